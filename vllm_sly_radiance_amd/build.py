@@ -1,9 +1,10 @@
-"""Build libw4a8_mxfp4.so in-tree with hipcc for gfx950 (one code object, no other target).
+"""Build libw4a8_mxfp4.so and libkv4_attn.so in-tree with hipcc for gfx950 (no other target).
 
     python -m vllm_sly_radiance_amd.build            # or __graft_entry__.build()
 
-The library is a plain C-ABI shared object (include/w4a8_mxfp4.h) loaded through ctypes; it links
-the HIP runtime by soname, so inside a torch process it binds to the runtime torch already loaded.
+The libraries are plain C-ABI shared objects (include/w4a8_mxfp4.h, include/kv4_attn.h) loaded
+through ctypes; they link the HIP runtime by soname, so inside a torch process they bind to the
+runtime torch already loaded.
 """
 from __future__ import annotations
 
@@ -23,6 +24,9 @@ ARCH = "gfx950"
 SOURCES = ["w4a8_api.hip", "w4a8_quant.hip", "w4a8_repack.hip", "w4a8_gemm_skinny.hip",
            "w4a8_gemm_stream.hip", "w4a8_gemm_ring.hip", "w4a8_gemm_tile.hip", "w4a8_gemm_band.hip",
            "w4a8_producers.hip", "w4a8_probe.hip"]
+
+KV4_LIB_PATH = os.path.join(PKG, "libkv4_attn.so")
+KV4_SOURCES = ["kv4_api.hip", "kv4_rope.hip", "kv4_pages.hip", "kv4_attn_rows.hip"]
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
@@ -44,23 +48,33 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (expected /opt/rocm/bin/hipcc)")
 
 
+def _command(sources, out) -> list[str]:
+    srcs = [os.path.join(CSRC, s) for s in sources]
+    return [hipcc(), *FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", out]
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every source into LIB_PATH (always rebuilds) and return the path."""
-    srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    tmp = LIB_PATH + ".tmp"
-    cmd = [hipcc(), *FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", tmp]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    # hipcc's host pass does not know the packed-fp32 target feature; that warning is expected
-    noise = [ln for ln in (res.stdout + res.stderr).splitlines()
-             if ln.strip() and "packed-fp32-ops" not in ln and "warning generated" not in ln
-             and "warnings generated" not in ln]
-    if res.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
-    if verbose and noise:
-        print("\n".join(noise), file=sys.stderr)
-    os.replace(tmp, LIB_PATH)
+    """Compile every source into LIB_PATH and KV4_LIB_PATH (always rebuilds, both at once) and
+    return LIB_PATH."""
+    jobs = []
+    for sources, path in ((SOURCES, LIB_PATH), (KV4_SOURCES, KV4_LIB_PATH)):
+        cmd = _command(sources, path + ".tmp")
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        jobs.append((path, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                            text=True)))
+    outputs = [(path, job.communicate()[0], job.returncode) for path, job in jobs]
+    for path, text, status in outputs:
+        # hipcc's host pass does not know the packed-fp32 target feature; that warning is expected
+        noise = [ln for ln in text.splitlines()
+                 if ln.strip() and "packed-fp32-ops" not in ln and "warning generated" not in ln
+                 and "warnings generated" not in ln]
+        if status != 0:
+            raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
+        if verbose and noise:
+            print("\n".join(noise), file=sys.stderr)
+    for path, _, _ in outputs:
+        os.replace(path + ".tmp", path)
     return LIB_PATH
 
 

@@ -1,0 +1,169 @@
+// Device helpers of the attention kernels over the 4-bit cache. Not part of the C ABI.
+#pragma once
+#include <type_traits>
+
+#include "kv4_internal.h"
+
+namespace kv4 {
+
+constexpr int kMaxChunk = 16384;   // tokens of a split at most: its page numbers fit in LDS
+
+int attn_row_fragments(int max_q, int Hq, int Hkv, int d);
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A sequence of the batch: its tokens, its first query row, its queries. Sizes that do not fit what
+// the launch was planned for make it bad: its rows are NaN.
+struct Sequence { int len, q0, n; bool bad; };
+__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
+  Sequence s;
+  s.len = a.lens[b];
+  s.q0 = a.starts[b];
+  s.n = a.starts[b + 1] - s.q0;
+  s.bad = s.len < 0 || s.len > a.max_len || ((long)s.len + (1 << a.page_shift) - 1) >> a.page_shift >
+          a.table_cols || s.q0 < 0 || s.n < 0 || s.n > a.max_q || s.q0 > a.total - s.n;
+  return s;
+}
+
+// Tokens [lo, hi) that the rows first .. last of a sequence see between them (lo rounded down to a
+// step), and [all_lo, all_hi) that each of them sees.
+struct Span { int lo, hi, all_lo, all_hi; };
+__device__ __forceinline__ Span tile_span(const AttnArgs& a, const Sequence& s, int first, int last,
+                                          int group_heads) {
+  const int p0 = s.len - s.n + first / group_heads, p1 = s.len - s.n + last / group_heads;
+  Span x;
+  x.hi = a.causal ? min(s.len, max(p1 + 1, 0)) : s.len;
+  x.all_hi = a.causal ? min(s.len, p0 + 1) : s.len;
+  x.lo = a.window > 0 ? max(p0 - a.window + 1, 0) & ~31 : 0;
+  x.all_lo = a.window > 0 ? p1 - a.window + 1 : 0;
+  return x;
+}
+
+// NaN to every output row of a bad sequence that lies in the output, for `heads` heads from h0.
+template <int D>
+__device__ __forceinline__ void nan_rows(const AttnArgs& a, const Sequence& s, int h0, int heads) {
+  const long first = max(s.q0, 0);
+  const long last = min((long)s.q0 + s.n, (long)a.total);
+  for (long i = first * heads * D + threadIdx.x; i < last * heads * D; i += blockDim.x) {
+    const long row = i / (heads * D), at = i % (heads * D);
+    a.out[(row * a.Hq + h0) * D + at] = 0x7FC0;
+  }
+}
+
+// 8 codes as a bf16 operand.
+__device__ __forceinline__ v8bf expand8(uint32_t codes, float scale) {
+  const v4i r = {(int)codes_bf16x2<0>(codes, scale), (int)codes_bf16x2<1>(codes, scale),
+                 (int)codes_bf16x2<2>(codes, scale), (int)codes_bf16x2<3>(codes, scale)};
+  return __builtin_bit_cast(v8bf, r);
+}
+
+__device__ __forceinline__ v8bf pack8bf(const float e[8]) {
+  const v4i r = {(int)bf16x2(e[0], e[1]), (int)bf16x2(e[2], e[3]), (int)bf16x2(e[4], e[5]),
+                 (int)bf16x2(e[6], e[7])};
+  return __builtin_bit_cast(v8bf, r);
+}
+
+__device__ __forceinline__ bool has_nan_scale(uint32_t four) {
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= ((four >> (8 * i)) & 0xFFu) == 0xFFu;
+  return any;
+}
+
+// The low (high) halves of two dwords, the first one's below.
+__device__ __forceinline__ int halves_lo(uint32_t x, uint32_t y) {
+  return (int)__builtin_amdgcn_perm(y, x, 0x05040100u);
+}
+__device__ __forceinline__ int halves_hi(uint32_t x, uint32_t y) {
+  return (int)__builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+
+// Byte B (channels 2 B, 2 B + 1 of the run) of 4 + 4 tokens' codes as the two channels' operands.
+template <int B, typename F>
+__device__ __forceinline__ void value_pair(v8bf& even, v8bf& odd, F codes, const float s[8]) {
+  uint32_t x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = codes(i, s[i], std::integral_constant<int, B>());
+  const v4i lo = {halves_lo(x[0], x[1]), halves_lo(x[2], x[3]), halves_lo(x[4], x[5]),
+                  halves_lo(x[6], x[7])};
+  const v4i hi = {halves_hi(x[0], x[1]), halves_hi(x[2], x[3]), halves_hi(x[4], x[5]),
+                  halves_hi(x[6], x[7])};
+  even = __builtin_bit_cast(v8bf, lo);
+  odd = __builtin_bit_cast(v8bf, hi);
+}
+
+// A run's channels as operands over the 8 tokens of a lane (4 g + i of two groups of 16).
+template <int D, typename Vec>
+__device__ __forceinline__ void value_operands(v8bf vf[Group<D>::kRun], Vec v0, uint32_t s0, Vec v1,
+                                               uint32_t s1) {
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s[i] = scale_of((s0 >> (8 * i)) & 0xFFu);
+    s[4 + i] = scale_of((s1 >> (8 * i)) & 0xFFu);
+  }
+  if constexpr (D >= 128) {
+    // dword i: token i's 4 bytes
+    auto codes = [&](int i, float sc, auto b) {
+      return codes_bf16x2<decltype(b)::value>((uint32_t)(i < 4 ? v0[i] : v1[i - 4]), sc);
+    };
+    value_pair<0>(vf[0], vf[1], codes, s);
+    value_pair<1>(vf[2], vf[3], codes, s);
+    value_pair<2>(vf[4], vf[5], codes, s);
+    value_pair<3>(vf[6], vf[7], codes, s);
+  } else {
+    // dword i / 2: tokens i, i + 1, 2 bytes each
+    auto codes = [&](int i, float sc, auto b) {
+      const uint32_t w = (uint32_t)(i < 4 ? v0[i >> 1] : v1[(i - 4) >> 1]);
+      constexpr int B = decltype(b)::value;
+      return i & 1 ? codes_bf16x2<B + 2>(w, sc) : codes_bf16x2<B>(w, sc);
+    };
+    value_pair<0>(vf[0], vf[1], codes, s);
+    value_pair<1>(vf[2], vf[3], codes, s);
+  }
+}
+
+// C consecutive channels of an output row: y / sum in bf16, zeros where nothing was summed.
+template <int C>
+__device__ __forceinline__ void store_row(uint16_t* out, const float y[C], float sum) {
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float z[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) z[i] = sum == 0.0f ? 0.0f : y[i] * inv;
+  if constexpr (C == 1) {
+    *out = (uint16_t)bf16x2(z[0], 0.0f);
+  } else {
+    uint32_t w[C / 2];
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i) w[i] = bf16x2(z[2 * i], z[2 * i + 1]);
+    __builtin_memcpy(__builtin_assume_aligned(out, 2 * C), w, 2 * C);
+  }
+}
+
+// Partial results: fp32 [batch][Hkv][splits][rows][D], then [..][rows][2] with the row's maximum (in
+// units of log2) and sum.
+__device__ __forceinline__ size_t part_index(const AttnArgs& a, int b, int h, int split, int row) {
+  const size_t rows = (size_t)a.max_q * (a.Hq / a.Hkv);
+  return (((size_t)b * a.Hkv + h) * a.splits + split) * rows + row;
+}
+__device__ __forceinline__ float* part_row(const AttnArgs& a, int D, int b, int h, int split, int row) {
+  return a.part + part_index(a, b, h, split, row) * D;
+}
+__device__ __forceinline__ float* part_stat(const AttnArgs& a, int D, int b, int h, int split,
+                                            int row) {
+  return a.part + part_index(a, a.batch, 0, 0, 0) * D + part_index(a, b, h, split, row) * 2;
+}
+template <int D, int C>
+__device__ __forceinline__ void store_part(const AttnArgs& a, int b, int h, int split, int row,
+                                           int ch, const float y[C], float top, float sum) {
+  float* o = part_row(a, D, b, h, split, row) + ch;
+#pragma unroll
+  for (int i = 0; i < C; i += 4)
+    *reinterpret_cast<v4f*>(o + i) = v4f{y[i], y[i + 1], y[i + 2], y[i + 3]};
+  if (ch == 0) {
+    float* st = part_stat(a, D, b, h, split, row);
+    st[0] = top, st[1] = sum;
+  }
+}
+
+}  // namespace kv4
