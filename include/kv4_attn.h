@@ -83,7 +83,7 @@ int kv4_qk_norm_rope(const void* q, long q_ts, long q_hs, const void* k, long k_
 /* kv4_qk_norm_rope with the new keys (rounded from fp32) and values bf16 [T, kv_heads, d] written
  * to the cache instead of a k_out: token t goes to slot slots[t] = page number * page + place (int64
  * [T]; a slot below 0 or past the last page is skipped, slots are distinct). page_stride: bytes from
- * one page to the next, a multiple of 16. */
+ * one page to the next, a multiple of 16 below 2^32. */
 int kv4_qk_norm_rope_append(const void* q, long q_ts, long q_hs, const void* k, long k_ts,
                             long k_hs, const void* v, long v_ts, long v_hs, const void* q_weight,
                             const void* k_weight, const void* cos_sin, long table_rows, int rot,

@@ -74,6 +74,29 @@ def test_long_context_is_split():
     b.check(run(b, max_q=9))
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 150])
+def test_many_sequences(n):
+    """The runs are found 64 sequences at a time; most sequences empty, short ones, a long one at either
+    end, and workgroups without work."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.choice([0, 0, 1, 17, 130, 300], n)]
+    lens[0], lens[-1], lens[n // 2] = 700, 1000, 900
+    qs = [int(x) for x in rng.choice([0, 1, 1, 2], n)]
+    qs[0] = qs[-1] = qs[n // 2] = 1
+    b = Batch(rng, lens, qs, 2, 1, 64, 16)
+    b.check(run(b))
+    b.check(run(b, window=40), window=40)
+
+
+def test_batches_longer_than_they_are():
+    """Limits far above the batch's lengths, as a graph's are: workgroups without work."""
+    b = Batch(np.random.default_rng(21), [3, 900, 1], [1, 1, 1], 4, 2, 128, 16)
+    b.check(run(b, max_len=1 << 20))
+    b.check(run(b, max_q=4, max_len=1 << 20))
+    b = Batch(np.random.default_rng(22), [1], [1], 4, 2, 256, 16)
+    b.check(run(b, max_len=1 << 20))
+
+
 def test_scores_far_apart_and_alike():
     """One key far above the others at either end; equal scores; large and tiny scales."""
     rng = np.random.default_rng(5)

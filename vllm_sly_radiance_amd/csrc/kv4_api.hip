@@ -57,9 +57,9 @@ int check_cache(const char* who, const void* cache, long pages, long page_stride
   if (pages < 0 || pages > 0x7FFFFFFFL)
     return fail(KV4_EINVAL, "%s: %ld pages", who, pages);
   const long bytes = (long)heads * (page / 16) * 17 * d;
-  if (page_stride < bytes || page_stride % 16)
-    return fail(KV4_EINVAL, "%s: page stride %ld is less than a page's %ld bytes or no multiple of 16",
-                who, page_stride, bytes);
+  if (page_stride < bytes || page_stride % 16 || page_stride >> 32)
+    return fail(KV4_EINVAL, "%s: page stride %ld is less than a page's %ld bytes, 2^32 or more, or no "
+                "multiple of 16", who, page_stride, bytes);
   if (!cache && pages) return fail(KV4_EINVAL, "%s: null cache", who);
   if (!aligned(cache, 16)) return fail(KV4_EINVAL, "%s: the cache is not 16-byte aligned", who);
   return KV4_OK;
@@ -119,6 +119,11 @@ int attn_sizes(const char* who, int batch, int max_q, int max_len, int q_heads, 
   if ((long)batch * q_heads * max_q > 0x7FFFFFFFL)
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d q_heads=%d are too many rows", who, batch, max_q,
                 q_heads);
+  // work is counted in granules of 128 tokens (fewer rows a tile make more of them)
+  if (((long)batch * kv_heads * (((long)max_q * (q_heads / kv_heads) + 15) / 16)) *
+          ((max_len + 127L) / 128) > (1L << 30))
+    return fail(KV4_EINVAL, "%s: batch=%d max_q=%d max_len=%d are too much for one call", who, batch,
+                max_q, max_len);
   return KV4_OK;
 }
 
@@ -242,8 +247,9 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   a.q_ts = q_ts, a.q_hs = q_hs, a.page_stride = page_stride, a.pages = pages;
   a.table_stride = table_stride, a.page_shift = page_shift(page), a.table_cols = table_cols;
   a.total = total, a.batch = batch, a.max_q = max_q, a.max_len = max_len;
-  a.Hq = q_heads, a.Hkv = kv_heads, a.window = window, a.scale = scale;
-  a.causal = flags & KV4_CAUSAL, a.chunk = plan.chunk, a.splits = plan.splits;
+  a.Hq = q_heads, a.Hkv = kv_heads, a.group = q_heads / kv_heads;
+  a.window = window, a.scale = scale;
+  a.causal = flags & KV4_CAUSAL, a.runs = plan.runs;
   return hip_status(launch_attn(a, d, (hipStream_t)stream), who);
 }
 

@@ -3,8 +3,8 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c s_j - m),  s_j = q . k_j,  c = scale * log2(e)
 //
 // The rows of one kv head are its sequence's queries times the query heads that share it; a
-// workgroup has 16 * RF of them and one chunk of the cached tokens, its four waves 32 tokens at a
-// time in turn. Keys and values are read once, straight into registers in matrix-operand order:
+// workgroup has 16 * RF of them and a run of the cached tokens, its W waves 32 tokens at a time in
+// turn. Keys and values are read once, straight into registers in matrix-operand order:
 //   S^T = K . Q^T   (16 tokens x 16 rows): lane (g = l / 16, r = l % 16) holds token r, one block of
 //                   32 channels per instruction group; its 16 bytes of codes and one scale.
 //   O^T = V^T . P^T (16 channels x 16 rows over 32 tokens): the scores' registers are already the
@@ -12,8 +12,14 @@
 //                   lane the same 8 tokens of the 8 channels of run r.
 // Codes become bf16 by v_cvt_scalef32_pk_bf16_fp4, exactly, with their block's scale. The running
 // maximum moves only when a score passes it by 2^8, so that most steps have no exchange between
-// lanes and no rescaling; what is above 1 costs no precision in fp32 and bf16. Waves meet in LDS,
-// chunks in a second launch that weighs the partial results.
+// lanes and no rescaling; what is above 1 costs no precision in fp32 and bf16. Waves meet in LDS.
+//
+// The work of a batch is the tokens of all its units (sequence, row tile, kv head), in granules of
+// 32 W. As many workgroups as the card holds at once take an equal run of granules each, found from
+// the lengths on the device: one round, no tail, whatever the lengths are, and a graph captured with
+// a batch's limits balances every replay. A unit inside one run is finished there; one that crosses
+// runs leaves partial results, at most two a workgroup, for a second launch to weigh. Short
+// contexts take a workgroup a unit and no second launch.
 //
 // Bounded by HBM where the cache is long; by the launches and three dependent reads (length, page,
 // tokens) where it is short.
@@ -23,7 +29,6 @@
 namespace kv4 {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kStep = 32;                   // tokens of a wave's step
 
 // The codes and scales of 16 tokens, as a lane holds them.
@@ -35,209 +40,338 @@ struct Raw {
   uint32_t ks[P], vs[P];
 };
 
+// group: the same in every lane; the lane's share of it is an unsigned 32-bit offset, so the loads
+// take a scalar base
 template <int D>
-__device__ __forceinline__ void load_group(Raw<D>& w, const uint8_t* group, int g, int r) {
+__device__ __forceinline__ void load_keys(Raw<D>& w, const uint8_t* group, uint32_t g, uint32_t r) {
   using G = Group<D>;
   typedef typename Raw<D>::Vec Vec;
-  constexpr int B = sizeof(Vec);
 #pragma unroll
   for (int p = 0; p < G::kPlanes; ++p) {
-    w.k[p] = *reinterpret_cast<const Vec*>(group + G::kKeys + r * (D / 2) + p * 64 + g * B);
-    w.v[p] = *reinterpret_cast<const Vec*>(group + G::kValues + ((p * 4 + g) * 16 + r) * B);
-    w.ks[p] = group[G::kKeyScales + r * (D / kBlock) + (D >= 128 ? 4 * p + g : g >> 1)];
+    w.k[p] = *reinterpret_cast<const Vec*>(
+        group + (uint32_t)(G::kKeys + r * (D / 2) + p * 64 + g * sizeof(Vec)));
+    w.ks[p] =
+        group[(uint32_t)(G::kKeyScales + r * (D / kBlock) + (D >= 128 ? 4 * p + g : g >> 1))];
+  }
+}
+template <int D>
+__device__ __forceinline__ void load_values(Raw<D>& w, const uint8_t* group, uint32_t g,
+                                            uint32_t r) {
+  using G = Group<D>;
+  typedef typename Raw<D>::Vec Vec;
+#pragma unroll
+  for (int p = 0; p < G::kPlanes; ++p) {
+    w.v[p] = *reinterpret_cast<const Vec*>(
+        group + (uint32_t)(G::kValues + ((p * 4 + g) * 16 + r) * sizeof(Vec)));
     w.vs[p] = *reinterpret_cast<const uint32_t*>(
-        group + G::kValueScales + (D >= 128 ? 4 * p + (r >> 2) : r >> 3) * kGroup + 4 * g);
+        group + (uint32_t)(G::kValueScales + (D >= 128 ? 4 * p + (r >> 2) : r >> 3) * kGroup + 4 * g));
   }
 }
 
-template <int D, int RF>
-__global__ __launch_bounds__(256) void attn_rows(AttnArgs a, int tiles) {
+// Granules of a sequence's units: each of tiles x kv heads units has as many as its visible tokens
+// take, one at least (a unit of no tokens writes its zeros, a bad sequence its NaN).
+struct Units { int per_unit, units, lo; };
+template <int kGranule>
+__device__ __forceinline__ Units units_of(const AttnArgs& a, const Sequence& s, int tile_rows) {
+  if (s.bad) return {1, a.Hkv, 0};
+  const int R = s.n * a.group;
+  if (R == 0) return {1, 0, 0};
+  const Span x = query_span(a, s, 0, s.n - 1);
+  return {x.hi > x.lo ? ceil_div(x.hi - x.lo, kGranule) : 1, ceil_div(R, tile_rows) * a.Hkv, x.lo};
+}
+
+// Inclusive scan over the wave: shifts inside rows of 16 lanes, then the rows' last lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast:15, rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast:31, rows 2 and 3
+  return x;
+}
+
+// A run of granules of the batch: its first sequence, the granule of that sequence's work, and how
+// many. Every wave finds it by itself, 64 sequences at a time: no exchange between waves.
+struct Run { Sequence s; int b; uint32_t off, left, share; };
+template <int kGranule>
+__device__ __forceinline__ Run find_run(const AttnArgs& a, int tile_rows, int lane) {
+  auto work = [&](int i, Sequence& s) {
+    s = {0, 0, 0, false};
+    if (i >= a.batch) return 0u;
+    s = sequence(a, i);
+    const Units x = units_of<kGranule>(a, s, tile_rows);
+    return (uint32_t)x.per_unit * (uint32_t)x.units;
+  };
+  Run run = {{0, 0, 0, false}, 0, 0, 0, 0};
+  Sequence s;
+  uint32_t w = work(lane, s), upto = wave_scan(w);
+  uint32_t total = __builtin_amdgcn_readlane(upto, 63);
+  for (int i0 = 64; i0 < a.batch; i0 += 64) {
+    Sequence other;
+    total += __builtin_amdgcn_readlane(wave_scan(work(i0 + lane, other)), 63);
+  }
+  run.share = a.by_runs(total + a.runs - 1);
+  const uint32_t at = run.share * blockIdx.x;
+  if (at >= total) return run;           // no work left for this workgroup
+  run.left = min(run.share, total - at);
+  uint32_t before = 0;
+  for (int i0 = 0; i0 < a.batch;) {
+    const uint32_t lo = before + upto - w;
+    const uint64_t here = __ballot(at >= lo && at - lo < w);
+    if (here) {
+      const int k = __builtin_ctzll(here);
+      run.b = i0 + k;
+      run.off = at - __builtin_amdgcn_readlane(lo, k);
+      run.s.len = __builtin_amdgcn_readlane(s.len, k);
+      run.s.q0 = __builtin_amdgcn_readlane(s.q0, k);
+      run.s.n = __builtin_amdgcn_readlane(s.n, k);
+      run.s.bad = __builtin_amdgcn_readlane(s.bad, k);
+      return run;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+    i0 += 64;
+    w = work(i0 + lane, s), upto = wave_scan(w);
+  }
+  run.left = 0;
+  return run;
+}
+
+template <int D, int RF, int W>
+struct Shared {
+  v4i q[RF * (D / 32)][64];
+  float stat[2][W][RF * 16];
+  float merge[W][16][D + 4];
+  int bad_page;
+};
+
+template <int D, int RF, int W, int NS>
+__global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs a) {
   using G = Group<D>;
   constexpr int P = G::kPlanes, M = G::kRun, KS = D / 32;   // planes, channels of a run, K steps
-  constexpr int kPad = D + 4;
-  __shared__ int pages[kMaxChunk / 16 + 1];
-  __shared__ int bad_page;
-  __shared__ float stat[2][kWaves][RF * 16];
-  __shared__ float merge[kWaves][16][kPad];
+  constexpr int kGranule = kStep * W, kTile = 16 * RF;
+  __shared__ Shared<D, RF, W> sh;
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group_heads = a.group;
 
-  // workgroups: [batch][row tiles][kv heads][splits]
-  const int group_heads = a.Hq / a.Hkv;
-  const int split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
-  const int h = rest % a.Hkv, tile = rest / a.Hkv % tiles, b = rest / a.Hkv / tiles;
-  const Sequence s = sequence(a, b);
-  if (s.bad) {
-    if (split == 0 && tile == 0) nan_rows<D>(a, s, h * group_heads, group_heads);
-    return;
+  Run run = {{0, 0, 0, false}, 0, 0, 0, 0};
+  if (a.tiles) {
+    // short contexts: one unit, workgroups [batch][tiles][kv heads]
+    const uint32_t per = a.tiles * a.Hkv;
+    run.b = blockIdx.x / per;
+    run.s = sequence_uniform(a, run.b);
+    const Units x = units_of<kGranule>(a, run.s, kTile);
+    const uint32_t u = blockIdx.x % per;
+    if (u >= (uint32_t)x.units) return;
+    run.off = u * x.per_unit, run.left = x.per_unit, run.share = 0;
+  } else {
+    run = find_run<kGranule>(a, kTile, lane);
+    if (tid == 0 && !a.by_unit) meta(a, kTile, D, blockIdx.x)[0] = 0;
+    if (!run.left) return;
   }
-  const int R = s.n * group_heads, r0 = tile * 16 * RF;
-  if (r0 >= R) return;
-  const Span span = tile_span(a, s, r0, min(r0 + 16 * RF, R) - 1, group_heads);
-  const int t0 = span.lo + split * a.chunk;
-  const int t1 = min(span.hi, t0 + a.chunk);
-  const bool direct = span.hi - span.lo <= a.chunk;     // one chunk: no partial results
-  if (t0 >= t1 && !(direct && split == 0)) return;
-
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, r = lane & 15;
-  const int first_page = t0 >> a.page_shift;
-  const int npages = t1 > t0 ? ((t1 - 1) >> a.page_shift) - first_page + 1 : 0;
-  if (tid == 0) bad_page = 0;
-  __syncthreads();
-  for (int i = tid; i < npages; i += 256) {
-    const int p = a.pages_of[(size_t)b * a.table_stride + first_page + i];
-    const bool ok = p >= 0 && p < a.pages;
-    pages[i] = ok ? p : 0;
-    if (!ok) bad_page = 1;
-  }
-
-  // this lane's rows: query operand, and the tokens they see
-  v8bf q[RF][KS];
-  int hi[RF], lo[RF];
-#pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    const int row = r0 + f * 16 + r;
-    const int qi = min(row, R - 1) / group_heads, head = min(row, R - 1) % group_heads;
-    const int place = s.len - s.n + qi;
-    hi[f] = a.causal ? min(place + 1, s.len) : s.len;
-    lo[f] = a.window > 0 ? place - a.window + 1 : 0;
-    const uint16_t* src = a.q + (size_t)(s.q0 + qi) * a.q_ts + (size_t)(h * group_heads + head) * a.q_hs;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-      q[f][k] = __builtin_bit_cast(
-          v8bf, *reinterpret_cast<const v4i*>(
-                    src + (D >= 128 ? 128 * (k >> 2) + 32 * g + 8 * (k & 3) : 16 * g + 8 * k)));
-  }
-  __syncthreads();
-
-  const uint8_t* head_base = a.cache + (size_t)(h << (a.page_shift - 4)) * G::kBytes;
-  const int group_mask = (1 << (a.page_shift - 4)) - 1;
-  auto group_at = [&](int t) {
-    const int i = min((t >> a.page_shift) - first_page, npages - 1);
-    const int p = __builtin_amdgcn_readfirstlane(pages[i]);
-    return head_base + (size_t)p * a.page_stride + (size_t)((t >> 4) & group_mask) * G::kBytes;
-  };
 
   const float c = a.scale * 1.44269504088896340736f;
   const float slack = 8.0f / c;
-  float m[RF], l[RF];                  // row maximum (raw scores), this lane's share of the sum
-  v4f o[RF][P][M];
-#pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    m[f] = -INFINITY, l[f] = 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int i = 0; i < M; ++i) o[f][p][i] = v4f{0, 0, 0, 0};
-  }
-
-  Raw<D> cur[2], nxt[2];
-  int t = t0 + wave * kStep;
-  if (t < t1) {
-    load_group<D>(cur[0], group_at(t), g, r);
-    load_group<D>(cur[1], group_at(t + 16), g, r);
-  }
-  for (; t < t1; t += kWaves * kStep) {
-    const int tn = t + kWaves * kStep;
-    if (tn < t1) {
-      load_group<D>(nxt[0], group_at(tn), g, r);
-      load_group<D>(nxt[1], group_at(tn + 16), g, r);
+  int unit = 0, gu = 0;       // unit of the sequence and granule of the unit that the run stands at
+  {
+    const Units un = units_of<kGranule>(a, run.s, kTile);
+    if (run.off) {
+      unit = __builtin_amdgcn_readfirstlane(run.off / (uint32_t)un.per_unit);
+      gu = run.off - unit * un.per_unit;
     }
-    // scores of 2 x 16 tokens: lane holds tokens 4 g + i of both, row r
-    v4f sc[RF][2];
+  }
+  while (true) {
+    const Sequence s = run.s;
+    const int b = run.b;
+    const Units un = units_of<kGranule>(a, s, kTile);
+    if (unit >= un.units) {                                 // the next sequence
+      if (++run.b >= a.batch) return;
+      unit = 0;
+      run.s = sequence_uniform(a, run.b);
+      continue;
+    }
+    const int take = min((uint32_t)(un.per_unit - gu), run.left);
+    const int tile = a.by_heads(unit), h = unit - tile * a.Hkv;
+    const bool whole = take == un.per_unit;
+    const int first_granule = gu, this_unit = unit;
+    run.left -= take, gu += take;
+    if (gu == un.per_unit) ++unit, gu = 0;
+    if (s.bad) {
+      nan_rows<D>(a, s, h * group_heads, group_heads);
+      if (!run.left) return;
+      continue;
+    }
+    const int R = s.n * group_heads, r0 = tile * kTile;
+    const Span span = query_span(a, s, a.by_group(r0), a.by_group(min(r0 + kTile, R) - 1));
+    const int t0 = un.lo + first_granule * kGranule;
+    const int t1 = min(span.hi, t0 + take * kGranule);
+
+    // the rows' query operands, asked for here and put into LDS for all waves behind the first loads
+    // of the cache; the tokens that this lane's rows see
+    constexpr int kOps = ceil_div(RF * KS, W);
+    v4i ops[kOps];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int j = 0; j < kOps; ++j) {
+      const int i = wave + j * W, k = i % KS;
+      const int row = min(r0 + min(i / KS, RF - 1) * 16 + r, R - 1), qi = a.by_group(row);
+      const uint16_t* src = a.q + (size_t)(s.q0 + qi) * a.q_ts +
+                            (size_t)(h * group_heads + row - qi * group_heads) * a.q_hs;
+      ops[j] = *reinterpret_cast<const v4i*>(
+          src + (D >= 128 ? 128 * (k >> 2) + 32 * g + 8 * (k & 3) : 16 * g + 8 * k));
+    }
+    int hi[RF], lo[RF];
 #pragma unroll
-      for (int f = 0; f < RF; ++f) sc[f][u] = v4f{0, 0, 0, 0};
+    for (int f = 0; f < RF; ++f) {
+      const int place = s.len - s.n + a.by_group(min(r0 + f * 16 + r, R - 1));
+      hi[f] = a.causal ? min(place + 1, s.len) : s.len;
+      lo[f] = a.window > 0 ? place - a.window + 1 : 0;
+    }
+
+    // The page of a step's 16 tokens: its number is read two steps ahead of the tokens' use. Tokens
+    // from t1 on read the last page that holds some before it.
+    const int* table = a.pages_of + (size_t)b * a.table_stride;
+    const uint8_t* head_base = a.cache + (size_t)(h << (a.page_shift - 4)) * G::kBytes;
+    const int group_mask = (1 << (a.page_shift - 4)) - 1;
+    const int last_page = (t1 - 1) >> a.page_shift;
+    bool bad = false;
+    auto page_of = [&](int t) { return scalar_load(table + min(t >> a.page_shift, last_page)); };
+    auto group_at = [&](int t, int page) {
+      const int p = __builtin_amdgcn_readfirstlane(page);
+      const bool ok = (uint32_t)p < (uint32_t)a.pages;
+      bad |= !ok;
+      return head_base + (uint64_t)(uint32_t)(ok ? p : 0) * (uint32_t)a.page_stride +
+             (uint32_t)((t >> 4) & group_mask) * (uint32_t)G::kBytes;
+    };
+
+    float m[RF], l[RF];                // row maximum (raw scores), this lane's share of the sum
+    v4f o[RF][P][M];
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+      m[f] = -INFINITY, l[f] = 0.0f;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < M; ++i) o[f][p][i] = v4f{0, 0, 0, 0};
+    }
+
+    // NS steps' codes in registers: the keys of the step NS on are asked for when this one's scores are
+    // done, its values when this one's products are. Past the end the segment's last step is asked
+    // for again (cache hits that nothing uses): loads that are always issued let the waits count
+    // those in flight instead of draining them.
+    Raw<D> ring[NS][2];
+    const int t_last = (t1 - 1 - t0) / kStep * kStep + t0;
+    int t = t0 + wave * kStep;
+    int na = 0, nb = 0;                // page numbers of the next step to ask for
+    if (t < t1) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const int tj = min(t + j * kGranule, t_last);
+        const uint8_t* ga = group_at(tj, page_of(tj));
+        const uint8_t* gb = group_at(tj + 16, page_of(tj + 16));
+        load_keys<D>(ring[j][0], ga, g, r), load_keys<D>(ring[j][1], gb, g, r);
+        load_values<D>(ring[j][0], ga, g, r), load_values<D>(ring[j][1], gb, g, r);
+      }
+      const int tj = min(t + NS * kGranule, t_last);
+      na = page_of(tj), nb = page_of(tj + 16);
+    }
+#pragma unroll
+    for (int j = 0; j < kOps; ++j)
+      if (wave + j * W < RF * KS) sh.q[wave + j * W][lane] = ops[j];
+    __syncthreads();
+    while (t < t1) {
+#pragma unroll
+     for (int j = 0; j < NS; ++j, t += kGranule) {
+      if (j && t >= t1) break;
+      Raw<D>(&w)[2] = ring[j];
+      // scores of 2 x 16 tokens: lane holds tokens 4 g + i of both, row r
+      v4f sc[RF][2];
+#pragma unroll
+      for (int f = 0; f < RF; ++f) sc[f][0] = sc[f][1] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int p = D >= 128 ? k >> 2 : 0;
-        const v8bf kf = expand8(cur[u].k[p][D >= 128 ? k & 3 : k], scale_of(cur[u].ks[p]));
+        const v8bf k0 = expand8(w[0].k[p][D >= 128 ? k & 3 : k], scale_of(w[0].ks[p]));
+        const v8bf k1 = expand8(w[1].k[p][D >= 128 ? k & 3 : k], scale_of(w[1].ks[p]));
+#pragma unroll
+        for (int f = 0; f < RF; ++f) {
+          const v8bf q = __builtin_bit_cast(v8bf, sh.q[f * KS + k][lane]);
+          sc[f][0] = mfma16(k0, q, sc[f][0]);
+          sc[f][1] = mfma16(k1, q, sc[f][1]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const int tn = min(t + NS * kGranule, t_last);
+      const uint8_t* ga = group_at(tn, na);
+      const uint8_t* gb = group_at(tn + 16, nb);
+      load_keys<D>(w[0], ga, g, r), load_keys<D>(w[1], gb, g, r);
+      const int tp = min(tn + kGranule, t_last);
+      na = page_of(tp), nb = page_of(tp + 16);
+      if (t + kStep > span.all_hi || t < span.all_lo) {   // tokens that some row does not see
 #pragma unroll
         for (int f = 0; f < RF; ++f)
-          sc[f][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[f][k], sc[f][u], 0, 0, 0);
-      }
-    }
-    // tokens that some row of the tile does not see
-    const bool edge = t + kStep > span.all_hi || t < span.all_lo;
-    if (edge) {
-#pragma unroll
-      for (int f = 0; f < RF; ++f)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tok = t + 16 * u + 4 * g + i;
-            if (tok >= hi[f] || tok < lo[f]) sc[f][u][i] = -INFINITY;
-          }
-      // what lies behind the last token that any row sees is not the sequence's: its values are
-      // zeroed, whatever they hold
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t + 16 * u + 4 * g + i >= t1)
-#pragma unroll
-            for (int p = 0; p < P; ++p) cur[u].vs[p] &= ~(0xFFu << (8 * i));
-    }
-    v8bf pr[RF];
-#pragma unroll
-    for (int f = 0; f < RF; ++f) {
-      float mx = fmaxf(fmaxf(fmaxf(sc[f][0][0], sc[f][0][1]), fmaxf(sc[f][0][2], sc[f][0][3])),
-                       fmaxf(fmaxf(sc[f][1][0], sc[f][1][1]), fmaxf(sc[f][1][2], sc[f][1][3])));
-      if (__ballot(mx > m[f] + slack)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m[f], mx);
-        const float alpha = mn == m[f] ? 1.0f : exp2_raw((m[f] - mn) * c);
-        m[f] = mn;
-        l[f] *= alpha;
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-#pragma unroll
-          for (int i = 0; i < M; ++i) o[f][p][i] *= alpha;
-      }
-      const float sub = m[f] == -INFINITY ? 0.0f : m[f] * c;
-      float e[8];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[4 * u + i] = exp2_raw(fmaf(sc[f][u][i], c, -sub));
-      l[f] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-      pr[f] = pack8bf(e);
-    }
-    if (edge) {
-      // A NaN block of a token that some rows see and others do not: its product with a weight of
-      // zero would reach the rows that do not. It is taken out of the values, and the rows that
-      // see it are marked through a product of its own.
-      bool any = false;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int p = 0; p < P; ++p) any |= has_nan_scale(cur[u].vs[p]);
-      if (__ballot(any)) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          float isnan[8];
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t e = (cur[u].vs[p] >> (8 * i)) & 0xFFu;
-              isnan[4 * u + i] = e == 0xFFu ? 1.0f : 0.0f;
-              if (e == 0xFFu) cur[u].vs[p] &= ~(0xFFu << (8 * i));
+              const int tok = t + 16 * u + 4 * g + i;
+              if (tok >= hi[f] || tok < lo[f]) sc[f][u][i] = -INFINITY;
             }
-          const v8bf mark = pack8bf(isnan);
+      }
+      v8bf pr[RF];
+#pragma unroll
+      for (int f = 0; f < RF; ++f) {
+        float mx = fmaxf(fmaxf(fmaxf(sc[f][0][0], sc[f][0][1]), fmaxf(sc[f][0][2], sc[f][0][3])),
+                         fmaxf(fmaxf(sc[f][1][0], sc[f][1][1]), fmaxf(sc[f][1][2], sc[f][1][3])));
+        if (__ballot(mx > m[f] + slack)) {
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float mn = fmaxf(m[f], mx);
+          const float alpha = mn == m[f] ? 1.0f : exp2_raw((m[f] - mn) * c);
+          m[f] = mn;
+          l[f] *= alpha;
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int i = 0; i < M; ++i) o[f][p][i] *= alpha;
+        }
+        const float sub = m[f] == -INFINITY ? 0.0f : m[f] * c;
+        float e[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[4 * u + i] = exp2_raw(fmaf(sc[f][u][i], c, -sub));
+        l[f] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        pr[f] = pack8bf(e);
+      }
+      // A NaN block of a token that a row does not see (a later query's, or nobody's behind the last
+      // token): its product with a weight of zero would reach the row. Such blocks are taken out of
+      // the values, and the rows that do see them are marked through a product of its own.
+      uint32_t nan = 0;
+#pragma unroll
+      for (int p = 0; p < P; ++p) nan |= nan_scales(w[0].vs[p]) | nan_scales(w[1].vs[p]);
+      if (__ballot(nan != 0)) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          float is[8];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t hit = nan_scales(w[u].vs[p]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) is[4 * u + i] = hit >> (8 * i) & 0xFFu ? 1.0f : 0.0f;
+            w[u].vs[p] &= ~((hit >> 7) * 0xFFu);
+          }
+          const v8bf mark = pack8bf(is);
 #pragma unroll
           for (int f = 0; f < RF; ++f) {
-            float sees[8];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int tok = t + 16 * u + 4 * g + i;
-                sees[4 * u + i] = tok < hi[f] && tok >= lo[f] ? 1.0f : 0.0f;
+                is[4 * u + i] = tok < hi[f] && tok >= lo[f] ? 1.0f : 0.0f;
               }
-            const v4f hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mark, pack8bf(sees),
-                                                                    v4f{0, 0, 0, 0}, 0, 0, 0);
+            const v4f hit = mfma16(mark, pack8bf(is), v4f{0, 0, 0, 0});
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -246,124 +380,194 @@ __global__ __launch_bounds__(256) void attn_rows(AttnArgs a, int tiles) {
           }
         }
       }
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        each_value_pair<D>(w[0].v[p], w[0].vs[p], w[1].v[p], w[1].vs[p],
+                           [&](auto pair, v8bf even, v8bf odd) {
+                             constexpr int i = 2 * decltype(pair)::value;
+#pragma unroll
+                             for (int f = 0; f < RF; ++f) {
+                               o[f][p][i] = mfma16(even, pr[f], o[f][p][i]);
+                               o[f][p][i + 1] = mfma16(odd, pr[f], o[f][p][i + 1]);
+                             }
+                             __builtin_amdgcn_sched_barrier(0);
+                           });
+      load_values<D>(w[0], ga, g, r), load_values<D>(w[1], gb, g, r);
+     }
     }
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      v8bf vf[M];
-      value_operands<D>(vf, cur[0].v[p], cur[0].vs[p], cur[1].v[p], cur[1].vs[p]);
-#pragma unroll
-      for (int i = 0; i < M; ++i)
-#pragma unroll
-        for (int f = 0; f < RF; ++f)
-          o[f][p][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[i], pr[f], o[f][p][i], 0, 0, 0);
-    }
-    cur[0] = nxt[0];
-    cur[1] = nxt[1];
-  }
 
-  // ---- the waves' shares -------------------------------------------------------------------------
+    // ---- the waves' shares -----------------------------------------------------------------------
+    {
+    // (tid pinned here, or the addresses below are kept in registers through the steps)
+    const int tid = pinned(threadIdx.x), lane = tid & 63, g = lane >> 4, r = lane & 15;
+    if (tid == 0) sh.bad_page = 0;
 #pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    l[f] += __shfl_xor(l[f], 16);
-    l[f] += __shfl_xor(l[f], 32);
-    if (g == 0) stat[0][wave][f * 16 + r] = m[f], stat[1][wave][f * 16 + r] = l[f];
-  }
-  __syncthreads();
-  const bool poison = bad_page != 0;
+    for (int f = 0; f < RF; ++f) {
+      l[f] += __shfl_xor(l[f], 16);
+      l[f] += __shfl_xor(l[f], 32);
+      if (g == 0) sh.stat[0][wave][f * 16 + r] = m[f], sh.stat[1][wave][f * 16 + r] = l[f];
+    }
+    __syncthreads();
+    if (bad) sh.bad_page = 1;
+    const int which = first_granule > 0 ? 0 : 1;
 #pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    float top = -INFINITY;
+    for (int f = 0; f < RF; ++f) {
+      float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stat[0][w][f * 16 + r]);
-    const float mine = m[f] == top ? 1.0f : exp2_raw((m[f] - top) * c);
+      for (int w = 0; w < W; ++w) top = fmaxf(top, sh.stat[0][w][f * 16 + r]);
+      const float mine = m[f] == top ? 1.0f : exp2_raw((m[f] - top) * c);
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+      for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        // channels of the plane: M * (4 g + x) + i
+        for (int x = 0; x < 4; ++x) {
+          // channels of the plane: M * (4 g + x) + i
 #pragma unroll
-        for (int i = 0; i < M; i += 4) {
-          const v4f y = {o[f][p][i][x] * mine, o[f][p][i + 1][x] * mine, o[f][p][i + 2][x] * mine,
-                         o[f][p][i + 3][x] * mine};
-          *reinterpret_cast<v4f*>(&merge[wave][r][p * 128 + M * (4 * g + x) + i]) = y;
+          for (int i = 0; i < M; i += 4) {
+            const v4f y = {o[f][p][i][x] * mine, o[f][p][i + 1][x] * mine,
+                           o[f][p][i + 2][x] * mine, o[f][p][i + 3][x] * mine};
+            *reinterpret_cast<v4f*>(&sh.merge[wave][r][p * 128 + M * (4 * g + x) + i]) = y;
+          }
         }
+      __syncthreads();
+      // 16 rows x D: each thread C channels of one row
+      constexpr int kThreads = 64 * W / 16, C = D / kThreads < 4 ? 4 : D / kThreads;
+      const int row = tid / kThreads, ch = tid % kThreads * C;
+      const int tr = r0 + f * 16 + row;
+      if (ch < D && tr < R) {
+        float tm = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) tm = fmaxf(tm, sh.stat[0][w][f * 16 + row]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float wm = sh.stat[0][w][f * 16 + row];
+          sum += sh.stat[1][w][f * 16 + row] * (wm == tm ? 1.0f : exp2_raw((wm - tm) * c));
+        }
+        if (sh.bad_page) sum = __uint_as_float(0x7FC00000u);
+        float y[C];
+#pragma unroll
+        for (int i = 0; i < C; i += 4) {
+          v4f acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            acc += *reinterpret_cast<const v4f*>(&sh.merge[w][row][ch + i]);
+          y[i] = acc[0], y[i + 1] = acc[1], y[i + 2] = acc[2], y[i + 3] = acc[3];
+        }
+        if (whole)
+          store_row<C>(out_row(a, D, s.q0, h, tr) + ch, y, sum);
+        else
+          store_part<C>(a, kTile, D, 2 * blockIdx.x + which, f * 16 + row, ch, y, tm * c, sum);
       }
-    __syncthreads();
-    // 16 rows x D: each thread D / 16 channels of one row
-    constexpr int C = D / 16;
-    const int row = tid >> 4, ch = (tid & 15) * C;
-    const int tr = r0 + f * 16 + row;
-    float tm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) tm = fmaxf(tm, stat[0][w][f * 16 + row]);
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float wm = stat[0][w][f * 16 + row];
-      sum += stat[1][w][f * 16 + row] * (wm == tm ? 1.0f : exp2_raw((wm - tm) * c));
+      __syncthreads();
     }
-    if (poison) sum = __uint_as_float(0x7FC00000u);
-    float y[C];
-#pragma unroll
-    for (int i = 0; i < C; i += 4) {
-      v4f acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        acc += *reinterpret_cast<const v4f*>(&merge[w][row][ch + i]);
-      y[i] = acc[0], y[i + 1] = acc[1], y[i + 2] = acc[2], y[i + 3] = acc[3];
     }
-    if (tr < R) {
-      if (direct)
-        store_row<C>(a.out + ((size_t)(s.q0 + tr / group_heads) * a.Hq + h * group_heads +
-                              tr % group_heads) * D + ch, y, sum);
-      else
-        store_part<D, C>(a, b, h, split, tr, ch, y, tm * c, sum);
+    if (a.runs && first_granule == 0 && tid == 0 && (a.by_unit || !whole)) {
+      // what attn_join is told of a unit: how many workgroups after this one finish it
+      int* mt = meta(a, kTile, D, a.by_unit ? b * a.units + this_unit : blockIdx.x);
+      mt[0] = (int)((un.per_unit - take + run.share - 1) / run.share);
+      mt[1] = b, mt[2] = this_unit, mt[3] = blockIdx.x;
     }
-    __syncthreads();
+    if (!run.left) return;
   }
 }
 
-// Partial results of a row's chunks, weighed: one wave a row.
-template <int D>
-__global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int rows) {
-  constexpr int C = D / 64;
-  const int lane = threadIdx.x & 63, fours = ceil_div(rows, 4);
-  const int rest = blockIdx.x / fours, h = rest % a.Hkv, b = rest / a.Hkv;
-  const int row = blockIdx.x % fours * 4 + (int)(threadIdx.x >> 6);
-  const int group_heads = a.Hq / a.Hkv;
-  const Sequence s = sequence(a, b);
-  const int R = s.n * group_heads;
-  if (s.bad || row >= rows || row >= R) return;
-  const int r0 = row / tile_rows * tile_rows;
-  const Span span = tile_span(a, s, r0, min(r0 + tile_rows, R) - 1, group_heads);
-  const int n = span.hi - span.lo <= a.chunk ? 1 : ceil_div(span.hi - span.lo, a.chunk);
-  if (n <= 1) return;                         // already written
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 64) top = fmaxf(top, part_stat(a, D, b, h, i, row)[0]);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-  float sum = 0.0f, y[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) y[i] = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const float* st = part_stat(a, D, b, h, i, row);
-    const float w = st[0] == top ? 1.0f : exp2_raw(st[0] - top);
-    const float* o = part_row(a, D, b, h, i, row) + lane * C;
-    sum += w * st[1];
-#pragma unroll
-    for (int k = 0; k < C; ++k) y[k] += w * o[k];
+// A unit that crosses runs: the partial results of workgroup i (its last) and of the n after it (their
+// first), weighed. D / 4 threads read a partial result of a row, S such teams share a row's. What a
+// unit's first workgroup has written is found by the unit, or by that workgroup where those are
+// fewer. The rows of 8 partial results a thread are read without waiting for the maxima that weigh
+// them.
+template <int D, int S>
+__global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int entries, int rows) {
+  constexpr int kLanes = D / 4, kTeams = 256 / kLanes, kRows = kTeams / S, kAhead = 8;
+  __shared__ v4f side[S > 1 ? kTeams : 1][kLanes];
+  __shared__ float sums[kTeams];
+  const int tid = threadIdx.x, lane = tid % kLanes, team = tid / kLanes, mine = team % S;
+  const int entry = blockIdx.x % entries, row = blockIdx.x / entries * kRows + team / S;
+  const int* mt = meta(a, tile_rows, D, entry);
+  int n = mt[0], b = mt[1], unit = mt[2];
+  const int i0 = mt[3];
+  if (a.by_unit) {
+    // a unit that the batch does not have was not written
+    b = entry / a.units, unit = entry % a.units;
+    const Sequence s = sequence_uniform(a, b);
+    if (s.bad || a.by_heads(unit) * tile_rows >= s.n * a.group) return;
   }
-  store_row<C>(a.out + ((size_t)(s.q0 + row / group_heads) * a.Hq + h * group_heads +
-                        row % group_heads) * D + lane * C, y, sum);
+  if (!n) return;
+  const int tile = a.by_heads(unit), h = unit - tile * a.Hkv;
+  const int q0 = scalar_load(a.starts + b), R = (scalar_load(a.starts + b + 1) - q0) * a.group;
+  const int tr = tile * tile_rows + row;
+  const int last = row < rows && tr < R ? n : -1;        // no partial results of a row beyond
+  // partial 0 is the last of workgroup i0, partial k > 0 the first of workgroup i0 + k
+  auto slot = [&](int k) { return 2 * (i0 + k) + (k == 0 ? 1 : 0); };
+  v4f part[kAhead];
+  float st[kAhead][2];
+  auto read = [&](int k0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = k0 + j * S;
+      if (k > last) break;
+      part[j] = *reinterpret_cast<const v4f*>(part_row(a, tile_rows, D, slot(k), row) + 4 * lane);
+      const float* p = part_stat(a, tile_rows, D, slot(k), row);
+      st[j][0] = p[0], st[j][1] = p[1];
+    }
+  };
+  read(mine);
+  float top = -INFINITY;
+  for (int k = lane; k <= last; k += kLanes)
+    top = fmaxf(top, part_stat(a, tile_rows, D, slot(k), row)[0]);
+#pragma unroll
+  for (int x = 1; x < kLanes; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  float sum = 0.0f;
+  v4f y = {0, 0, 0, 0};
+  for (int k0 = mine; k0 <= last;) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (k0 + j * S > last) break;
+      const float w = st[j][0] == top ? 1.0f : exp2_raw(st[j][0] - top);
+      sum += w * st[j][1];
+      y += w * part[j];
+    }
+    k0 += kAhead * S;
+    read(k0);
+  }
+  if constexpr (S > 1) {
+    side[team][lane] = y;
+    if (lane == 0) sums[team] = sum;
+    __syncthreads();
+    if (mine) return;
+#pragma unroll
+    for (int k = 1; k < S; ++k) y += side[team + k][lane], sum += sums[team + k];
+  }
+  if (last < 0) return;
+  const float out[4] = {y[0], y[1], y[2], y[3]};
+  store_row<4>(out_row(a, D, q0, h, tr) + 4 * lane, out, sum);
 }
 
 template <int D, int RF>
-hipError_t launch(const AttnArgs& a, hipStream_t stream) {
-  const int rows = a.max_q * (a.Hq / a.Hkv);
-  const int tiles = ceil_div(rows, 16 * RF);
-  attn_rows<D, RF><<<a.batch * tiles * a.Hkv * a.splits, 256, 0, stream>>>(a, tiles);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess || a.splits == 1) return e;
-  attn_join<D><<<a.batch * a.Hkv * ceil_div(rows, 4), 256, 0, stream>>>(a, 16 * RF, rows);
+hipError_t launch(AttnArgs a, hipStream_t stream) {
+  constexpr int W = kRunWaves, NS = attn_stages(D, RF);
+  const int rows = a.max_q * a.group;
+  a.by_group = divisor(a.group), a.by_heads = divisor(a.Hkv), a.by_runs = divisor(a.runs ? a.runs : 1);
+  if (!a.runs) {
+    a.tiles = ceil_div(rows, 16 * RF);
+    constexpr int WW = attn_whole_waves(RF);
+    attn_rows<D, RF, WW, NS><<<a.batch * a.tiles * a.Hkv, 64 * WW, 0, stream>>>(a);
+    return hipGetLastError();
+  }
+  a.tiles = 0;
+  a.units = ceil_div(rows, 16 * RF) * a.Hkv;
+  a.by_unit = (long)a.batch * a.units <= a.runs;
+  attn_rows<D, RF, W, NS><<<a.runs, 64 * W, 0, stream>>>(a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  const int entries = a.by_unit ? a.batch * a.units : a.runs;
+  const int tile_rows = rows < 16 * RF ? rows : 16 * RF;
+  // A row to a workgroup where the rows are few: many workgroups' partial results each. A row to a
+  // team where they are many (of few partial results each).
+  constexpr int kTeams = 1024 / D;
+  if ((long)entries * tile_rows <= 2048)
+    attn_join<D, kTeams><<<entries * tile_rows, 256, 0, stream>>>(a, 16 * RF, entries, tile_rows);
+  else
+    attn_join<D, 1><<<entries * ceil_div(tile_rows, kTeams), 256, 0, stream>>>(a, 16 * RF, entries,
+                                                                             tile_rows);
   return hipGetLastError();
 }
 
@@ -389,19 +593,19 @@ int attn_row_fragments(int max_q, int Hq, int Hkv, int d) {
 
 AttnPlan attn_plan(int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window) {
   const long rows = (long)max_q * (Hq / Hkv);
-  const int tile = 16 * attn_row_fragments(max_q, Hq, Hkv, d);
+  const int rf = attn_row_fragments(max_q, Hq, Hkv, d), tile = 16 * rf;
   const long units = (long)batch * Hkv * ((rows + tile - 1) / tile);
-  // tokens that a tile can see
+  // tokens that a tile can see, in granules
   long span = max_len;
   if (window > 0 && (long)window + max_q + 31 < span) span = (long)window + max_q + 31;
-  const int grain = kWaves * kStep;
-  long chunk = (span * units / 2048 + grain - 1) / grain * grain;
-  chunk = chunk < grain ? grain : chunk > kMaxChunk ? kMaxChunk : chunk;
-  AttnPlan p;
-  p.chunk = (int)chunk;
-  p.splits = (int)((span + chunk - 1) / chunk);
-  if (p.splits < 1) p.splits = 1;
-  p.workspace = p.splits == 1 ? 0 : (size_t)batch * Hkv * p.splits * rows * (d + 2) * sizeof(float);
+  AttnPlan p = {0, 0};
+  // Two steps a wave: a workgroup a unit, and no second launch.
+  if (span <= 2L * kStep * attn_whole_waves(rf)) return p;
+  // as many workgroups as the card's 256 CUs hold at once, or a granule each
+  const long granules = (span + kStep * kRunWaves - 1) / (kStep * kRunWaves);
+  const long most = 256L * 4 * attn_waves(d, rf) / kRunWaves;
+  p.runs = (int)(units * granules < most ? units * granules : most);
+  p.workspace = (size_t)p.runs * ((size_t)2 * tile * (d + 2) * sizeof(float) + 16);
   return p;
 }
 

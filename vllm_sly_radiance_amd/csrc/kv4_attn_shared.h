@@ -6,31 +6,69 @@
 
 namespace kv4 {
 
-constexpr int kMaxChunk = 16384;   // tokens of a split at most: its page numbers fit in LDS
-
 int attn_row_fragments(int max_q, int Hq, int Hkv, int d);
+
+// Waves of a workgroup of attn_rows, and waves a SIMD is to hold (registers allow no more).
+constexpr int kRunWaves = 4;                                          // sharing the batch's tokens
+constexpr int attn_whole_waves(int rf) { return rf <= 2 ? 8 : 4; }    // a workgroup a unit
+constexpr int attn_waves(int d, int rf) { return d * rf <= 128 ? 4 : d * rf <= 256 || d < 256 ? 2 : 1; }
+constexpr int attn_stages(int d, int rf) { return 1; }
+
+__device__ __forceinline__ v4f mfma16(v8bf a, v8bf b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// A scalar load: the address is the same in every lane, and nothing writes there while the kernel
+// runs.
+__device__ __forceinline__ int scalar_load(const int* p) {
+  return *(const __attribute__((address_space(4))) int*)(uintptr_t)p;
+}
+
+// x, which the compiler computes with from here on and not earlier.
+__device__ __forceinline__ int pinned(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A value that is the same in every lane, as a scalar.
+__device__ __forceinline__ long uniform(long x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)x);
+  return ((long)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | lo;
+}
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A sequence of the batch: its tokens, its first query row, its queries. Sizes that do not fit what
 // the launch was planned for make it bad: its rows are NaN.
 struct Sequence { int len, q0, n; bool bad; };
+__device__ __forceinline__ bool misfit(const AttnArgs& a, const Sequence& s) {
+  const long pages = ((long)s.len + (1 << a.page_shift) - 1) >> a.page_shift;
+  return s.len < 0 || s.len > a.max_len || pages > a.table_cols || s.q0 < 0 || s.n < 0 ||
+         s.n > a.max_q || s.q0 > a.total - s.n;
+}
 __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b) {
   Sequence s;
   s.len = a.lens[b];
   s.q0 = a.starts[b];
   s.n = a.starts[b + 1] - s.q0;
-  s.bad = s.len < 0 || s.len > a.max_len || ((long)s.len + (1 << a.page_shift) - 1) >> a.page_shift >
-          a.table_cols || s.q0 < 0 || s.n < 0 || s.n > a.max_q || s.q0 > a.total - s.n;
+  s.bad = misfit(a, s);
+  return s;
+}
+// the same of a b that is the same in every lane
+__device__ __forceinline__ Sequence sequence_uniform(const AttnArgs& a, int b) {
+  Sequence s;
+  s.len = scalar_load(a.lens + b);
+  s.q0 = scalar_load(a.starts + b);
+  s.n = scalar_load(a.starts + b + 1) - s.q0;
+  s.bad = misfit(a, s);
   return s;
 }
 
-// Tokens [lo, hi) that the rows first .. last of a sequence see between them (lo rounded down to a
+// Tokens [lo, hi) that the queries first .. last of a sequence see between them (lo rounded down to a
 // step), and [all_lo, all_hi) that each of them sees.
 struct Span { int lo, hi, all_lo, all_hi; };
-__device__ __forceinline__ Span tile_span(const AttnArgs& a, const Sequence& s, int first, int last,
-                                          int group_heads) {
-  const int p0 = s.len - s.n + first / group_heads, p1 = s.len - s.n + last / group_heads;
+__device__ __forceinline__ Span query_span(const AttnArgs& a, const Sequence& s, int first, int last) {
+  const int p0 = s.len - s.n + first, p1 = s.len - s.n + last;
   Span x;
   x.hi = a.causal ? min(s.len, max(p1 + 1, 0)) : s.len;
   x.all_hi = a.causal ? min(s.len, p0 + 1) : s.len;
@@ -50,6 +88,12 @@ __device__ __forceinline__ void nan_rows(const AttnArgs& a, const Sequence& s, i
   }
 }
 
+// The output of row `row` (queries times the heads of a group) of a sequence's kv head.
+__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int D, int q0, int h, int row) {
+  const int qi = a.by_group(row);
+  return a.out + ((size_t)(q0 + qi) * a.Hq + h * a.group + row - qi * a.group) * D;
+}
+
 // 8 codes as a bf16 operand.
 __device__ __forceinline__ v8bf expand8(uint32_t codes, float scale) {
   const v4i r = {(int)codes_bf16x2<0>(codes, scale), (int)codes_bf16x2<1>(codes, scale),
@@ -63,11 +107,9 @@ __device__ __forceinline__ v8bf pack8bf(const float e[8]) {
   return __builtin_bit_cast(v8bf, r);
 }
 
-__device__ __forceinline__ bool has_nan_scale(uint32_t four) {
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) any |= ((four >> (8 * i)) & 0xFFu) == 0xFFu;
-  return any;
+// Bit 7 of each of four scale bytes that is 255.
+__device__ __forceinline__ uint32_t nan_scales(uint32_t four) {
+  return ((four & 0x7F7F7F7Fu) + 0x01010101u) & four & 0x80808080u;
 }
 
 // The low (high) halves of two dwords, the first one's below.
@@ -92,34 +134,35 @@ __device__ __forceinline__ void value_pair(v8bf& even, v8bf& odd, F codes, const
   odd = __builtin_bit_cast(v8bf, hi);
 }
 
-// A run's channels as operands over the 8 tokens of a lane (4 g + i of two groups of 16).
-template <int D, typename Vec>
-__device__ __forceinline__ void value_operands(v8bf vf[Group<D>::kRun], Vec v0, uint32_t s0, Vec v1,
-                                               uint32_t s1) {
+// A run's channels as operands over the 8 tokens of a lane (4 g + i of two groups of 16), two
+// channels at a time: use(index of the pair, channel 2 x index, the one after).
+template <int D, typename Vec, typename Use>
+__device__ __forceinline__ void each_value_pair(Vec v0, uint32_t s0, Vec v1, uint32_t s1, Use use) {
   float s[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     s[i] = scale_of((s0 >> (8 * i)) & 0xFFu);
     s[4 + i] = scale_of((s1 >> (8 * i)) & 0xFFu);
   }
-  if constexpr (D >= 128) {
-    // dword i: token i's 4 bytes
-    auto codes = [&](int i, float sc, auto b) {
-      return codes_bf16x2<decltype(b)::value>((uint32_t)(i < 4 ? v0[i] : v1[i - 4]), sc);
-    };
-    value_pair<0>(vf[0], vf[1], codes, s);
-    value_pair<1>(vf[2], vf[3], codes, s);
-    value_pair<2>(vf[4], vf[5], codes, s);
-    value_pair<3>(vf[6], vf[7], codes, s);
-  } else {
-    // dword i / 2: tokens i, i + 1, 2 bytes each
-    auto codes = [&](int i, float sc, auto b) {
+  auto codes = [&](int i, float sc, auto b) {
+    constexpr int B = decltype(b)::value;
+    if constexpr (D >= 128) {         // dword i: token i's 4 bytes
+      return codes_bf16x2<B>((uint32_t)(i < 4 ? v0[i] : v1[i - 4]), sc);
+    } else {                          // dword i / 2: tokens i, i + 1, 2 bytes each
       const uint32_t w = (uint32_t)(i < 4 ? v0[i >> 1] : v1[(i - 4) >> 1]);
-      constexpr int B = decltype(b)::value;
-      return i & 1 ? codes_bf16x2<B + 2>(w, sc) : codes_bf16x2<B>(w, sc);
-    };
-    value_pair<0>(vf[0], vf[1], codes, s);
-    value_pair<1>(vf[2], vf[3], codes, s);
+      return i & 1 ? codes_bf16x2<(B + 2) % 4>(w, sc) : codes_bf16x2<B>(w, sc);
+    }
+  };
+  v8bf even, odd;
+  value_pair<0>(even, odd, codes, s);
+  use(std::integral_constant<int, 0>(), even, odd);
+  value_pair<1>(even, odd, codes, s);
+  use(std::integral_constant<int, 1>(), even, odd);
+  if constexpr (D >= 128) {
+    value_pair<2>(even, odd, codes, s);
+    use(std::integral_constant<int, 2>(), even, odd);
+    value_pair<3>(even, odd, codes, s);
+    use(std::integral_constant<int, 3>(), even, odd);
   }
 }
 
@@ -140,28 +183,30 @@ __device__ __forceinline__ void store_row(uint16_t* out, const float y[C], float
   }
 }
 
-// Partial results: fp32 [batch][Hkv][splits][rows][D], then [..][rows][2] with the row's maximum (in
-// units of log2) and sum.
-__device__ __forceinline__ size_t part_index(const AttnArgs& a, int b, int h, int split, int row) {
-  const size_t rows = (size_t)a.max_q * (a.Hq / a.Hkv);
-  return (((size_t)b * a.Hkv + h) * a.splits + split) * rows + row;
+// Workspace of attn_rows: partial results fp32 [2 runs][tile rows][D], [2 runs][tile rows][2] with
+// the row's maximum (in units of log2) and sum, and int [runs][4]: what attn_join is told (of a unit,
+// by its index b * units + unit, or of the one that begins in a run).
+__device__ __forceinline__ float* part_row(const AttnArgs& a, int tile_rows, int D, int slot,
+                                           int row) {
+  return a.part + ((size_t)slot * tile_rows + row) * D;
 }
-__device__ __forceinline__ float* part_row(const AttnArgs& a, int D, int b, int h, int split, int row) {
-  return a.part + part_index(a, b, h, split, row) * D;
-}
-__device__ __forceinline__ float* part_stat(const AttnArgs& a, int D, int b, int h, int split,
+__device__ __forceinline__ float* part_stat(const AttnArgs& a, int tile_rows, int D, int slot,
                                             int row) {
-  return a.part + part_index(a, a.batch, 0, 0, 0) * D + part_index(a, b, h, split, row) * 2;
+  return a.part + (size_t)2 * a.runs * tile_rows * D + ((size_t)slot * tile_rows + row) * 2;
 }
-template <int D, int C>
-__device__ __forceinline__ void store_part(const AttnArgs& a, int b, int h, int split, int row,
-                                           int ch, const float y[C], float top, float sum) {
-  float* o = part_row(a, D, b, h, split, row) + ch;
+__device__ __forceinline__ int* meta(const AttnArgs& a, int tile_rows, int D, int entry) {
+  return reinterpret_cast<int*>(a.part + (size_t)2 * a.runs * tile_rows * (D + 2)) + 4 * entry;
+}
+template <int C>
+__device__ __forceinline__ void store_part(const AttnArgs& a, int tile_rows, int D, int slot,
+                                           int row, int ch, const float y[C], float top,
+                                           float sum) {
+  float* o = part_row(a, tile_rows, D, slot, row) + ch;
 #pragma unroll
   for (int i = 0; i < C; i += 4)
     *reinterpret_cast<v4f*>(o + i) = v4f{y[i], y[i + 1], y[i + 2], y[i + 3]};
   if (ch == 0) {
-    float* st = part_stat(a, D, b, h, split, row);
+    float* st = part_stat(a, tile_rows, D, slot, row);
     st[0] = top, st[1] = sum;
   }
 }

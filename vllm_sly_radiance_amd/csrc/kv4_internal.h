@@ -117,6 +117,24 @@ struct MoveArgs {
 // pairs: n <= kMovePairs of them (src, dst), sorted by src
 hipError_t launch_move(const MoveArgs& a, const int* pairs, int n, hipStream_t stream);
 
+// Division of 0 <= n < 2^31 by a divisor that the host knows: a multiplication by m =
+// floor(2^(31 + s) / d) + 1, s = ceil(log2 d), whose error m d - 2^(31 + s) <= d <= 2^s stays below
+// what moves a quotient. The integer division in its place is some 40 dependent instructions, and
+// several stood before a workgroup's first loads.
+struct Divisor {
+  int d;
+  uint32_t m;
+  int shift;              // s - 1
+  __device__ __forceinline__ int operator()(int n) const {
+    return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> shift);
+  }
+};
+inline Divisor divisor(int d) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return {d, d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)d + 1), s - 1};
+}
+
 struct AttnArgs {
   const uint16_t* q;
   const uint8_t* cache;
@@ -126,13 +144,18 @@ struct AttnArgs {
   uint16_t* out;
   float* part;            // partial results, or null
   long q_ts, q_hs, page_stride, pages, table_stride;
-  int page_shift, table_cols, total, batch, max_q, max_len, Hq, Hkv, window;
+  int page_shift, table_cols, total, batch, max_q, max_len, Hq, Hkv, group, window;   // group: Hq / Hkv
   float scale;
   bool causal;
-  int chunk, splits;      // tokens of a split, splits at most
+  int runs;               // workgroups that share the batch's tokens; 0: one a unit
+  // set at the launch: row tiles of a sequence at most, where runs is 0; units of a sequence at most,
+  // and whether attn_join goes by units (there are no more of them than runs) or by runs
+  int tiles, units;
+  bool by_unit;
+  Divisor by_group, by_heads, by_runs;   // of Hq / Hkv, Hkv, runs
 };
-// How the cached tokens are split over workgroups, and the bytes of partial results that takes.
-struct AttnPlan { int chunk, splits; size_t workspace; };
+// How the cached tokens are spread over workgroups, and the workspace that takes.
+struct AttnPlan { int runs; size_t workspace; };
 AttnPlan attn_plan(int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window);
 hipError_t launch_attn(const AttnArgs& a, int d, hipStream_t stream);
 
