@@ -121,8 +121,8 @@ int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache, long p
 
 /* Bytes of workspace kv4_attention needs for these sizes (the partial results of long contexts
  * split over workgroups). */
-int kv4_attention_workspace(int batch, int max_q, int max_len, int q_heads, int kv_heads, int d,
-                            int window, size_t* bytes);
+int kv4_attention_workspace(int total, int batch, int max_q, int max_len, int q_heads, int kv_heads,
+                            int d, int window, size_t* bytes);
 
 /* Copies page src to page dst for each of the n pairs (int32 [n][2] = src, dst, in HOST memory, read
  * before the call returns) in `layers` caches layer_stride bytes apart, and where tables is not null

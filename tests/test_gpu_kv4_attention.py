@@ -68,7 +68,7 @@ def test_long_context_is_split():
     """Chunks over workgroups, joined in a second launch; the same through a larger max_len, whose
     chunks are longer."""
     b = Batch(np.random.default_rng(4), [5000, 4097, 3, 129], [1, 2, 1, 2], 8, 2, 128, 64)
-    assert _native_kv4.attention_workspace(4, 2, 5000, 8, 2, 128, 0) > 0
+    assert _native_kv4.attention_workspace(6, 4, 2, 5000, 8, 2, 128, 0) > 0
     b.check(run(b))
     b.check(run(b, max_len=200000))
     b.check(run(b, max_q=9))

@@ -209,3 +209,28 @@ def test_fakes_give_the_outputs_shapes():
         assert a.shape == b.shape == (5, 2, 128) and a.dtype == torch.bfloat16
         o = K.attention(q, cache, table, n, torch.empty(4, dtype=torch.int32, device="cuda"), 5, 60)
         assert o.shape == q.shape and o.dtype == torch.bfloat16
+
+
+def workspace(lib, *sizes):
+    n = ctypes.c_size_t()
+    assert lib.kv4_attention_workspace(*sizes, ctypes.byref(n)) == 0
+    return n.value
+
+
+def test_what_serves_a_call(lib):
+    """(total, batch, max_q, max_len, q heads, kv heads, d, window): few rows over a long context are
+    split over workgroups, which takes a workspace; many rows (more than 128 a kv head, 64 at head size
+    256, and 700 times half that in all) are not, unless sequences of few rows may stand beside them."""
+    assert workspace(lib, 1, 1, 1, 512, 32, 8, 128, 0) == 0
+    assert workspace(lib, 1, 1, 1, 513, 32, 8, 128, 0) > 0
+    assert workspace(lib, 0, 1, 0, 4096, 32, 8, 128, 0) == 0
+    assert workspace(lib, 1399, 1, 1399, 4096, 32, 8, 128, 0) > 0
+    assert workspace(lib, 1400, 1, 1400, 4096, 32, 8, 128, 0) == 0
+    assert workspace(lib, 1401, 2, 1400, 4096, 32, 8, 128, 0) > 0
+    assert workspace(lib, 64 * 32, 64, 32, 4096, 32, 8, 128, 0) > 0
+    assert workspace(lib, 64 * 33, 64, 33, 4096, 32, 8, 128, 0) == 0
+    assert workspace(lib, 1399, 1, 1399, 4096, 16, 2, 256, 0) > 0
+    assert workspace(lib, 1400, 1, 1400, 4096, 16, 2, 256, 0) == 0
+    # beside chunks: rows of one query of the group's heads, if they fit attn_rows' 64 (32)
+    assert workspace(lib, 1401, 2, 1400, 4096, 65, 1, 128, 0) == 0
+    assert workspace(lib, 1401, 2, 1400, 4096, 64, 1, 128, 0) > 0

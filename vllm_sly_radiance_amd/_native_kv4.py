@@ -30,7 +30,7 @@ SIGNATURES = {
     "kv4_attention": (_int, [_vp, _long, _long, _vp, _long, _long, _int, _vp, _long, _int, _vp, _vp,
                              _vp, _vp, _sz, _int, _int, _int, _int, _int, _int, _int, _f, _int,
                              _int, _vp]),
-    "kv4_attention_workspace": (_int, [_int, _int, _int, _int, _int, _int, _int, _psz]),
+    "kv4_attention_workspace": (_int, [_int, _int, _int, _int, _int, _int, _int, _int, _psz]),
     "kv4_move_pages": (_int, [_vp, _int, _long, _long, _long, _sz, _vp, _int, _vp, _int, _int,
                               _long, _vp]),
 }
@@ -74,8 +74,8 @@ def page_bytes(heads: int, page: int, d: int) -> int:
     return n.value
 
 
-def attention_workspace(batch, max_q, max_len, q_heads, kv_heads, d, window) -> int:
+def attention_workspace(total, batch, max_q, max_len, q_heads, kv_heads, d, window) -> int:
     n = _sz()
-    check(lib().kv4_attention_workspace(batch, max_q, max_len, q_heads, kv_heads, d, window,
+    check(lib().kv4_attention_workspace(total, batch, max_q, max_len, q_heads, kv_heads, d, window,
                                         _c.byref(n)))
     return n.value

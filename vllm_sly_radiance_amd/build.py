@@ -26,7 +26,8 @@ SOURCES = ["w4a8_api.hip", "w4a8_quant.hip", "w4a8_repack.hip", "w4a8_gemm_skinn
            "w4a8_producers.hip", "w4a8_probe.hip"]
 
 KV4_LIB_PATH = os.path.join(PKG, "libkv4_attn.so")
-KV4_SOURCES = ["kv4_api.hip", "kv4_rope.hip", "kv4_pages.hip", "kv4_attn_rows.hip"]
+KV4_SOURCES = ["kv4_api.hip", "kv4_rope.hip", "kv4_pages.hip", "kv4_attn_rows.hip",
+               "kv4_attn_tiles.hip"]
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",

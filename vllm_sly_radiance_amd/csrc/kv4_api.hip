@@ -113,7 +113,7 @@ int attn_sizes(const char* who, int batch, int max_q, int max_len, int q_heads, 
   if (int rc = check_heads(who, q_heads, d)) return rc;
   if (q_heads % kv_heads)
     return fail(KV4_EINVAL, "%s: %d query heads over %d kv heads", who, q_heads, kv_heads);
-  if (batch < 0 || max_q < 0 || max_len < 0 || max_len > 0x7FFFFF00 || window < 0)
+  if (batch < 0 || max_q < 0 || max_len < 0 || max_len > 0x7FFFF000 || window < 0)
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d max_len=%d window=%d", who, batch, max_q, max_len,
                 window);
   if ((long)batch * q_heads * max_q > 0x7FFFFFFFL)
@@ -206,13 +206,14 @@ KV4_API int kv4_gather(const void* cache, long pages, long page_stride, int page
   return hip_status(launch_gather(a, d, (hipStream_t)stream), who);
 }
 
-KV4_API int kv4_attention_workspace(int batch, int max_q, int max_len, int q_heads, int kv_heads,
-                                    int d, int window, size_t* bytes) {
+KV4_API int kv4_attention_workspace(int total, int batch, int max_q, int max_len, int q_heads,
+                                    int kv_heads, int d, int window, size_t* bytes) {
   if (!bytes) return fail(KV4_EINVAL, "attention_workspace: null output");
   if (int rc = attn_sizes("attention_workspace", batch, max_q, max_len, q_heads, kv_heads, d, window))
     return rc;
-  *bytes = batch && max_q ? attn_plan(batch, max_q, max_len, q_heads, kv_heads, d, window).workspace
-                          : 0;
+  *bytes = total > 0 && batch && max_q
+               ? attn_plan(total, batch, max_q, max_len, q_heads, kv_heads, d, window).workspace
+               : 0;
   return KV4_OK;
 }
 
@@ -237,7 +238,7 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
     return fail(KV4_EINVAL, "%s: null pointer", who);
   if (!aligned(seq_lens, 4) || !aligned(q_starts, 4) || !aligned(page_table, 4) || !aligned(out, 16))
     return fail(KV4_EINVAL, "%s: misaligned pointer", who);
-  const AttnPlan plan = attn_plan(batch, max_q, max_len, q_heads, kv_heads, d, window);
+  const AttnPlan plan = attn_plan(total, batch, max_q, max_len, q_heads, kv_heads, d, window);
   if (plan.workspace > workspace_bytes || (plan.workspace && (!workspace || !aligned(workspace, 16))))
     return fail(KV4_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who,
                 plan.workspace, workspace_bytes);
@@ -249,8 +250,11 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   a.total = total, a.batch = batch, a.max_q = max_q, a.max_len = max_len;
   a.Hq = q_heads, a.Hkv = kv_heads, a.group = q_heads / kv_heads;
   a.window = window, a.scale = scale;
-  a.causal = flags & KV4_CAUSAL, a.runs = plan.runs;
-  return hip_status(launch_attn(a, d, (hipStream_t)stream), who);
+  a.causal = flags & KV4_CAUSAL;
+  a.fragments = plan.fragments, a.runs = plan.runs, a.few_rows = plan.few_rows;
+  if (plan.tiles)
+    if (int rc = hip_status(launch_attn_tiles(a, d, (hipStream_t)stream), who)) return rc;
+  return plan.rows ? hip_status(launch_attn_rows(a, d, (hipStream_t)stream), who) : KV4_OK;
 }
 
 KV4_API int kv4_move_pages(void* cache, int layers, long layer_stride, long pages, long page_stride,

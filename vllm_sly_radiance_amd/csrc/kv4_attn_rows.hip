@@ -75,20 +75,9 @@ template <int kGranule>
 __device__ __forceinline__ Units units_of(const AttnArgs& a, const Sequence& s, int tile_rows) {
   if (s.bad) return {1, a.Hkv, 0};
   const int R = s.n * a.group;
-  if (R == 0) return {1, 0, 0};
+  if (R == 0 || (a.few_rows && R > a.few_rows)) return {1, 0, 0};
   const Span x = query_span(a, s, 0, s.n - 1);
   return {x.hi > x.lo ? ceil_div(x.hi - x.lo, kGranule) : 1, ceil_div(R, tile_rows) * a.Hkv, x.lo};
-}
-
-// Inclusive scan over the wave: shifts inside rows of 16 lanes, then the rows' last lanes.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr:1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast:15, rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast:31, rows 2 and 3
-  return x;
 }
 
 // A run of granules of the batch: its first sequence, the granule of that sequence's work, and how
@@ -145,7 +134,7 @@ struct Shared {
   int bad_page;
 };
 
-template <int D, int RF, int W, int NS>
+template <int D, int RF, int W>
 __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs a) {
   using G = Group<D>;
   constexpr int P = G::kPlanes, M = G::kRun, KS = D / 32;   // planes, channels of a run, K steps
@@ -255,35 +244,27 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
         for (int i = 0; i < M; ++i) o[f][p][i] = v4f{0, 0, 0, 0};
     }
 
-    // NS steps' codes in registers: the keys of the step NS on are asked for when this one's scores are
-    // done, its values when this one's products are. Past the end the segment's last step is asked
-    // for again (cache hits that nothing uses): loads that are always issued let the waits count
-    // those in flight instead of draining them.
-    Raw<D> ring[NS][2];
+    // A step's codes in registers: the next step's keys are asked for when this one's scores are done,
+    // its values when this one's products are (two and three steps ahead measured the same). Past the
+    // end the segment's last step is asked for again (cache hits that nothing uses): loads that are
+    // always issued let the waits count those in flight instead of draining them.
+    Raw<D> w[2];
     const int t_last = (t1 - 1 - t0) / kStep * kStep + t0;
     int t = t0 + wave * kStep;
     int na = 0, nb = 0;                // page numbers of the next step to ask for
     if (t < t1) {
-#pragma unroll
-      for (int j = 0; j < NS; ++j) {
-        const int tj = min(t + j * kGranule, t_last);
-        const uint8_t* ga = group_at(tj, page_of(tj));
-        const uint8_t* gb = group_at(tj + 16, page_of(tj + 16));
-        load_keys<D>(ring[j][0], ga, g, r), load_keys<D>(ring[j][1], gb, g, r);
-        load_values<D>(ring[j][0], ga, g, r), load_values<D>(ring[j][1], gb, g, r);
-      }
-      const int tj = min(t + NS * kGranule, t_last);
-      na = page_of(tj), nb = page_of(tj + 16);
+      const uint8_t* ga = group_at(t, page_of(t));
+      const uint8_t* gb = group_at(t + 16, page_of(t + 16));
+      load_keys<D>(w[0], ga, g, r), load_keys<D>(w[1], gb, g, r);
+      load_values<D>(w[0], ga, g, r), load_values<D>(w[1], gb, g, r);
+      const int tn = min(t + kGranule, t_last);
+      na = page_of(tn), nb = page_of(tn + 16);
     }
 #pragma unroll
     for (int j = 0; j < kOps; ++j)
       if (wave + j * W < RF * KS) sh.q[wave + j * W][lane] = ops[j];
     __syncthreads();
-    while (t < t1) {
-#pragma unroll
-     for (int j = 0; j < NS; ++j, t += kGranule) {
-      if (j && t >= t1) break;
-      Raw<D>(&w)[2] = ring[j];
+    for (; t < t1; t += kGranule) {
       // scores of 2 x 16 tokens: lane holds tokens 4 g + i of both, row r
       v4f sc[RF][2];
 #pragma unroll
@@ -301,7 +282,7 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      const int tn = min(t + NS * kGranule, t_last);
+      const int tn = min(t + kGranule, t_last);
       const uint8_t* ga = group_at(tn, na);
       const uint8_t* gb = group_at(tn + 16, nb);
       load_keys<D>(w[0], ga, g, r), load_keys<D>(w[1], gb, g, r);
@@ -393,7 +374,6 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
                              __builtin_amdgcn_sched_barrier(0);
                            });
       load_values<D>(w[0], ga, g, r), load_values<D>(w[1], gb, g, r);
-     }
     }
 
     // ---- the waves' shares -----------------------------------------------------------------------
@@ -489,7 +469,8 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int 
     // a unit that the batch does not have was not written
     b = entry / a.units, unit = entry % a.units;
     const Sequence s = sequence_uniform(a, b);
-    if (s.bad || a.by_heads(unit) * tile_rows >= s.n * a.group) return;
+    const int R = s.n * a.group;
+    if (s.bad || a.by_heads(unit) * tile_rows >= R || (a.few_rows && R > a.few_rows)) return;
   }
   if (!n) return;
   const int tile = a.by_heads(unit), h = unit - tile * a.Hkv;
@@ -544,19 +525,19 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int 
 
 template <int D, int RF>
 hipError_t launch(AttnArgs a, hipStream_t stream) {
-  constexpr int W = kRunWaves, NS = attn_stages(D, RF);
-  const int rows = a.max_q * a.group;
+  constexpr int W = kRunWaves;
+  const int rows = a.few_rows ? a.few_rows : a.max_q * a.group;   // of a sequence at most
   a.by_group = divisor(a.group), a.by_heads = divisor(a.Hkv), a.by_runs = divisor(a.runs ? a.runs : 1);
   if (!a.runs) {
     a.tiles = ceil_div(rows, 16 * RF);
     constexpr int WW = attn_whole_waves(RF);
-    attn_rows<D, RF, WW, NS><<<a.batch * a.tiles * a.Hkv, 64 * WW, 0, stream>>>(a);
+    attn_rows<D, RF, WW><<<a.batch * a.tiles * a.Hkv, 64 * WW, 0, stream>>>(a);
     return hipGetLastError();
   }
   a.tiles = 0;
   a.units = ceil_div(rows, 16 * RF) * a.Hkv;
   a.by_unit = (long)a.batch * a.units <= a.runs;
-  attn_rows<D, RF, W, NS><<<a.runs, 64 * W, 0, stream>>>(a);
+  attn_rows<D, RF, W><<<a.runs, 64 * W, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   const int entries = a.by_unit ? a.batch * a.units : a.runs;
   const int tile_rows = rows < 16 * RF ? rows : 16 * RF;
@@ -573,43 +554,62 @@ hipError_t launch(AttnArgs a, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_d(const AttnArgs& a, hipStream_t stream) {
-  switch (attn_row_fragments(a.max_q, a.Hq, a.Hkv, D)) {
+  switch (a.fragments) {
     case 1: return launch<D, 1>(a, stream);
     case 2: return launch<D, 2>(a, stream);
     default:
       if constexpr (D <= 128) return launch<D, 4>(a, stream);
-      return launch<D, 2>(a, stream);
+      return hipErrorInvalidValue;
   }
 }
 
 }  // namespace
 
-// Row fragments of a workgroup: the fewest of 1, 2, 4 that hold a sequence's rows, 4 (2 at D = 256,
-// whose accumulators are twice as wide) beyond.
-int attn_row_fragments(int max_q, int Hq, int Hkv, int d) {
-  const long rows = (long)max_q * (Hq / Hkv);
-  return rows <= 16 ? 1 : rows <= 32 || d == 256 ? 2 : 4;
-}
-
-AttnPlan attn_plan(int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window) {
-  const long rows = (long)max_q * (Hq / Hkv);
-  const int rf = attn_row_fragments(max_q, Hq, Hkv, d), tile = 16 * rf;
-  const long units = (long)batch * Hkv * ((rows + tile - 1) / tile);
+AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window) {
+  const int group = Hq / Hkv;
+  const long rows = (long)max_q * group;
+  AttnPlan p = {};
+  // Row fragments: the fewest of 1, 2, 4 that hold a sequence's rows, 4 (2 at D = 256, whose
+  // accumulators are twice as wide) beyond.
+  auto fragments = [d](long n) { return n <= 16 ? 1 : n <= 32 || d == 256 ? 2 : 4; };
+  long few = rows;
+  // attn_tiles or attn_rows: a workgroup of attn_tiles does what four row tiles (of 64 rows, 32 at
+  // D = 256) of attn_rows do, in the time of 2.6 of them, but it walks over all its tokens by itself
+  // and has a CU to itself: below some 700 row tiles in the batch, 2.7 for each CU, spreading the
+  // tokens over all CUs wins. Against 4096 cached tokens, attn_tiles and attn_rows with its join in us:
+  //   d = 128, 32 query and 8 kv heads      d = 256, 24 and 4              d = 64, 64 and 8
+  //   1 x 256 queries   128 tiles 105  42   4 x 128  384 tiles 183  125    256 queries   256 tiles 84  45
+  //   1 x 512           256       109  62   1 x 512  384       186  124    512           512       88  70
+  //   1 x 1024          512       118  96   4 x 256  768       192  226    2 x 512      1024       99 134
+  //   1 x 4096         2048       158 345
+  //   32 x 17 (68 rows) 512       135  98
+  const long rows_tile = d == 256 ? 32 : 64;
+  if (rows > 2 * rows_tile && (long)total * Hq >= 700 * rows_tile) {
+    p.tiles = true;
+    // Sequences of fewer queries beside: those of one query are attn_rows'.
+    if (total == (long)batch * max_q) return p;
+    const int fit = group <= 16 ? 16 : group <= 32 || d == 256 ? 32 : 64;
+    if (group > fit) return p;
+    few = p.few_rows = fit;
+  }
+  p.rows = true;
+  p.fragments = fragments(few);
+  const int tile = 16 * p.fragments;
+  const long units = (long)batch * Hkv * ((few + tile - 1) / tile);
   // tokens that a tile can see, in granules
   long span = max_len;
   if (window > 0 && (long)window + max_q + 31 < span) span = (long)window + max_q + 31;
-  AttnPlan p = {0, 0};
   // Two steps a wave: a workgroup a unit, and no second launch.
-  if (span <= 2L * kStep * attn_whole_waves(rf)) return p;
+  if (span <= 2L * kStep * attn_whole_waves(p.fragments)) return p;
   // as many workgroups as the card's 256 CUs hold at once, or a granule each
   const long granules = (span + kStep * kRunWaves - 1) / (kStep * kRunWaves);
-  const long most = 256L * 4 * attn_waves(d, rf) / kRunWaves;
+  const long most = 256L * 4 * attn_waves(d, p.fragments) / kRunWaves;
   p.runs = (int)(units * granules < most ? units * granules : most);
   p.workspace = (size_t)p.runs * ((size_t)2 * tile * (d + 2) * sizeof(float) + 16);
   return p;
 }
 
-hipError_t launch_attn(const AttnArgs& a, int d, hipStream_t stream) {
+hipError_t launch_attn_rows(const AttnArgs& a, int d, hipStream_t stream) {
   return d == 64 ? launch_d<64>(a, stream)
                  : d == 128 ? launch_d<128>(a, stream) : launch_d<256>(a, stream);
 }

@@ -6,13 +6,10 @@
 
 namespace kv4 {
 
-int attn_row_fragments(int max_q, int Hq, int Hkv, int d);
-
 // Waves of a workgroup of attn_rows, and waves a SIMD is to hold (registers allow no more).
 constexpr int kRunWaves = 4;                                          // sharing the batch's tokens
 constexpr int attn_whole_waves(int rf) { return rf <= 2 ? 8 : 4; }    // a workgroup a unit
 constexpr int attn_waves(int d, int rf) { return d * rf <= 128 ? 4 : d * rf <= 256 || d < 256 ? 2 : 1; }
-constexpr int attn_stages(int d, int rf) { return 1; }
 
 __device__ __forceinline__ v4f mfma16(v8bf a, v8bf b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -25,7 +22,8 @@ __device__ __forceinline__ int scalar_load(const int* p) {
 }
 
 // x, which the compiler computes with from here on and not earlier.
-__device__ __forceinline__ int pinned(int x) {
+template <typename I>
+__device__ __forceinline__ I pinned(I x) {
   asm volatile("" : "+v"(x));
   return x;
 }
@@ -37,6 +35,17 @@ __device__ __forceinline__ long uniform(long x) {
 }
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Inclusive scan over the wave: shifts inside rows of 16 lanes, then the rows' last lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // row_bcast:15, rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // row_bcast:31, rows 2 and 3
+  return x;
+}
 
 // A sequence of the batch: its tokens, its first query row, its queries. Sizes that do not fit what
 // the launch was planned for make it bad: its rows are NaN.

@@ -147,16 +147,20 @@ struct AttnArgs {
   int page_shift, table_cols, total, batch, max_q, max_len, Hq, Hkv, group, window;   // group: Hq / Hkv
   float scale;
   bool causal;
+  int fragments;          // row fragments of attn_rows' workgroups
   int runs;               // workgroups that share the batch's tokens; 0: one a unit
+  int few_rows;           // attn_rows has the sequences of at most so many rows, attn_tiles the
+                          // others; 0: one of them has all
   // set at the launch: row tiles of a sequence at most, where runs is 0; units of a sequence at most,
   // and whether attn_join goes by units (there are no more of them than runs) or by runs
   int tiles, units;
   bool by_unit;
   Divisor by_group, by_heads, by_runs;   // of Hq / Hkv, Hkv, runs
 };
-// How the cached tokens are spread over workgroups, and the workspace that takes.
-struct AttnPlan { int runs; size_t workspace; };
-AttnPlan attn_plan(int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window);
-hipError_t launch_attn(const AttnArgs& a, int d, hipStream_t stream);
+// What serves a call (attn_tiles, attn_rows or both), and the workspace that takes.
+struct AttnPlan { bool tiles, rows; int fragments, runs, few_rows; size_t workspace; };
+AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window);
+hipError_t launch_attn_rows(const AttnArgs& a, int d, hipStream_t stream);
+hipError_t launch_attn_tiles(const AttnArgs& a, int d, hipStream_t stream);
 
 }  // namespace kv4

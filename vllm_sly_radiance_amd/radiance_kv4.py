@@ -342,7 +342,7 @@ def _kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tenso
         out = torch.empty((total, Hq, d), dtype=torch.bfloat16, device=dev)
         if total == 0 or B == 0:
             return out
-        need = _native.attention_workspace(B, max_q, max_len, Hq, Hkv, d, window)
+        need = _native.attention_workspace(total, B, max_q, max_len, Hq, Hkv, d, window)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _native.check(_native.lib().kv4_attention(
             q.data_ptr(), *_strides(q), cache.data_ptr(), cache.shape[0], stride, page,
