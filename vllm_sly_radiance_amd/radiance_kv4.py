@@ -6,7 +6,8 @@ and output projections (radiance_mxfp4 has those).
   attention            softmax attention of ragged queries over the cached tokens
   gather               tokens of the cache as bf16
   move_pages           page copies over all layers, and the remapped page table, in one launch
-  PagePool             the host's side: allocate, extend, fork, free, compact
+
+kv4_pool.PagePool is the host's side: allocate, extend, fork, truncate, free, compact.
 
 The cache is MXFP4, as the weights are: e2m1 codes with a power-of-two scale for each 32 channels of a
 token, 4.25 bits an element. new_cache() makes one: uint8 [pages, kv heads, page / 16, 17 d], or
