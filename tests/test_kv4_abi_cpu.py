@@ -234,3 +234,25 @@ def test_what_serves_a_call(lib):
     # beside chunks: rows of one query of the group's heads, if they fit attn_rows' 64 (32)
     assert workspace(lib, 1401, 2, 1400, 4096, 65, 1, 128, 0) == 0
     assert workspace(lib, 1401, 2, 1400, 4096, 64, 1, 128, 0) > 0
+
+
+def test_binding_refuses():
+    """What is no tensor, no number or too many is a Python exception, not a crash."""
+    ops = N.ops()
+    t = torch.zeros((2, 2, 128), dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    for call, error, what in (
+            (lambda: ops.gather(t), RuntimeError, "gather: 1 arguments in place of 2"),
+            (lambda: ops.gather(t, 3), RuntimeError, "argument 1 must be a tensor"),
+            (lambda: ops.gather(None, t), RuntimeError, "argument 0 must be a tensor"),
+            (lambda: ops.gather(t, i), RuntimeError, "on the GPU, got cpu"),
+            (lambda: ops.move_pages(t, i, None), RuntimeError, "on the GPU"),
+            (lambda: ops.attention(t, t, i, i, i, 2 ** 40, 1, 1.0, True, 0), RuntimeError,
+             "max_q=1099511627776 is out of range"),
+            (lambda: ops.attention(t, t, i, i, i, 1, -2 ** 70, 1.0, True, 0), OverflowError, ""),
+            (lambda: ops.attention(t, t, i, i, i, "1", 1, 1.0, True, 0), TypeError, ""),
+            (lambda: ops.attention(t, t, i, i, i, 1, 1, None, True, 0), TypeError, ""),
+            (lambda: ops.qk_norm_rope(t, t, None, None, None, None, None, 1e-6, 0, 0), RuntimeError,
+             "on the GPU")):
+        with pytest.raises(error, match=what or None):
+            call()

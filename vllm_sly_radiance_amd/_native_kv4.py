@@ -1,9 +1,11 @@
-"""ctypes binding of libkv4_attn.so (C ABI: include/kv4_attn.h), loaded as _native loads the linear
-path's library: after torch, with no fallback. A missing or stale library raises, and so does every
-nonzero status (RuntimeError carrying kv4_last_error())."""
+"""Loading of libkv4_attn.so (C ABI: include/kv4_attn.h): ops(), its binding to torch tensors, and lib(),
+the C functions through ctypes. Loaded as _native loads the linear path's library: after torch, with
+no fallback. A missing or stale library raises, and so does every nonzero status (RuntimeError
+carrying kv4_last_error())."""
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
 
@@ -36,7 +38,7 @@ SIGNATURES = {
 }
 
 _lock = threading.Lock()
-_lib = None
+_lib = _ops = None
 
 
 def load_cdll(path: str = LIB_PATH) -> ctypes.CDLL:
@@ -61,6 +63,19 @@ def lib() -> ctypes.CDLL:
                 import torch  # noqa: F401  (bind to torch's HIP runtime before dlopen)
                 _lib = load_cdll()
     return _lib
+
+
+def ops():
+    """The ops on torch tensors (csrc/kv4_torch.cpp)."""
+    global _ops
+    if _ops is None:
+        lib()                       # raises where it is not built, or not this ABI
+        try:
+            _ops = importlib.import_module("._kv4_torch", __package__)
+        except ImportError as e:
+            raise RuntimeError("_kv4_torch.so is not built for this torch: run "
+                               f"__graft_entry__.build() first ({e})") from e
+    return _ops
 
 
 def check(rc: int) -> None:

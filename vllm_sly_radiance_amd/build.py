@@ -1,10 +1,12 @@
-"""Build libw4a8_mxfp4.so and libkv4_attn.so in-tree with hipcc for gfx950 (no other target).
+"""Build libw4a8_mxfp4.so and libkv4_attn.so in-tree with hipcc for gfx950 (no other target), and
+_kv4_torch.so, the latter's binding to torch tensors, with the host compiler.
 
     python -m vllm_sly_radiance_amd.build            # or __graft_entry__.build()
 
 The libraries are plain C-ABI shared objects (include/w4a8_mxfp4.h, include/kv4_attn.h) loaded
 through ctypes; they link the HIP runtime by soname, so inside a torch process they bind to the
-runtime torch already loaded.
+runtime torch already loaded. _kv4_torch.so is a CPython module over libkv4_attn.so, built against the
+installed torch's headers.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -28,6 +31,8 @@ SOURCES = ["w4a8_api.hip", "w4a8_quant.hip", "w4a8_repack.hip", "w4a8_gemm_skinn
 KV4_LIB_PATH = os.path.join(PKG, "libkv4_attn.so")
 KV4_SOURCES = ["kv4_api.hip", "kv4_rope.hip", "kv4_pages.hip", "kv4_attn_rows.hip",
                "kv4_attn_tiles.hip"]
+KV4_TORCH_PATH = os.path.join(PKG, "_kv4_torch.so")
+KV4_TORCH_SOURCE = "kv4_torch.cpp"
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
@@ -54,12 +59,31 @@ def _command(sources, out) -> list[str]:
     return [hipcc(), *FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", out]
 
 
+def _torch_commands(out) -> tuple[list[str], list[str]]:
+    """Compile and link the torch binding (the link needs libkv4_attn.so, found again beside it)."""
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cxx = os.environ.get("CXX") or "g++"
+    system = [os.path.join(base, "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    compile_ = [cxx, "-c", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
+                "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}",
+                *(a for d in system for a in ("-isystem", d)),
+                os.path.join(CSRC, KV4_TORCH_SOURCE), "-o", out + ".o"]
+    link = [cxx, "-shared", out + ".o", "-o", out, f"-L{PKG}", "-l:" + os.path.basename(KV4_LIB_PATH),
+            f"-L{os.path.join(base, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+            "-Wl,-rpath,$ORIGIN"]
+    return compile_, link
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every source into LIB_PATH and KV4_LIB_PATH (always rebuilds, both at once) and
-    return LIB_PATH."""
+    """Compile every source into LIB_PATH, KV4_LIB_PATH and KV4_TORCH_PATH (always rebuilds, all at
+    once) and return LIB_PATH."""
+    compile_, link = _torch_commands(KV4_TORCH_PATH + ".tmp")
     jobs = []
-    for sources, path in ((SOURCES, LIB_PATH), (KV4_SOURCES, KV4_LIB_PATH)):
-        cmd = _command(sources, path + ".tmp")
+    for cmd, path in ((_command(SOURCES, LIB_PATH + ".tmp"), LIB_PATH),
+                      (_command(KV4_SOURCES, KV4_LIB_PATH + ".tmp"), KV4_LIB_PATH),
+                      (compile_, None)):
         if verbose:
             print(" ".join(cmd), flush=True)
         jobs.append((path, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
@@ -71,11 +95,17 @@ def build(verbose: bool = False) -> str:
                  if ln.strip() and "packed-fp32-ops" not in ln and "warning generated" not in ln
                  and "warnings generated" not in ln]
         if status != 0:
-            raise RuntimeError("hipcc failed:\n" + "\n".join(noise))
+            raise RuntimeError("the compiler failed:\n" + "\n".join(noise))
         if verbose and noise:
             print("\n".join(noise), file=sys.stderr)
     for path, _, _ in outputs:
-        os.replace(path + ".tmp", path)
+        if path:
+            os.replace(path + ".tmp", path)
+    done = subprocess.run(link, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if done.returncode:
+        raise RuntimeError("the linker failed:\n" + done.stdout)
+    os.remove(KV4_TORCH_PATH + ".tmp.o")
+    os.replace(KV4_TORCH_PATH + ".tmp", KV4_TORCH_PATH)
     return LIB_PATH
 
 

@@ -26,7 +26,6 @@ with a fake, opaque to a compiler. The functions are the same with defaults.
 """
 from __future__ import annotations
 
-import functools
 import math
 from typing import Optional, Sequence
 
@@ -73,170 +72,28 @@ def rotary_axes(sections: Sequence[int], interleaved: bool = False, device="cuda
     return torch.tensor(axes, dtype=torch.int32, device=device)
 
 
-# ---- checks -------------------------------------------------------------------------------------
-# The calls below are a few microseconds of GPU work where a batch is small, so the host's share is kept
-# small as well: shapes, strides and pointers are read once, and where nothing watches ops by name
-# the body is called without the dispatcher (one token through qk_norm_rope, 5 us on the GPU: 18.9
-# us a call with the dispatcher and separate helpers, 13.3 now, 2.7 of them the launch).
-def _heads(op: str, name: str, x: torch.Tensor):
-    """bf16 [T, heads, d] whose heads are 16-byte aligned runs, other layouts copied: (x, T, heads, d,
-    its address, token and head strides; those of an axis of one, which may be anything, as 0)."""
-    if x.dtype is not torch.bfloat16 or x.dim() != 3:
-        _fail(op, f"{name} must be bf16 [tokens, heads, head size], got {x.dtype} {tuple(x.shape)}")
-    T, H, d = x.shape
-    if d not in HEAD_SIZES:
-        _fail(op, f"head size {d} of {name} is none of {HEAD_SIZES}")
-    st, sh, sc = x.stride()
-    at = x.data_ptr()
-    if T <= 1:
-        st = 0
-    if H <= 1:
-        sh = 0
-    if (sc != 1 or (st | sh) & 7 or at & 15) and T:
-        x = x.clone(memory_format=torch.contiguous_format)
-        return _heads(op, name, x)
-    return x, T, H, d, at, st, sh
-
-
-def _cache(op: str, cache: torch.Tensor, d: Optional[int] = None, heads: Optional[int] = None):
-    """(pages, kv heads, page size, head size, page stride) of a layer's cache."""
-    if cache.dtype is not torch.uint8 or cache.dim() != 4 or cache.shape[3] % 17 \
-            or cache.shape[3] // 17 not in HEAD_SIZES or cache.shape[2] * GROUP not in PAGE_SIZES:
-        _fail(op, f"cache must be uint8 [pages, kv heads, page / 16, 17 * head size], got "
-                  f"{cache.dtype} {tuple(cache.shape)}")
-    pages, H, n, b = cache.shape
-    sp, sh, sn, sb = cache.stride()
-    if (sb != 1 or (n > 1 and sn != b) or (H > 1 and sh != n * b) or cache.data_ptr() & 15) \
-            and cache.numel():
-        _fail(op, "a page of the cache must be contiguous and 16-byte aligned")
-    if d is not None and b != 17 * d:
-        _fail(op, f"cache of head size {b // 17} against {d}")
-    if heads is not None and H != heads:
-        _fail(op, f"cache of {H} kv heads against {heads}")
-    return pages, H, n * GROUP, b // 17, sp if pages > 1 else H * n * b
-
-
-def _same_device(op: str, *tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        _fail(op, f"tensors must be on the GPU, got {dev}")
-    for t in tensors[1:]:
-        if t is not None and t.device != dev:
-            _fail(op, f"tensors on {dev} and {t.device}")
-    return dev
-
-
-def _entry(op, body):
-    """The body, called on the tensors' device; through `op`, whose name a compiler, a tracer or a mode
-    then sees and whose backward raises, where one watches or a gradient may be asked for."""
-    ns, name = op._qualname.split("::")
+def _entry(op, name):
+    """The native op `name`, called without the dispatcher (3 us a call) where nothing watches ops by name
+    and no gradient can be asked for; else `op`, whose name a compiler, a tracer or a mode sees and
+    whose backward raises."""
+    ns, public = op._qualname.split("::")
     space = getattr(torch.ops, ns)
 
     def call(*args):
         if _rmx._watched() or type(args[0]) is not torch.Tensor \
                 or (torch.is_grad_enabled() and _rmx._asks_gradient(args)):
-            return getattr(space, name)(*args)
-        return body(*args)
+            return getattr(space, public)(*args)
+        return getattr(_native.ops(), name)(*args)
     return call
 
 
-def _on_device(body):
-    """body with the device of its first argument, a GPU's tensor, as the current one."""
-    @functools.wraps(body)
-    def run(first, *args):
-        if first.is_cuda and first.get_device() != torch._C._cuda_getDevice():
-            with torch.cuda.device(first.device):
-                return body(first, *args)
-        return body(first, *args)
-    return run
-
-
-def _stream(dev) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _slots(op: str, slots: torch.Tensor, T: int) -> torch.Tensor:
-    if slots.dtype is not torch.int64 or slots.dim() != 1 or slots.shape[0] != T:
-        _fail(op, f"slots must be int64 [{T}], got {slots.dtype} {tuple(slots.shape)}")
-    return slots.contiguous()
-
-
 # ---- norm and rotation --------------------------------------------------------------------------
-def _rope_args(op, T, d, q_weight, k_weight, cos_sin, positions, axis, plus_one, adjacent):
-    """(the C call's arguments from the weights to the axes, flags, tensors that they point into)."""
-    flags = (_native.PLUS_ONE if plus_one else 0) | (_native.ADJACENT if adjacent else 0)
-    weights, at = [], []
-    for w in (q_weight, k_weight):
-        p = 0
-        if w is not None:
-            if w.dtype is not torch.bfloat16 or w.dim() != 1 or w.shape[0] != d:
-                _fail(op, f"{'k_weight' if weights else 'q_weight'} must be bf16 [{d}], got {w.dtype} "
-                          f"{tuple(w.shape)}")
-            p = w.data_ptr()
-            if p & 15 or w.stride(0) != 1:
-                w = w.clone(memory_format=torch.contiguous_format)
-                p = w.data_ptr()
-        weights.append(w)
-        at.append(p)
-    if cos_sin is None:
-        return (*at, 0, 0, 0, 0, 0, 1, 0), flags, weights
-    fp32 = cos_sin.dtype is torch.float32
-    if not (fp32 or cos_sin.dtype is torch.bfloat16) or cos_sin.dim() != 2:
-        _fail(op, f"cos_sin must be fp32 or bf16 [positions, rotated channels], got "
-                  f"{cos_sin.dtype} {tuple(cos_sin.shape)}")
-    rows, rot = cos_sin.shape
-    if rot == 0 or rot > d or rot % 16:
-        _fail(op, f"{rot} rotated channels: need a multiple of 16 up to the head size {d}")
-    cos_sin = cos_sin.contiguous()
-    dims = 0 if positions is None else positions.dim()
-    i32 = dims and positions.dtype is torch.int32
-    if dims not in (1, 2) or not (i32 or positions.dtype is torch.int64) \
-            or positions.shape[-1] != T or positions.shape[0] == 0 and dims == 2:
-        _fail(op, f"positions must be int64 or int32 [{T}] or [axes, {T}], got "
-                  f"{None if positions is None else (positions.dtype, tuple(positions.shape))}")
-    axes = positions.shape[0] if dims == 2 else 1
-    if axes > 1 and axis is None:
-        _fail(op, f"positions on {axes} axes need the axis of each pair (rotary_axes)")
-    if axis is not None:
-        if axis.dtype is not torch.int32 or tuple(axis.shape) != (rot // 2,):
-            _fail(op, f"axis must be int32 [{rot // 2}], got {axis.dtype} {tuple(axis.shape)}")
-        axis = axis.contiguous()
-    if positions.stride(-1) != 1 or (axes > 1 and positions.stride(0) < T):
-        positions = positions.contiguous()
-    flags |= (0 if fp32 else _native.TABLE_BF16) | (_native.POS_I32 if i32 else 0)
-    return ((*at, cos_sin.data_ptr(), rows, rot, positions.data_ptr(),
-             positions.stride(0) if axes > 1 else T, axes, _ptr(axis)), flags,
-            (weights, cos_sin, positions, axis))
-
-
-def _same_tokens(op, T, d, name, x, xT, xd):
-    if xT != T or xd != d:
-        _fail(op, f"{name} {tuple(x.shape)} does not match q [{T}, ..., {d}]")
-
-
-@_on_device
 def _qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
                   k_weight: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor],
                   positions: Optional[torch.Tensor], axis: Optional[torch.Tensor], eps: float,
                   plus_one: bool, adjacent: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    op = "qk_norm_rope"
-    dev = _same_device(op, q, k, q_weight, k_weight, cos_sin, positions, axis)
-    q, T, Hq, d, qp, qt, qh = _heads(op, "q", q)
-    k, kT, Hkv, kd, kp, kt, kh = _heads(op, "k", k)
-    _same_tokens(op, T, d, "k", k, kT, kd)
-    tail, flags, keep = _rope_args(op, T, d, q_weight, k_weight, cos_sin, positions, axis, plus_one,
-                                   adjacent)
-    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ko = torch.empty_like(k, memory_format=torch.contiguous_format)
-    # (q, k and keep may be copies: stream-ordered, reused only after this launch)
-    _native.check(_native.lib().kv4_qk_norm_rope(
-        qp, qt, qh, kp, kt, kh, *tail, qo.data_ptr(), ko.data_ptr(), T, Hq, Hkv, d, eps, flags,
-        _stream(dev)))
-    return qo, ko
+    return _native.ops().qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, axis, eps,
+                                      plus_one, adjacent)
 
 
 def _qk_norm_rope_fake(q, k, q_weight, k_weight, cos_sin, positions, axis, eps, plus_one, adjacent):
@@ -246,7 +103,7 @@ def _qk_norm_rope_fake(q, k, q_weight, k_weight, cos_sin, positions, axis, eps, 
 
 qk_norm_rope_op = torch.library.custom_op("radiance::qk_norm_rope", _qk_norm_rope, mutates_args=())
 qk_norm_rope_op.register_fake(_qk_norm_rope_fake)
-_call_qk_norm_rope = _entry(qk_norm_rope_op, _qk_norm_rope)
+_call_qk_norm_rope = _entry(qk_norm_rope_op, "qk_norm_rope")
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, *, axis=None, eps: float = 1e-6,
@@ -261,31 +118,13 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, *, axis=None, eps
                               bool(plus_one), bool(adjacent))
 
 
-@_on_device
 def _qk_norm_rope_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
                       cos_sin: Optional[torch.Tensor], positions: Optional[torch.Tensor],
                       cache: torch.Tensor, slots: torch.Tensor, axis: Optional[torch.Tensor],
                       eps: float, plus_one: bool, adjacent: bool) -> torch.Tensor:
-    op = "qk_norm_rope_append"
-    dev = _same_device(op, q, k, v, q_weight, k_weight, cos_sin, positions, cache, slots, axis)
-    q, T, Hq, d, qp, qt, qh = _heads(op, "q", q)
-    k, kT, Hkv, kd, kp, kt, kh = _heads(op, "k", k)
-    v, vT, Hv, vd, vp, vt, vh = _heads(op, "v", v)
-    _same_tokens(op, T, d, "k", k, kT, kd)
-    _same_tokens(op, T, d, "v", v, vT, vd)
-    if Hv != Hkv:
-        _fail(op, f"v {tuple(v.shape)} does not match k {tuple(k.shape)}")
-    tail, flags, keep = _rope_args(op, T, d, q_weight, k_weight, cos_sin, positions, axis, plus_one,
-                                   adjacent)
-    pages, _, page, _, stride = _cache(op, cache, d, Hkv)
-    slots = _slots(op, slots, T)
-    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-    # (the inputs may be copies: stream-ordered, reused only after this launch)
-    _native.check(_native.lib().kv4_qk_norm_rope_append(
-        qp, qt, qh, kp, kt, kh, vp, vt, vh, *tail, qo.data_ptr(), cache.data_ptr(), pages, stride,
-        page, slots.data_ptr(), T, Hq, Hkv, d, eps, flags, _stream(dev)))
-    return qo
+    return _native.ops().qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, cache,
+                                             slots, axis, eps, plus_one, adjacent)
 
 
 def _qk_norm_rope_kv4_fake(q, k, v, q_weight, k_weight, cos_sin, positions, cache, slots, axis, eps,
@@ -296,7 +135,7 @@ def _qk_norm_rope_kv4_fake(q, k, v, q_weight, k_weight, cos_sin, positions, cach
 qk_norm_rope_kv4_op = torch.library.custom_op("radiance::qk_norm_rope_kv4", _qk_norm_rope_kv4,
                                               mutates_args=("cache",))
 qk_norm_rope_kv4_op.register_fake(_qk_norm_rope_kv4_fake)
-_call_qk_norm_rope_kv4 = _entry(qk_norm_rope_kv4_op, _qk_norm_rope_kv4)
+_call_qk_norm_rope_kv4 = _entry(qk_norm_rope_kv4_op, "qk_norm_rope_append")
 
 
 def qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, cache, slots, *, axis=None,
@@ -308,18 +147,8 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, cache, 
 
 
 # ---- reading back -------------------------------------------------------------------------------
-@_on_device
 def _kv4_gather(cache: torch.Tensor, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    op = "gather"
-    dev = _same_device(op, cache, slots)
-    pages, H, page, d, stride = _cache(op, cache)
-    slots = _slots(op, slots, slots.shape[0] if slots.dim() else 0)
-    T = slots.shape[0]
-    k = torch.empty((T, H, d), dtype=torch.bfloat16, device=dev)
-    v = torch.empty_like(k)
-    _native.check(_native.lib().kv4_gather(cache.data_ptr(), pages, stride, page, slots.data_ptr(),
-                                           k.data_ptr(), v.data_ptr(), T, H, d, _stream(dev)))
-    return k, v
+    return _native.ops().gather(cache, slots)
 
 
 def _kv4_gather_fake(cache, slots):
@@ -330,7 +159,7 @@ def _kv4_gather_fake(cache, slots):
 
 kv4_gather_op = torch.library.custom_op("radiance::kv4_gather", _kv4_gather, mutates_args=())
 kv4_gather_op.register_fake(_kv4_gather_fake)
-_call_kv4_gather = _entry(kv4_gather_op, _kv4_gather)
+_call_kv4_gather = _entry(kv4_gather_op, "gather")
 
 
 def gather(cache, slots):
@@ -340,39 +169,11 @@ def gather(cache, slots):
 
 
 # ---- attention ----------------------------------------------------------------------------------
-@_on_device
 def _kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor,
                    seq_lens: torch.Tensor, q_starts: torch.Tensor, max_q: int, max_len: int,
                    scale: float, causal: bool, window: int) -> torch.Tensor:
-    op = "attention"
-    dev = _same_device(op, q, cache, page_table, seq_lens, q_starts)
-    q, total, Hq, d, qp, qt, qh = _heads(op, "q", q)
-    pages, Hkv, page, _, stride = _cache(op, cache, d)
-    B = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    if seq_lens.dtype is not torch.int32 or B < 0:
-        _fail(op, f"seq_lens must be int32 [batch], got {seq_lens.dtype} {tuple(seq_lens.shape)}")
-    if q_starts.dtype is not torch.int32 or q_starts.dim() != 1 or q_starts.shape[0] != B + 1:
-        _fail(op, f"q_starts must be int32 [{B + 1}], got {q_starts.dtype} {tuple(q_starts.shape)}")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
-        _fail(op, f"page_table must be int32 [{B}, pages of a sequence], got "
-                  f"{page_table.dtype} {tuple(page_table.shape)}")
-    seq_lens, q_starts = seq_lens.contiguous(), q_starts.contiguous()
-    row, col = page_table.stride()
-    if col != 1:
-        page_table = page_table.contiguous()
-        row = page_table.stride(0)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if total == 0 or B == 0:
-        return out
-    need = _native.attention_workspace(total, B, max_q, max_len, Hq, Hkv, d, window)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    # (the workspace and inputs that are copies: stream-ordered, reused only after this launch)
-    _native.check(_native.lib().kv4_attention(
-        qp, qt, qh, cache.data_ptr(), pages, stride, page, page_table.data_ptr(), row if B > 1 else 0,
-        page_table.shape[1], seq_lens.data_ptr(), q_starts.data_ptr(), out.data_ptr(), _ptr(ws), need,
-        total, B, max_q, max_len, Hq, Hkv, d, scale, window, _native.CAUSAL if causal else 0,
-        _stream(dev)))
-    return out
+    return _native.ops().attention(q, cache, page_table, seq_lens, q_starts, max_q, max_len, scale,
+                                   causal, window)
 
 
 def _kv4_attention_fake(q, cache, page_table, seq_lens, q_starts, max_q, max_len, scale, causal,
@@ -383,7 +184,7 @@ def _kv4_attention_fake(q, cache, page_table, seq_lens, q_starts, max_q, max_len
 kv4_attention_op = torch.library.custom_op("radiance::kv4_attention", _kv4_attention,
                                            mutates_args=())
 kv4_attention_op.register_fake(_kv4_attention_fake)
-_call_kv4_attention = _entry(kv4_attention_op, _kv4_attention)
+_call_kv4_attention = _entry(kv4_attention_op, "attention")
 
 
 def attention(q, cache, page_table, seq_lens, q_starts, max_q: int, max_len: int, *,
@@ -403,33 +204,9 @@ def attention(q, cache, page_table, seq_lens, q_starts, max_q: int, max_len: int
 
 
 # ---- pages --------------------------------------------------------------------------------------
-@_on_device
 def _kv4_move_pages(cache: torch.Tensor, pairs: torch.Tensor,
                     page_table: Optional[torch.Tensor]) -> None:
-    op = "move_pages"
-    dev = _same_device(op, cache, page_table)
-    layers = cache.shape[0] if cache.dim() == 5 else 1
-    one = cache[0] if cache.dim() == 5 and layers else cache
-    if layers == 0:
-        return
-    pages, heads, page, d, stride = _cache(op, one)
-    if pairs.device.type != "cpu" or pairs.dtype != torch.int32 or pairs.dim() != 2 \
-            or pairs.shape[1] != 2:
-        _fail(op, f"pairs must be int32 [n, 2] (from, to) on the host, got {pairs.dtype} "
-                  f"{tuple(pairs.shape)} on {pairs.device}")
-    pairs = pairs.contiguous()
-    rows = cols = table_stride = 0
-    if page_table is not None:
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 \
-                or (page_table.numel() and page_table.stride(1) != 1 and page_table.shape[1] > 1):
-            _fail(op, f"page_table must be int32 [sequences, pages] with contiguous rows, got "
-                      f"{page_table.dtype} {tuple(page_table.shape)}")
-        rows, cols = page_table.shape
-        table_stride = page_table.stride(0) if rows > 1 else cols
-    _native.check(_native.lib().kv4_move_pages(
-        cache.data_ptr(), layers, cache.stride(0) if layers > 1 else 0, pages, stride,
-        heads * page // GROUP * 17 * d, pairs.data_ptr(), pairs.shape[0],
-        _ptr(page_table) if rows * cols else 0, rows, cols, table_stride, _stream(dev)))
+    return _native.ops().move_pages(cache, pairs, page_table)
 
 
 def _kv4_move_pages_fake(cache, pairs, page_table):
@@ -439,7 +216,7 @@ def _kv4_move_pages_fake(cache, pairs, page_table):
 kv4_move_pages_op = torch.library.custom_op("radiance::kv4_move_pages", _kv4_move_pages,
                                             mutates_args=("cache", "page_table"))
 kv4_move_pages_op.register_fake(_kv4_move_pages_fake)
-_call_kv4_move_pages = _entry(kv4_move_pages_op, _kv4_move_pages)
+_call_kv4_move_pages = _entry(kv4_move_pages_op, "move_pages")
 
 
 def move_pages(cache, pairs, page_table=None) -> None:
