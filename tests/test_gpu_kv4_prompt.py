@@ -22,8 +22,8 @@ def _lib(gpu_lib):
 
 def run(batch, max_q=None, max_len=None, **kw):
     q, cache, table, lens, starts, mq, ml = batch.device()
-    # rows enough for a workgroup of many rows (tests/test_kv4_abi_cpu.py has the rule)
-    assert q.shape[0] * q.shape[1] >= 700 * (32 if batch.d == 256 else 64)
+    # rows enough for workgroups of many rows (tests/test_kv4_abi_cpu.py has the rule)
+    assert q.shape[0] * q.shape[1] >= 200 * (32 if batch.d == 256 else 64)
     print(f"[kv4] lens={batch.lens} q={batch.qs} heads={q.shape[1]}/{batch.Hkv} d={batch.d} "
           f"page={batch.page} {kw}", flush=True)
     out = K.attention(q, cache, table, lens, starts, max_q or mq, max_len or ml, **kw)
@@ -68,6 +68,46 @@ def test_more_sequences_than_lanes():
     qs = [(20, 1, 0, 13)[i % 4] for i in range(150)]
     b = Batch(rng, [n + int(rng.integers(0, 60)) for n in qs], qs, 64, 2, 64, 16)
     b.check(run(b))
+
+
+PARTS = [(16, 2, 64, 16, [1500], [800]), (8, 2, 256, 64, [1400], [801]), (32, 2, 128, 32, [1100], [401]),
+         (32, 2, 128, 32, [1100, 1000], [399, 399]),        # every sequence alike but for its length
+         (32, 2, 128, 16, [1300, 900, 20], [300, 290, 1])]
+
+
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 333)])
+@pytest.mark.parametrize("i", range(len(PARTS)))
+def test_units_in_parts(i, causal, window):
+    """Few units over long contexts: their tokens are cut into parts, some of which a row sees none of."""
+    Hq, Hkv, d, page, lens, qs = PARTS[i]
+    b = Batch(np.random.default_rng(20 + i), lens, qs, Hq, Hkv, d, page)
+    # (a window leaves some of them too few tokens to be cut)
+    assert _native_kv4.attention_workspace(sum(qs), len(qs), max(qs), max(lens), Hq, Hkv, d, 0) > 4096
+    b.check(run(b, causal=causal, window=window), causal=causal, window=window)
+
+
+def test_parts_with_nan_blocks_bad_pages_and_bad_lengths():
+    b = Batch(np.random.default_rng(30), [1200, 1100, 1150], [300, 300, 300], 16, 2, 128, 16)
+    for s, tok, head, what in ((0, 100, 0, "v"), (0, 700, 1, "k"), (0, 1150, 1, "v"), (2, 1149, 0, "v")):
+        slot = b.slots(s)[tok]
+        pk, pv, sk, sv = KO.places(int(slot % 16), 128)
+        b.cache[slot // 16, head, 0][(sk if what == "k" else sv)[tok % 4]] = 255
+    b.check(run(b))
+    page = b.table[1, 60]
+    b.table[1, 60] = -1
+    out = run(b)
+    got = O.bf16_to_f32(host_u16(out))
+    # rows of the second sequence that come after token 960, and those of their workgroup
+    assert np.isnan(got[300 + 160:600]).all()
+    b.check(out, only=(0, 2))
+    b.table[1, 60] = page
+    q, cache, table, lens, starts, mq, ml = b.device()
+    for bad in (0, 1, 2):
+        wrong = lens.clone()
+        wrong[bad] = 5000
+        got = O.bf16_to_f32(host_u16(K.attention(q, cache, table, wrong, starts, mq, ml)))
+        assert np.isnan(got[300 * bad:300 * bad + 300]).all()
+        b.check(K.attention(q, cache, table, wrong, starts, mq, ml), only={0, 1, 2} - {bad})
 
 
 @pytest.mark.parametrize("window", [1, 31, 64, 200, 5000])

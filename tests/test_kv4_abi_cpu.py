@@ -218,22 +218,25 @@ def workspace(lib, *sizes):
 
 
 def test_what_serves_a_call(lib):
-    """(total, batch, max_q, max_len, q heads, kv heads, d, window): few rows over a long context are
-    split over workgroups, which takes a workspace; many rows (more than 128 a kv head, 64 at head size
-    256, and 700 times half that in all) are not, unless sequences of few rows may stand beside them."""
+    """(total, batch, max_q, max_len, q heads, kv heads, d, window) and the workspace: few rows over a long
+    context are shared out over 512 workgroups, two partial results each; many rows (more than 128 a kv
+    head, 64 at head size 256, and 200 times half that in all) take a workgroup for each 256 (128), the
+    last round's in parts; sequences of few rows beside them, both."""
+    few = lambda runs, rows, d: runs * (2 * rows * (d + 2) * 4 + 16)  # noqa: E731
+    many = lambda parts, rows, d: parts * rows * (d + 2) * 4 + 4096  # noqa: E731
     assert workspace(lib, 1, 1, 1, 512, 32, 8, 128, 0) == 0
-    assert workspace(lib, 1, 1, 1, 513, 32, 8, 128, 0) > 0
+    assert workspace(lib, 1, 1, 1, 513, 32, 8, 128, 0) == few(8 * 5, 16, 128)
     assert workspace(lib, 0, 1, 0, 4096, 32, 8, 128, 0) == 0
-    assert workspace(lib, 1399, 1, 1399, 4096, 32, 8, 128, 0) > 0
-    assert workspace(lib, 1400, 1, 1400, 4096, 32, 8, 128, 0) == 0
-    assert workspace(lib, 1401, 2, 1400, 4096, 32, 8, 128, 0) > 0
-    assert workspace(lib, 64 * 32, 64, 32, 4096, 32, 8, 128, 0) > 0
-    assert workspace(lib, 64 * 33, 64, 33, 4096, 32, 8, 128, 0) == 0
-    assert workspace(lib, 1399, 1, 1399, 4096, 16, 2, 256, 0) > 0
-    assert workspace(lib, 1400, 1, 1400, 4096, 16, 2, 256, 0) == 0
-    # beside chunks: rows of one query of the group's heads, if they fit attn_rows' 64 (32)
-    assert workspace(lib, 1401, 2, 1400, 4096, 65, 1, 128, 0) == 0
-    assert workspace(lib, 1401, 2, 1400, 4096, 64, 1, 128, 0) > 0
+    assert workspace(lib, 399, 1, 399, 4096, 32, 8, 128, 0) == few(512, 64, 128)
+    assert workspace(lib, 400, 1, 400, 4096, 32, 8, 128, 0) == many(56 * 4, 256, 128)
+    assert workspace(lib, 400, 1, 400, 400, 32, 8, 128, 0) == 0
+    assert workspace(lib, 64 * 32, 64, 32, 4096, 32, 8, 128, 0) == few(512, 64, 128)
+    assert workspace(lib, 64 * 33, 64, 33, 4096, 32, 8, 128, 0) == 0      # 512 units, two rounds
+    assert workspace(lib, 400, 1, 400, 4096, 16, 2, 256, 0) == many(50 * 5, 128, 256)
+    assert workspace(lib, 400, 1, 400, 4096, 64, 64, 64, 0) == many(128 * 2, 256, 64)
+    # beside chunks: rows of one query of the group's heads, if they fit attn_rows' 64
+    assert workspace(lib, 401, 2, 400, 4096, 65, 1, 128, 0) == many(512, 256, 128)
+    assert workspace(lib, 401, 2, 400, 4096, 64, 1, 128, 0) == many(512, 256, 128) + few(64, 64, 128)
 
 
 def test_binding_refuses():

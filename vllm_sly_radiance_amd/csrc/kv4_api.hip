@@ -251,9 +251,13 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   a.Hq = q_heads, a.Hkv = kv_heads, a.group = q_heads / kv_heads;
   a.window = window, a.scale = scale;
   a.causal = flags & KV4_CAUSAL;
-  a.fragments = plan.fragments, a.runs = plan.runs, a.few_rows = plan.few_rows;
-  if (plan.tiles)
+  a.few_rows = plan.few_rows;
+  if (plan.tiles) {
+    a.entries = plan.entries, a.span = plan.span;
     if (int rc = hip_status(launch_attn_tiles(a, d, (hipStream_t)stream), who)) return rc;
+    a.entries = 0, a.part += plan.tiles_workspace / sizeof(float);
+  }
+  a.fragments = plan.fragments, a.runs = plan.runs;
   return plan.rows ? hip_status(launch_attn_rows(a, d, (hipStream_t)stream), who) : KV4_OK;
 }
 

@@ -50,9 +50,16 @@ __device__ __forceinline__ void load_keys(Raw<D>& w, const uint8_t* group, uint3
   for (int p = 0; p < G::kPlanes; ++p) {
     w.k[p] = *reinterpret_cast<const Vec*>(
         group + (uint32_t)(G::kKeys + r * (D / 2) + p * 64 + g * sizeof(Vec)));
-    w.ks[p] =
-        group[(uint32_t)(G::kKeyScales + r * (D / kBlock) + (D >= 128 ? 4 * p + g : g >> 1))];
+    // the word that holds the scale (a byte carried to the next step would be masked where it is loaded,
+    // with a wait for all that is in flight)
+    w.ks[p] = *reinterpret_cast<const uint32_t*>(
+        group + (uint32_t)(G::kKeyScales + (D >= 128 ? r * (D / kBlock) + 4 * p : 4 * (r >> 1))));
   }
+}
+// The bit of its key scales' words that a lane's scale begins at.
+template <int D>
+__device__ __forceinline__ uint32_t key_scale_bit(uint32_t g, uint32_t r) {
+  return D >= 128 ? 8 * g : 16 * (r & 1) + 8 * (g >> 1);
 }
 template <int D>
 __device__ __forceinline__ void load_values(Raw<D>& w, const uint8_t* group, uint32_t g,
@@ -249,6 +256,7 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
     // end the segment's last step is asked for again (cache hits that nothing uses): loads that are
     // always issued let the waits count those in flight instead of draining them.
     Raw<D> w[2];
+    const uint32_t ks_bit = key_scale_bit<D>(g, r);
     const int t_last = (t1 - 1 - t0) / kStep * kStep + t0;
     int t = t0 + wave * kStep;
     int na = 0, nb = 0;                // page numbers of the next step to ask for
@@ -272,8 +280,8 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int p = D >= 128 ? k >> 2 : 0;
-        const v8bf k0 = expand8(w[0].k[p][D >= 128 ? k & 3 : k], scale_of(w[0].ks[p]));
-        const v8bf k1 = expand8(w[1].k[p][D >= 128 ? k & 3 : k], scale_of(w[1].ks[p]));
+        const v8bf k0 = expand8(w[0].k[p][D >= 128 ? k & 3 : k], scale_of((w[0].ks[p] >> ks_bit) & 0xFFu));
+        const v8bf k1 = expand8(w[1].k[p][D >= 128 ? k & 3 : k], scale_of((w[1].ks[p] >> ks_bit) & 0xFFu));
 #pragma unroll
         for (int f = 0; f < RF; ++f) {
           const v8bf q = __builtin_bit_cast(v8bf, sh.q[f * KS + k][lane]);
@@ -478,7 +486,8 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int 
   const int tr = tile * tile_rows + row;
   const int last = row < rows && tr < R ? n : -1;        // no partial results of a row beyond
   // partial 0 is the last of workgroup i0, partial k > 0 the first of workgroup i0 + k
-  auto slot = [&](int k) { return 2 * (i0 + k) + (k == 0 ? 1 : 0); };
+  // (those of a unit that attn_tiles did in parts lie one after the other)
+  auto slot = [&](int k) { return a.by_parts ? i0 + k : 2 * (i0 + k) + (k == 0 ? 1 : 0); };
   v4f part[kAhead];
   float st[kAhead][2];
   auto read = [&](int k0) {
@@ -523,6 +532,20 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int 
   store_row<4>(out_row(a, D, q0, h, tr) + 4 * lane, out, sum);
 }
 
+// rows: of a sequence at most
+template <int D>
+hipError_t join(const AttnArgs& a, int tile_rows, int entries, int rows, hipStream_t stream) {
+  if (rows > tile_rows) rows = tile_rows;
+  // A row to a workgroup where the rows are few: many workgroups' partial results each. A row to a
+  // team where they are many (of few partial results each).
+  constexpr int kTeams = 1024 / D;
+  if ((long)entries * rows <= 2048)
+    attn_join<D, kTeams><<<entries * rows, 256, 0, stream>>>(a, tile_rows, entries, rows);
+  else
+    attn_join<D, 1><<<entries * ceil_div(rows, kTeams), 256, 0, stream>>>(a, tile_rows, entries, rows);
+  return hipGetLastError();
+}
+
 template <int D, int RF>
 hipError_t launch(AttnArgs a, hipStream_t stream) {
   constexpr int W = kRunWaves;
@@ -539,17 +562,7 @@ hipError_t launch(AttnArgs a, hipStream_t stream) {
   a.by_unit = (long)a.batch * a.units <= a.runs;
   attn_rows<D, RF, W><<<a.runs, 64 * W, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  const int entries = a.by_unit ? a.batch * a.units : a.runs;
-  const int tile_rows = rows < 16 * RF ? rows : 16 * RF;
-  // A row to a workgroup where the rows are few: many workgroups' partial results each. A row to a
-  // team where they are many (of few partial results each).
-  constexpr int kTeams = 1024 / D;
-  if ((long)entries * tile_rows <= 2048)
-    attn_join<D, kTeams><<<entries * tile_rows, 256, 0, stream>>>(a, 16 * RF, entries, tile_rows);
-  else
-    attn_join<D, 1><<<entries * ceil_div(tile_rows, kTeams), 256, 0, stream>>>(a, 16 * RF, entries,
-                                                                             tile_rows);
-  return hipGetLastError();
+  return join<D>(a, 16 * RF, a.by_unit ? a.batch * a.units : a.runs, rows, stream);
 }
 
 template <int D>
@@ -565,6 +578,15 @@ hipError_t launch_d(const AttnArgs& a, hipStream_t stream) {
 
 }  // namespace
 
+hipError_t launch_attn_join(const AttnArgs& a, int d, int tile_rows, int entries, hipStream_t stream) {
+  return d == 64 ? join<64>(a, tile_rows, entries, tile_rows, stream)
+                 : d == 128 ? join<128>(a, tile_rows, entries, tile_rows, stream)
+                            : join<256>(a, tile_rows, entries, tile_rows, stream);
+}
+
+// Partial results of attn_tiles at most: two for each CU, 68 MB.
+constexpr int kMostEntries = 2 * kCUs;
+
 AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window) {
   const int group = Hq / Hkv;
   const long rows = (long)max_q * group;
@@ -572,22 +594,40 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   // Row fragments: the fewest of 1, 2, 4 that hold a sequence's rows, 4 (2 at D = 256, whose
   // accumulators are twice as wide) beyond.
   auto fragments = [d](long n) { return n <= 16 ? 1 : n <= 32 || d == 256 ? 2 : 4; };
+  // tokens that a row tile can see
+  long span = max_len;
+  if (window > 0 && (long)window + max_q + 31 < span) span = (long)window + max_q + 31;
   long few = rows;
   // attn_tiles or attn_rows: a workgroup of attn_tiles does what four row tiles (of 64 rows, 32 at
-  // D = 256) of attn_rows do, in the time of 2.6 of them, but it walks over all its tokens by itself
-  // and has a CU to itself: below some 700 row tiles in the batch, 2.7 for each CU, spreading the
-  // tokens over all CUs wins. Against 4096 cached tokens, attn_tiles and attn_rows with its join in us:
-  //   d = 128, 32 query and 8 kv heads      d = 256, 24 and 4              d = 64, 64 and 8
-  //   1 x 256 queries   128 tiles 105  42   4 x 128  384 tiles 183  125    256 queries   256 tiles 84  45
-  //   1 x 512           256       109  62   1 x 512  384       186  124    512           512       88  70
-  //   1 x 1024          512       118  96   4 x 256  768       192  226    2 x 512      1024       99 134
-  //   1 x 4096         2048       158 345
-  //   32 x 17 (68 rows) 512       135  98
+  // D = 256) of attn_rows do, in the time of 2.6 of them; but it has a CU to itself, so that few of
+  // them are cut into parts, each with a start, an end and partial results of its own. Against 4096
+  // cached tokens, attn_tiles and attn_rows with attn_join in us:
+  //   d = 128, 32 query and 8 kv heads      d = 256, 24 and 4               d = 64, 64 and 8
+  //   1 x 128 queries    64 tiles  31  32   1 x 100  76 tiles  41  43       1 x 64    64 tiles  23  22
+  //   1 x 256           128        40  41   1 x 512 384       104 122       1 x 512  512        60  70
+  //   1 x 512           256        53  61   4 x 256 768       173 226
+  //   1 x 1024          512        85  96   and 32 and 32 heads of 64:
+  //   1 x 4096         2048       153 300                                   1 x 600  320        55  54
+  //   16 x 33 (132 rows) 384       79  86
   const long rows_tile = d == 256 ? 32 : 64;
-  if (rows > 2 * rows_tile && (long)total * Hq >= 700 * rows_tile) {
+  if (rows > 2 * rows_tile && (long)total * Hq >= 200 * rows_tile) {
     p.tiles = true;
+    // The last round of row tiles is done in parts: into how many is known here where all sequences have
+    // max_q queries.
+    const bool even = total == (long)batch * max_q;
+    const long tile_rows = attn_tile_rows(d), units = (rows + tile_rows - 1) / tile_rows * batch * Hkv;
+    p.span = span;
+    if (even) {
+      const int rest = (int)(units % kCUs), parts = attn_parts(rest, span, kMostEntries);
+      p.entries = parts > 1 ? rest * parts : 0;
+    } else {
+      p.entries = (int)(units * 16 < kMostEntries ? units * 16 : kMostEntries);
+    }
+    if (p.entries)
+      p.tiles_workspace = p.workspace =
+          (size_t)(p.entries + 1) / 2 * 2 * tile_rows * (d + 2) * sizeof(float) + kCUs * 16;
     // Sequences of fewer queries beside: those of one query are attn_rows'.
-    if (total == (long)batch * max_q) return p;
+    if (even) return p;
     const int fit = group <= 16 ? 16 : group <= 32 || d == 256 ? 32 : 64;
     if (group > fit) return p;
     few = p.few_rows = fit;
@@ -596,16 +636,13 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   p.fragments = fragments(few);
   const int tile = 16 * p.fragments;
   const long units = (long)batch * Hkv * ((few + tile - 1) / tile);
-  // tokens that a tile can see, in granules
-  long span = max_len;
-  if (window > 0 && (long)window + max_q + 31 < span) span = (long)window + max_q + 31;
   // Two steps a wave: a workgroup a unit, and no second launch.
   if (span <= 2L * kStep * attn_whole_waves(p.fragments)) return p;
   // as many workgroups as the card's 256 CUs hold at once, or a granule each
   const long granules = (span + kStep * kRunWaves - 1) / (kStep * kRunWaves);
   const long most = 256L * 4 * attn_waves(d, p.fragments) / kRunWaves;
   p.runs = (int)(units * granules < most ? units * granules : most);
-  p.workspace = (size_t)p.runs * ((size_t)2 * tile * (d + 2) * sizeof(float) + 16);
+  p.workspace += (size_t)p.runs * ((size_t)2 * tile * (d + 2) * sizeof(float) + 16);
   return p;
 }
 

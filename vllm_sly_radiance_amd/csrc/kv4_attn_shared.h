@@ -194,7 +194,8 @@ __device__ __forceinline__ void store_row(uint16_t* out, const float y[C], float
 
 // Workspace of attn_rows: partial results fp32 [2 runs][tile rows][D], [2 runs][tile rows][2] with
 // the row's maximum (in units of log2) and sum, and int [runs][4]: what attn_join is told (of a unit,
-// by its index b * units + unit, or of the one that begins in a run).
+// by its index b * units + unit, or of the one that begins in a run). attn_tiles' has the same parts,
+// a partial result for each part of each entry (2 runs of them at least), and int [256][4], by entry.
 __device__ __forceinline__ float* part_row(const AttnArgs& a, int tile_rows, int D, int slot,
                                            int row) {
   return a.part + ((size_t)slot * tile_rows + row) * D;

@@ -14,11 +14,16 @@
 // both go on at once: the scores of the next 32 tokens run under the weights of these 32, the sums
 // under the conversion of codes, instruction by instruction.
 //
-// 4096 causal tokens, 32 query and 8 kv heads of 128: 155 us, 887 TFLOP/s of visible products; the
+// A batch's row tiles seldom fill the CUs evenly. Whole rounds of them take a workgroup each; the last
+// round's are cut along the tokens into as many parts as pay (attn_parts), which attn_join weighs:
+// 300 units of 128 rows against 4096 tokens each at D = 256 took 310 us in two rounds of whole
+// units, and take 222 and 8 for the join with 44 of them in 5 parts.
+//
+// 4096 causal tokens, 32 query and 8 kv heads of 128: 152 us, 900 TFLOP/s of visible products; the
 // cores are busy half of the cycles, at the 1.7 GHz that this load leaves the clock (a large library
 // product of bf16 matrices reaches 1206). Whole steps pipelined in place of
-// 32 tokens and 2 to 10 operands read ahead were slower or the same; steps of 64 tokens took 178 us
-// (a barrier and a start of the operand reads each).
+// 32 tokens, 2 to 10 operands read ahead and a second accumulator for the scores were slower or the
+// same; steps of 64 tokens took 178 us (a barrier and a start of the operand reads each).
 #include <utility>
 
 #include "kv4_attn.h"
@@ -103,7 +108,7 @@ struct Fill {
   using G = Group<D>;
   typedef typename std::conditional<D >= 128, v4i, v2i>::type Vec;
   uint32_t k[T::kKeyUnits];
-  uint32_t ks[(T::kKeyUnits + 3) / 4];
+  uint32_t ks;             // the word that holds the units' key scales (a byte for each 4), from bit ks_bit
   Vec v[2];
   uint32_t vs[2];
   float s[8];              // while they are converted: the tokens' scales, one byte's values
@@ -111,14 +116,15 @@ struct Fill {
   // This lane's places, in bytes: of its keys, their scales, its values and their scales in the group,
   // and in LDS (of a buffer) of its keys and of the two channels of a byte of its values. They are
   // pinned where they are used: 64-bit forms of them would be kept in registers through the loop.
-  uint32_t key_at, key_scale_at, value_at, value_scale_at, key_to, even_to, odd_to, nan_to;
+  uint32_t key_at, key_scale_at, ks_bit, value_at, value_scale_at, key_to, even_to, odd_to, nan_to;
   int byte;
   bool has_values;
 
   __device__ __forceinline__ void place(int grp, int part, int lane) {
     const int l = part * 64 + lane, token = l & 15, run = l >> 4, u = l / T::kByteLanes;
     key_at = G::kKeys + token * (D / 2) + run * (4 * T::kKeyUnits);
-    key_scale_at = G::kKeyScales + token * (D / kBlock) + run * T::kKeyUnits / 4;
+    const int scale = token * (D / kBlock) + run * T::kKeyUnits / 4;
+    key_scale_at = G::kKeyScales + (scale & ~3), ks_bit = 8 * (scale & 3);
     const int unit = run * T::kKeyUnits, tok = 16 * grp + token;
     key_to = (((tok >> 5) * (D / 16) + (unit >> 1)) * 64 + (unit & 1) * 32 + (tok & 31)) * 16;
     has_values = u < T::kValueUnits;
@@ -146,9 +152,9 @@ struct Fill {
       const v2i x = *reinterpret_cast<const v2i*>(kp);
       k[0] = x[0], k[1] = x[1];
     }
-    const uint8_t* sp = group + (uint32_t)pinned(key_scale_at);
-#pragma unroll
-    for (int i = 0; i < (T::kKeyUnits + 3) / 4; ++i) ks[i] = sp[i];
+    // (a word and not the bytes: bytes carried to the next step are masked where they are loaded, with a
+    // wait for all that is in flight)
+    ks = *reinterpret_cast<const uint32_t*>(group + (uint32_t)pinned(key_scale_at));
   }
   // (lanes without values read those of group byte 0 on: they are not used)
   __device__ __forceinline__ void load_values(const uint8_t* group) {
@@ -183,7 +189,7 @@ struct Fill {
     if constexpr (I < T::kKeyUnits) {
       // units I and I + 1 are the two halves of an instruction's channels
       uint8_t* to = reinterpret_cast<uint8_t*>(&sh.k[kbuf][0][0][0]) + pinned(key_to);
-      const v4i y = __builtin_bit_cast(v4i, expand8(k[I], scale_of(ks[I / 4])));
+      const v4i y = __builtin_bit_cast(v4i, expand8(k[I], scale_of((ks >> (ks_bit + 8 * (I / 4))) & 0xFFu)));
       *reinterpret_cast<v4i*>(to + (I >> 1) * 1024 + (I & 1) * 512) = y;
     } else if constexpr (I == T::kKeyUnits) {
 #pragma unroll
@@ -217,19 +223,21 @@ struct Fill {
   }
 };
 
-// The x-th tile from the end of the batch's: a sequence of more rows than attn_rows takes has as many as
-// its rows fill, a bad one has one.
+// Row tiles of sequence i: as many as its rows fill where it has more than attn_rows takes; a bad one has
+// one, which writes its NaN.
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, int tile_rows, int i) {
+  if (i >= a.batch) return 0;
+  const Sequence s = sequence(a, i);
+  const int R = s.bad ? 0 : s.n * a.group;
+  return s.bad ? 1 : R > a.few_rows ? ceil_div(R, tile_rows) : 0;
+}
+
+// The x-th row tile from the end of the batch's.
 struct Place { int b, tile; };
 __device__ __forceinline__ Place find_tile(const AttnArgs& a, int tile_rows, int x, int lane) {
   int left = x;
   for (int i0 = (a.batch - 1) & ~63; i0 >= 0; i0 -= 64) {
-    const int i = i0 + 63 - lane;          // lanes in descending order of the sequences
-    int n = 0;
-    if (i < a.batch) {
-      const Sequence s = sequence(a, i);
-      const int R = s.n * a.group;
-      n = s.bad ? 1 : R > a.few_rows ? ceil_div(R, tile_rows) : 0;
-    }
+    const int n = tiles_of(a, tile_rows, i0 + 63 - lane);   // lanes in descending order
     const int upto = wave_scan(n);
     const uint64_t here = __ballot(left >= upto - n && left < upto);
     if (here) {
@@ -241,6 +249,25 @@ __device__ __forceinline__ Place find_tile(const AttnArgs& a, int tile_rows, int
   return {-1, 0};
 }
 
+// What workgroup x does: one of `parts` parts of the tokens of unit `unit` (row tile and kv head), whose
+// partial results are those of entry `entry`. Units that fill whole rounds of the CUs are done by a
+// workgroup each; those of the last round, which would leave CUs idle, in parts.
+struct Work { int unit, part, parts, entry; };
+__device__ __forceinline__ Work find_work(const AttnArgs& a, int tile_rows, int x, int lane) {
+  if (!a.entries) return {x, 0, 1, 0};
+  int tiles = 0;
+  for (int i0 = 0; i0 < a.batch; i0 += 64)
+    tiles += __builtin_amdgcn_readlane(wave_scan(tiles_of(a, tile_rows, i0 + lane)), 63);
+  const int units = tiles * a.Hkv, rest = units % kCUs, first = units - rest;
+  const int parts = attn_parts(rest, a.span, a.entries);
+  // (attn_join looks at the entries that there may be)
+  if (x < a.entries && x < kCUs && x >= rest && threadIdx.x == 0) meta(a, tile_rows, a.d, x)[0] = 0;
+  if (x < first) return {x, 0, 1, -1};
+  const int y = x - first, part = rest ? y / rest : parts;
+  if (part >= parts) return {units, 0, 1, -1};
+  return {first + y - part * rest, part, parts, y - part * rest};
+}
+
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
   using T = Tiles<D, W>;
@@ -250,15 +277,20 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // Workgroups [tiles of the batch, the last first][kv heads]. The tiles that the batch has come first, so
-  // that the workgroups without one are the grid's last and the others spread over all dies; a
-  // sequence's last tiles, which see most tokens, begin first; and where the kv heads are a multiple of
-  // 8 a head's keys and values stay in one die's L2.
-  const int x = a.by_heads(blockIdx.x), h = blockIdx.x - x * a.Hkv;
+  // Units [tiles of the batch, the last first][kv heads]. A sequence's last tiles, which see most tokens,
+  // begin first; and where the kv heads are a multiple of 8 a head's keys and values stay in one
+  // die's L2.
+  const Work work = find_work(a, T::kRows, blockIdx.x, lane);
+  const int x = a.by_heads(work.unit), h = work.unit - x * a.Hkv;
   const Place at = find_tile(a, T::kRows, x, lane);
   if (at.b < 0) return;
   const int b = at.b, tile = at.tile;
   const Sequence s = sequence_uniform(a, b);
+  if (a.entries && work.entry >= 0 && work.part == 0 && tid == 0) {
+    int* mt = meta(a, T::kRows, D, work.entry);
+    mt[0] = s.bad ? 0 : work.parts - 1;
+    mt[1] = b, mt[2] = tile * a.Hkv + h, mt[3] = work.entry * work.parts;
+  }
   if (s.bad) {
     nan_rows<D>(a, s, h * a.group, a.group);
     return;
@@ -287,7 +319,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
   const int* table = a.pages_of + (size_t)b * a.table_stride;
   const uint8_t* head_base = a.cache + (size_t)(h << (a.page_shift - 4)) * G::kBytes;
   const int group_mask = (1 << (a.page_shift - 4)) - 1;
-  const int t0 = all.lo, t1 = all.hi, last_page = (t1 - 1) >> a.page_shift;
+  // this workgroup's part of the tokens, in steps
+  const int share = ceil_div(ceil_div(max(all.hi - all.lo, 0), kTile), work.parts) * kTile;
+  const int t0 = all.lo + work.part * share, t1 = min(all.hi, t0 + share);
+  const int last_page = (t1 - 1) >> a.page_shift;
   bool bad = false;
   // The numbers of 128 pages from page_base on, a lane each of two registers: a step's is read from them
   // without a wait. (A scalar load would share its counter with the LDS reads and stall them.)
@@ -343,8 +378,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
     } else {
       keys_from = g1;
     }
-    fill.load_values(g1);
     fill.load_keys(keys_from);
+    fill.load_values(g1);
     lds_barrier();
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc[0][j] = 0.0f;
@@ -352,6 +387,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
     for (int k = 0; k < KS; ++k)
       sc[0] = mfma32(__builtin_bit_cast(v8bf, sh.k[0][0][k][lane]), q[k], sc[0]);
   }
+  // The queries are here: without this the compiler waits for them inside the loop, each step, and with
+  // them for the loads just asked for.
+  __builtin_amdgcn_s_waitcnt(0x0F70);     // vmcnt(0)
   int buf = 0;                            // of step t; buf ^ 1 of step t + 1
   for (int t = t0; t < t1; t += kTile, buf ^= 1) {
     // all have written what this step reads, and read what it overwrites
@@ -428,9 +466,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
             sh, grp < 2 ? buf : buf ^ 1, buf ^ 1);
       });
     });
-    fill.load_values(grp < 2 ? keys_from : group_at(t + 2 * kTile));
+    const uint8_t* values_from = grp < 2 ? keys_from : group_at(t + 2 * kTile);
     keys_from = group_at(t + (key_ahead + 1) * kTile);
-    fill.load_keys(keys_from);
+    fill.load_keys(keys_from);             // needed first
+    fill.load_values(values_from);
     if (nan_here) {
       // Rows that see a token with a NaN block: its 32 channels are NaN. 2^127 for the block times
       // 2^127 for the row that sees it is infinite; the same once more with the other sign is NaN.
@@ -473,20 +512,31 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float y[4] = {o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
-      store_row<4>(out + 32 * i + 8 * g + 4 * half, y, sum);
+      const int ch = 32 * i + 8 * g + 4 * half;
+      if (work.parts == 1)
+        store_row<4>(out + ch, y, sum);
+      else
+        store_part<4>(a, T::kRows, D, work.entry * work.parts + work.part, row - r0, ch, y, m * c, sum);
     }
 }
 
 template <int D, int W>
 hipError_t launch(AttnArgs a, hipStream_t stream) {
+  constexpr int kRows = Tiles<D, W>::kRows;
   a.by_group = divisor(a.group), a.by_heads = divisor(a.Hkv);
-  a.tiles = ceil_div(a.max_q * a.group, Tiles<D, W>::kRows);
-  attn_tiles<D, W><<<a.tiles * a.batch * a.Hkv, 64 * W, 0, stream>>>(a);
-  return hipGetLastError();
+  a.d = D, a.runs = (a.entries + 1) / 2;
+  const int units = ceil_div(a.max_q * a.group, kRows) * a.batch * a.Hkv;
+  attn_tiles<D, W><<<units + a.entries, 64 * W, 0, stream>>>(a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (!a.entries) return hipSuccess;
+  a.by_parts = true;
+  const int entries = a.entries < kCUs ? a.entries : kCUs - 1;
+  return launch_attn_join(a, D, kRows, entries < units ? entries : units, stream);
 }
 
 }  // namespace
 
+int attn_tile_rows(int d) { return d == 256 ? Tiles<256, 4>::kRows : Tiles<128, 8>::kRows; }
 
 hipError_t launch_attn_tiles(const AttnArgs& a, int d, hipStream_t stream) {
   return d == 64 ? launch<64, 8>(a, stream)

@@ -155,12 +155,37 @@ struct AttnArgs {
   // and whether attn_join goes by units (there are no more of them than runs) or by runs
   int tiles, units;
   bool by_unit;
+  // attn_tiles: partial results that the workspace holds (0: no unit is done in parts), tokens that a
+  // row tile sees at most; the head size; and, for attn_join, that partial results lie by entry and part
+  int entries, span, d;
+  bool by_parts;
   Divisor by_group, by_heads, by_runs;   // of Hq / Hkv, Hkv, runs
 };
-// What serves a call (attn_tiles, attn_rows or both), and the workspace that takes.
-struct AttnPlan { bool tiles, rows; int fragments, runs, few_rows; size_t workspace; };
+constexpr int kCUs = 256;
+
+// Into how many parts of their tokens the `rest` < 256 units of attn_tiles' last round are cut, at most
+// `entries` in all. Counted in the time of a unit's token: the parts' rounds, with 140 for a
+// workgroup's start and end, and 2 for each partial result's way through memory.
+__host__ __device__ inline int attn_parts(int rest, int span, int entries) {
+  int best = 1, least = span + 140;
+#pragma unroll
+  for (int s = 2; s <= 16; ++s) {       // (unrolled, the divisions are multiplications)
+    const int cost = (rest * s + kCUs - 1) / kCUs * (span / s + 140) + 2 * rest * s;
+    if (rest * s <= entries && cost < least) least = cost, best = s;
+  }
+  return best;
+}
+
+// What serves a call (attn_tiles, attn_rows or both), and the workspace that takes: attn_tiles' first.
+struct AttnPlan {
+  bool tiles, rows;
+  int fragments, runs, few_rows, entries, span;
+  size_t tiles_workspace, workspace;
+};
 AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window);
+int attn_tile_rows(int d);          // rows of a workgroup of attn_tiles
 hipError_t launch_attn_rows(const AttnArgs& a, int d, hipStream_t stream);
 hipError_t launch_attn_tiles(const AttnArgs& a, int d, hipStream_t stream);
+hipError_t launch_attn_join(const AttnArgs& a, int d, int tile_rows, int entries, hipStream_t stream);
 
 }  // namespace kv4
