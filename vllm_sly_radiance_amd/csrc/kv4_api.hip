@@ -119,9 +119,10 @@ int attn_sizes(const char* who, int batch, int max_q, int max_len, int q_heads, 
   if ((long)batch * q_heads * max_q > 0x7FFFFFFFL)
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d q_heads=%d are too many rows", who, batch, max_q,
                 q_heads);
-  // work is counted in granules of 128 tokens (fewer rows a tile make more of them)
-  if (((long)batch * kv_heads * (((long)max_q * (q_heads / kv_heads) + 15) / 16)) *
-          ((max_len + 127L) / 128) > (1L << 30))
+  // attn_rows counts work in granules of 128 tokens of a row tile, and two for its start, in 31 bits
+  const long rows = (long)max_q * (q_heads / kv_heads);
+  const long tile = rows <= 16 ? 16 : rows <= 32 || d == 256 ? 32 : 64;
+  if ((long)batch * kv_heads * ((rows + tile - 1) / tile) * ((max_len + 127L) / 128) > (1L << 29))
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d max_len=%d are too much for one call", who, batch,
                 max_q, max_len);
   return KV4_OK;

@@ -15,14 +15,18 @@
 // lanes and no rescaling; what is above 1 costs no precision in fp32 and bf16. Waves meet in LDS.
 //
 // The work of a batch is the tokens of all its units (sequence, row tile, kv head), in granules of
-// 32 W. As many workgroups as the card holds at once take an equal run of granules each, found from
-// the lengths on the device: one round, no tail, whatever the lengths are, and a graph captured with
-// a batch's limits balances every replay. A unit inside one run is finished there; one that crosses
-// runs leaves partial results, at most two a workgroup, for a second launch to weigh. Short
-// contexts take a workgroup a unit and no second launch.
+// 32 W, and a little for each unit's start. As many workgroups as the card holds at once take an equal
+// run of it each, found from the lengths on the device: one round, no tail, whatever the lengths are,
+// and a graph captured with a batch's limits balances every replay. A unit inside one run is finished
+// there; one that crosses runs leaves partial results, at most two a workgroup, for a second launch to
+// weigh. Short contexts take a workgroup a unit and no second launch.
 //
-// Bounded by HBM where the cache is long; by the launches and three dependent reads (length, page,
-// tokens) where it is short.
+// Bounded by HBM where the cache is long and rows are few: 48 sequences of up to 8000 tokens, 32 query
+// and 8 kv heads of 128, 208 MB: 44 us, 4.7 TB/s (6.05 is what plain reads reach); one sequence of
+// 131072 tokens, 143 MB: 30 us. By the vector units with 16 to 64 rows (the codes' conversion is the
+// same for every row, the weights are not): 8 x 8 queries of 48 + 16 heads against up to 4000 tokens,
+// 49 MB: 20 us. By the launches and three dependent reads (length, page, tokens) where it is short: 500
+// tokens 7.5 us. The join behind it takes 3 to 6.
 #include "kv4_attn.h"
 #include "kv4_attn_shared.h"
 
@@ -75,6 +79,12 @@ __device__ __forceinline__ void load_values(Raw<D>& w, const uint8_t* group, uin
   }
 }
 
+// What a unit costs besides its granules (its queries, the first reads of its pages and tokens, the
+// waves' shares, what is written), in granules: 4.5 us against 1.1 to 2.2 a granule. Without it a run of
+// several short units was the last to end: 30 sequences of up to 8000 tokens, 4 kv heads of 256: 37.6
+// us, 32.4 with it; 8 times 8 queries against up to 4000 tokens: 22.0 and 20.0.
+constexpr int kStart = 2;
+
 // Granules of a sequence's units: each of tiles x kv heads units has as many as its visible tokens
 // take, one at least (a unit of no tokens writes its zeros, a bad sequence its NaN).
 struct Units { int per_unit, units, lo; };
@@ -87,32 +97,42 @@ __device__ __forceinline__ Units units_of(const AttnArgs& a, const Sequence& s, 
   return {x.hi > x.lo ? ceil_div(x.hi - x.lo, kGranule) : 1, ceil_div(R, tile_rows) * a.Hkv, x.lo};
 }
 
-// A run of granules of the batch: its first sequence, the granule of that sequence's work, and how
-// many. Every wave finds it by itself, 64 sequences at a time: no exchange between waves.
-struct Run { Sequence s; int b; uint32_t off, left, share; };
+// A run of the batch's work, which is for each unit `start` and its granules: the run's first sequence,
+// where in that sequence's work it begins, how much it is, and the runs' size. start is kStart, or 0
+// where every unit is a whole number of runs and none begins inside one. Every wave finds its run by
+// itself, 64 sequences at a time: no exchange between waves.
+struct Run { Sequence s; int b, start; uint32_t off, left, share; };
 template <int kGranule>
 __device__ __forceinline__ Run find_run(const AttnArgs& a, int tile_rows, int lane) {
-  auto work = [&](int i, Sequence& s) {
-    s = {0, 0, 0, false};
-    if (i >= a.batch) return 0u;
+  Run run = {{0, 0, 0, false}, 0, 0, 0, 0, 0};
+  Sequence s = {0, 0, 0, false};
+  Units x = {1, 0, 0};
+  auto look = [&](int i) {
+    s = {0, 0, 0, false}, x = {1, 0, 0};
+    if (i >= a.batch) return;
     s = sequence(a, i);
-    const Units x = units_of<kGranule>(a, s, tile_rows);
-    return (uint32_t)x.per_unit * (uint32_t)x.units;
+    x = units_of<kGranule>(a, s, tile_rows);
   };
-  Run run = {{0, 0, 0, false}, 0, 0, 0, 0};
-  Sequence s;
-  uint32_t w = work(lane, s), upto = wave_scan(w);
-  uint32_t total = __builtin_amdgcn_readlane(upto, 63);
-  for (int i0 = 64; i0 < a.batch; i0 += 64) {
-    Sequence other;
-    total += __builtin_amdgcn_readlane(wave_scan(work(i0 + lane, other)), 63);
+  auto sum = [](uint32_t n) { return (uint32_t)__builtin_amdgcn_readlane(wave_scan(n), 63); };
+  uint32_t granules = 0, units = 0;
+  for (int i0 = (a.batch - 1) & ~63; i0 >= 0; i0 -= 64) {
+    look(i0 + lane);
+    granules += sum((uint32_t)x.per_unit * (uint32_t)x.units), units += sum(x.units);
   }
-  run.share = a.by_runs(total + a.runs - 1);
-  const uint32_t at = run.share * blockIdx.x;
+  run.share = a.by_runs(granules + a.runs - 1);
+  bool crosses = false;
+  for (int i0 = (a.batch - 1) & ~63; i0 >= 0 && !crosses; i0 -= 64) {
+    if (a.batch > 64) look(i0 + lane);
+    crosses = __ballot(x.units && run.share && x.per_unit % run.share) != 0;
+  }
+  if (crosses) run.start = kStart, run.share = a.by_runs(granules + kStart * units + a.runs - 1);
+  const uint32_t total = granules + run.start * units, at = run.share * blockIdx.x;
   if (at >= total) return run;           // no work left for this workgroup
   run.left = min(run.share, total - at);
   uint32_t before = 0;
-  for (int i0 = 0; i0 < a.batch;) {
+  for (int i0 = 0; i0 < a.batch; i0 += 64) {
+    if (a.batch > 64) look(i0 + lane);
+    const uint32_t w = (uint32_t)(x.per_unit + run.start) * (uint32_t)x.units, upto = wave_scan(w);
     const uint32_t lo = before + upto - w;
     const uint64_t here = __ballot(at >= lo && at - lo < w);
     if (here) {
@@ -126,8 +146,6 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, int tile_rows, int la
       return run;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
-    i0 += 64;
-    w = work(i0 + lane, s), upto = wave_scan(w);
   }
   run.left = 0;
   return run;
@@ -151,7 +169,7 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group_heads = a.group;
 
-  Run run = {{0, 0, 0, false}, 0, 0, 0, 0};
+  Run run = {{0, 0, 0, false}, 0, 0, 0, 0, 0};
   if (a.tiles) {
     // short contexts: one unit, workgroups [batch][tiles][kv heads]
     const uint32_t per = a.tiles * a.Hkv;
@@ -169,12 +187,13 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
 
   const float c = a.scale * 1.44269504088896340736f;
   const float slack = 8.0f / c;
-  int unit = 0, gu = 0;       // unit of the sequence and granule of the unit that the run stands at
+  const int start = run.start;
+  int unit = 0, at = 0;       // the unit of the sequence and the place in its work that the run stands at
   {
-    const Units un = units_of<kGranule>(a, run.s, kTile);
+    const int work = units_of<kGranule>(a, run.s, kTile).per_unit + start;
     if (run.off) {
-      unit = __builtin_amdgcn_readfirstlane(run.off / (uint32_t)un.per_unit);
-      gu = run.off - unit * un.per_unit;
+      unit = __builtin_amdgcn_readfirstlane(run.off / (uint32_t)work);
+      at = run.off - unit * work;
     }
   }
   while (true) {
@@ -187,12 +206,16 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
       run.s = sequence_uniform(a, run.b);
       continue;
     }
-    const int take = min((uint32_t)(un.per_unit - gu), run.left);
+    const int rest = un.per_unit + start - at, part = min((uint32_t)rest, run.left), this_unit = unit;
+    const int first_granule = max(at - start, 0), take = max(at + part - start, 0) - first_granule;
     const int tile = a.by_heads(unit), h = unit - tile * a.Hkv;
     const bool whole = take == un.per_unit;
-    const int first_granule = gu, this_unit = unit;
-    run.left -= take, gu += take;
-    if (gu == un.per_unit) ++unit, gu = 0;
+    run.left -= part, at += part;
+    if (part == rest) ++unit, at = 0;
+    if (take == 0) {          // the run ends within a unit's start: the next one begins it
+      if (!run.left) return;
+      continue;
+    }
     if (s.bad) {
       nan_rows<D>(a, s, h * group_heads, group_heads);
       if (!run.left) return;
@@ -451,7 +474,7 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
     if (a.runs && first_granule == 0 && tid == 0 && (a.by_unit || !whole)) {
       // what attn_join is told of a unit: how many workgroups after this one finish it
       int* mt = meta(a, kTile, D, a.by_unit ? b * a.units + this_unit : blockIdx.x);
-      mt[0] = (int)((un.per_unit - take + run.share - 1) / run.share);
+      mt[0] = (int)((rest - part + run.share - 1) / run.share);
       mt[1] = b, mt[2] = this_unit, mt[3] = blockIdx.x;
     }
     if (!run.left) return;
