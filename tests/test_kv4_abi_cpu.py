@@ -224,8 +224,12 @@ def test_what_serves_a_call(lib):
     last round's in parts; sequences of few rows beside them, both."""
     few = lambda runs, rows, d: runs * (2 * rows * (d + 2) * 4 + 16)  # noqa: E731
     many = lambda parts, rows, d: parts * rows * (d + 2) * 4 + 4096  # noqa: E731
-    assert workspace(lib, 1, 1, 1, 512, 32, 8, 128, 0) == 0
-    assert workspace(lib, 1, 1, 1, 513, 32, 8, 128, 0) == few(8 * 5, 16, 128)
+    assert workspace(lib, 1, 1, 1, 1024, 32, 8, 128, 0) == 0
+    assert workspace(lib, 1, 1, 1, 1025, 32, 8, 128, 0) == few(8 * 9, 16, 128)
+    assert workspace(lib, 16, 16, 1, 2048, 32, 8, 128, 0) == 0            # 128 units of 8 steps
+    assert workspace(lib, 15, 15, 1, 2048, 32, 8, 128, 0) == few(1024, 16, 128)
+    assert workspace(lib, 99, 99, 1, 4097, 32, 8, 128, 0) == few(1024, 16, 128)
+    assert workspace(lib, 99, 99, 1, 9999, 32, 8, 128, 1000) == 0         # what a window leaves
     assert workspace(lib, 0, 1, 0, 4096, 32, 8, 128, 0) == 0
     assert workspace(lib, 399, 1, 399, 4096, 32, 8, 128, 0) == few(512, 64, 128)
     assert workspace(lib, 400, 1, 400, 4096, 32, 8, 128, 0) == many(56 * 4, 256, 128)

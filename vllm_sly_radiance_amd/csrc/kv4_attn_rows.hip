@@ -19,7 +19,7 @@
 // run of it each, found from the lengths on the device: one round, no tail, whatever the lengths are,
 // and a graph captured with a batch's limits balances every replay. A unit inside one run is finished
 // there; one that crosses runs leaves partial results, at most two a workgroup, for a second launch to
-// weigh. Short contexts take a workgroup a unit and no second launch.
+// weigh. Short contexts, and many units of middling ones, take a workgroup a unit and no second launch.
 //
 // Bounded by HBM where the cache is long and rows are few: 48 sequences of up to 8000 tokens, 32 query
 // and 8 kv heads of 128, 208 MB: 44 us, 4.7 TB/s (6.05 is what plain reads reach); one sequence of
@@ -659,8 +659,16 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   p.fragments = fragments(few);
   const int tile = 16 * p.fragments;
   const long units = (long)batch * Hkv * ((few + tile - 1) / tile);
-  // Two steps a wave: a workgroup a unit, and no second launch.
-  if (span <= 2L * kStep * attn_whole_waves(p.fragments)) return p;
+  // A workgroup a unit, and no second launch, where its waves have few steps to go, or the units are many
+  // and of like length enough. Equal lengths L, such workgroups and runs with the join, us (d = 128,
+  // 32 query and 8 kv heads unless said):
+  //   L = 1000, 1 sequence  10.4  11.8    L = 2000, 1    14.4  11.5    L = 3000, 32     25.0  29.7
+  //                    16   11.1  17.6              4    14.6  13.2             100     70.6  75.5
+  //                    64   17.5  24.0             16    15.3  18.9    L = 6000, 16     32.8  31.8
+  //   8 queries (32 rows)                         200    88.2  98.7    200 .. 6000, 48  47.3  45.7
+  //   L = 800, 8 sequences  13.0  20.0    8 x 3 rows, 16 kv heads, L = 2000: 20.2  22.0, L = 3000: 25.2  24.9
+  const long waves_step = kStep * attn_whole_waves(p.fragments), steps = (span + waves_step - 1) / waves_step;
+  if (steps <= 4 || (span <= (p.fragments == 1 ? 4096 : 2048) && units >= 16 * steps)) return p;
   // as many workgroups as the card's 256 CUs hold at once, or a granule each
   const long granules = (span + kStep * kRunWaves - 1) / (kStep * kRunWaves);
   const long most = 256L * 4 * attn_waves(d, p.fragments) / kRunWaves;
