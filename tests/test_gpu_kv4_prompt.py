@@ -62,6 +62,19 @@ def test_chunks_beside_decoding_sequences(d, Hq, Hkv, qs):
         assert not out[at:at + 10].any() and out[at + 10].any()
 
 
+@pytest.mark.parametrize("d,Hq,Hkv,qs", [(64, 32, 8, [350, 8, 7, 9, 8, 16, 17, 1]),
+                                         (128, 32, 8, [8, 9, 7, 350, 8, 16, 17, 0]),
+                                         (128, 32, 4, [5, 400, 4, 1, 2, 4, 5, 3]),
+                                         (256, 24, 4, [4, 300, 5, 6, 3, 4])])
+def test_chunk_beside_drafts(d, Hq, Hkv, qs):
+    """Sequences of a few queries each beside a chunk: up to what the others have on average, and beyond."""
+    rng = np.random.default_rng(50)
+    lens = [n + int(rng.integers(0, 500)) for n in qs]
+    b = Batch(rng, lens, qs, Hq, Hkv, d, 16)
+    b.check(run(b))
+    b.check(run(b, window=150), window=150)
+
+
 def test_more_sequences_than_lanes():
     """The tiles of a batch are found 64 sequences at a time."""
     rng = np.random.default_rng(3)
@@ -244,3 +257,23 @@ def test_same_bits_every_time_and_on_another_stream():
     s.synchronize()
     for out in outs:
         assert np.array_equal(host_u16(out), want)
+
+
+def test_one_chunk_among_many_decoding_and_bad_sequences():
+    """Far fewer row tiles than the longest chunk's times the batch, and bad sequences among them."""
+    rng = np.random.default_rng(40)
+    qs = [1] * 70
+    qs[33] = 600
+    lens = [int(n) for n in rng.integers(1, 90, 70)]
+    lens[33] = 650
+    b = Batch(rng, lens, qs, 32, 2, 64, 16)
+    b.check(run(b))
+    q, cache, table, dl, starts, mq, ml = b.device()
+    bad = (0, 7, 32, 34, 69)
+    for i in bad:
+        dl[i] = ml + 1 + i
+    out = K.attention(q, cache, table, dl, starts, mq, ml)
+    got = O.bf16_to_f32(host_u16(out))
+    for i in bad:
+        assert np.isnan(got[b.starts[i]:b.starts[i + 1]]).all()
+    b.check(out, only=set(range(70)) - set(bad))

@@ -254,7 +254,7 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   a.causal = flags & KV4_CAUSAL;
   a.few_rows = plan.few_rows;
   if (plan.tiles) {
-    a.entries = plan.entries, a.span = plan.span;
+    a.units = plan.units, a.entries = plan.entries, a.span = plan.span;
     if (int rc = hip_status(launch_attn_tiles(a, d, (hipStream_t)stream), who)) return rc;
     a.entries = 0, a.part += plan.tiles_workspace / sizeof(float);
   }

@@ -632,14 +632,24 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   //   1 x 1024          512        85  96   and 32 and 32 heads of 64:
   //   1 x 4096         2048       153 300                                   1 x 600  320        55  54
   //   16 x 33 (132 rows) 384       79  86
+  // Decoding sequences beside a chunk in attn_rows are read with the chunk's 64 rows: with 100 MB of cache
+  // and more that costs more than the two launches of attn_rows beside attn_tiles do: one chunk and 47
+  // sequences of 4000 tokens, d = 128, 64 queries: 74 and 89, 256: 79 and 92; 100 queries and 7
+  // sequences of 3000: 37 and 26.
   const long rows_tile = d == 256 ? 32 : 64;
-  if (rows > 2 * rows_tile && (long)total * Hq >= 200 * rows_tile) {
+  // all sequences have max_q queries
+  const bool even = total == (long)batch * max_q;
+  // Row tiles of the batch at most: a sequence (or bad one) has one that is not full.
+  auto tiles_of_batch = [&](long tile) {
+    const long each = batch * ((rows + tile - 1) / tile), all = (long)total * group / tile + batch;
+    return even || each < all ? each : all;
+  };
+  if (rows > 2 * rows_tile && ((long)total * Hq >= 200 * rows_tile || (!even && (long)batch * span * Hkv * d >= 100000000))) {
     p.tiles = true;
-    // The last round of row tiles is done in parts: into how many is known here where all sequences have
-    // max_q queries.
-    const bool even = total == (long)batch * max_q;
-    const long tile_rows = attn_tile_rows(d), units = (rows + tile_rows - 1) / tile_rows * batch * Hkv;
+    const long tile_rows = attn_tile_rows(d), units = tiles_of_batch(tile_rows) * Hkv;
+    p.units = (int)units;
     p.span = span;
+    // The last round of row tiles is done in parts: into how many is known here where the batch is even.
     if (even) {
       const int rest = (int)(units % kCUs), parts = attn_parts(rest, span, kMostEntries);
       p.entries = parts > 1 ? rest * parts : 0;
@@ -649,16 +659,21 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
     if (p.entries)
       p.tiles_workspace = p.workspace =
           (size_t)(p.entries + 1) / 2 * 2 * tile_rows * (d + 2) * sizeof(float) + kCUs * 16;
-    // Sequences of fewer queries beside: those of one query are attn_rows'.
+    // Sequences of fewer queries beside: those of one query are attn_rows', and those of as many as the
+    // others have beside the longest on average, where they fit (40 sequences of 8 queries and 3000 tokens
+    // beside a chunk of 300, d = 128: 81 us, 150 in attn_tiles).
     if (even) return p;
-    const int fit = group <= 16 ? 16 : group <= 32 || d == 256 ? 32 : 64;
+    const long others = batch > 1 ? ((long)total - max_q + batch - 2) / (batch - 1) * group : 0;
+    const long want = others <= rows_tile && others > group ? others : group;
+    const int fit = want <= 16 ? 16 : want <= 32 || d == 256 ? 32 : 64;
     if (group > fit) return p;
     few = p.few_rows = fit;
   }
   p.rows = true;
   p.fragments = fragments(few);
   const int tile = 16 * p.fragments;
-  const long units = (long)batch * Hkv * ((few + tile - 1) / tile);
+  const long most_units = (long)batch * Hkv * ((few + tile - 1) / tile);
+  const long units = p.few_rows ? most_units : tiles_of_batch(tile) * Hkv;
   // A workgroup a unit, and no second launch, where its waves have few steps to go, or the units are many
   // and of like length enough. Equal lengths L, such workgroups and runs with the join, us (d = 128,
   // 32 query and 8 kv heads unless said):
@@ -668,7 +683,9 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   //   8 queries (32 rows)                         200    88.2  98.7    200 .. 6000, 48  47.3  45.7
   //   L = 800, 8 sequences  13.0  20.0    8 x 3 rows, 16 kv heads, L = 2000: 20.2  22.0, L = 3000: 25.2  24.9
   const long waves_step = kStep * attn_whole_waves(p.fragments), steps = (span + waves_step - 1) / waves_step;
-  if (steps <= 4 || (span <= (p.fragments == 1 ? 4096 : 2048) && units >= 16 * steps)) return p;
+  // (not where most of those workgroups would have nothing to do)
+  if (most_units <= 2 * units && (steps <= 4 || (span <= (p.fragments == 1 ? 4096 : 2048) && units >= 16 * steps)))
+    return p;
   // as many workgroups as the card's 256 CUs hold at once, or a granule each
   const long granules = (span + kStep * kRunWaves - 1) / (kStep * kRunWaves);
   const long most = 256L * 4 * attn_waves(d, p.fragments) / kRunWaves;

@@ -525,13 +525,12 @@ hipError_t launch(AttnArgs a, hipStream_t stream) {
   constexpr int kRows = Tiles<D, W>::kRows;
   a.by_group = divisor(a.group), a.by_heads = divisor(a.Hkv);
   a.d = D, a.runs = (a.entries + 1) / 2;
-  const int units = ceil_div(a.max_q * a.group, kRows) * a.batch * a.Hkv;
-  attn_tiles<D, W><<<units + a.entries, 64 * W, 0, stream>>>(a);
+  attn_tiles<D, W><<<a.units + a.entries, 64 * W, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (!a.entries) return hipSuccess;
   a.by_parts = true;
   const int entries = a.entries < kCUs ? a.entries : kCUs - 1;
-  return launch_attn_join(a, D, kRows, entries < units ? entries : units, stream);
+  return launch_attn_join(a, D, kRows, entries < a.units ? entries : a.units, stream);
 }
 
 }  // namespace

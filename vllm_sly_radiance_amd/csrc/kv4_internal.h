@@ -151,8 +151,9 @@ struct AttnArgs {
   int runs;               // workgroups that share the batch's tokens; 0: one a unit
   int few_rows;           // attn_rows has the sequences of at most so many rows, attn_tiles the
                           // others; 0: one of them has all
-  // set at the launch: row tiles of a sequence at most, where runs is 0; units of a sequence at most,
-  // and whether attn_join goes by units (there are no more of them than runs) or by runs
+  // set at the launch: row tiles of a sequence at most, where runs is 0; units of a sequence at most
+  // (attn_tiles: of the batch, from the plan), and whether attn_join goes by units (there are no more of
+  // them than runs) or by runs
   int tiles, units;
   bool by_unit;
   // attn_tiles: partial results that the workspace holds (0: no unit is done in parts), tokens that a
@@ -179,7 +180,8 @@ __host__ __device__ inline int attn_parts(int rest, int span, int entries) {
 // What serves a call (attn_tiles, attn_rows or both), and the workspace that takes: attn_tiles' first.
 struct AttnPlan {
   bool tiles, rows;
-  int fragments, runs, few_rows, entries, span;
+  int fragments, runs, few_rows;
+  int units, entries, span;             // of attn_tiles; units: at most
   size_t tiles_workspace, workspace;
 };
 AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window);
