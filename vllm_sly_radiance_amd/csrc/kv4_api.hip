@@ -200,7 +200,7 @@ KV4_API int kv4_gather(const void* cache, long pages, long page_stride, int page
   if (!slots || !aligned(slots, 8)) return fail(KV4_EINVAL, "%s: null or misaligned slots", who);
   if (!k || !v || !aligned(k, 16) || !aligned(v, 16))
     return fail(KV4_EINVAL, "%s: null or misaligned output", who);
-  if ((long)T * heads * (d / 8) / 256 > kMaxGrid)
+  if ((long)T * heads > 0x7FFFFFFFL || (long)T * heads * (d / 8) / 256 > kMaxGrid)
     return fail(KV4_EINVAL, "%s: T=%d is too large", who, T);
   GatherArgs a = {(const uint8_t*)cache, slots, (uint16_t*)k, (uint16_t*)v, pages, page_stride,
                   page_shift(page), T, heads};

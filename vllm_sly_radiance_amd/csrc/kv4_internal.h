@@ -72,6 +72,24 @@ __device__ __forceinline__ uint32_t codes8(const float y[8], uint32_t e) {
   return r;
 }
 
+// Division of 0 <= n < 2^31 by a divisor that the host knows: a multiplication by m =
+// floor(2^(31 + s) / d) + 1, s = ceil(log2 d), whose error m d - 2^(31 + s) <= d <= 2^s stays below
+// what moves a quotient. The integer division in its place is some 40 dependent instructions, and
+// several stood before a workgroup's first loads.
+struct Divisor {
+  int d;
+  uint32_t m;
+  int shift;              // s - 1
+  __device__ __forceinline__ int operator()(int n) const {
+    return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> shift);
+  }
+};
+inline Divisor divisor(int d) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  return {d, d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)d + 1), s - 1};
+}
+
 // ---- arguments of the launchers -----------------------------------------------------------------
 struct Heads {            // bf16 [T][heads][d] with unit channel stride
   const uint16_t* p;
@@ -101,7 +119,8 @@ struct GatherArgs {
   uint16_t* k;
   uint16_t* v;
   long pages, page_stride;
-  int page_shift, T, H;
+  int page_shift, T, H;   // T * H < 2^31
+  Divisor by_heads;       // of H, set at the launch
 };
 hipError_t launch_gather(const GatherArgs& a, int d, hipStream_t stream);
 
@@ -116,24 +135,6 @@ struct MoveArgs {
 };
 // pairs: n <= kMovePairs of them (src, dst), sorted by src
 hipError_t launch_move(const MoveArgs& a, const int* pairs, int n, hipStream_t stream);
-
-// Division of 0 <= n < 2^31 by a divisor that the host knows: a multiplication by m =
-// floor(2^(31 + s) / d) + 1, s = ceil(log2 d), whose error m d - 2^(31 + s) <= d <= 2^s stays below
-// what moves a quotient. The integer division in its place is some 40 dependent instructions, and
-// several stood before a workgroup's first loads.
-struct Divisor {
-  int d;
-  uint32_t m;
-  int shift;              // s - 1
-  __device__ __forceinline__ int operator()(int n) const {
-    return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> shift);
-  }
-};
-inline Divisor divisor(int d) {
-  int s = 0;
-  while (((int64_t)1 << s) < d) ++s;
-  return {d, d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)d + 1), s - 1};
-}
 
 struct AttnArgs {
   const uint16_t* q;
