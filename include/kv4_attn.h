@@ -106,8 +106,9 @@ int kv4_gather(const void* cache, long pages, long page_stride, int page, const 
  * KV4_CAUSAL j <= p, and with window > 0 j > p - window. A query that sees nothing gives zeros.
  * What a masked token holds, NaN included, has no effect. page_table int32 [batch][table_cols]
  * with row stride table_stride: the sequence's pages in order; entries past its last page are not
- * read. A page number outside the cache, or a sequence longer than the table's row, makes the
- * outputs of the queries that would read it NaN. Query head h reads kv head h / (q_heads / kv_heads).
+ * read. A page number outside the cache makes the outputs of the queries that would read it NaN; a
+ * sequence longer than the table's row or max_len, of more queries than max_q, or with tokens in a
+ * cache of no pages, all of its. Query head h reads kv head h / (q_heads / kv_heads).
  * out bf16 [total, q_heads, d], contiguous. scale > 0. Scores, softmax statistics and sums are fp32;
  * the weights of the values are rounded to bf16 for the matrix cores.
  * workspace: kv4_attention_workspace() bytes, 16-byte aligned (may be null for 0), free again when

@@ -247,7 +247,10 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   a.q = (const uint16_t*)q, a.cache = (const uint8_t*)cache, a.pages_of = page_table;
   a.lens = seq_lens, a.starts = q_starts, a.out = (uint16_t*)out, a.part = (float*)workspace;
   a.q_ts = q_ts, a.q_hs = q_hs, a.page_stride = page_stride, a.pages = pages;
-  a.table_stride = table_stride, a.page_shift = page_shift(page), a.table_cols = table_cols;
+  a.table_stride = table_stride, a.page_shift = page_shift(page);
+  // An unusable page is read as page 0, which a cache of no pages does not have: no token of it has a
+  // page, so that every sequence with tokens is longer than its row of the table (NaN).
+  a.table_cols = pages ? table_cols : 0;
   a.total = total, a.batch = batch, a.max_q = max_q, a.max_len = max_len;
   a.Hq = q_heads, a.Hkv = kv_heads, a.group = q_heads / kv_heads;
   a.window = window, a.scale = scale;
