@@ -156,7 +156,6 @@ struct Shared {
   v4i q[RF * (D / 32)][64];
   float stat[2][W][RF * 16];
   float merge[W][16][D + 4];
-  int bad_page;
 };
 
 template <int D, int RF, int W>
@@ -253,14 +252,9 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
     const uint8_t* head_base = a.cache + (size_t)(h << (a.page_shift - 4)) * G::kBytes;
     const int group_mask = (1 << (a.page_shift - 4)) - 1;
     const int last_page = (t1 - 1) >> a.page_shift;
-    bool bad = false;
     auto page_of = [&](int t) { return scalar_load(table + min(t >> a.page_shift, last_page)); };
     auto group_at = [&](int t, int page) {
-      const int p = __builtin_amdgcn_readfirstlane(page);
-      const bool ok = (uint32_t)p < (uint32_t)a.pages;
-      bad |= !ok;
-      return head_base + (uint64_t)(uint32_t)(ok ? p : 0) * (uint32_t)a.page_stride +
-             (uint32_t)((t >> 4) & group_mask) * (uint32_t)G::kBytes;
+      return tokens_at(a, head_base, __builtin_amdgcn_readfirstlane(page), (t >> 4) & group_mask, G::kBytes);
     };
 
     float m[RF], l[RF];                // row maximum (raw scores), this lane's share of the sum
@@ -283,11 +277,11 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
     const int t_last = (t1 - 1 - t0) / kStep * kStep + t0;
     int t = t0 + wave * kStep;
     int na = 0, nb = 0;                // page numbers of the next step to ask for
+    Tokens ta = {}, tb = {};           // whose keys are in w
     if (t < t1) {
-      const uint8_t* ga = group_at(t, page_of(t));
-      const uint8_t* gb = group_at(t + 16, page_of(t + 16));
-      load_keys<D>(w[0], ga, g, r), load_keys<D>(w[1], gb, g, r);
-      load_values<D>(w[0], ga, g, r), load_values<D>(w[1], gb, g, r);
+      ta = group_at(t, page_of(t)), tb = group_at(t + 16, page_of(t + 16));
+      load_keys<D>(w[0], ta.group, g, r), load_keys<D>(w[1], tb.group, g, r);
+      load_values<D>(w[0], ta.group, g, r), load_values<D>(w[1], tb.group, g, r);
       const int tn = min(t + kGranule, t_last);
       na = page_of(tn), nb = page_of(tn + 16);
     }
@@ -296,6 +290,10 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
       if (wave + j * W < RF * KS) sh.q[wave + j * W][lane] = ops[j];
     __syncthreads();
     for (; t < t1; t += kGranule) {
+      if (ta.nan | tb.nan) {           // (a branch: two more values in the products' loop spill registers)
+#pragma unroll
+        for (int p = 0; p < P; ++p) w[0].ks[p] |= ta.nan, w[1].ks[p] |= tb.nan;
+      }
       // scores of 2 x 16 tokens: lane holds tokens 4 g + i of both, row r
       v4f sc[RF][2];
 #pragma unroll
@@ -314,9 +312,8 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
       }
       __builtin_amdgcn_sched_barrier(0);
       const int tn = min(t + kGranule, t_last);
-      const uint8_t* ga = group_at(tn, na);
-      const uint8_t* gb = group_at(tn + 16, nb);
-      load_keys<D>(w[0], ga, g, r), load_keys<D>(w[1], gb, g, r);
+      ta = group_at(tn, na), tb = group_at(tn + 16, nb);
+      load_keys<D>(w[0], ta.group, g, r), load_keys<D>(w[1], tb.group, g, r);
       const int tp = min(tn + kGranule, t_last);
       na = page_of(tp), nb = page_of(tp + 16);
       if (t + kStep > span.all_hi || t < span.all_lo) {   // tokens that some row does not see
@@ -404,14 +401,13 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
                              }
                              __builtin_amdgcn_sched_barrier(0);
                            });
-      load_values<D>(w[0], ga, g, r), load_values<D>(w[1], gb, g, r);
+      load_values<D>(w[0], ta.group, g, r), load_values<D>(w[1], tb.group, g, r);
     }
 
     // ---- the waves' shares -----------------------------------------------------------------------
     {
     // (tid pinned here, or the addresses below are kept in registers through the steps)
     const int tid = pinned(threadIdx.x), lane = tid & 63, g = lane >> 4, r = lane & 15;
-    if (tid == 0) sh.bad_page = 0;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
       l[f] += __shfl_xor(l[f], 16);
@@ -419,7 +415,6 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
       if (g == 0) sh.stat[0][wave][f * 16 + r] = m[f], sh.stat[1][wave][f * 16 + r] = l[f];
     }
     __syncthreads();
-    if (bad) sh.bad_page = 1;
     const int which = first_granule > 0 ? 0 : 1;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
@@ -453,7 +448,6 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
           const float wm = sh.stat[0][w][f * 16 + row];
           sum += sh.stat[1][w][f * 16 + row] * (wm == tm ? 1.0f : exp2_raw((wm - tm) * c));
         }
-        if (sh.bad_page) sum = __uint_as_float(0x7FC00000u);
         float y[C];
 #pragma unroll
         for (int i = 0; i < C; i += 4) {

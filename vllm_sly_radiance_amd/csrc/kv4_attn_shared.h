@@ -73,6 +73,17 @@ __device__ __forceinline__ Sequence sequence_uniform(const AttnArgs& a, int b) {
   return s;
 }
 
+// A group of 16 tokens. Those of a page number outside the cache are read from page 0, and `nan` (all ones;
+// 0 for others), set in the words of their key scales, makes their scores NaN: the masks keep that from the
+// rows that do not see them.
+struct Tokens { const uint8_t* group; uint32_t nan; };
+__device__ __forceinline__ Tokens tokens_at(const AttnArgs& a, const uint8_t* head_base, int page, int group,
+                                            int group_bytes) {
+  const bool ok = (uint32_t)page < (uint32_t)a.pages;
+  return {head_base + (uint64_t)(uint32_t)(ok ? page : 0) * (uint32_t)a.page_stride +
+              (uint32_t)group * (uint32_t)group_bytes, ok ? 0u : ~0u};
+}
+
 // Tokens [lo, hi) that the queries first .. last of a sequence see between them (lo rounded down to a
 // step), and [all_lo, all_hi) that each of them sees.
 struct Span { int lo, hi, all_lo, all_hi; };

@@ -77,7 +77,6 @@ struct Shared {
   v4i v[2][D / 32][kTile / kGroup][64];   // [buffer][32 channels][16 tokens][lane, in value_slot's order]
   uint8_t nan[2][D / 32][kTile];          // value scales of a step that has NaN blocks
   int has_nan[2];
-  int bad_page;
 };
 
 // Where channel c of 32, half h of the tokens, lies among the 64 operands of a matrix instruction. In
@@ -109,6 +108,7 @@ struct Fill {
   typedef typename std::conditional<D >= 128, v4i, v2i>::type Vec;
   uint32_t k[T::kKeyUnits];
   uint32_t ks;             // the word that holds the units' key scales (a byte for each 4), from bit ks_bit
+  uint32_t key_nan;        // and their tokens' Tokens::nan
   Vec v[2];
   uint32_t vs[2];
   float s[8];              // while they are converted: the tokens' scales, one byte's values
@@ -138,7 +138,9 @@ struct Fill {
     nan_to = block * T::kTile + 16 * grp + 4 * h;
   }
 
-  __device__ __forceinline__ void load_keys(const uint8_t* group) {
+  __device__ __forceinline__ void load_keys(const Tokens& tokens) {
+    const uint8_t* group = tokens.group;
+    key_nan = tokens.nan;
     const uint8_t* kp = group + (uint32_t)pinned(key_at);
     if constexpr (T::kKeyUnits >= 4) {
 #pragma unroll
@@ -189,7 +191,8 @@ struct Fill {
     if constexpr (I < T::kKeyUnits) {
       // units I and I + 1 are the two halves of an instruction's channels
       uint8_t* to = reinterpret_cast<uint8_t*>(&sh.k[kbuf][0][0][0]) + pinned(key_to);
-      const v4i y = __builtin_bit_cast(v4i, expand8(k[I], scale_of((ks >> (ks_bit + 8 * (I / 4))) & 0xFFu)));
+      const uint32_t e = (ks >> (ks_bit + 8 * (I / 4))) & 0xFFu;
+      const v4i y = __builtin_bit_cast(v4i, expand8(k[I], bits_f32(e << 23 | key_nan)));
       *reinterpret_cast<v4i*>(to + (I >> 1) * 1024 + (I & 1) * 512) = y;
     } else if constexpr (I == T::kKeyUnits) {
 #pragma unroll
@@ -323,7 +326,6 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
   const int share = ceil_div(ceil_div(max(all.hi - all.lo, 0), kTile), work.parts) * kTile;
   const int t0 = all.lo + work.part * share, t1 = min(all.hi, t0 + share);
   const int last_page = (t1 - 1) >> a.page_shift;
-  bool bad = false;
   // The numbers of 128 pages from page_base on, a lane each of two registers: a step's is read from them
   // without a wait. (A scalar load would share its counter with the LDS reads and stall them.)
   auto pages_from = [&](int first) { return table[min(first + lane, last_page)]; };
@@ -336,11 +338,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
       pages_now = pages_next;
       pages_next = pages_from(page_base + 64);
     }
-    const int p = __builtin_amdgcn_readlane(pages_now, e - page_base);
-    const bool ok = (uint32_t)p < (uint32_t)a.pages;
-    bad |= !ok;
-    return head_base + (uint64_t)(uint32_t)(ok ? p : 0) * (uint32_t)a.page_stride +
-           (uint32_t)((t >> 4) & group_mask) * (uint32_t)G::kBytes;
+    return tokens_at(a, head_base, __builtin_amdgcn_readlane(pages_now, e - page_base),
+                     (t >> 4) & group_mask, G::kBytes);
   };
 
   const float c = a.scale * 1.44269504088896340736f;
@@ -358,17 +357,17 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
   const int value_lane = value_slot(half, lane & 31);
   Fill<D, W> fill;
   fill.place(grp, wave % T::kParts, lane);
-  const uint8_t* keys_from = nullptr;     // the group whose keys are in `fill`
-  if (tid == 0) sh.has_nan[0] = sh.has_nan[1] = sh.bad_page = 0;
+  Tokens keys_from = {};                  // whose keys are in `fill`
+  if (tid == 0) sh.has_nan[0] = sh.has_nan[1] = 0;
   for (int i = tid; i < 2 * CT * kTile; i += 64 * W) (&sh.nan[0][0][0])[i] = 0;
   lds_barrier();
   if (t0 < t1) {
     page_base = t0 >> a.page_shift;
     pages_now = pages_from(page_base), pages_next = pages_from(page_base + 64);
-    const uint8_t* g0 = group_at(t0);
-    const uint8_t* g1 = group_at(t0 + kTile);
+    const Tokens g0 = group_at(t0);
+    const Tokens g1 = group_at(t0 + kTile);
     fill.load_keys(g0);
-    fill.load_values(g0);
+    fill.load_values(g0.group);
     fill.take_out_nan(sh, 0);
     fill.template slices<0, Fill<D, W>::kSlices>(sh, 0, 0);
     if (grp < 2) {
@@ -379,7 +378,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
       keys_from = g1;
     }
     fill.load_keys(keys_from);
-    fill.load_values(g1);
+    fill.load_values(g1.group);
     lds_barrier();
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc[0][j] = 0.0f;
@@ -466,7 +465,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
             sh, grp < 2 ? buf : buf ^ 1, buf ^ 1);
       });
     });
-    const uint8_t* values_from = grp < 2 ? keys_from : group_at(t + 2 * kTile);
+    const uint8_t* values_from = (grp < 2 ? keys_from : group_at(t + 2 * kTile)).group;
     keys_from = group_at(t + (key_ahead + 1) * kTile);
     fill.load_keys(keys_from);             // needed first
     fill.load_values(values_from);
@@ -501,11 +500,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
     }
   }
 
-  if (bad) sh.bad_page = 1;
-  lds_barrier();
   l += __shfl_xor(l, 32);
   if (w0 + (lane & 31) >= R) return;
-  const float sum = sh.bad_page ? __uint_as_float(0x7FC00000u) : l;
   uint16_t* out = out_row(a, D, s.q0, h, row);
 #pragma unroll
   for (int i = 0; i < CT; ++i)
@@ -514,9 +510,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
       const float y[4] = {o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
       const int ch = 32 * i + 8 * g + 4 * half;
       if (work.parts == 1)
-        store_row<4>(out + ch, y, sum);
+        store_row<4>(out + ch, y, l);
       else
-        store_part<4>(a, T::kRows, D, work.entry * work.parts + work.part, row - r0, ch, y, m * c, sum);
+        store_part<4>(a, T::kRows, D, work.entry * work.parts + work.part, row - r0, ch, y, m * c, l);
     }
 }
 
