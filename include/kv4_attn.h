@@ -21,7 +21,8 @@
  *   key scales   [16 tokens][d / 32]
  *   value scales [d / 32][16 tokens]
  * Codes are e2m1, the low nibble the even channel; a scale byte E is 2^(E - 127) for 32 consecutive
- * channels of one token, 255 for a block that held a value that is not finite (it reads as NaN).
+ * channels of one token, 255 for a block that held a value that is not finite. A byte above 252 reads
+ * as NaN, whoever wrote it.
  * E is the smallest exponent with amax <= 7 * 2^(E - 127), within 1 .. 252, so that rounding to the
  * nearest code is off by at most 2^(E - 127) at the top; codes round to nearest, ties to even. The
  * value layout puts 4 tokens of a run side by side: a lane of the attention kernels holds the codes

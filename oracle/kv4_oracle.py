@@ -35,9 +35,9 @@ def quantize(x: np.ndarray):
 
 
 def dequantize(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
-    """-> float64 [..., d]; a block of scale 255 is NaN."""
+    """-> float64 [..., d]; a block of a scale above 252, the largest that quantize gives, is NaN."""
     s = np.ldexp(1.0, scales.astype(np.int64) - 127)
-    s = np.where(scales == 255, np.nan, s)
+    s = np.where(scales > 252, np.nan, s)
     return E2M1[codes] * np.repeat(s, 32, axis=-1)
 
 

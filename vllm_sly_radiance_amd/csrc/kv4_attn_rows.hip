@@ -301,8 +301,8 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int p = D >= 128 ? k >> 2 : 0;
-        const v8bf k0 = expand8(w[0].k[p][D >= 128 ? k & 3 : k], scale_of((w[0].ks[p] >> ks_bit) & 0xFFu));
-        const v8bf k1 = expand8(w[1].k[p][D >= 128 ? k & 3 : k], scale_of((w[1].ks[p] >> ks_bit) & 0xFFu));
+        const v8bf k0 = expand8(w[0].k[p][D >= 128 ? k & 3 : k], stored_scale((w[0].ks[p] >> ks_bit) & 0xFFu));
+        const v8bf k1 = expand8(w[1].k[p][D >= 128 ? k & 3 : k], stored_scale((w[1].ks[p] >> ks_bit) & 0xFFu));
 #pragma unroll
         for (int f = 0; f < RF; ++f) {
           const v8bf q = __builtin_bit_cast(v8bf, sh.q[f * KS + k][lane]);

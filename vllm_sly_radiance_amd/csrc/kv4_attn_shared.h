@@ -127,9 +127,9 @@ __device__ __forceinline__ v8bf pack8bf(const float e[8]) {
   return __builtin_bit_cast(v8bf, r);
 }
 
-// Bit 7 of each of four scale bytes that is 255.
+// Bit 7 of each of four scale bytes above 252, which read as NaN.
 __device__ __forceinline__ uint32_t nan_scales(uint32_t four) {
-  return ((four & 0x7F7F7F7Fu) + 0x01010101u) & four & 0x80808080u;
+  return ((four & 0x7F7F7F7Fu) + 0x03030303u) & four & 0x80808080u;
 }
 
 // The low (high) halves of two dwords, the first one's below.

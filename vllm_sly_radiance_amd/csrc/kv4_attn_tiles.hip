@@ -191,8 +191,8 @@ struct Fill {
     if constexpr (I < T::kKeyUnits) {
       // units I and I + 1 are the two halves of an instruction's channels
       uint8_t* to = reinterpret_cast<uint8_t*>(&sh.k[kbuf][0][0][0]) + pinned(key_to);
-      const uint32_t e = (ks >> (ks_bit + 8 * (I / 4))) & 0xFFu;
-      const v4i y = __builtin_bit_cast(v4i, expand8(k[I], bits_f32(e << 23 | key_nan)));
+      const uint32_t e = ((ks | key_nan) >> (ks_bit + 8 * (I / 4))) & 0xFFu;
+      const v4i y = __builtin_bit_cast(v4i, expand8(k[I], stored_scale(e)));
       *reinterpret_cast<v4i*>(to + (I >> 1) * 1024 + (I & 1) * 512) = y;
     } else if constexpr (I == T::kKeyUnits) {
 #pragma unroll

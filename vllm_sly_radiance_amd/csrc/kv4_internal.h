@@ -49,6 +49,9 @@ __device__ __forceinline__ uint32_t codes_bf16x2(uint32_t codes, float scale) {
                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, B));
 }
 __device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float(e << 23); }
+// The same with bytes above 252, which scale_byte never gives, as 255: with 253 and 254 some codes pass the
+// range of bf16, and an infinite value would reach rows that do not see it through a weight of zero.
+__device__ __forceinline__ float stored_scale(uint32_t e) { return scale_of(e > 252u ? 255u : e); }
 
 // A block's scale byte from the largest magnitude's bits: the smallest exponent with amax <= 7 x
 // scale. Adding 0x1FFFFF carries into the exponent exactly where the mantissa is above 1.75.

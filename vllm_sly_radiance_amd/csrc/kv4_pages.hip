@@ -34,8 +34,8 @@ __global__ __launch_bounds__(256) void gather_tokens(GatherArgs a, long items) {
                            (size_t)(place >> 4) * G::kBytes;
     const uint32_t kc =
         *reinterpret_cast<const uint32_t*>(group + G::kKeys + token * (D / 2) + 4 * j);
-    const float ks = scale_of(group[G::kKeyScales + token * (D / kBlock) + (j >> 2)]);
-    const float vs = scale_of(group[G::kValueScales + (j >> 2) * kGroup + token]);
+    const float ks = stored_scale(group[G::kKeyScales + token * (D / kBlock) + (j >> 2)]);
+    const float vs = stored_scale(group[G::kValueScales + (j >> 2) * kGroup + token]);
     const int g = token >> 2, i = token & 3;
     uint32_t vc;
     if constexpr (G::kRun == 8) {
