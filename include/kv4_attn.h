@@ -101,10 +101,11 @@ int kv4_gather(const void* cache, long pages, long page_stride, int page, const 
 /* Softmax attention of the last tokens of `batch` sequences over their cached tokens:
  *   o_i = sum_j softmax_j(scale * q_i . k_j) v_j
  * q bf16 [total, q_heads, d] (token and head strides in elements, multiples of 8; 16-byte aligned),
- * sequence b's queries are rows q_starts[b] .. q_starts[b + 1] - 1 (int32 [batch + 1], ascending, at
- * most max_q apart) and stand at the end of its seq_lens[b] cached tokens (int32 [batch], at most
- * max_len): query i of n at place p = seq_len - n + i. It sees the tokens j < seq_len, with
- * KV4_CAUSAL j <= p, and with window > 0 j > p - window. A query that sees nothing gives zeros.
+ * sequence b's queries are rows q_starts[b] .. q_starts[b + 1] - 1 (int32 [batch + 1], at most max_q
+ * apart, ascending: with starts that go back, outputs are unspecified) and stand at the end of its
+ * seq_lens[b] cached tokens (int32 [batch], at most max_len): query i of n at place p = seq_len - n + i.
+ * It sees the tokens j < seq_len, with KV4_CAUSAL j <= p, and with window > 0 j > p - window. A query
+ * that sees nothing gives zeros.
  * What a masked token holds, NaN included, has no effect. page_table int32 [batch][table_cols]
  * with row stride table_stride: the sequence's pages in order; entries past its last page are not
  * read. A page number outside the cache makes the outputs of the queries that would read it NaN; a

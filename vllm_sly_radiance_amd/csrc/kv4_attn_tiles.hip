@@ -261,7 +261,9 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int tile_rows, int 
   int tiles = 0;
   for (int i0 = 0; i0 < a.batch; i0 += 64)
     tiles += __builtin_amdgcn_readlane(wave_scan(tiles_of(a, tile_rows, i0 + lane)), 63);
-  const int units = tiles * a.Hkv, rest = units % kCUs, first = units - rest;
+  // (more units than the launch was planned for, which starts that overlap would make, are not cut: the
+  // workgroups that would tell attn_join of them may not be there)
+  const int units = tiles * a.Hkv, rest = units <= a.units ? units % kCUs : 0, first = units - rest;
   const int parts = attn_parts(rest, a.span, a.entries);
   // (attn_join looks at the entries that there may be)
   if (x < a.entries && x < kCUs && x >= rest && threadIdx.x == 0) meta(a, tile_rows, a.d, x)[0] = 0;
