@@ -1,0 +1,34 @@
+"""Attention over the 4-bit cache under limits far above what a batch holds."""
+import numpy as np
+import pytest
+import torch
+
+from tests._kv4 import Batch
+from vllm_sly_radiance_amd import _native_kv4
+from vllm_sly_radiance_amd import radiance_kv4 as K
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _lib(gpu_lib):
+    return _native_kv4.lib()
+
+
+@pytest.mark.parametrize("Hq,Hkv,d,n,chunk,max_q", [(32, 8, 128, 512, 150, 4096), (48, 16, 128, 256, 70, 4096),
+                                                    (16, 2, 256, 300, 1, 8192)])
+def test_a_chunk_beside_many_decoding_sequences(Hq, Hkv, d, n, chunk, max_q):
+    """Limits of 131072 tokens and thousands of queries a sequence, as of a server's captured graph."""
+    rng = np.random.default_rng(n)
+    qs = [1] * n
+    qs[n // 3] = chunk
+    lens = [int(x) for x in rng.integers(1, 40, n)]
+    lens[n // 3] = chunk + 60
+    b = Batch(rng, lens, qs, Hq, Hkv, d, 16)
+    q, cache, table, dl, starts, _, _ = b.device()
+    rows = torch.zeros((n - 1 + max_q, Hq, d), dtype=torch.bfloat16, device="cuda")
+    rows[:q.shape[0]] = q
+    wide = torch.full((n, 131072 // 16), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    print(f"[kv4] {n} sequences, heads={Hq}/{Hkv} d={d} chunk {chunk} of {max_q}", flush=True)
+    b.check(K.attention(rows, cache, wide, dl, starts, max_q, 131072)[:q.shape[0]])

@@ -107,8 +107,9 @@ int rope(const char* who, RopeArgs a, int q_heads, int kv_heads, int d, hipStrea
   return hip_status(launch_rope(a, d, stream), who);
 }
 
-int attn_sizes(const char* who, int batch, int max_q, int max_len, int q_heads, int kv_heads, int d,
-               int window) {
+// Checks the sizes of an attention call and plans it (an empty plan where there is nothing to do).
+int plan_attention(const char* who, int total, int batch, int max_q, int max_len, int q_heads,
+                   int kv_heads, int d, int window, AttnPlan* plan) {
   if (int rc = check_heads(who, kv_heads, d)) return rc;
   if (int rc = check_heads(who, q_heads, d)) return rc;
   if (q_heads % kv_heads)
@@ -116,15 +117,20 @@ int attn_sizes(const char* who, int batch, int max_q, int max_len, int q_heads, 
   if (batch < 0 || max_q < 0 || max_len < 0 || max_len > 0x7FFFF000 || window < 0)
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d max_len=%d window=%d", who, batch, max_q, max_len,
                 window);
-  if ((long)batch * q_heads * max_q > 0x7FFFFFFFL)
+  // what the counts below need to be exact: rows at the limits, and row tiles of 16 of them, which is
+  // what the kernels count in 32 bits whatever the starts on the device are
+  const long heads = (long)batch * q_heads, rows = (long)std::min(max_q, std::max(total, 0)) * q_heads;
+  if ((max_q && heads > (1L << 40) / max_q) || rows > 0x7FFFF000L ||
+      batch * (rows / 16 + kv_heads) > 0x7FFFFFFFL)
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d q_heads=%d are too many rows", who, batch, max_q,
                 q_heads);
-  // attn_rows counts work in granules of 128 tokens of a row tile, and two for its start, in 31 bits
-  const long rows = (long)max_q * (q_heads / kv_heads);
-  const long tile = rows <= 16 ? 16 : rows <= 32 || d == 256 ? 32 : 64;
-  if ((long)batch * kv_heads * ((rows + tile - 1) / tile) * ((max_len + 127L) / 128) > (1L << 29))
-    return fail(KV4_EINVAL, "%s: batch=%d max_q=%d max_len=%d are too much for one call", who, batch,
-                max_q, max_len);
+  *plan = {};
+  if (total <= 0 || !batch || !max_q) return KV4_OK;
+  *plan = attn_plan(total, batch, std::min(max_q, total), max_len, q_heads, kv_heads, d, window);
+  // attn_rows counts its work in 31 bits, a launch its threads in 32
+  if (plan->work > 0x7FFFFFFFL - 4 * kCUs || plan->threads >> 32)
+    return fail(KV4_EINVAL, "%s: batch=%d total=%d max_len=%d are too much for one call", who, batch, total,
+                max_len);
   return KV4_OK;
 }
 
@@ -210,11 +216,11 @@ KV4_API int kv4_gather(const void* cache, long pages, long page_stride, int page
 KV4_API int kv4_attention_workspace(int total, int batch, int max_q, int max_len, int q_heads,
                                     int kv_heads, int d, int window, size_t* bytes) {
   if (!bytes) return fail(KV4_EINVAL, "attention_workspace: null output");
-  if (int rc = attn_sizes("attention_workspace", batch, max_q, max_len, q_heads, kv_heads, d, window))
+  AttnPlan plan;
+  if (int rc = plan_attention("attention_workspace", total, batch, max_q, max_len, q_heads, kv_heads, d,
+                              window, &plan))
     return rc;
-  *bytes = total > 0 && batch && max_q
-               ? attn_plan(total, batch, max_q, max_len, q_heads, kv_heads, d, window).workspace
-               : 0;
+  *bytes = plan.workspace;
   return KV4_OK;
 }
 
@@ -225,7 +231,9 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
                           int max_len, int q_heads, int kv_heads, int d, float scale, int window,
                           int flags, void* stream) {
   const char* who = "attention";
-  if (int rc = attn_sizes(who, batch, max_q, max_len, q_heads, kv_heads, d, window)) return rc;
+  AttnPlan plan;
+  if (int rc = plan_attention(who, total, batch, max_q, max_len, q_heads, kv_heads, d, window, &plan))
+    return rc;
   if (int rc = check_cache(who, cache, pages, page_stride, page, kv_heads, d)) return rc;
   if (!(scale > 0.0f) || scale > 3.0e38f)
     return fail(KV4_EINVAL, "%s: scale must be positive and finite", who);
@@ -239,7 +247,6 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
     return fail(KV4_EINVAL, "%s: null pointer", who);
   if (!aligned(seq_lens, 4) || !aligned(q_starts, 4) || !aligned(page_table, 4) || !aligned(out, 16))
     return fail(KV4_EINVAL, "%s: misaligned pointer", who);
-  const AttnPlan plan = attn_plan(total, batch, max_q, max_len, q_heads, kv_heads, d, window);
   if (plan.workspace > workspace_bytes || (plan.workspace && (!workspace || !aligned(workspace, 16))))
     return fail(KV4_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who,
                 plan.workspace, workspace_bytes);
@@ -251,7 +258,8 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   // An unusable page is read as page 0, which a cache of no pages does not have: no token of it has a
   // page, so that every sequence with tokens is longer than its row of the table (NaN).
   a.table_cols = pages ? table_cols : 0;
-  a.total = total, a.batch = batch, a.max_q = max_q, a.max_len = max_len;
+  a.total = total, a.batch = batch, a.max_len = max_len;
+  a.max_q = std::min(max_q, total);     // (a sequence of more queries than rows is bad either way)
   a.Hq = q_heads, a.Hkv = kv_heads, a.group = q_heads / kv_heads;
   a.window = window, a.scale = scale;
   a.causal = flags & KV4_CAUSAL;

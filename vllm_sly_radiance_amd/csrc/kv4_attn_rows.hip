@@ -27,6 +27,8 @@
 // same for every row, the weights are not): 8 x 8 queries of 48 + 16 heads against up to 4000 tokens,
 // 49 MB: 20 us. By the launches and three dependent reads (length, page, tokens) where it is short: 500
 // tokens 7.5 us. The join behind it takes 3 to 6.
+#include <algorithm>
+
 #include "kv4_attn.h"
 #include "kv4_attn_shared.h"
 
@@ -468,7 +470,8 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
     if (a.runs && first_granule == 0 && tid == 0 && (a.by_unit || !whole)) {
       // what attn_join is told of a unit: how many workgroups after this one finish it
       int* mt = meta(a, kTile, D, a.by_unit ? b * a.units + this_unit : blockIdx.x);
-      mt[0] = (int)((rest - part + run.share - 1) / run.share);
+      // (no more than there are: starts that go back can make more work than 32 bits count)
+      mt[0] = min((int)((rest - part + run.share - 1) / run.share), a.runs - 1 - (int)blockIdx.x);
       mt[1] = b, mt[2] = this_unit, mt[3] = blockIdx.x;
     }
     if (!run.left) return;
@@ -650,6 +653,7 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
     } else {
       p.entries = (int)(units * 16 < kMostEntries ? units * 16 : kMostEntries);
     }
+    p.threads = (units + p.entries) * attn_tile_rows(d) * 2;     // 64 for each 32 rows
     if (p.entries)
       p.tiles_workspace = p.workspace =
           (size_t)(p.entries + 1) / 2 * 2 * tile_rows * (d + 2) * sizeof(float) + kCUs * 16;
@@ -678,12 +682,16 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   //   L = 800, 8 sequences  13.0  20.0    8 x 3 rows, 16 kv heads, L = 2000: 20.2  22.0, L = 3000: 25.2  24.9
   const long waves_step = kStep * attn_whole_waves(p.fragments), steps = (span + waves_step - 1) / waves_step;
   // (not where most of those workgroups would have nothing to do)
-  if (most_units <= 2 * units && (steps <= 4 || (span <= (p.fragments == 1 ? 4096 : 2048) && units >= 16 * steps)))
+  if (most_units <= 2 * units && (steps <= 4 || (span <= (p.fragments == 1 ? 4096 : 2048) && units >= 16 * steps))) {
+    p.threads = std::max(p.threads, most_units * 64 * attn_whole_waves(p.fragments));
     return p;
+  }
   // as many workgroups as the card's 256 CUs hold at once, or a granule each
   const long granules = (span + kStep * kRunWaves - 1) / (kStep * kRunWaves);
   const long most = 256L * 4 * attn_waves(d, p.fragments) / kRunWaves;
   p.runs = (int)(units * granules < most ? units * granules : most);
+  // (where attn_join looks at every unit there may be, all of them count)
+  p.work = (most_units <= p.runs ? most_units : units) * (granules + kStart);
   p.workspace += (size_t)p.runs * ((size_t)2 * tile * (d + 2) * sizeof(float) + 16);
   return p;
 }

@@ -187,6 +187,8 @@ struct AttnPlan {
   int fragments, runs, few_rows;
   int units, entries, span;             // of attn_tiles; units: at most
   size_t tiles_workspace, workspace;
+  long work;                            // granules of attn_rows and starts of its units, where runs share them
+  long threads;                         // of the largest launch
 };
 AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv, int d, int window);
 int attn_tile_rows(int d);          // rows of a workgroup of attn_tiles
