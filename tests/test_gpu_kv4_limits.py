@@ -32,3 +32,17 @@ def test_a_chunk_beside_many_decoding_sequences(Hq, Hkv, d, n, chunk, max_q):
     wide[:, :table.shape[1]] = table
     print(f"[kv4] {n} sequences, heads={Hq}/{Hkv} d={d} chunk {chunk} of {max_q}", flush=True)
     b.check(K.attention(rows, cache, wide, dl, starts, max_q, 131072)[:q.shape[0]])
+
+
+@pytest.mark.parametrize("max_len", [30, 100000])
+@pytest.mark.parametrize("d,qs", [(128, [2, 0, 1]), (64, [300, 1, 200]), (256, [0, 0, 0])])
+def test_no_queries_allowed(d, qs, max_len):
+    """max_q = 0: every sequence with queries has more than that, and its rows are NaN as under any max_q."""
+    cache = K.new_cache(4, 2, 16, d)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.ones((sum(qs) + 3, 8, d), dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros((3, 7000), dtype=torch.int32, device="cuda")
+    starts = i32(0, qs[0], qs[0] + qs[1], sum(qs))
+    print(f"[kv4] max_q=0 q={qs} d={d} max_len={max_len}", flush=True)
+    for lens in (i32(30, 20, 25), i32(0, 0, 0)):
+        assert K.attention(q, cache, table, lens, starts, 0, max_len)[:sum(qs)].isnan().all()

@@ -52,3 +52,12 @@ def test_a_limit_above_the_rows_is_the_rows(lib):
 def test_refused(lib, sizes, msg):
     rc, _, error = ask(lib, *sizes)
     assert rc == 1 and msg in error, error
+
+
+def test_rows_under_a_limit_of_no_queries_are_not_nothing_to_do(lib):
+    """Their outputs have to be written (NaN), so that the call needs its tensors."""
+    call = lambda total: lib.kv4_attention(  # noqa: E731
+        None, 0, 0, None, 0, 17 * 128, 16, None, 0, 0, None, None, None, None, 0, total, 2, 0, 10, 2, 1, 128,
+        1.0, 0, 0, None)
+    assert call(0) == 0
+    assert call(5) == 1 and b"null q" in lib.kv4_last_error()

@@ -125,8 +125,9 @@ int plan_attention(const char* who, int total, int batch, int max_q, int max_len
     return fail(KV4_EINVAL, "%s: batch=%d max_q=%d q_heads=%d are too many rows", who, batch, max_q,
                 q_heads);
   *plan = {};
-  if (total <= 0 || !batch || !max_q) return KV4_OK;
-  *plan = attn_plan(total, batch, std::min(max_q, total), max_len, q_heads, kv_heads, d, window);
+  if (total <= 0 || !batch) return KV4_OK;
+  // (where no sequence may have queries, those that do are written as NaN: planned as for one each)
+  *plan = attn_plan(total, batch, std::max(std::min(max_q, total), 1), max_len, q_heads, kv_heads, d, window);
   // attn_rows counts its work in 31 bits, a launch its threads in 32
   if (plan->work > 0x7FFFFFFFL - 4 * kCUs || plan->threads >> 32)
     return fail(KV4_EINVAL, "%s: batch=%d total=%d max_len=%d are too much for one call", who, batch, total,
@@ -241,7 +242,7 @@ KV4_API int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache
   if (total < 0 || table_cols < 0 || table_stride < 0)
     return fail(KV4_EINVAL, "%s: total=%d table_cols=%d table_stride=%ld", who, total, table_cols,
                 table_stride);
-  if (!total || !batch || !max_q) return KV4_OK;
+  if (!total || !batch) return KV4_OK;
   if (int rc = check_rows(who, "q", q, q_ts, q_hs)) return rc;
   if (!seq_lens || !q_starts || (!page_table && table_cols) || !out)
     return fail(KV4_EINVAL, "%s: null pointer", who);

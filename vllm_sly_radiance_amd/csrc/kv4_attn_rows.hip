@@ -569,7 +569,7 @@ hipError_t join(const AttnArgs& a, int tile_rows, int entries, int rows, hipStre
 template <int D, int RF>
 hipError_t launch(AttnArgs a, hipStream_t stream) {
   constexpr int W = kRunWaves;
-  const int rows = a.few_rows ? a.few_rows : a.max_q * a.group;   // of a sequence at most
+  const int rows = a.few_rows ? a.few_rows : std::max(a.max_q, 1) * a.group;   // of a sequence at most
   a.by_group = divisor(a.group), a.by_heads = divisor(a.Hkv), a.by_runs = divisor(a.runs ? a.runs : 1);
   if (!a.runs) {
     a.tiles = ceil_div(rows, 16 * RF);
