@@ -1,13 +1,14 @@
 // The 4-bit cache's ops on torch tensors: argument checks, outputs, workspaces and the current stream,
 // then one call of the C ABI (kv4_attn.h). A CPython module without the dispatcher in front: a decode
 // step's ops are a few microseconds of GPU work each, and the host has to keep up with them. One
-// token through qk_norm_rope takes 7 us a call from Python, 2.7 of them the launch, where the
+// token through qk_norm_rope takes 6.4 us a call from Python, 2.7 of them the launch, where the
 // same checks in Python and a ctypes call took 13.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -331,23 +332,52 @@ PyObject* move_pages(const Args& a) {
   Py_RETURN_NONE;
 }
 
+// Whether the tensors among the arguments may be taken as they are, past the dispatcher: none is of a
+// subclass, a transform's (vmap's have no storage), or one that a gradient is asked of.
+bool plain(PyObject* const* args, Py_ssize_t n) {
+  const bool grad = c10::GradMode::is_enabled();
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* x = args[i];
+    if (x == Py_None || PyLong_Check(x) || PyFloat_Check(x)) continue;
+    if (!THPVariable_CheckExact(x)) {     // (a Parameter is exact)
+      if (THPVariable_Check(x)) return false;
+      continue;
+    }
+    const Tensor& t = THPVariable_Unpack(x);
+    const c10::DispatchKeySet keys = t.key_set();
+    if (keys.has(c10::DispatchKey::FuncTorchBatched) || keys.has(c10::DispatchKey::FuncTorchGradWrapper) ||
+        keys.has(c10::DispatchKey::Functionalize) || keys.has(c10::DispatchKey::Python) ||
+        (grad && t.requires_grad()))
+      return false;
+  }
+  return true;
+}
+
 // Nothing thrown leaves an entry: torch's handlers turn it into the Python exception.
-template <PyObject* (*F)(const Args&), int N>
+template <PyObject* (*F)(const Args&), int N, bool IfPlain>
 PyObject* entry(const char* op, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != N) fail(op, str(n) + " arguments in place of " + str(N));
+  if (IfPlain && !plain(args, n)) Py_RETURN_NOTIMPLEMENTED;
   return F(Args{op, args});
   END_HANDLE_TH_ERRORS
 }
-#define ENTRY(name, n)                                                                             \
-  {#name, (PyCFunction)(void (*)(void))(_PyCFunctionFast)[](PyObject*, PyObject* const* a,         \
-                                                           Py_ssize_t k)->PyObject* {              \
-     return entry<name, n>(#name, a, k);                                                           \
-   },                                                                                              \
-   METH_FASTCALL, nullptr}
+PyObject* is_plain(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(plain(args, n));
+  END_HANDLE_TH_ERRORS
+}
+#define METHOD(name, f) {name, (PyCFunction)(void (*)(void))(_PyCFunctionFast)f, METH_FASTCALL, nullptr}
+#define ENTRY(name, n, if_plain)                                                                 \
+  [](PyObject*, PyObject* const* a, Py_ssize_t k) -> PyObject* {                                 \
+    return entry<name, n, if_plain>(#name, a, k);                                                \
+  }
+// name, and name_if_plain, which returns NotImplemented where the tensors are not
+#define ENTRIES(name, n) METHOD(#name, ENTRY(name, n, false)), METHOD(#name "_if_plain", ENTRY(name, n, true))
 
-PyMethodDef methods[] = {ENTRY(qk_norm_rope, 10), ENTRY(qk_norm_rope_append, 13), ENTRY(gather, 2),
-                         ENTRY(attention, 10),    ENTRY(move_pages, 3),           {}};
+PyMethodDef methods[] = {ENTRIES(qk_norm_rope, 10), ENTRIES(qk_norm_rope_append, 13), ENTRIES(gather, 2),
+                         ENTRIES(attention, 10),    ENTRIES(move_pages, 3),           METHOD("is_plain", is_plain),
+                         {}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv4_torch", nullptr, -1, methods};
 
 }  // namespace
