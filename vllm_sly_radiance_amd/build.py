@@ -76,36 +76,58 @@ def _torch_commands(out) -> tuple[list[str], list[str]]:
     return compile_, link
 
 
+def _run(cmd, verbose):
+    """The command's process, started."""
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def _end(job, verbose) -> None:
+    """Waits for a compiler; RuntimeError with its words where it failed."""
+    text = job.communicate()[0]
+    # hipcc's host pass does not know the packed-fp32 target feature; that warning is expected
+    noise = [ln for ln in text.splitlines()
+             if ln.strip() and "packed-fp32-ops" not in ln and "warning generated" not in ln
+             and "warnings generated" not in ln]
+    if job.returncode != 0:
+        raise RuntimeError("the compiler failed:\n" + "\n".join(noise))
+    if verbose and noise:
+        print("\n".join(noise), file=sys.stderr)
+
+
 def build(verbose: bool = False) -> str:
     """Compile every source into LIB_PATH, KV4_LIB_PATH and KV4_TORCH_PATH (always rebuilds, all at
-    once) and return LIB_PATH."""
-    compile_, link = _torch_commands(KV4_TORCH_PATH + ".tmp")
-    jobs = []
-    for cmd, path in ((_command(SOURCES, LIB_PATH + ".tmp"), LIB_PATH),
-                      (_command(KV4_SOURCES, KV4_LIB_PATH + ".tmp"), KV4_LIB_PATH),
-                      (compile_, None)):
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        jobs.append((path, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
-                                            text=True)))
-    outputs = [(path, job.communicate()[0], job.returncode) for path, job in jobs]
-    for path, text, status in outputs:
-        # hipcc's host pass does not know the packed-fp32 target feature; that warning is expected
-        noise = [ln for ln in text.splitlines()
-                 if ln.strip() and "packed-fp32-ops" not in ln and "warning generated" not in ln
-                 and "warnings generated" not in ln]
-        if status != 0:
-            raise RuntimeError("the compiler failed:\n" + "\n".join(noise))
-        if verbose and noise:
-            print("\n".join(noise), file=sys.stderr)
-    for path, _, _ in outputs:
-        if path:
+    once) and return LIB_PATH. What compiles is put in place whatever becomes of the rest: the linear
+    path's library needs hipcc only. RuntimeError at the end where something did not."""
+    libraries = [(path, _run(_command(sources, path + ".tmp"), verbose))
+                 for sources, path in ((SOURCES, LIB_PATH), (KV4_SOURCES, KV4_LIB_PATH))]
+    tmp, errors, link = KV4_TORCH_PATH + ".tmp", [], None
+    try:
+        compile_, link = _torch_commands(tmp)
+        binding = _run(compile_, verbose)
+    except (OSError, ImportError, AttributeError) as e:        # no host compiler, no torch or not its headers
+        binding, link = None, None
+        errors.append(f"_kv4_torch cannot be built: {e}")
+    for path, job in libraries:
+        try:
+            _end(job, verbose)
             os.replace(path + ".tmp", path)
-    done = subprocess.run(link, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if done.returncode:
-        raise RuntimeError("the linker failed:\n" + done.stdout)
-    os.remove(KV4_TORCH_PATH + ".tmp.o")
-    os.replace(KV4_TORCH_PATH + ".tmp", KV4_TORCH_PATH)
+        except RuntimeError as e:
+            errors.append(str(e))
+            if path == KV4_LIB_PATH:
+                link = None
+    try:
+        if binding:
+            _end(binding, verbose)
+            if link:
+                _end(_run(link, verbose), verbose)
+                os.replace(tmp, KV4_TORCH_PATH)
+            os.remove(tmp + ".o")
+    except RuntimeError as e:
+        errors.append(str(e))
+    if errors:
+        raise RuntimeError("\n".join(errors))
     return LIB_PATH
 
 
