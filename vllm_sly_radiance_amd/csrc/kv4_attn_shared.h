@@ -199,7 +199,7 @@ __device__ __forceinline__ void store_row(uint16_t* out, const float y[C], float
     uint32_t w[C / 2];
 #pragma unroll
     for (int i = 0; i < C / 2; ++i) w[i] = bf16x2(z[2 * i], z[2 * i + 1]);
-    __builtin_memcpy(__builtin_assume_aligned(out, 2 * C), w, 2 * C);
+    __builtin_memcpy(__builtin_assume_aligned(out, 2 * C < 16 ? 2 * C : 16), w, 2 * C);
   }
 }
 
