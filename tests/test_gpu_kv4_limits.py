@@ -46,3 +46,17 @@ def test_no_queries_allowed(d, qs, max_len):
     print(f"[kv4] max_q=0 q={qs} d={d} max_len={max_len}", flush=True)
     for lens in (i32(30, 20, 25), i32(0, 0, 0)):
         assert K.attention(q, cache, table, lens, starts, 0, max_len)[:sum(qs)].isnan().all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 8, 1 << 20, 130])
+@pytest.mark.parametrize("d,Hq,Hkv,lens,qs", [(128, 4, 2, [5, 0, 20], [9, 3, 1]), (64, 4, 2, [2500, 7], [1, 30]),
+                                              (128, 64, 8, [120, 130], [250, 130])])
+def test_windows_longer_than_any_sequence(d, Hq, Hkv, lens, qs, window, causal):
+    """As large as an int: queries that stand before the sequence (more of them than tokens) reach far below
+    zero."""
+    b = Batch(np.random.default_rng(d), lens, qs, Hq, Hkv, d, 16)
+    q, cache, table, dl, starts, mq, ml = b.device()
+    print(f"[kv4] lens={lens} q={qs} d={d} window={window} causal={causal}", flush=True)
+    out = K.attention(q, cache, table, dl, starts, mq, ml, causal=causal, window=window)
+    b.check(out, causal=causal, window=window)

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
     for (int f = 0; f < RF; ++f) {
       const int place = s.len - s.n + a.by_group(min(r0 + f * 16 + r, R - 1));
       hi[f] = a.causal ? min(place + 1, s.len) : s.len;
-      lo[f] = a.window > 0 ? place - a.window + 1 : 0;
+      lo[f] = first_seen(a, place);
     }
 
     // The page of a step's 16 tokens: its number is read two steps ahead of the tokens' use. Tokens

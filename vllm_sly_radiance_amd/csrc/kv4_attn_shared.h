@@ -84,6 +84,13 @@ __device__ __forceinline__ Tokens tokens_at(const AttnArgs& a, const uint8_t* he
               (uint32_t)group * (uint32_t)group_bytes, ok ? 0u : ~0u};
 }
 
+// The first token that a query at `place` sees; at most 0: no bound. A query before the sequence (more
+// queries than tokens) counts as at its start, where a window ends before the tokens too: its own place less
+// a window as large as an int would wrap, to a start far behind the pages.
+__device__ __forceinline__ int first_seen(const AttnArgs& a, int place) {
+  return a.window > 0 ? max(place, 0) - a.window + 1 : 0;
+}
+
 // Tokens [lo, hi) that the queries first .. last of a sequence see between them (lo rounded down to a
 // step), and [all_lo, all_hi) that each of them sees.
 struct Span { int lo, hi, all_lo, all_hi; };
@@ -92,8 +99,8 @@ __device__ __forceinline__ Span query_span(const AttnArgs& a, const Sequence& s,
   Span x;
   x.hi = a.causal ? min(s.len, max(p1 + 1, 0)) : s.len;
   x.all_hi = a.causal ? min(s.len, p0 + 1) : s.len;
-  x.lo = a.window > 0 ? max(p0 - a.window + 1, 0) & ~31 : 0;
-  x.all_lo = a.window > 0 ? p1 - a.window + 1 : 0;
+  x.lo = max(first_seen(a, p0), 0) & ~31;
+  x.all_lo = first_seen(a, p1);
   return x;
 }
 

@@ -309,7 +309,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
   const Span mine = query_span(a, s, a.by_group(min(w0, R - 1)), a.by_group(min(w0 + 32, R) - 1));
   const int place = s.len - s.n + qi;
   const int hi = a.causal ? min(place + 1, s.len) : s.len;
-  const int lo = a.window > 0 ? place - a.window + 1 : 0;
+  const int lo = first_seen(a, place);
   v8bf q[KS];
   {
     const uint16_t* src = a.q + (size_t)(s.q0 + qi) * a.q_ts +
