@@ -261,12 +261,13 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int tile_rows, int 
   int tiles = 0;
   for (int i0 = 0; i0 < a.batch; i0 += 64)
     tiles += __builtin_amdgcn_readlane(wave_scan(tiles_of(a, tile_rows, i0 + lane)), 63);
-  // (more units than the launch was planned for, which starts that overlap would make, are not cut: the
-  // workgroups that would tell attn_join of them may not be there)
-  const int units = tiles * a.Hkv, rest = units <= a.units ? units % kCUs : 0, first = units - rest;
+  const int units = tiles * a.Hkv, rest = units % kCUs, first = units - rest;
   const int parts = attn_parts(rest, a.span, a.entries);
-  // (attn_join looks at the entries that there may be)
-  if (x < a.entries && x < kCUs && x >= rest && threadIdx.x == 0) meta(a, tile_rows, a.d, x)[0] = 0;
+  // attn_join looks at the entries that there may be. Those past the batch's have nothing for it, nor have
+  // those whose workgroup was not launched, where starts that go back make more units than were planned for
+  // (asked here only: `rest` from a.units at the top cost 4 us of 225 on chunks_wide's sizes).
+  if (x < a.entries && x < kCUs && threadIdx.x == 0 && (x >= rest || first + x >= a.units + a.entries))
+    meta(a, tile_rows, a.d, x)[0] = 0;
   if (x < first) return {x, 0, 1, -1};
   const int y = x - first, part = rest ? y / rest : parts;
   if (part >= parts) return {units, 0, 1, -1};
