@@ -459,10 +459,12 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
             acc += *reinterpret_cast<const v4f*>(&sh.merge[w][row][ch + i]);
           y[i] = acc[0], y[i + 1] = acc[1], y[i + 2] = acc[2], y[i + 3] = acc[3];
         }
-        if (whole)
+        if (whole) {
+          if (!sees_any(a, s.len, s.len - s.n + a.by_group(tr))) sum = INFINITY;
           store_row<C>(out_row(a, D, s.q0, h, tr) + ch, y, sum);
-        else
+        } else {
           store_part<C>(a, kTile, D, 2 * blockIdx.x + which, f * 16 + row, ch, y, tm * c, sum);
+        }
       }
       __syncthreads();
     }
@@ -502,7 +504,8 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int 
   }
   if (!n) return;
   const int tile = a.by_heads(unit), h = unit - tile * a.Hkv;
-  const int q0 = scalar_load(a.starts + b), R = (scalar_load(a.starts + b + 1) - q0) * a.group;
+  const int len = scalar_load(a.lens + b), q0 = scalar_load(a.starts + b);
+  const int queries = scalar_load(a.starts + b + 1) - q0, R = queries * a.group;
   const int tr = tile * tile_rows + row;
   const int last = row < rows && tr < R ? n : -1;        // no partial results of a row beyond
   // partial 0 is the last of workgroup i0, partial k > 0 the first of workgroup i0 + k
@@ -549,6 +552,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a, int tile_rows, int 
   }
   if (last < 0) return;
   const float out[4] = {y[0], y[1], y[2], y[3]};
+  if (!sees_any(a, len, len - queries + a.by_group(tr))) sum = INFINITY;
   store_row<4>(out_row(a, D, q0, h, tr) + 4 * lane, out, sum);
 }
 

@@ -91,6 +91,11 @@ __device__ __forceinline__ int first_seen(const AttnArgs& a, int place) {
   return a.window > 0 ? max(place, 0) - a.window + 1 : 0;
 }
 
+// Whether a query at `place` of a sequence of len tokens sees any.
+__device__ __forceinline__ bool sees_any(const AttnArgs& a, int len, int place) {
+  return (a.causal ? min(place + 1, len) : len) > max(first_seen(a, place), 0);
+}
+
 // Tokens [lo, hi) that the queries first .. last of a sequence see between them (lo rounded down to a
 // step), and [all_lo, all_hi) that each of them sees.
 struct Span { int lo, hi, all_lo, all_hi; };
@@ -193,13 +198,14 @@ __device__ __forceinline__ void each_value_pair(Vec v0, uint32_t s0, Vec v1, uin
   }
 }
 
-// C consecutive channels of an output row: y / sum in bf16, zeros where nothing was summed.
+// C consecutive channels of an output row: y / sum in bf16. A query that sees nothing has y = 0 and is given
+// an infinite sum, for zeros; one whose scores are all -infinity has y = 0 and sum = 0, for NaN.
 template <int C>
 __device__ __forceinline__ void store_row(uint16_t* out, const float y[C], float sum) {
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = 1.0f / sum;
   float z[C];
 #pragma unroll
-  for (int i = 0; i < C; ++i) z[i] = sum == 0.0f ? 0.0f : y[i] * inv;
+  for (int i = 0; i < C; ++i) z[i] = y[i] * inv;
   if constexpr (C == 1) {
     *out = (uint16_t)bf16x2(z[0], 0.0f);
   } else {

@@ -505,6 +505,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void attn_tiles(AttnArgs a) {
 
   l += __shfl_xor(l, 32);
   if (w0 + (lane & 31) >= R) return;
+  if (work.parts == 1 && hi <= max(lo, 0)) l = INFINITY;
   uint16_t* out = out_row(a, D, s.q0, h, row);
 #pragma unroll
   for (int i = 0; i < CT; ++i)
