@@ -61,3 +61,27 @@ def test_threads_on_streams_of_their_own():
     for i in range(4):
         for o in outs[i]:
             assert np.array_equal(host_u16(o), want[i])
+
+
+def test_writes_into_the_cache_are_seen_by_autograd():
+    """A tensor saved for a backward pass and written since is noticed, as after any op in place."""
+    bf = lambda *s: torch.ones(s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    slots = torch.arange(3, device="cuda")
+    for write in (lambda c, t: K.qk_norm_rope_append(bf(3, 4, 64), bf(3, 2, 64), bf(3, 2, 64), None, None, None,
+                                                     None, c, slots),
+                  lambda c, t: K.move_pages(c, torch.tensor([[0, 1]], dtype=torch.int32), t)):
+        for mode in (torch.enable_grad, torch.no_grad, torch.inference_mode):
+            cache, table = K.new_cache(3, 2, 16, 64), torch.zeros((1, 2), dtype=torch.int32, device="cuda")
+            w = torch.ones((), device="cuda", requires_grad=True)
+            y = (w * cache).sum()
+            before = cache._version
+            with mode():
+                write(cache, table)
+            assert cache._version > before
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                y.backward()
+    assert table._version > 0
+    with torch.inference_mode():                # made there: no versions, and none asked for
+        cache = K.new_cache(3, 2, 16, 64)
+        K.move_pages(cache, torch.tensor([[0, 1]], dtype=torch.int32))
+        assert not cache.any()

@@ -88,6 +88,11 @@ void launch(c10::Device dev, F f) {
   check(status);
 }
 
+// A tensor that a launch has written: what autograd saved of it before is out of date.
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor new_bf16(c10::Device dev, at::IntArrayRef shape) {
   return at::empty(shape, at::TensorOptions().dtype(at::kBFloat16).device(dev));
 }
@@ -237,6 +242,7 @@ PyObject* qk_norm_rope_append(const Args& a) {
         address_as<const int>(r.axis), address_as<void>(qo), c.p, c.pages, c.stride, c.page,
         address_as<const int64_t>(slots), q.T, q.H, k.H, q.d, eps, r.flags, stream);
   });
+  written(cache);
   return THPVariable_Wrap(qo);
 }
 
@@ -329,6 +335,7 @@ PyObject* move_pages(const Args& a) {
                             address_as<const int>(pairs), n,
                             rows && cols ? address_as<int>(table) : nullptr, rows, cols, row, stream);
     });
+  written(cache), written(table);
   Py_RETURN_NONE;
 }
 
