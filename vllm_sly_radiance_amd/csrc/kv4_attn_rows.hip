@@ -292,7 +292,10 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
       if (wave + j * W < RF * KS) sh.q[wave + j * W][lane] = ops[j];
     __syncthreads();
     for (; t < t1; t += kGranule) {
-      if (ta.nan | tb.nan) {           // (a branch: two more values in the products' loop spill registers)
+      // (A branch: two more values in the products' loop spill registers. Here and below the compiler is
+      // told that it is seldom taken: without, 4 sequences of 500 tokens, 5 queries, 24 and 4 heads of 256
+      // took 16.9 us in place of 16.0.)
+      if (__builtin_expect((ta.nan | tb.nan) != 0, 0)) {
 #pragma unroll
         for (int p = 0; p < P; ++p) w[0].ks[p] |= ta.nan, w[1].ks[p] |= tb.nan;
       }
@@ -361,7 +364,7 @@ __global__ __launch_bounds__(64 * W, attn_waves(D, RF)) void attn_rows(AttnArgs 
       uint32_t nan = 0;
 #pragma unroll
       for (int p = 0; p < P; ++p) nan |= nan_scales(w[0].vs[p]) | nan_scales(w[1].vs[p]);
-      if (__ballot(nan != 0)) {
+      if (__builtin_expect(__ballot(nan != 0) != 0, 0)) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
           float is[8];
