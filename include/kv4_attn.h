@@ -112,7 +112,8 @@ int kv4_gather(const void* cache, long pages, long page_stride, int page, const 
  * sequence longer than the table's row or max_len, of more queries than max_q, or with tokens in a
  * cache of no pages, all of its. Query head h reads kv head h / (q_heads / kv_heads).
  * out bf16 [total, q_heads, d], contiguous. scale > 0. Scores, softmax statistics and sums are fp32;
- * the weights of the values are rounded to bf16 for the matrix cores.
+ * the weights of the values are rounded to bf16 for the matrix cores. They are relative to a running
+ * maximum that may lag by 2^8, so that sums over values beyond 2^100 may pass fp32's range.
  * workspace: kv4_attention_workspace() bytes, 16-byte aligned (may be null for 0), free again when
  * the launches have run. */
 int kv4_attention(const void* q, long q_ts, long q_hs, const void* cache, long pages,

@@ -628,18 +628,18 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   // attn_tiles or attn_rows: a workgroup of attn_tiles does what four row tiles (of 64 rows, 32 at
   // D = 256) of attn_rows do, in the time of 2.6 of them; but it has a CU to itself, so that few of
   // them are cut into parts, each with a start, an end and partial results of its own. Against 4096
-  // cached tokens, attn_tiles and attn_rows with attn_join in us:
-  //   d = 128, 32 query and 8 kv heads      d = 256, 24 and 4               d = 64, 64 and 8
-  //   1 x 128 queries    64 tiles  31  32   1 x 100  76 tiles  41  43       1 x 64    64 tiles  23  22
-  //   1 x 256           128        40  41   1 x 512 384       104 122       1 x 512  512        60  70
-  //   1 x 512           256        53  61   4 x 256 768       173 226
-  //   1 x 1024          512        85  96   and 32 and 32 heads of 64:
-  //   1 x 4096         2048       153 300                                   1 x 600  320        55  54
-  //   16 x 33 (132 rows) 384       79  86
+  // cached tokens, attn_tiles and attn_rows with attn_join in us a call:
+  //   d = 128, 32 query and 8 kv heads        d = 256, 24 and 4                 d = 64, 64 and 8
+  //   1 x 128 queries    64 tiles  28  32     1 x 100  76 tiles  39  42         1 x 64    64 tiles  20  23
+  //   1 x 256           128        38  40     1 x 512 384        96 124         1 x 512  512        53  61
+  //   1 x 512           256        49  57     4 x 256 768       161 229
+  //   1 x 1024          512        79  83                                       and 32 and 32 heads of 64:
+  //   1 x 4096         2048       137 273                                       1 x 600  320        51  52
+  //   16 x 33 (132 rows) 384       74  80
   // Decoding sequences beside a chunk in attn_rows are read with the chunk's 64 rows: with 100 MB of cache
   // and more that costs more than the two launches of attn_rows beside attn_tiles do: one chunk and 47
-  // sequences of 4000 tokens, d = 128, 64 queries: 74 and 89, 256: 79 and 92; 100 queries and 7
-  // sequences of 3000: 37 and 26.
+  // sequences of 4000 tokens, d = 128, 64 queries: 73 and 78, 256: 83 and 83; 100 queries and 7
+  // sequences of 3000: 42 and 35.
   const long rows_tile = d == 256 ? 32 : 64;
   // all sequences have max_q queries
   const bool even = total == (long)batch * max_q;
@@ -680,13 +680,13 @@ AttnPlan attn_plan(int total, int batch, int max_q, int max_len, int Hq, int Hkv
   const long most_units = (long)batch * Hkv * ((few + tile - 1) / tile);
   const long units = p.few_rows ? most_units : tiles_of_batch(tile) * Hkv;
   // A workgroup a unit, and no second launch, where its waves have few steps to go, or the units are many
-  // and of like length enough. Equal lengths L, such workgroups and runs with the join, us (d = 128,
+  // and of like length enough. Equal lengths L, such workgroups and runs with the join, us a call (d = 128,
   // 32 query and 8 kv heads unless said):
-  //   L = 1000, 1 sequence  10.4  11.8    L = 2000, 1    14.4  11.5    L = 3000, 32     25.0  29.7
-  //                    16   11.1  17.6              4    14.6  13.2             100     70.6  75.5
-  //                    64   17.5  24.0             16    15.3  18.9    L = 6000, 16     32.8  31.8
-  //   8 queries (32 rows)                         200    88.2  98.7    200 .. 6000, 48  47.3  45.7
-  //   L = 800, 8 sequences  13.0  20.0    8 x 3 rows, 16 kv heads, L = 2000: 20.2  22.0, L = 3000: 25.2  24.9
+  //   L = 1000, 1 sequence   9.7   9.9    L = 2000, 1    13.8  10.2    L = 3000, 32     20.5  25.5
+  //                    16   10.0  14.3              4    14.1  11.6             100     66.2  68.1
+  //                    64   16.5  22.3             16    14.3  16.1    L = 6000, 16     30.2  26.9
+  //   8 queries (32 rows)                         200    85.5  96.6    200 .. 6000, 48  43.1  36.8
+  //   L = 800, 8 sequences  12.4  17.6    8 x 3 rows, 16 kv heads, L = 2000: 14.0  15.9, L = 3000: 18.4  17.9
   const long waves_step = kStep * attn_whole_waves(p.fragments), steps = (span + waves_step - 1) / waves_step;
   // (not where most of those workgroups would have nothing to do)
   if (most_units <= 2 * units && (steps <= 4 || (span <= (p.fragments == 1 ? 4096 : 2048) && units >= 16 * steps))) {
