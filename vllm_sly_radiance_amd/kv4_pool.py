@@ -127,7 +127,7 @@ class PagePool:
     def extend(self, sequences: Sequence[int], counts: Sequence[int]) -> Step:
         """Room for counts[i] more tokens of each sequence, and the step that fills it. The last, partly
         filled page of a sequence that shares it is copied first (in all layers, one launch, on the
-        current stream). RuntimeError, with nothing changed, where the free pages do not suffice."""
+        current stream). RuntimeError where the free pages do not suffice; what fails changes nothing."""
         if len(sequences) != len(counts) or len(set(sequences)) != len(sequences):
             _fail(f"extend of sequences {list(sequences)} by {list(counts)}")
         batch = [self._get(i) for i in sequences]
@@ -146,22 +146,36 @@ class PagePool:
             need += -(-(s.length + n) // self.page) - len(s.pages) + copy
         if need > len(self._free):
             _fail(f"{need} pages needed, {len(self._free)} of {self.pages} free")
-        pairs = []
-        for s, n, copy in zip(batch, counts, copies):
-            if copy:
-                new = heapq.heappop(self._free)
-                pairs.append((s.pages[-1], new))
-                self._refs[s.pages[-1]] -= 1
-                self._refs[new] = 1
-                s.pages[-1] = new
-            s.length += n
-            while len(s.pages) * self.page < s.length:
-                new = heapq.heappop(self._free)
-                self._refs[new] = 1
-                s.pages.append(new)
-        if pairs:
-            _kv4.move_pages(self.cache, torch.tensor(pairs, dtype=torch.int32))
-        return self._step(batch, counts)
+        pairs, taken, old = [], [], []
+
+        def take():
+            taken.append(heapq.heappop(self._free))
+            self._refs[taken[-1]] = 1
+            return taken[-1]
+        try:
+            for s, n, copy in zip(batch, counts, copies):
+                old.append((s, len(s.pages), s.length, s.pages[-1] if copy else None))
+                if copy:
+                    pairs.append((s.pages[-1], take()))
+                    self._refs[s.pages[-1]] -= 1
+                    s.pages[-1] = taken[-1]
+                s.length += n
+                while len(s.pages) * self.page < s.length:
+                    s.pages.append(take())
+            if pairs:
+                _kv4.move_pages(self.cache, torch.tensor(pairs, dtype=torch.int32))
+            return self._step(batch, counts)
+        except Exception:               # of the launch or an allocation
+            for s, pages, length, shared_page in old:
+                del s.pages[pages:]
+                s.length = length
+                if shared_page is not None:
+                    s.pages[-1] = shared_page
+                    self._refs[shared_page] += 1
+            for p in taken:
+                self._refs[p] = 0
+                heapq.heappush(self._free, p)
+            raise
 
     def _step(self, batch, counts) -> Step:
         # One host buffer and one copy: slots and positions (8 bytes each), then the int32 parts.
