@@ -22,11 +22,18 @@
 // weigh. Short contexts, and many units of middling ones, take a workgroup a unit and no second launch.
 //
 // Bounded by HBM where the cache is long and rows are few: 48 sequences of up to 8000 tokens, 32 query
-// and 8 kv heads of 128, 208 MB: 44 us, 4.7 TB/s (6.05 is what plain reads reach); one sequence of
-// 131072 tokens, 143 MB: 30 us. By the vector units with 16 to 64 rows (the codes' conversion is the
-// same for every row, the weights are not): 8 x 8 queries of 48 + 16 heads against up to 4000 tokens,
-// 49 MB: 20 us. By the launches and three dependent reads (length, page, tokens) where it is short: 500
-// tokens 7.5 us. The join behind it takes 3 to 6.
+// and 8 kv heads of 128, 208 MB: 46 us, 4.5 TB/s (6.05 is what plain reads reach); one sequence of
+// 131072 tokens, 143 MB: 31 us. By the start and the end of a unit where its tokens are few: 8 x 8
+// queries of 48 + 16 heads against up to 4000 tokens, 49 MB: 21 us, 8 of them the longest runs' six
+// granules, at the read rate. By a step's fixed work (maxima, masks, exchanges, addresses) at heads of 64,
+// whose steps read half the bytes: 48 sequences, 32 kv heads, 415 MB: 94 us, 4.4 TB/s. By the launches and
+// three dependent reads (length, page, tokens) where it is short: 500 tokens 8 us. The join behind it takes
+// 4 to 6.
+//
+// Every instance keeps 53 to 84 scalars more than there are registers in lanes of vector registers. Three
+// spill vector registers to memory, for the most part on the path of NaN blocks: 64 rows at D = 128 (17), 32
+// rows at D = 64 (2) and 32 rows at D = 256 in workgroups of 8 waves (39; 4 waves, whose registers suffice,
+// took 17.4 us where these took 15.6).
 #include <algorithm>
 
 #include "kv4_attn.h"

@@ -17,13 +17,14 @@
 // A batch's row tiles seldom fill the CUs evenly. Whole rounds of them take a workgroup each; the last
 // round's are cut along the tokens into as many parts as pay (attn_parts), which attn_join weighs:
 // 300 units of 128 rows against 4096 tokens each at D = 256 took 310 us in two rounds of whole
-// units, and take 222 and 8 for the join with 44 of them in 5 parts.
+// units, and take 206 and 8 for the join with 44 of them in 5 parts.
 //
-// 4096 causal tokens, 32 query and 8 kv heads of 128: 152 us, 900 TFLOP/s of visible products; the
-// cores are busy half of the cycles, at the 1.7 GHz that this load leaves the clock (a large library
-// product of bf16 matrices reaches 1206). Whole steps pipelined in place of
-// 32 tokens, 2 to 10 operands read ahead and a second accumulator for the scores were slower or the
-// same; steps of 64 tokens took 178 us (a barrier and a start of the operand reads each).
+// 4096 causal tokens, 32 query and 8 kv heads of 128: 138 us, 1000 TFLOP/s of visible products, once the
+// card is warm (the first passes 151; a large library product of bf16 matrices reaches 1206). The matrix
+// cores are busy 44 % of the cycles, the vector units 48 %. Whole steps pipelined in place of 32 tokens, 2
+// to 10 operands read ahead and a second accumulator for the scores were slower or the same; steps of 64
+// tokens were 15 % slower (a barrier and a start of the operand reads each). The instance for heads of 128
+// spills 2 vector registers, outside of its loop.
 #include <utility>
 
 #include "kv4_attn.h"
@@ -265,7 +266,7 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int tile_rows, int 
   const int parts = attn_parts(rest, a.span, a.entries);
   // attn_join looks at the entries that there may be. Those past the batch's have nothing for it, nor have
   // those whose workgroup was not launched, where starts that go back make more units than were planned for
-  // (asked here only: `rest` from a.units at the top cost 4 us of 225 on chunks_wide's sizes).
+  // (asked here only: `rest` chosen by a.units cost 4 us of 225 with 300 units at D = 256).
   if (x < a.entries && x < kCUs && threadIdx.x == 0 && (x >= rest || first + x >= a.units + a.entries))
     meta(a, tile_rows, a.d, x)[0] = 0;
   if (x < first) return {x, 0, 1, -1};

@@ -1,7 +1,8 @@
 // Reading tokens back from the 4-bit cache, and moving its pages, for gfx950. Both only move bytes:
-// HBM bounds them where there is enough to move (4096 tokens of 16 heads of 128 read back, 43 MB: 11.1
-// us, 3.8 TB/s; 600 pages of 24 layers moved, 501 MB: 107 us, 4.7 TB/s of the 5.1 that a large copy
-// reaches), launch latency where there is not (61 tokens 2.8 us, 4 pages of 24 layers 3.2).
+// HBM bounds them where there is enough to move (600 pages of 24 layers moved, 501 MB: 107 us, 4.7 TB/s of
+// the 5.1 that a large copy reaches; 4096 tokens of 16 heads of 128 read back, 43 MB: 11.6 us, 3.7 TB/s, with
+// one item a lane in flight, whose codes and scales wait for its slot), launch latency where there is not (61
+// tokens 2.8 us, 4 pages of 24 layers 3.2).
 #include "kv4_attn.h"
 #include "kv4_internal.h"
 

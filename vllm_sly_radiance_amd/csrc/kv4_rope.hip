@@ -12,7 +12,7 @@
 //
 // Bounded by HBM: 4096 tokens of 48 query, 16 key and 16 value heads of 128 with their cache slots, 143
 // MB, 34 us, 4.2 TB/s of the 5.1 that a large copy reaches (vector work alone would take half of it);
-// 3777 tokens of 24 + 4 heads of 256, three axes: 108 MB, 27 us, 4.0 TB/s. Two or four heads in flight
+// 3777 tokens of 24 + 4 heads of 256, three axes: 111 MB, 26 us, 4.2 TB/s. Two or four heads in flight
 // were no faster (fewer waves fit). One token: 4 us, the latency of three dependent reads.
 //
 // Every floating-point step is fixed (no contraction into fused multiply-adds), so the outputs and
