@@ -115,3 +115,18 @@ def test_what_is_plain():
     torch.func.vmap(lambda x: (is_plain(x) and pytest.fail("a batched tensor")) or x * 2)(torch.zeros(2, 2))
     torch.func.grad(lambda x: (is_plain(x) and pytest.fail("a tensor under grad")) or x.sum())(t)
     torch.func.jvp(lambda x: (is_plain(x) and pytest.fail("a tensor under jvp")) or x * 2, (t,), (t,))
+
+
+def test_views_that_are_not_their_bytes_are_not_plain():
+    """A negated view, or a tensor of zeros without memory: the dispatcher makes plain ones of them."""
+    is_plain = K._native.ops().is_plain
+    t = torch.arange(3.0)
+    assert not is_plain(torch._neg_view(t)) and not is_plain(torch._efficientzerotensor((3,)))
+    assert is_plain(torch._neg_view(t).resolve_neg(), t[::2], t.expand(2, 3))
+
+
+def test_a_negated_view_is_what_it_says(seen):
+    q, k = q_k()
+    a, b = K.qk_norm_rope(torch._neg_view(q), k, None, None, None, None)
+    assert torch.equal(a, -2 * q) and torch.equal(b, 3 * k)
+    assert not seen[0][0].is_neg()

@@ -339,8 +339,15 @@ PyObject* move_pages(const Args& a) {
   Py_RETURN_NONE;
 }
 
+// What the dispatcher resolves before an op sees it: the tensors of transforms (vmap's have no storage),
+// subclasses with a dispatch of their own, views that stand for other values than their bytes.
+constexpr c10::DispatchKeySet kNotPlain({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                         c10::DispatchKey::Functionalize, c10::DispatchKey::Python,
+                                         c10::DispatchKey::Negative, c10::DispatchKey::Conjugate,
+                                         c10::DispatchKey::ZeroTensor});
+
 // Whether the tensors among the arguments may be taken as they are, past the dispatcher: none is of a
-// subclass, a transform's (vmap's have no storage), or one that a gradient is asked of.
+// subclass or of those keys, and no gradient is asked of any.
 bool plain(PyObject* const* args, Py_ssize_t n) {
   const bool grad = c10::GradMode::is_enabled();
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -351,11 +358,7 @@ bool plain(PyObject* const* args, Py_ssize_t n) {
       continue;
     }
     const Tensor& t = THPVariable_Unpack(x);
-    const c10::DispatchKeySet keys = t.key_set();
-    if (keys.has(c10::DispatchKey::FuncTorchBatched) || keys.has(c10::DispatchKey::FuncTorchGradWrapper) ||
-        keys.has(c10::DispatchKey::Functionalize) || keys.has(c10::DispatchKey::Python) ||
-        (grad && t.requires_grad()))
-      return false;
+    if (t.key_set().has_any(kNotPlain) || (grad && t.requires_grad())) return false;
   }
   return true;
 }
