@@ -7,6 +7,10 @@ vllm-sly-radiance (sly/mxfp4/radiance_mxfp4.py + radiance_mxfp4_fp8.hip).
                    attention, gather, page moves (ops radiance::kv4_*, radiance::qk_norm_rope*)
   kv4_pool         the host's side of that cache: pages, forks, steps of a batch
   _native_kv4      ctypes binding of libkv4_attn.so (C ABI in include/kv4_attn.h)
+  radiance_gdn     linear-attention layers between their projections: causal convolution, gated delta
+                   rule (ops radiance::causal_conv, ::gated_delta_rule)
+  radiance_sample  tokens from logits: temperature, top-k, top-p, min-p (op radiance::sample)
+  _native_decode   ctypes binding of libdecode_ops.so (C ABI in include/decode_ops.h)
   synthetic        seeded operands with the benchmark distributions
   build            hipcc recipe for the libraries
 """

@@ -1,12 +1,13 @@
-"""Build libw4a8_mxfp4.so and libkv4_attn.so in-tree with hipcc for gfx950 (no other target), and
-_kv4_torch.so, the latter's binding to torch tensors, with the host compiler.
+"""Build libw4a8_mxfp4.so, libkv4_attn.so and libdecode_ops.so in-tree with hipcc for gfx950 (no other
+target), and _kv4_torch.so and _decode_torch.so, the latter two's bindings to torch tensors, with the host
+compiler.
 
     python -m vllm_sly_radiance_amd.build            # or __graft_entry__.build()
 
-The libraries are plain C-ABI shared objects (include/w4a8_mxfp4.h, include/kv4_attn.h) loaded
-through ctypes; they link the HIP runtime by soname, so inside a torch process they bind to the
-runtime torch already loaded. _kv4_torch.so is a CPython module over libkv4_attn.so, built against the
-installed torch's headers.
+The libraries are plain C-ABI shared objects (include/w4a8_mxfp4.h, include/kv4_attn.h,
+include/decode_ops.h) loaded through ctypes; they link the HIP runtime by soname, so inside a torch process
+they bind to the runtime torch already loaded. The bindings are CPython modules over them, built against
+the installed torch's headers.
 """
 from __future__ import annotations
 
@@ -32,7 +33,12 @@ KV4_LIB_PATH = os.path.join(PKG, "libkv4_attn.so")
 KV4_SOURCES = ["kv4_api.hip", "kv4_rope.hip", "kv4_pages.hip", "kv4_attn_rows.hip",
                "kv4_attn_tiles.hip"]
 KV4_TORCH_PATH = os.path.join(PKG, "_kv4_torch.so")
-KV4_TORCH_SOURCE = "kv4_torch.cpp"
+DECODE_LIB_NAME = "libdecode_ops.so"
+DECODE_SOURCES = ["dec_api.hip", "dec_conv.hip", "dec_delta_steps.hip", "dec_sample.hip"]
+DECODE_TORCH_NAME = "_decode_torch.so"
+# binding -> its source and the library that it is over
+BINDINGS = {os.path.basename(KV4_TORCH_PATH): ("kv4_torch.cpp", os.path.basename(KV4_LIB_PATH)),
+            DECODE_TORCH_NAME: ("decode_torch.cpp", DECODE_LIB_NAME)}
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
@@ -60,8 +66,10 @@ def _command(sources, out) -> list[str]:
 
 
 def _torch_commands(out) -> tuple[list[str], list[str]]:
-    """Compile and link the torch binding (the link needs libkv4_attn.so, found again beside it)."""
+    """Compile and link the torch binding that `out` (with .tmp) is to be (the link needs its library,
+    found again beside it)."""
     import torch
+    source, library = BINDINGS[os.path.basename(out).removesuffix(".tmp")]
     base = os.path.dirname(torch.__file__)
     cxx = os.environ.get("CXX") or "g++"
     system = [os.path.join(base, "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
@@ -69,8 +77,8 @@ def _torch_commands(out) -> tuple[list[str], list[str]]:
                 "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}",
                 *(a for d in system for a in ("-isystem", d)),
-                os.path.join(CSRC, KV4_TORCH_SOURCE), "-o", out + ".o"]
-    link = [cxx, "-shared", out + ".o", "-o", out, f"-L{PKG}", "-l:" + os.path.basename(KV4_LIB_PATH),
+                os.path.join(CSRC, source), "-o", out + ".o"]
+    link = [cxx, "-shared", out + ".o", "-o", out, f"-L{PKG}", "-l:" + library,
             f"-L{os.path.join(base, 'lib')}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
             "-Wl,-rpath,$ORIGIN"]
     return compile_, link
@@ -97,35 +105,38 @@ def _end(job, verbose) -> None:
 
 
 def build(verbose: bool = False) -> str:
-    """Compile every source into LIB_PATH, KV4_LIB_PATH and KV4_TORCH_PATH (always rebuilds, all at
-    once) and return LIB_PATH. What compiles is put in place whatever becomes of the rest: the linear
-    path's library needs hipcc only. RuntimeError at the end where something did not."""
+    """Compile every source into the libraries and their bindings (always rebuilds, all at once) and
+    return LIB_PATH. What compiles is put in place whatever becomes of the rest: the linear path's library
+    needs hipcc only. RuntimeError at the end where something did not."""
+    decode_lib, decode_torch = (os.path.join(os.path.dirname(LIB_PATH), n)
+                                for n in (DECODE_LIB_NAME, DECODE_TORCH_NAME))
     libraries = [(path, _run(_command(sources, path + ".tmp"), verbose))
-                 for sources, path in ((SOURCES, LIB_PATH), (KV4_SOURCES, KV4_LIB_PATH))]
-    tmp, errors, link = KV4_TORCH_PATH + ".tmp", [], None
-    try:
-        compile_, link = _torch_commands(tmp)
-        binding = _run(compile_, verbose)
-    except (OSError, ImportError, AttributeError) as e:        # no host compiler, no torch or not its headers
-        binding, link = None, None
-        errors.append(f"_kv4_torch cannot be built: {e}")
+                 for sources, path in ((SOURCES, LIB_PATH), (KV4_SOURCES, KV4_LIB_PATH),
+                                       (DECODE_SOURCES, decode_lib))]
+    errors, bindings = [], []
+    for path, library in ((KV4_TORCH_PATH, KV4_LIB_PATH), (decode_torch, decode_lib)):
+        try:
+            compile_, link = _torch_commands(path + ".tmp")
+            bindings.append((path, library, _run(compile_, verbose), link))
+        except (OSError, ImportError, AttributeError) as e:    # no host compiler, no torch or not its headers
+            errors.append(f"{os.path.basename(path).removesuffix('.so')} cannot be built: {e}")
+    built = set()
     for path, job in libraries:
         try:
             _end(job, verbose)
             os.replace(path + ".tmp", path)
+            built.add(path)
         except RuntimeError as e:
             errors.append(str(e))
-            if path == KV4_LIB_PATH:
-                link = None
-    try:
-        if binding:
-            _end(binding, verbose)
-            if link:
+    for path, library, job, link in bindings:
+        try:
+            _end(job, verbose)
+            if library in built:
                 _end(_run(link, verbose), verbose)
-                os.replace(tmp, KV4_TORCH_PATH)
-            os.remove(tmp + ".o")
-    except RuntimeError as e:
-        errors.append(str(e))
+                os.replace(path + ".tmp", path)
+            os.remove(path + ".tmp.o")
+        except RuntimeError as e:
+            errors.append(str(e))
     if errors:
         raise RuntimeError("\n".join(errors))
     return LIB_PATH

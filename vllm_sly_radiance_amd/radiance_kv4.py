@@ -76,11 +76,11 @@ _compiling, _jit_tracing = _rmx._compiling, _rmx._jit_tracing
 _dispatch_modes, _function_modes = _rmx._dispatch_modes, _rmx._function_modes
 
 
-def _entry(op, name):
-    """The native op `name`, called without the dispatcher (3 us a call) where nothing watches ops by name
-    and every tensor is plain; else `op`, whose name a compiler, a tracer, a mode or a subclass sees, which
-    vmap maps and whose backward raises. The binding looks at the tensors (kv4_torch.cpp), 1 us a call less
-    than fewer of these checks took here."""
+def _entry(op, name, native=_native):
+    """The op `name` of `native`'s binding, called without the dispatcher (3 us a call) where nothing watches
+    ops by name and every tensor is plain; else `op`, whose name a compiler, a tracer, a mode or a subclass
+    sees, which vmap maps and whose backward raises. The binding looks at the tensors (torch_args.h), 1 us a
+    call less than fewer of these checks took here."""
     ns, public = op._qualname.split("::")
     space = getattr(torch.ops, ns)
     name += "_if_plain"
@@ -89,7 +89,7 @@ def _entry(op, name):
         # _rmx._watched() inline, as in its own call sites
         if not (_compiling() or _dispatch_modes() or _jit_tracing()
                 or (_function_modes() and _rmx._function_mode_watches())):
-            out = getattr(_native.ops(), name)(*args)
+            out = getattr(native.ops(), name)(*args)
             if out is not NotImplemented:
                 return out
         return getattr(space, public)(*args)
