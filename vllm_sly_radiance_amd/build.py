@@ -34,7 +34,8 @@ KV4_SOURCES = ["kv4_api.hip", "kv4_rope.hip", "kv4_pages.hip", "kv4_attn_rows.hi
                "kv4_attn_tiles.hip"]
 KV4_TORCH_PATH = os.path.join(PKG, "_kv4_torch.so")
 DECODE_LIB_NAME = "libdecode_ops.so"
-DECODE_SOURCES = ["dec_api.hip", "dec_conv.hip", "dec_delta_steps.hip", "dec_sample.hip"]
+DECODE_SOURCES = ["dec_api.hip", "dec_conv.hip", "dec_delta_steps.hip", "dec_delta_chunks.hip",
+                  "dec_sample.hip"]
 DECODE_TORCH_NAME = "_decode_torch.so"
 # binding -> its source and the library that it is over
 BINDINGS = {os.path.basename(KV4_TORCH_PATH): ("kv4_torch.cpp", os.path.basename(KV4_LIB_PATH)),

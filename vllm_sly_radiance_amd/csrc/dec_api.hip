@@ -67,8 +67,8 @@ int check_delta_sizes(const char* who, int total, int batch, int max_q, int writ
     return fail(DEC_EINVAL, "%s: %d value heads over %d key heads", who, v_heads, k_heads);
   if ((dk != 64 && dk != 128) || (dv != 64 && dv != 128))
     return fail(DEC_EINVAL, "%s: heads of %d and %d channels are none of 64, 128", who, dk, dv);
-  if ((long)batch * v_heads * (dv / 16) > kMaxGrid)
-    return fail(DEC_EINVAL, "%s: batch=%d of %d heads is too large", who, batch, v_heads);
+  if ((long)batch * v_heads * (dv / 16) > kMaxGrid || ((long)total / kChunk + batch) * v_heads > kMaxGrid)
+    return fail(DEC_EINVAL, "%s: total=%d batch=%d of %d heads is too large", who, total, batch, v_heads);
   return DEC_OK;
 }
 
@@ -149,6 +149,10 @@ DEC_API int dec_gated_delta(const void* q, long q_ts, long q_hs, const void* k, 
   d.a = (const uint16_t*)a, d.a_ts = a_ts, d.b = (const uint16_t*)b, d.b_ts = b_ts;
   d.a_log = a_log, d.dt_bias = dt_bias, d.state = state, d.out = (uint16_t*)out, d.workspace = workspace;
   d.Hk = k_heads, d.Hv = v_heads, d.scale = scale, d.eps = eps;
+  if (plan.chunks) {
+    d.kt = plan.kt;
+    return hip_status(launch_delta_chunks(d, dk, dv, (hipStream_t)stream), who);
+  }
   return hip_status(launch_delta_steps(d, dk, dv, (hipStream_t)stream), who);
 }
 

@@ -110,6 +110,4 @@ hipError_t launch_delta_steps(const DeltaArgs& a, int dk, int dv, hipStream_t st
   return dv == 128 ? launch<64, 128>(a, stream) : launch<64, 64>(a, stream);
 }
 
-DeltaPlan delta_plan(int, int, int, int, int, int, int, int) { return {}; }
-
 }  // namespace dec

@@ -66,6 +66,7 @@ struct DeltaArgs {
   float* state;
   uint16_t* out;
   void* workspace;
+  size_t kt;              // where in it the chunks' K^T begin
   long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, a_ts, b_ts;
   Sequences s;
   int Hk, Hv;
@@ -73,10 +74,12 @@ struct DeltaArgs {
   Divisor by_units, by_heads, by_group;   // set at the launch
 };
 struct DeltaPlan {
-  bool chunks;
-  size_t workspace;
+  bool chunks;            // in chunks, or token after token
+  size_t kt, workspace;
 };
+constexpr int kChunk = 64;
 DeltaPlan delta_plan(int total, int batch, int max_q, int write_cols, int Hk, int Hv, int dk, int dv);
+hipError_t launch_delta_chunks(const DeltaArgs& a, int dk, int dv, hipStream_t stream);
 hipError_t launch_delta_steps(const DeltaArgs& a, int dk, int dv, hipStream_t stream);
 
 struct SampleArgs {
