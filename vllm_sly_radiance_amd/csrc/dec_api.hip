@@ -150,7 +150,7 @@ DEC_API int dec_gated_delta(const void* q, long q_ts, long q_hs, const void* k, 
   d.a_log = a_log, d.dt_bias = dt_bias, d.state = state, d.out = (uint16_t*)out, d.workspace = workspace;
   d.Hk = k_heads, d.Hv = v_heads, d.scale = scale, d.eps = eps;
   if (plan.chunks) {
-    d.kt = plan.kt;
+    d.keys = plan.keys;
     return hip_status(launch_delta_chunks(d, dk, dv, (hipStream_t)stream), who);
   }
   return hip_status(launch_delta_steps(d, dk, dv, (hipStream_t)stream), who);

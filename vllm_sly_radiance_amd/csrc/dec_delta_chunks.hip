@@ -5,18 +5,21 @@
 //   (1 + A) U = diag(beta) (V - diag(e^G) K S),   A_ij = beta_i e^(G_i - G_j) k_i . k_j for j < i
 //   O = scale (diag(e^G) Q S + P U),              P_ij = e^(G_i - G_j) q_i . k_j for j <= i
 //   S <- e^(G_63) S + K^T diag(e^(G_63 - G)) U
-// A and P do not depend on the state: delta_prepare makes (1 + A)^-1 diag(beta), P and K^T of every chunk and
+// A and P do not depend on the state: delta_prepare makes T = (1 + A)^-1 diag(beta) and P of every chunk and
 // head at once, and delta_chunks goes through a sequence's chunks with the state in registers.
 //
-// delta_chunks: a wave has 16 columns of a state, which do not meet others, so that its products need no
-// other wave. As a matrix instruction's result a column is a lane and 4 rows of 16 lie in a lane's registers;
-// as its operand a column is a lane and 8 of the 32 terms lie in them. The sums run over whatever order of
-// terms both operands have, so with rows 8 g + 4 e + r of 32 in tile e, lane group g and register r, two
-// result tiles are one operand as they are: S, X = V - K S and U go from product to product without
-// leaving their lanes. The other operands are rows of 8 consecutive elements in memory.
+// Operands are fp16. A row of K or Q is scaled by a power of two and then exact; what comes from sums in fp32 is
+// scaled likewise (T and P by 2^12, columns of S, X = V - diag(e^G) K S and U by their largest element) and
+// split into two parts that add up to it, the second the rounding of what the first leaves: 22 bits, and
+// products of two such as three instructions. Two parts of bf16 hold 16 bits, and three of them took 182
+// instructions a chunk in place of 132. A state is as far from the definition as a plain evaluation in fp32.
 //
-// The operands that come from sums are in fp32 and a bf16 operand holds 8 bits: they are split into parts
-// that add up to them, K and Q are exact.
+// A wave has 16 columns of a state, which do not meet others, so that its products need no other wave. As a
+// matrix instruction's result a column is a lane and 4 rows of 16 lie in a lane's registers; as its operand a
+// column is a lane and 8 of the 32 terms lie in them. The sums run over whatever order of terms both
+// operands have, so with rows 8 g + 4 e + r of 32 in tile e, lane group g and register r (place(), below),
+// two result tiles are one operand as they are: S, X and U go from product to product without leaving their
+// lanes. The other operands come from memory in the order in which lanes want them.
 #include "decode_ops.h"
 #include "dec_delta.h"
 #include "dec_internal.h"
@@ -24,43 +27,86 @@
 namespace dec {
 namespace {
 
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* global_ptr;
+
 constexpr int C = kChunk;
-constexpr int kTParts = 3, kPParts = 2, kSParts = 3, kXParts = 3, kUParts = 2, kQParts = 2;
 constexpr int kPad = 68;                // floats of a row of a chunk's matrices in LDS
+constexpr int kFrag = 1024;             // bytes of an operand: 64 lanes of 16
+constexpr int kLower = 6;               // operands of T or P: row tiles 0, 1 with terms 0..31, tiles 2, 3 with all
+constexpr float kUnit = 4096.0f;        // what T and P are scaled by
 
 // A chunk and head's part of the workspace.
 struct ChunkHead {
-  uint16_t t[kTParts][C][C];
-  uint16_t p[kPParts][C][C];
-  float k_factor[C], q_factor[C], u_factor[C];   // e^G / |k|, scale e^G / |q|, e^(G_63 - G) / |k|
-  float decay, pad[3];                           // e^(G_63)
+  v8h t[2][kLower][64];
+  float k_factor[C], u_factor[C];       // e^G / |k|, e^(G_63 - G) / |k|, for the scaled k
+  float decay, pad[C - 1];              // e^(G_63)
+  float q_factor[C];                    // e^G / |q|, for the scaled q
+  v8h p[2][kLower][64];
 };
+constexpr int kHeadStage = 13 * kFrag;  // of it, what delta_chunks takes through LDS
+// A chunk and key head's: K as rows and as columns of the products, and Q.
+template <int DK>
+struct ChunkKeys {
+  v8h k[4][DK / 32][64], kt[DK / 16][2][64], q[4][DK / 32][64];
+};
+template <int DK>
+constexpr int kKeysStage = (4 * (DK / 32) + 2 * (DK / 16)) * kFrag;
 
-__device__ __forceinline__ v4f mfma(v8bf a, v8bf b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+// Token (or key channel) of row m of a tile: the order that makes two result tiles an operand.
+__device__ __forceinline__ int place(int tile, int m) {
+  return 32 * (tile >> 1) + 8 * (m >> 2) + 4 * (tile & 1) + (m & 3);
 }
-__device__ __forceinline__ v8bf load8(const uint16_t* p) { return *reinterpret_cast<const v8bf*>(p); }
+// Operand of row tile t and terms 32 k .. 32 k + 31 among the kLower.
+__device__ __forceinline__ constexpr int lower(int t, int k) { return t < 2 ? t : 2 * t - 2 + k; }
 
-// Parts of 8 fp32 values, each the rounding of what the ones before it leave.
-template <int N>
-__device__ __forceinline__ void split(const float x[8], v8bf part[N]) {
-  uint32_t u[N][4];
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ v2h half2(float a, float b) { return __builtin_convertvector(v2f{a, b}, v2h); }
+
+// x as two parts that add up to it, 8 values.
+__device__ __forceinline__ void split(const float x[8], v8h& hi, v8h& lo) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float lo = x[2 * i], hi = x[2 * i + 1];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      u[n][i] = bf16x2(lo, hi);
-      if (n + 1 < N) lo -= bf16_lo(u[n][i]), hi -= bf16_hi(u[n][i]);
-    }
+  for (int i = 0; i < 8; i += 2) {
+    const v2h a = half2(x[i], x[i + 1]), b = half2(x[i] - (float)a[0], x[i + 1] - (float)a[1]);
+    hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
   }
-#pragma unroll
-  for (int n = 0; n < N; ++n) part[n] = __builtin_bit_cast(v8bf, v4i{(int)u[n][0], (int)u[n][1], (int)u[n][2], (int)u[n][3]});
 }
 
-// K^T of a chunk and key head, [DK][C] bf16.
-__device__ __forceinline__ uint16_t* delta_kt(const DeltaArgs& a, int dk, int c, int hk) {
-  return (uint16_t*)((char*)a.workspace + a.kt) + ((size_t)c * a.Hk + hk) * dk * C;
+// The power of two that brings a magnitude (its bits) to 2^13 .. 2^14, and one over it. What is below 2^-113
+// counts as that; what is not finite stays so.
+__device__ __forceinline__ float scale_to(uint32_t top) { return __uint_as_float((267u - max(top >> 23, 14u)) << 23); }
+__device__ __forceinline__ float scale_back(uint32_t top) { return __uint_as_float((max(top >> 23, 14u) - 13u) << 23); }
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Over the four lanes that have the same column (or row).
+__device__ __forceinline__ uint32_t max_groups(uint32_t x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max((uint32_t)a[0], (uint32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max((uint32_t)b[0], (uint32_t)b[1]);
+}
+__device__ __forceinline__ float sum_groups(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t y = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ v4i load8(const uint16_t* p) { return *reinterpret_cast<const v4i*>(p); }
+// Element i of 8 bf16.
+__device__ __forceinline__ float element(v4i x, int i) { return i & 1 ? bf16_hi((uint32_t)x[i / 2]) : bf16_lo((uint32_t)x[i / 2]); }
+
+// Keys and queries of a chunk slot and key head, behind the heads' parts.
+template <int DK>
+__device__ __forceinline__ ChunkKeys<DK>& delta_keys(const DeltaArgs& a, int c, int hk) {
+  return ((ChunkKeys<DK>*)((char*)a.workspace + a.keys))[(size_t)c * a.Hk + hk];
 }
 
 // Chunk slots: sequence b's begin at starts[b] / 64 + b, so that total / 64 + batch slots hold all.
@@ -81,21 +127,15 @@ __device__ __forceinline__ int sequence_of(const Sequences& s, int c) {
   return count - 1;
 }
 
-__device__ __forceinline__ float sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
-
-template <int DK>
 struct PrepareShared {
-  float a[C][kPad], t[C][kPad], p[C][kPad];
+  float a[C][kPad], t[C][kPad];
   float g_hi[C], g_lo[C], beta[C], rk[C], rq[C];
 };
 
 // One workgroup makes one chunk's matrices for one value head; wave w has rows 16 w .. 16 w + 15.
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
-  __shared__ __attribute__((aligned(16))) PrepareShared<DK> s;
+  __shared__ __attribute__((aligned(16))) PrepareShared s;
   const int c = a.by_heads((int)blockIdx.x), h = (int)blockIdx.x - c * a.Hv;
   const int hk = a.by_group(h);
   const int b = sequence_of(a.s, c);
@@ -112,16 +152,30 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
   const auto load = [&](const uint16_t* p, long ts, long hs, int tile, int step) {
     return load8(p + (row0 + min(16 * tile + col, m - 1)) * ts + hk * hs + 32 * step + 8 * g);
   };
-  v8bf kf[kSteps], qf[kSteps];
-  float kk = 0.0f, qq = 0.0f;
+  // a row scaled to fp16, its sum of squares and its scale
+  const auto scaled = [&](const v4i x[kSteps], v8h y[kSteps], float& squares, float& scale) {
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    kf[i] = load(a.k, a.k_ts, a.k_hs, w, i), qf[i] = load(a.q, a.q_ts, a.q_hs, w, i);
+    for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) kk = fmaf((float)kf[i][j], (float)kf[i][j], kk), qq = fmaf((float)qf[i][j], (float)qf[i][j], qq);
-  }
-  kk = sum_groups(kk), qq = sum_groups(qq);
-  if (g == 0) s.rk[16 * w + col] = 1.0f / sqrtf(kk + a.eps), s.rq[16 * w + col] = a.scale / sqrtf(qq + a.eps);
+      for (int j = 0; j < 8; ++j) top = max(top, magnitude(element(x[i], j)));
+    scale = scale_to(max_groups(top)), squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float z = element(x[i], j) * scale;
+        y[i][j] = (_Float16)z, squares = fmaf(z, z, squares);
+      }
+    squares = sum_groups(squares);
+  };
+  v4i raw[4][kSteps], raw_q[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) raw_q[i] = load(a.q, a.q_ts, a.q_hs, w, i);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) raw[t][i] = load(a.k, a.k_ts, a.k_hs, t, i);
   if (w == 0) {
     // (decays below e^-200 are 0 either way; held to that, the sums stay finite)
     double sum = 0.0;
@@ -139,26 +193,43 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
     // two floats: differences of nearby sums keep the bits of what lies between them
     s.g_hi[lane] = (float)sum, s.g_lo[lane] = (float)(sum - (double)(float)sum), s.beta[lane] = beta;
   }
-  __syncthreads();
+  v8h kf[4][kSteps], qf[kSteps];
+  float rk[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    float squares, scale;
+    scaled(raw[t], kf[t], squares, scale);
+    rk[t] = 1.0f / sqrtf(fmaf(a.eps * scale, scale, squares));
+    if (t == w && g == 0) s.rk[16 * w + col] = rk[t];
+  }
   {
-    const v4f rk = *(const v4f*)&s.rk[16 * w + 4 * g], rq = *(const v4f*)&s.rq[16 * w + 4 * g];
+    float squares, scale;
+    scaled(raw_q, qf, squares, scale);
+    if (g == 0) s.rq[16 * w + col] = 1.0f / sqrtf(fmaf(a.eps * scale, scale, squares));
+  }
+  __syncthreads();
+  v4f p[4] = {};
+  {
+    v8h mine[kSteps];                   // (the row tile is a number that the compiler does not know)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) mine[i] = w < 2 ? (w ? kf[1][i] : kf[0][i]) : w == 2 ? kf[2][i] : kf[3][i];
+    const v4f rki = *(const v4f*)&s.rk[16 * w + 4 * g], rqi = *(const v4f*)&s.rq[16 * w + 4 * g];
     const v4f hi = *(const v4f*)&s.g_hi[16 * w + 4 * g], lo = *(const v4f*)&s.g_lo[16 * w + 4 * g];
     const v4f beta = *(const v4f*)&s.beta[16 * w + 4 * g];
-    for (int tile = 0; tile <= (w | 1); ++tile) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (t > (w | 1)) break;
       v4f ak = {}, aq = {};
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const v8bf f = load(a.k, a.k_ts, a.k_hs, tile, i);
-        ak = mfma(kf[i], f, ak), aq = mfma(qf[i], f, aq);
-      }
-      const int j = 16 * tile + col;
-      const float rkj = s.rk[j], hj = s.g_hi[j], lj = s.g_lo[j];
+      for (int i = 0; i < kSteps; ++i) ak = mfma(mine[i], kf[t][i], ak), aq = mfma(qf[i], kf[t][i], aq);
+      const int j = 16 * t + col;
+      const float hj = s.g_hi[j], lj = s.g_lo[j];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * w + 4 * g + r;
-        const float d = j <= i ? expf((hi[r] - hj) + (lo[r] - lj)) * rkj : 0.0f;
-        s.a[i][j] = j < i ? beta[r] * d * rk[r] * ak[r] : 0.0f;
-        s.p[i][j] = j <= i ? d * rq[r] * aq[r] : 0.0f;
+        const float d = j <= i ? expf((hi[r] - hj) + (lo[r] - lj)) * rk[t] : 0.0f;
+        s.a[i][j] = j < i ? beta[r] * d * rki[r] * ak[r] : 0.0f;
+        p[t][r] = j <= i ? d * rqi[r] * aq[r] : 0.0f;
       }
     }
   }
@@ -210,22 +281,27 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
     }
   }
   __syncthreads();
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    if (t <= (w | 1))
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.a[16 * w + 4 * g + r][16 * t + col] = p[t][r];
+  __syncthreads();
   ChunkHead& out = ((ChunkHead*)a.workspace)[(size_t)c * a.Hv + h];
-  const int i = tid >> 2;
-  if (i >= 32 || (tid & 3) < 2)         // (the blocks that delta_chunks reads)
 #pragma unroll
-    for (int j0 = 0; j0 < 16; j0 += 8) {
-      const int j = (tid & 3) * 16 + j0;
-      float x[8], y[8];
+  for (int x = tid; x < 2 * kLower * 64; x += 256) {
+    const bool is_p = x >= kLower * 64;
+    const int f = (is_p ? x - kLower * 64 : x) >> 6;       // operand, and its row tile and terms
+    const int t = f < 2 ? f : 2 + (f - 2) / 2, k = f < 2 ? 0 : (f - 2) & 1;
+    const int i = place(t, col), j = 32 * k + 8 * g;
+    float y[8];
 #pragma unroll
-      for (int l = 0; l < 8; ++l) x[l] = s.t[i][j + l] * s.beta[j + l], y[l] = s.p[i][j + l];
-      v8bf tp[kTParts], pp[kPParts];
-      split<kTParts>(x, tp), split<kPParts>(y, pp);
-#pragma unroll
-      for (int l = 0; l < kTParts; ++l) *(v8bf*)&out.t[l][i][j] = tp[l];
-#pragma unroll
-      for (int l = 0; l < kPParts; ++l) *(v8bf*)&out.p[l][i][j] = pp[l];
-    }
+    for (int l = 0; l < 8; ++l) y[l] = is_p ? s.a[i][j + l] * kUnit : s.t[i][j + l] * (s.beta[j + l] * kUnit);
+    v8h hi, lo;
+    split(y, hi, lo);
+    v8h(*to)[kLower][64] = is_p ? out.p : out.t;
+    to[0][f][lane] = hi, to[1][f][lane] = lo;
+  }
   if (w == 0) {
     const float hi = s.g_hi[lane], lo = s.g_lo[lane], last = s.g_hi[C - 1], rest = s.g_lo[C - 1];
     const float in = expf(hi), there = lane < m ? 1.0f : 0.0f;
@@ -234,36 +310,183 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
     out.u_factor[lane] = there * (expf((last - hi) + (rest - lo)) * s.rk[lane]);
     if (lane == 0) out.decay = expf(last);
   }
-  if (hk * (a.Hv / a.Hk) == h) {        // K^T once for the heads that share it
+  if (hk * (a.Hv / a.Hk) == h) {        // K and Q once for the heads that share them
+    ChunkKeys<DK>& keys = delta_keys<DK>(a, c, hk);
+    const int token = 16 * w + col, tile = 2 * (token >> 5) + ((token >> 2) & 1);
+    const int row = 4 * ((token >> 3) & 3) + (token & 3);
     __syncthreads();
-    uint16_t(*kt)[C + 8] = (uint16_t(*)[C + 8]) s.a;       // [DK][C], over a and t
+    _Float16(*kt)[C + 8] = (_Float16(*)[C + 8]) s.a;       // [DK][C], over a and t
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const v4i k = __builtin_bit_cast(v4i, kf[step]);
+      const v8h x = w < 2 ? (w ? kf[1][step] : kf[0][step]) : w == 2 ? kf[2][step] : kf[3][step];
+      keys.k[tile][step][16 * g + row] = x;
+      keys.q[tile][step][16 * g + row] = qf[step];
 #pragma unroll
-      for (int l = 0; l < 8; ++l) kt[32 * step + 8 * g + l][16 * w + col] = (uint16_t)((uint32_t)k[l / 2] >> (16 * (l & 1)));
+      for (int l = 0; l < 8; ++l) kt[32 * step + 8 * g + l][token] = x[l];
     }
     __syncthreads();
-    uint16_t* to = delta_kt(a, DK, c, hk);
-    for (int x = tid; x < DK * C / 8; x += 256)
-      *(v8bf*)(to + 8 * x) = *(const v8bf*)&kt[x / (C / 8)][x % (C / 8) * 8];
+#pragma unroll
+    for (int x = tid; x < DK / 8 * 64; x += 256) {
+      const int j = x >> 7, k = (x >> 6) & 1;
+      keys.kt[j][k][lane] = *(const v8h*)&kt[place(j, col)][32 * k + 8 * g];
+    }
   }
 }
 
-// Token (or key channel) of row m of a tile: the order that makes two result tiles an operand.
-__device__ __forceinline__ int place(int tile, int m) { return 32 * (tile >> 1) + 8 * (m >> 2) + 4 * (tile & 1) + (m & 3); }
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
 
-template <int DK>
-__global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a, int dv) {
+// What the waves of a workgroup of delta_chunks share.
+template <int DK, int NW>
+struct ChunkShared {
+  struct Stage {
+    union {
+      struct {
+        v8h t[2][kLower][64];
+        float k_factor[C], u_factor[C], decay, pad[C - 1], unused[C];
+      };
+      char head[kHeadStage];
+    };
+    v8h k[4][DK / 32][64], kt[DK / 16][2][64];
+  } stage[2];
+  struct {
+    v8h s[2][DK / 32][64];              // parts of the state before the chunk
+    v4f u[4][64];
+    float s_back[16], u_back[16];       // one over the columns' scales
+    int done;                           // the outputs are written already
+  } wave[NW];
+};
+
+// A workgroup has 16 NW columns of a sequence and head's state. Waves 0 .. NW - 1 have 16 of them each and go
+// through the chunks; wave NW + i makes the outputs of wave i's columns, a chunk behind, and moves the next
+// chunk's operands to LDS.
+template <int DK, int NW>
+__global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
   constexpr int kSteps = DK / 32, kTiles = DK / 16;
-  const int blocks = dv / 64;
-  const int bh = (int)blockIdx.x / blocks;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  ChunkShared<DK, NW>& sh = *(ChunkShared<DK, NW>*)lds;
+  // a head's parts on one of the 8 dies, which have an L2 each
+  const int part = (int)(blockIdx.x >> 3) % parts, bh = (int)(blockIdx.x >> 3) / parts * 8 + (int)(blockIdx.x & 7);
+  if (bh >= sequences) return;
   const int b = a.by_heads(bh), h = bh - b * a.Hv, hk = a.by_group(h);
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int col0 = ((int)blockIdx.x % blocks) * 64 + (threadIdx.x >> 6) * 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool outputs = wave >= NW;
+  const int mine = outputs ? wave - NW : wave;
+  const int col0 = (part * NW + mine) * 16;
+  auto& ex = sh.wave[mine];
   int first, n;
   rows_of(a.s, b, first, n);
-  const int c0 = first_chunk(a.s, b);
+  const int chunks = ceil_div(n, C), c0 = first_chunk(a.s, b);
+  const auto head_of = [&](int c) -> const ChunkHead& { return ((const ChunkHead*)a.workspace)[(size_t)(c0 + c) * a.Hv + h]; };
+
+  if (outputs) {
+    // ---- operands of chunk c to stage c % 2, this wave's share of them
+    const auto move = [&](int c) {
+      const char* head = (const char*)&head_of(c);
+      const char* keys = (const char*)&delta_keys<DK>(a, c0 + c, hk);
+      auto& to = sh.stage[c & 1];
+      constexpr int kHead = kHeadStage / kFrag, kAll = kHead + kKeysStage<DK> / kFrag;
+#pragma unroll
+      for (int x = 0; x < ceil_div(kAll, NW); ++x) {
+        const int i = x * NW + mine;
+        if (i >= kAll) break;
+        const char* from = i < kHead ? head + i * kFrag : keys + (i - kHead) * kFrag;
+        char* at = i < kHead ? to.head + i * kFrag : (char*)to.k + (i - kHead) * kFrag;
+        __builtin_amdgcn_global_load_lds((global_ptr)(from + 16 * lane), (lds_ptr)at, 16, 0, 0);
+      }
+    };
+    if (chunks) move(0);
+    v8h q[4][kSteps], p[2][kLower], sp[2][kSteps];
+    v4f u[4], s_back;
+    float q_factor[4];
+    bool done = false;
+    const auto load = [&](int c) {
+      const ChunkHead& head = head_of(c);
+      const ChunkKeys<DK>& keys = delta_keys<DK>(a, c0 + c, hk);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        q_factor[t] = head.q_factor[place(t, col)];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) q[t][i] = keys.q[t][i][lane];
+      }
+#pragma unroll
+      for (int l = 0; l < 2; ++l)
+#pragma unroll
+        for (int f = 0; f < kLower; ++f) p[l][f] = head.p[l][f][lane];
+    };
+    for (int c = 0; c <= chunks; ++c) {
+      wait_loads();
+      lds_barrier();                    // A: stage c is there, and all have taken what chunk c - 1 left
+      if (c + 1 < chunks) move(c + 1);
+      if (c > 0 && !done) {
+        // outputs of chunk c - 1: rows are columns of the state, columns tokens
+        uint32_t top = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top = max(top, magnitude(u[t][r]));
+        top = max_groups(top);
+        const float up = scale_to(top);
+        if (g == 0) ex.u_back[col] = scale_back(top) * (1.0f / kUnit);
+        v8h uh[2], ul[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = u[2 * k + i / 4][i & 3] * up;
+          split(y, uh[k], ul[k]);
+        }
+        v4f o[4] = {}, x[4] = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int l = 1; l >= 0; --l)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) o[t] = mfma(sp[l][i], q[t][i], o[t]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int l = 0; l < 3; ++l)
+#pragma unroll
+            for (int t = 2 * k; t < 4; ++t)
+              x[t] = mfma(l == 0 ? ul[k] : uh[k], p[l == 1][lower(t, k)], x[t]);
+        const v4f u_back = *(const v4f*)&ex.u_back[4 * g];
+        const int m = min(n - (c - 1) * C, C);
+        uint16_t* out = a.out + (((size_t)first + (c - 1) * C) * a.Hv + h) * dv + col0 + 4 * g;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int token = place(t, col);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t][r] = a.scale * fmaf(o[t][r], s_back[r] * q_factor[t], x[t][r] * u_back[r]);
+          if (token < m)
+            *reinterpret_cast<uint2*>(out + (size_t)token * a.Hv * dv) =
+                make_uint2(bf16x2(o[t][0], o[t][1]), bf16x2(o[t][2], o[t][3]));
+        }
+      }
+      if (c == chunks) break;
+      load(c);
+      lds_barrier();                    // B: wave `mine` has left what the outputs of chunk c take
+      done = ex.done;
+      s_back = *(const v4f*)&ex.s_back[4 * g];
+#pragma unroll
+      for (int l = 0; l < 2; ++l)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) sp[l][i] = ex.s[l][i][lane];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) u[t] = ex.u[t][lane];
+    }
+    return;
+  }
 
   v4f S[kTiles];
   const int read = a.s.read[b], write = a.s.write[b * a.s.write_stride];
@@ -276,141 +499,154 @@ __global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a, int dv) {
       S[j][r] = read >= 0 && read < a.s.slots
                     ? a.state[read * a.s.slot_stride + at + (size_t)place(j, 4 * g + r) * dv]
                     : fill;
-
-  for (int i0 = 0; i0 < n; i0 += C) {
-    const int m = min(n - i0, C);
-    const size_t row0 = (size_t)first + i0;
-    const ChunkHead& ch = ((const ChunkHead*)a.workspace)[(size_t)(c0 + i0 / C) * a.Hv + h];
-    const uint16_t* kt = delta_kt(a, DK, c0 + i0 / C, hk);
-    v4f x[4] = {}, o[4] = {};
+  // values of chunk c, rows as results have them
+  uint32_t v[16];
+  const auto values = [&](int c) {
+    const uint16_t* from = a.v + ((size_t)first + c * C) * a.v_ts + h * a.v_hs + col0 + col;
+    const int m = min(n - c * C, C);
 #pragma unroll
-    for (int step = 0; step < kSteps; ++step) {
-      v8bf sp[kSParts];
-      const float y[8] = {S[2 * step][0],     S[2 * step][1],     S[2 * step][2],     S[2 * step][3],
-                          S[2 * step + 1][0], S[2 * step + 1][1], S[2 * step + 1][2], S[2 * step + 1][3]};
-      split<kSParts>(y, sp);
+    for (int i = 0; i < 16; ++i) {
+      const int token = place(i >> 2, 4 * g + (i & 3));
+      v[i] = from[(size_t)min(token, m - 1) * a.v_ts];
+    }
+  };
+  if (chunks) values(0);
+  for (int c = 0; c < chunks; ++c) {
+    const auto& st = sh.stage[c & 1];
+    const int m = min(n - c * C, C);
+    uint32_t top = 0;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const size_t row = row0 + min(place(t, col), m - 1);
-        const v8bf kf = load8(a.k + row * a.k_ts + hk * a.k_hs + 32 * step + 8 * g);
-        const v8bf qf = load8(a.q + row * a.q_ts + hk * a.q_hs + 32 * step + 8 * g);
+    for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-        for (int p = kSParts - 1; p >= 0; --p) x[t] = mfma(kf, sp[p], x[t]);
+      for (int r = 0; r < 4; ++r) top = max(top, magnitude(S[j][r]));
+    top = max_groups(top);
+    const float s_to = scale_to(top), s_back = scale_back(top);
+    v8h sh_[kSteps], sl[kSteps];
 #pragma unroll
-        for (int p = kQParts - 1; p >= 0; --p) o[t] = mfma(sp[p], qf, o[t]);
+    for (int i = 0; i < kSteps; ++i) {
+      float y[8];
+#pragma unroll
+      for (int l = 0; l < 8; ++l) y[l] = S[2 * i + l / 4][l & 3] * s_to;
+      split(y, sh_[i], sl[i]);
+    }
+    lds_barrier();                      // A
+    if (g == 0) ex.s_back[col] = s_back;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) ex.s[0][i][lane] = sh_[i], ex.s[1][i][lane] = sl[i];
+    v4f x[4] = {};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int l = 1; l >= 0; --l)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = mfma(st.k[t][i][lane], l ? sl[i] : sh_[i], x[t]);
+    top = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const v4f f = *(const v4f*)&st.k_factor[place(t, 4 * g)];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float y = place(t, 4 * g + r) < m ? __uint_as_float(v[4 * t + r] << 16) : 0.0f;
+        x[t][r] = fmaf(-(f[r] * s_back), x[t][r], y);
+        top = max(top, magnitude(x[t][r]));
       }
     }
-    v8bf xp[2][kXParts];
+    if (c + 1 < chunks) values(c + 1);
+    top = max_groups(top);
+    const float x_to = scale_to(top), x_back = scale_back(top) * (1.0f / kUnit);
+    v8h xh[2], xl[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const v4f f = *(const v4f*)&ch.k_factor[32 * k + 8 * g + 4 * e];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int token = 32 * k + 8 * g + 4 * e + r;
-          const float v = bf16_f32(a.v[(row0 + min(token, m - 1)) * a.v_ts + h * a.v_hs + col0 + col]);
-          y[4 * e + r] = (token < m ? v : 0.0f) - f[r] * x[2 * k + e][r];
-        }
-      }
-      split<kXParts>(y, xp[k]);
+      for (int l = 0; l < 8; ++l) y[l] = x[2 * k + l / 4][l & 3] * x_to;
+      split(y, xh[k], xl[k]);
     }
     v4f u[4] = {};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int l = 0; l < 3; ++l)       // small products first
+#pragma unroll
+        for (int t = 2 * k; t < 4; ++t)
+          u[t] = mfma(st.t[l == 1][lower(t, k)][lane], l == 0 ? xl[k] : xh[k], u[t]);
     float bad = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int k = 0; k <= t / 2; ++k) {
-        v8bf tf[kTParts];
-#pragma unroll
-        for (int p = 0; p < kTParts; ++p) tf[p] = load8(&ch.t[p][place(t, col)][32 * k + 8 * g]);
-#pragma unroll
-        for (int sum = (kTParts > kXParts ? kTParts : kXParts) - 1; sum >= 0; --sum)    // small products first
-#pragma unroll
-          for (int p = 0; p <= sum; ++p)
-            if (p < kTParts && sum - p < kXParts) u[t] = mfma(tf[p], xp[k][sum - p], u[t]);
-      }
+      u[t] = u[t] * x_back;
+      ex.u[t][lane] = u[t];
 #pragma unroll
       for (int r = 0; r < 4; ++r) bad = fmaf(u[t][r], 0.0f, bad);
     }
-    if (__any(bad != bad)) {
+    const bool replay = __any(bad != bad);
+    if (lane == 0) ex.done = replay;
+    lds_barrier();                      // B
+    if (replay) {
       // Something is not finite: token after token, so that no token sees a later one through a product
       // with zero.
       const float rate = decay_rate(a.a_log[h]), dt = a.dt_bias[h];
       for (int t = 0; t < m; ++t) {
-        const size_t row = row0 + t;
+        const size_t row = (size_t)first + c * C + t;
         const float alpha = expf(log_decay(bf16_f32(a.a[row * a.a_ts + h]), rate, dt));
         const float beta = sigmoid(bf16_f32(a.b[row * a.b_ts + h]));
-        const float v = bf16_f32(a.v[row * a.v_ts + h * a.v_hs + col0 + col]);
+        const float vt = bf16_f32(a.v[row * a.v_ts + h * a.v_hs + col0 + col]);
         float kk = 0.0f, qq = 0.0f, sk = 0.0f, sq = 0.0f;
-        v8bf kf[kSteps], qf[kSteps];
+        v4i kf[kSteps], qf[kSteps];
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-          kf[step] = load8(a.k + row * a.k_ts + hk * a.k_hs + 32 * step + 8 * g);
-          qf[step] = load8(a.q + row * a.q_ts + hk * a.q_hs + 32 * step + 8 * g);
+        for (int i = 0; i < kSteps; ++i) {
+          kf[i] = load8(a.k + row * a.k_ts + hk * a.k_hs + 32 * i + 8 * g);
+          qf[i] = load8(a.q + row * a.q_ts + hk * a.q_hs + 32 * i + 8 * g);
 #pragma unroll
           for (int l = 0; l < 8; ++l) {
-            const float k = (float)kf[step][l], q = (float)qf[step][l];
-            kk = fmaf(k, k, kk), qq = fmaf(q, q, qq), sk = fmaf(S[2 * step + l / 4][l & 3], k, sk);
+            const float kx = element(kf[i], l), qx = element(qf[i], l);
+            kk = fmaf(kx, kx, kk), qq = fmaf(qx, qx, qq), sk = fmaf(S[2 * i + l / 4][l & 3], kx, sk);
           }
         }
         kk = sum_groups(kk), qq = sum_groups(qq), sk = sum_groups(sk);
         const float rk = 1.0f / sqrtf(kk + a.eps), rq = a.scale / sqrtf(qq + a.eps);
-        const float ut = beta * (v - alpha * rk * sk) * rk;
+        const float ut = beta * (vt - alpha * rk * sk) * rk;
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
           for (int l = 0; l < 8; ++l) {
-            const float y = fmaf((float)kf[step][l], ut, alpha * S[2 * step + l / 4][l & 3]);
-            S[2 * step + l / 4][l & 3] = y;
-            sq = fmaf(y, (float)qf[step][l], sq);
+            const float y = fmaf(element(kf[i], l), ut, alpha * S[2 * i + l / 4][l & 3]);
+            S[2 * i + l / 4][l & 3] = y;
+            sq = fmaf(y, element(qf[i], l), sq);
           }
         sq = rq * sum_groups(sq);
         if (g == 0) a.out[(row * a.Hv + h) * dv + col0 + col] = (uint16_t)bf16x2(sq, sq);
       }
       continue;
     }
-    v8bf up[2][kUParts], sp[2][kSParts];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float y[8], z[8];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const v4f f = *(const v4f*)&ch.u_factor[32 * k + 8 * g + 4 * e];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[4 * e + r] = u[2 * k + e][r], z[4 * e + r] = f[r] * u[2 * k + e][r];
-      }
-      split<kUParts>(y, up[k]), split<kSParts>(z, sp[k]);
-    }
-    const float decay = ch.decay;
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      S[j] = S[j] * decay;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const v8bf f = load8(kt + (size_t)place(j, col) * C + 32 * k + 8 * g);
-#pragma unroll
-        for (int p = kSParts - 1; p >= 0; --p) S[j] = mfma(f, sp[k][p], S[j]);
-      }
-    }
+    top = 0;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int token = place(t, col);
-      o[t] = o[t] * ch.q_factor[token];
+      u[t] = u[t] * *(const v4f*)&st.u_factor[place(t, 4 * g)];
 #pragma unroll
-      for (int k = 0; k <= t / 2; ++k)
+      for (int r = 0; r < 4; ++r) top = max(top, magnitude(u[t][r]));
+    }
+    top = max_groups(top);
+    const float u_to = scale_to(top), u_back = scale_back(top), decay = st.decay;
+    v8h uh[2], ul[2];
 #pragma unroll
-        for (int p = 0; p < kPParts; ++p) {
-          const v8bf f = load8(&ch.p[p][token][32 * k + 8 * g]);
+    for (int k = 0; k < 2; ++k) {
+      float y[8];
 #pragma unroll
-          for (int l = 0; l < kUParts && l + p < 2; ++l) o[t] = mfma(up[k][l], f, o[t]);
-        }
-      if (token < m)
-        *reinterpret_cast<uint2*>(a.out + ((row0 + token) * a.Hv + h) * dv + col0 + 4 * g) =
-            make_uint2(bf16x2(o[t][0], o[t][1]), bf16x2(o[t][2], o[t][3]));
+      for (int l = 0; l < 8; ++l) y[l] = u[2 * k + l / 4][l & 3] * u_to;
+      split(y, uh[k], ul[k]);
+    }
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      v4f y = {};
+#pragma unroll
+      for (int l = 1; l >= 0; --l)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) y = mfma(st.kt[j][k][lane], l ? ul[k] : uh[k], y);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[j][r] = fmaf(S[j][r], decay, y[r] * u_back);
     }
   }
+  lds_barrier();                        // (the other waves' last A)
   if (write >= 0 && write < a.s.slots)
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
@@ -419,14 +655,23 @@ __global__ __launch_bounds__(256) void delta_chunks(DeltaArgs a, int dv) {
         a.state[write * a.s.slot_stride + at + (size_t)place(j, 4 * g + r) * dv] = S[j][r];
 }
 
+template <int DK, int NW>
+hipError_t launch_chunks(const DeltaArgs& a, int dv, hipStream_t stream) {
+  const int parts = dv / (16 * NW), sequences = a.s.batch * a.Hv;
+  constexpr int kBytes = sizeof(ChunkShared<DK, NW>);
+  static_assert(kBytes <= 160 * 1024, "LDS of a workgroup");
+  if (hipError_t e = hipFuncSetAttribute((const void*)delta_chunks<DK, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes)) return e;
+  delta_chunks<DK, NW><<<(unsigned)(ceil_div(sequences, 8) * 8 * parts), 128 * NW, kBytes, stream>>>(a, dv, parts, sequences);
+  return hipGetLastError();
+}
+
 template <int DK>
 hipError_t launch(DeltaArgs a, int dv, hipStream_t stream) {
   a.by_heads = divisor(a.Hv), a.by_group = divisor(a.Hv / a.Hk);
   const int chunks = a.s.total / C + a.s.batch;
   delta_prepare<DK><<<(unsigned)(chunks * a.Hv), 256, 0, stream>>>(a);
   if (hipError_t e = hipGetLastError()) return e;
-  delta_chunks<DK><<<(unsigned)(a.s.batch * a.Hv * (dv / 64)), 256, 0, stream>>>(a, dv);
-  return hipGetLastError();
+  return launch_chunks<DK, 2>(a, dv, stream);
 }
 
 }  // namespace
@@ -440,8 +685,8 @@ DeltaPlan delta_plan(int total, int batch, int max_q, int write_cols, int Hk, in
   p.chunks = max_q > 16 && !write_cols && total > 0;
   if (p.chunks) {
     const size_t chunks = total / C + batch;
-    p.kt = chunks * Hv * sizeof(ChunkHead);
-    p.workspace = p.kt + chunks * Hk * dk * C * 2;
+    p.keys = chunks * Hv * sizeof(ChunkHead);
+    p.workspace = p.keys + chunks * Hk * (dk == 128 ? sizeof(ChunkKeys<128>) : sizeof(ChunkKeys<64>));
   }
   return p;
 }

@@ -66,7 +66,7 @@ struct DeltaArgs {
   float* state;
   uint16_t* out;
   void* workspace;
-  size_t kt;              // where in it the chunks' K^T begin
+  size_t keys;            // where in it the chunks' keys begin
   long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, a_ts, b_ts;
   Sequences s;
   int Hk, Hv;
@@ -75,7 +75,7 @@ struct DeltaArgs {
 };
 struct DeltaPlan {
   bool chunks;            // in chunks, or token after token
-  size_t kt, workspace;
+  size_t keys, workspace;
 };
 constexpr int kChunk = 64;
 DeltaPlan delta_plan(int total, int batch, int max_q, int write_cols, int Hk, int Hv, int dk, int dv);
