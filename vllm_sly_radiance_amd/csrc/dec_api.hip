@@ -135,6 +135,8 @@ DEC_API int dec_gated_delta(const void* q, long q_ts, long q_hs, const void* k, 
     if (int rc = check_rows(who, "q", q, q_ts, q_hs)) return rc;
     if (int rc = check_rows(who, "k", k, k_ts, k_hs)) return rc;
     if (int rc = check_rows(who, "v", v, v_ts, v_hs)) return rc;
+    if (v_ts > 1 << 23)                 // (rows of a chunk are counted in 32 bits)
+      return fail(DEC_EINVAL, "%s: v's tokens are %ld elements apart: need 2^23 at most", who, v_ts);
     if (!a || !b || !aligned(a, 2) || !aligned(b, 2) || a_ts < 0 || b_ts < 0)
       return fail(DEC_EINVAL, "%s: null or misaligned a or b, or strides %ld and %ld", who, a_ts, b_ts);
     if (!out || !aligned(out, 16)) return fail(DEC_EINVAL, "%s: null or misaligned output", who);

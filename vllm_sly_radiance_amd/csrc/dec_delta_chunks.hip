@@ -47,13 +47,11 @@ struct ChunkHead {
   v8h p[2][kLower][64];
 };
 constexpr int kHeadStage = 13 * kFrag;  // of it, what delta_chunks takes through LDS
-// A chunk and key head's: K as rows and as columns of the products, and Q.
+// A chunk and key head's: K as rows and as columns of the products (which go through LDS), and Q.
 template <int DK>
 struct ChunkKeys {
   v8h k[4][DK / 32][64], kt[DK / 16][2][64], q[4][DK / 32][64];
 };
-template <int DK>
-constexpr int kKeysStage = (4 * (DK / 32) + 2 * (DK / 16)) * kFrag;
 
 // Token (or key channel) of row m of a tile: the order that makes two result tiles an operand.
 __device__ __forceinline__ int place(int tile, int m) {
@@ -82,6 +80,7 @@ __device__ __forceinline__ void split(const float x[8], v8h& hi, v8h& lo) {
 __device__ __forceinline__ float scale_to(uint32_t top) { return __uint_as_float((267u - max(top >> 23, 14u)) << 23); }
 __device__ __forceinline__ float scale_back(uint32_t top) { return __uint_as_float((max(top >> 23, 14u) - 13u) << 23); }
 
+__device__ __forceinline__ float larger(float top, float x) { return fmaxf(top, fabsf(x)); }
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
 // Over the four lanes that have the same column (or row).
@@ -333,15 +332,29 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
   }
 }
 
+// The last word of a buffer descriptor: plain bytes, loads past its end give zero.
+constexpr int kBufferWord3 = 0x00020000;
+
+// 64 lanes of 16 bytes, offset bytes behind a buffer's beginning.
+template <typename Buffer>
+__device__ __forceinline__ v8h load_frag(Buffer p, int lane16, int offset) {
+  return __builtin_bit_cast(v8h, __builtin_amdgcn_raw_buffer_load_b128(p, lane16, offset, 0));
+}
+
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// LDS reads above this are not moved below it, nor those below above.
+__device__ __forceinline__ void hold_reads() { __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x8 | 0x10 | 0x200 | 0x400); }
+
+// Waits for all loads but the last N.
+template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+  __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));   // vmcnt(N)
   asm volatile("" ::: "memory");
 }
 
@@ -357,12 +370,11 @@ struct ChunkShared {
       char head[kHeadStage];
     };
     v8h k[4][DK / 32][64], kt[DK / 16][2][64];
-  } stage[2];
+  } stage[3];
   struct {
     v8h s[2][DK / 32][64];              // parts of the state before the chunk
     v4f u[4][64];
-    float s_back[16], u_back[16];       // one over the columns' scales
-    int done;                           // the outputs are written already
+    float s_back[16], x_back[16], u_back[16];      // one over the columns' scales
   } wave[NW];
 };
 
@@ -370,7 +382,8 @@ struct ChunkShared {
 // through the chunks; wave NW + i makes the outputs of wave i's columns, a chunk behind, and moves the next
 // chunk's operands to LDS.
 template <int DK, int NW>
-__global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
+__global__ __launch_bounds__(128 * NW) __attribute__((amdgpu_waves_per_eu(NW / 2, NW / 2)))
+void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
   constexpr int kSteps = DK / 32, kTiles = DK / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   ChunkShared<DK, NW>& sh = *(ChunkShared<DK, NW>*)lds;
@@ -390,54 +403,62 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
   const auto head_of = [&](int c) -> const ChunkHead& { return ((const ChunkHead*)a.workspace)[(size_t)(c0 + c) * a.Hv + h]; };
 
   if (outputs) {
-    // ---- operands of chunk c to stage c % 2, this wave's share of them
+    // operands of chunk c to stage c % 3, this wave's share of them: kMoves loads or one more
+    const int lane16 = lane * 16;
+    constexpr int kHead = kHeadStage / kFrag, kKeys = 4 * kSteps + 2 * kTiles, kMoves = kKeys / NW + kHead / NW;
     const auto move = [&](int c) {
-      const char* head = (const char*)&head_of(c);
-      const char* keys = (const char*)&delta_keys<DK>(a, c0 + c, hk);
-      auto& to = sh.stage[c & 1];
-      constexpr int kHead = kHeadStage / kFrag, kAll = kHead + kKeysStage<DK> / kFrag;
+      const auto head = __builtin_amdgcn_make_buffer_rsrc((char*)&head_of(c) + mine * kFrag, 0, kHeadStage - mine * kFrag, kBufferWord3);
+      const auto keys = __builtin_amdgcn_make_buffer_rsrc((char*)&delta_keys<DK>(a, c0 + c, hk) + mine * kFrag, 0, kKeys * kFrag, kBufferWord3);
+      char* to = sh.stage[c % 3].head + mine * kFrag;
+      char* to_keys = (char*)sh.stage[c % 3].k + mine * kFrag;
 #pragma unroll
-      for (int x = 0; x < ceil_div(kAll, NW); ++x) {
-        const int i = x * NW + mine;
-        if (i >= kAll) break;
-        const char* from = i < kHead ? head + i * kFrag : keys + (i - kHead) * kFrag;
-        char* at = i < kHead ? to.head + i * kFrag : (char*)to.k + (i - kHead) * kFrag;
-        __builtin_amdgcn_global_load_lds((global_ptr)(from + 16 * lane), (lds_ptr)at, 16, 0, 0);
-      }
+      for (int x = 0; x < kKeys; x += NW)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(keys, (lds_ptr)(to_keys + x * kFrag), 16, lane16, x * kFrag, 0, 0);
+#pragma unroll
+      for (int x = 0; x < kHead; x += NW)
+        if (x + NW <= kHead || x + mine < kHead)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(head, (lds_ptr)(to + x * kFrag), 16, lane16, x * kFrag, 0, 0);
     };
-    if (chunks) move(0);
+    if (chunks > 0) move(0);
+    if (chunks > 1) move(1);
+    wait_loads<kMoves>();               // (of one chunk only: all but one load, which has until B)
+    if (chunks == 1) wait_loads<0>();
+    lds_barrier();                      // stage 0 is there
     v8h q[4][kSteps], p[2][kLower], sp[2][kSteps];
     v4f u[4], s_back;
-    float q_factor[4];
-    bool done = false;
+    float q_factor[4], o_factor[4], x_back;
     const auto load = [&](int c) {
-      const ChunkHead& head = head_of(c);
-      const ChunkKeys<DK>& keys = delta_keys<DK>(a, c0 + c, hk);
+      const auto head = __builtin_amdgcn_make_buffer_rsrc((void*)&head_of(c), 0, (int)sizeof(ChunkHead), kBufferWord3);
+      const auto keys = __builtin_amdgcn_make_buffer_rsrc((void*)delta_keys<DK>(a, c0 + c, hk).q, 0, (int)sizeof(ChunkKeys<DK>::q), kBufferWord3);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        q_factor[t] = head.q_factor[place(t, col)];
+        q_factor[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+            head, 4 * place(t, col), offsetof(ChunkHead, q_factor), 0));
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) q[t][i] = keys.q[t][i][lane];
+        for (int i = 0; i < kSteps; ++i) q[t][i] = load_frag(keys, lane16, (t * kSteps + i) * kFrag);
       }
 #pragma unroll
       for (int l = 0; l < 2; ++l)
 #pragma unroll
-        for (int f = 0; f < kLower; ++f) p[l][f] = head.p[l][f][lane];
+        for (int f = 0; f < kLower; ++f)
+          p[l][f] = load_frag(head, lane16, (int)offsetof(ChunkHead, p) + (l * kLower + f) * kFrag);
     };
     for (int c = 0; c <= chunks; ++c) {
-      wait_loads();
-      lds_barrier();                    // A: stage c is there, and all have taken what chunk c - 1 left
-      if (c + 1 < chunks) move(c + 1);
-      if (c > 0 && !done) {
-        // outputs of chunk c - 1: rows are columns of the state, columns tokens
-        uint32_t top = 0;
+      lds_barrier();                    // A: all have taken what chunk c - 1 left
+      uint32_t top = 0;
+      if (c > 0) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int r = 0; r < 4; ++r) top = max(top, magnitude(u[t][r]));
         top = max_groups(top);
+      }
+      const bool mine_to_write = c > 0 && !__any(top >= 0x7F800000u);    // (else the other wave writes them)
+      v4f o[4] = {}, x[4] = {};
+      if (mine_to_write) {
+        // outputs of chunk c - 1: rows are columns of the state, columns tokens
         const float up = scale_to(top);
-        if (g == 0) ex.u_back[col] = scale_back(top) * (1.0f / kUnit);
+        if (g == 0) ex.u_back[col] = scale_back(top) * x_back * (1.0f / kUnit);
         v8h uh[2], ul[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -446,7 +467,6 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
           for (int i = 0; i < 8; ++i) y[i] = u[2 * k + i / 4][i & 3] * up;
           split(y, uh[k], ul[k]);
         }
-        v4f o[4] = {}, x[4] = {};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
@@ -460,23 +480,28 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
 #pragma unroll
             for (int t = 2 * k; t < 4; ++t)
               x[t] = mfma(l == 0 ? ul[k] : uh[k], p[l == 1][lower(t, k)], x[t]);
-        const v4f u_back = *(const v4f*)&ex.u_back[4 * g];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o_factor[t] = a.scale * q_factor[t];
+      }
+      wait_loads<0>();                  // stage c + 1 is there
+      if (c < chunks) load(c);
+      if (mine_to_write) {
+        const v4f u_back = *(const v4f*)&ex.u_back[4 * g] * a.scale;
         const int m = min(n - (c - 1) * C, C);
         uint16_t* out = a.out + (((size_t)first + (c - 1) * C) * a.Hv + h) * dv + col0 + 4 * g;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int token = place(t, col);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[t][r] = a.scale * fmaf(o[t][r], s_back[r] * q_factor[t], x[t][r] * u_back[r]);
+          for (int r = 0; r < 4; ++r) o[t][r] = fmaf(o[t][r], s_back[r] * o_factor[t], x[t][r] * u_back[r]);
           if (token < m)
             *reinterpret_cast<uint2*>(out + (size_t)token * a.Hv * dv) =
                 make_uint2(bf16x2(o[t][0], o[t][1]), bf16x2(o[t][2], o[t][3]));
         }
       }
       if (c == chunks) break;
-      load(c);
       lds_barrier();                    // B: wave `mine` has left what the outputs of chunk c take
-      done = ex.done;
+      x_back = ex.x_back[col];
       s_back = *(const v4f*)&ex.s_back[4 * g];
 #pragma unroll
       for (int l = 0; l < 2; ++l)
@@ -484,6 +509,7 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
         for (int i = 0; i < kSteps; ++i) sp[l][i] = ex.s[l][i][lane];
 #pragma unroll
       for (int t = 0; t < 4; ++t) u[t] = ex.u[t][lane];
+      if (c + 2 < chunks) move(c + 2);  // (to where chunk c - 1 was, which all are through with)
     }
     return;
   }
@@ -499,61 +525,130 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
       S[j][r] = read >= 0 && read < a.s.slots
                     ? a.state[read * a.s.slot_stride + at + (size_t)place(j, 4 * g + r) * dv]
                     : fill;
-  // values of chunk c, rows as results have them
+  // values of chunk c, rows as results have them; rows past the sequence read as zero
   uint32_t v[16];
+  const int v_row = (int)a.v_ts * 2, v_at = 8 * g * v_row + 2 * col;
   const auto values = [&](int c) {
-    const uint16_t* from = a.v + ((size_t)first + c * C) * a.v_ts + h * a.v_hs + col0 + col;
-    const int m = min(n - c * C, C);
+    const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + ((size_t)first + c * C) * a.v_ts + h * a.v_hs + col0), 0,
+                                                        (min(n - c * C, C) - 1) * v_row + 32, kBufferWord3);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int token = place(i >> 2, 4 * g + (i & 3));
-      v[i] = from[(size_t)min(token, m - 1) * a.v_ts];
-    }
+    for (int i = 0; i < 16; ++i)
+      v[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(from, v_at + place(i >> 2, i & 3) * v_row, 0, 0);
   };
   if (chunks) values(0);
-  for (int c = 0; c < chunks; ++c) {
-    const auto& st = sh.stage[c & 1];
-    const int m = min(n - c * C, C);
-    uint32_t top = 0;
+  // What chunk c adds to the state, K^T U, is formed with the products that chunk c + 1 takes of it, tile
+  // pair after tile pair: the vector instructions on one pair under the matrix instructions on the next.
+  v8h uh[2], ul[2];                     // U of the chunk before, decayed to its end
+  float u_back = 0.0f, decay = 0.0f, u_most = 0.0f, s_top = 0.0f;
+  bool adds = false;
+  const auto added = [&](const v8h kt[2][2], v4f y[2]) {
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j)
+    for (int e = 0; e < 2; ++e) y[e] = v4f{};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) top = max(top, magnitude(S[j][r]));
-    top = max_groups(top);
-    const float s_to = scale_to(top), s_back = scale_back(top);
-    v8h sh_[kSteps], sl[kSteps];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      float y[8];
-#pragma unroll
-      for (int l = 0; l < 8; ++l) y[l] = S[2 * i + l / 4][l & 3] * s_to;
-      split(y, sh_[i], sl[i]);
-    }
-    lds_barrier();                      // A
-    if (g == 0) ex.s_back[col] = s_back;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) ex.s[0][i][lane] = sh_[i], ex.s[1][i][lane] = sl[i];
-    v4f x[4] = {};
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int l = 1; l >= 0; --l)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = mfma(st.k[t][i][lane], l ? sl[i] : sh_[i], x[t]);
-    top = 0;
+        for (int e = 0; e < 2; ++e) y[e] = mfma(kt[e][k], l ? ul[k] : uh[k], y[e]);
+  };
+  const auto add = [&](int i, const v4f y[2]) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[2 * i + e][r] = fmaf(S[2 * i + e][r], decay, y[e][r] * u_back);
+  };
+  lds_barrier();                        // (stage 0 is there)
+  for (int c = 0, place_of = 0, last = 2; c < chunks; ++c) {
+    const auto& st = sh.stage[place_of];
+    const auto& before = sh.stage[last];
+    last = place_of, place_of = place_of == 2 ? 0 : place_of + 1;
+    const int m = min(n - c * C, C);
+    v8h kf[2][4], kt[3][2][2], tf[2][kLower];
+    const auto read_k = [&](int i) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) kf[i & 1][t] = st.k[t][i][lane];
+    };
+    const auto read_kt = [&](int i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) kt[i % 3][e][k] = before.kt[2 * i + e][k][lane];
+    };
+    read_kt(0), read_k(0), read_kt(1);
+    hold_reads();
+    lds_barrier();                      // A
+    // The scale of the state's columns: by their largest element, or where the state is still to be
+    // formed by a bound of it, decay max |S| + 64 max |u| (keys are no longer than 1).
+    if (!adds) {
+      s_top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_top = larger(s_top, S[j][r]);
+      s_top = __uint_as_float(max_groups(__float_as_uint(s_top)));
+    }
+    const uint32_t bound = __float_as_uint(adds ? fmaf(decay, s_top, 64.0f * u_most) : s_top);
+    const float s_to = scale_to(bound), s_back = scale_back(bound);
+    if (g == 0) ex.s_back[col] = s_back;
+    s_top = 0.0f;
+    v4f x[4] = {};
+    const auto step = [&](int i) {
+      float y[8];
+#pragma unroll
+      for (int l = 0; l < 8; ++l) {
+        const float z = S[2 * i + l / 4][l & 3];
+        y[l] = z * s_to, s_top = larger(s_top, z);
+      }
+      v8h hi, lo;
+      split(y, hi, lo);
+      ex.s[0][i][lane] = hi, ex.s[1][i][lane] = lo;
+#pragma unroll
+      for (int l = 1; l >= 0; --l)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = mfma(kf[i & 1][t], l ? lo : hi, x[t]);
+    };
+    const auto read_t = [&](int l) {
+#pragma unroll
+      for (int f = 0; f < kLower; ++f) tf[l][f] = st.t[l][f][lane];
+    };
+    // (operands are read a step before their products: alone on its SIMD, a wave waits for every read)
+    if (adds) {
+      v4f y[2][2];
+      added(kt[0], y[0]);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (i + 2 < kSteps) read_kt(i + 2);
+        if (i + 1 < kSteps) read_k(i + 1);
+        if (i == kSteps - 2) read_t(0);
+        if (i == kSteps - 1) read_t(1);
+        hold_reads();
+        if (i + 1 < kSteps) added(kt[(i + 1) % 3], y[(i + 1) & 1]);
+        add(i, y[i & 1]);
+        step(i);
+      }
+    } else {
+      read_t(0), read_t(1);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (i + 1 < kSteps) read_k(i + 1);
+        step(i);
+      }
+    }
+    s_top = __uint_as_float(max_groups(__float_as_uint(s_top)));
+    float x_top = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const v4f f = *(const v4f*)&st.k_factor[place(t, 4 * g)];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float y = place(t, 4 * g + r) < m ? __uint_as_float(v[4 * t + r] << 16) : 0.0f;
-        x[t][r] = fmaf(-(f[r] * s_back), x[t][r], y);
-        top = max(top, magnitude(x[t][r]));
+        x[t][r] = fmaf(-(f[r] * s_back), x[t][r], __uint_as_float(v[4 * t + r] << 16));
+        x_top = larger(x_top, x[t][r]);
       }
     }
     if (c + 1 < chunks) values(c + 1);
-    top = max_groups(top);
-    const float x_to = scale_to(top), x_back = scale_back(top) * (1.0f / kUnit);
+    const uint32_t x_most = max_groups(__float_as_uint(x_top));
+    const float x_to = scale_to(x_most), x_back = scale_back(x_most) * (1.0f / kUnit);
+    if (g == 0) ex.x_back[col] = x_back;
     v8h xh[2], xl[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -562,26 +657,30 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
       for (int l = 0; l < 8; ++l) y[l] = x[2 * k + l / 4][l & 3] * x_to;
       split(y, xh[k], xl[k]);
     }
-    v4f u[4] = {};
+    v4f u[4] = {};                      // U, in X's scale
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int l = 0; l < 3; ++l)       // small products first
 #pragma unroll
         for (int t = 2 * k; t < 4; ++t)
-          u[t] = mfma(st.t[l == 1][lower(t, k)][lane], l == 0 ? xl[k] : xh[k], u[t]);
-    float bad = 0.0f;
+          u[t] = mfma(tf[l == 1][lower(t, k)], l == 0 ? xl[k] : xh[k], u[t]);
+    uint32_t top = 0;
+    float f_top = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      u[t] = u[t] * x_back;
       ex.u[t][lane] = u[t];
+      const v4f f = *(const v4f*)&st.u_factor[place(t, 4 * g)];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) bad = fmaf(u[t][r], 0.0f, bad);
+      for (int r = 0; r < 4; ++r) {
+        top = max(top, magnitude(u[t][r]));
+        u[t][r] *= f[r], f_top = larger(f_top, u[t][r]);
+      }
     }
-    const bool replay = __any(bad != bad);
-    if (lane == 0) ex.done = replay;
+    top = max_groups(top);
     lds_barrier();                      // B
-    if (replay) {
+    if (__any(top >= 0x7F800000u)) {
+      adds = false;                     // (the state is the one before this chunk by now)
       // Something is not finite: token after token, so that no token sees a later one through a product
       // with zero.
       const float rate = decay_rate(a.a_log[h]), dt = a.dt_bias[h];
@@ -618,16 +717,9 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
       }
       continue;
     }
-    top = 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      u[t] = u[t] * *(const v4f*)&st.u_factor[place(t, 4 * g)];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) top = max(top, magnitude(u[t][r]));
-    }
-    top = max_groups(top);
-    const float u_to = scale_to(top), u_back = scale_back(top), decay = st.decay;
-    v8h uh[2], ul[2];
+    const uint32_t f_most = max_groups(__float_as_uint(f_top));
+    const float u_to = scale_to(f_most);
+    u_back = scale_back(f_most) * x_back, u_most = __uint_as_float(top) * x_back, decay = st.decay;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float y[8];
@@ -635,15 +727,19 @@ __global__ __launch_bounds__(128 * NW) void delta_chunks(DeltaArgs a, int dv, in
       for (int l = 0; l < 8; ++l) y[l] = u[2 * k + l / 4][l & 3] * u_to;
       split(y, uh[k], ul[k]);
     }
+    adds = true;
+  }
+  if (adds) {
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      v4f y = {};
+    for (int i = 0; i < kSteps; ++i) {
+      v8h kt[2][2];
+      v4f y[2];
 #pragma unroll
-      for (int l = 1; l >= 0; --l)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) y = mfma(st.kt[j][k][lane], l ? ul[k] : uh[k], y);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) S[j][r] = fmaf(S[j][r], decay, y[r] * u_back);
+        for (int k = 0; k < 2; ++k) kt[e][k] = sh.stage[(chunks + 2) % 3].kt[2 * i + e][k][lane];
+      added(kt, y);
+      add(i, y);
     }
   }
   lds_barrier();                        // (the other waves' last A)

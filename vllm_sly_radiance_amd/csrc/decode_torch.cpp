@@ -48,7 +48,7 @@ bool rows_fit(const Tensor& x) {
   const long n = x.dim();
   if (x.stride(n - 1) != 1 || ((uintptr_t)address(x) & 15)) return false;
   for (long i = 0; i < n - 1; ++i)
-    if (x.size(i) > 1 && ((x.stride(i) & 7) || x.stride(i) < 0)) return false;
+    if (x.size(i) > 1 && ((x.stride(i) & 7) || x.stride(i) < 0 || (i == 0 && x.stride(i) > 1 << 23))) return false;
   return true;
 }
 Tensor rows(const Args& a, const char* name, const Tensor& x, at::IntArrayRef shape) {
