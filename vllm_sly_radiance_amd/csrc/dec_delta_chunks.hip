@@ -113,105 +113,122 @@ __device__ __forceinline__ int first_chunk(const Sequences& s, int b) {
   return min(max(s.starts[b], 0), s.total) / C + b;
 }
 
-// The sequence that chunk slot c belongs to: the last whose slots begin at it or before; -1 for none.
-__device__ __forceinline__ int sequence_of(const Sequences& s, int c) {
+// The sequence that chunk slot c belongs to, the last whose slots begin at it or before (-1 for none), its first
+// row and its number of rows.
+__device__ __forceinline__ int sequence_of(const Sequences& s, int c, int& first, int& n) {
   const int lane = threadIdx.x & 63;
-  int count = 0;
+  int b = -1;
   for (int b0 = 0; b0 < s.batch; b0 += 64) {
-    const int b = b0 + lane;
-    const int m = __popcll(__ballot(b < s.batch && first_chunk(s, min(b, s.batch - 1)) <= c));
-    count += m;
+    const int start = s.starts[min(b0 + lane, s.batch)];
+    const int m = __popcll(__ballot(b0 + lane < s.batch && min(max(start, 0), s.total) / C + b0 + lane <= c));
+    b += m;
+    if (m < 64 && m) {                  // its start and the next are here
+      first = min(max(__builtin_amdgcn_readlane(start, m - 1), 0), s.total);
+      n = max(min(__builtin_amdgcn_readlane(start, m), s.total) - first, 0);
+      return b;
+    }
     if (m < 64) break;
   }
-  return count - 1;
+  if (b >= 0) rows_of(s, b, first, n);
+  return b;
 }
 
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ double wave_sums(double x) {
+#define STEP(ctrl, rows)                                                                                      \
+  {                                                                                                           \
+    const uint64_t u = (uint64_t)__double_as_longlong(x);                                                     \
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, ctrl, rows, 0xF, false);    \
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), ctrl, rows, 0xF, false); \
+    x += __longlong_as_double((long long)((uint64_t)hi << 32 | lo));                                          \
+  }
+  STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF)     // row_shr:1, 2, 4, 8
+  STEP(0x142, 0xA) STEP(0x143, 0xC)                                       // row_bcast:15 and 31
+#undef STEP
+  return x;
+}
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <int DK>
 struct PrepareShared {
-  float a[C][kPad], t[C][kPad];
-  float g_hi[C], g_lo[C], beta[C], rk[C], rq[C];
+  float a[C][kPad];
+  union {
+    float t[C][kPad];
+    v8h k[4][DK / 32][64];              // K until its products are formed
+  };
+  float g_hi[C], g_lo[C], beta[C], rk[C], rq[C];           // G in units of ln 2
 };
 
 // One workgroup makes one chunk's matrices for one value head; wave w has rows 16 w .. 16 w + 15.
 template <int DK>
-__global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
-  __shared__ __attribute__((aligned(16))) PrepareShared s;
+__global__ __launch_bounds__(256, 4) void delta_prepare(DeltaArgs a) {
+  __shared__ __attribute__((aligned(16))) PrepareShared<DK> s;
   const int c = a.by_heads((int)blockIdx.x), h = (int)blockIdx.x - c * a.Hv;
   const int hk = a.by_group(h);
-  const int b = sequence_of(a.s, c);
-  if (b < 0) return;
   int first, n;
-  rows_of(a.s, b, first, n);
-  const int i0 = (c - first_chunk(a.s, b)) * C;
+  const int b = sequence_of(a.s, c, first, n);
+  if (b < 0) return;
+  const int i0 = (c - first / C - b) * C;
   if (i0 >= n) return;
   const int m = min(n - i0, C);
   const size_t row0 = (size_t)first + i0;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
 
   constexpr int kSteps = DK / 32;
-  const auto load = [&](const uint16_t* p, long ts, long hs, int tile, int step) {
-    return load8(p + (row0 + min(16 * tile + col, m - 1)) * ts + hk * hs + 32 * step + 8 * g);
-  };
-  // a row scaled to fp16, its sum of squares and its scale
-  const auto scaled = [&](const v4i x[kSteps], v8h y[kSteps], float& squares, float& scale) {
-    uint32_t top = 0;
+  uint16_t gate_a = 0, gate_b = 0;
+  if (w == 0) {
+    const size_t row = row0 + min(lane, m - 1);
+    gate_a = a.a[row * a.a_ts + h], gate_b = a.b[row * a.b_ts + h];
+  }
+  v4i raw_k[kSteps], raw_q[kSteps];
+  {
+    const size_t row = row0 + min(16 * w + col, m - 1);
+    const uint16_t* k = a.k + row * a.k_ts + hk * a.k_hs + 8 * g;
+    const uint16_t* q = a.q + row * a.q_ts + hk * a.q_hs + 8 * g;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+    for (int i = 0; i < kSteps; ++i) raw_k[i] = load8(k + 32 * i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, magnitude(element(x[i], j)));
-    scale = scale_to(max_groups(top)), squares = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float z = element(x[i], j) * scale;
-        y[i][j] = (_Float16)z, squares = fmaf(z, z, squares);
-      }
-    squares = sum_groups(squares);
-  };
-  v4i raw[4][kSteps], raw_q[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) raw_q[i] = load(a.q, a.q_ts, a.q_hs, w, i);
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) raw[t][i] = load(a.k, a.k_ts, a.k_hs, t, i);
+    for (int i = 0; i < kSteps; ++i) raw_q[i] = load8(q + 32 * i);
+  }
   if (w == 0) {
     // (decays below e^-200 are 0 either way; held to that, the sums stay finite)
-    double sum = 0.0;
-    float beta = 0.0f;
-    if (lane < m) {
-      const float x = log_decay(bf16_f32(a.a[(row0 + lane) * a.a_ts + h]), decay_rate(a.a_log[h]), a.dt_bias[h]);
-      sum = x < -200.0f ? -200.0f : x;
-      beta = sigmoid(bf16_f32(a.b[(row0 + lane) * a.b_ts + h]));
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double y = __shfl_up(sum, d);
-      if (lane >= d) sum += y;
-    }
+    const float x = log_decay(bf16_f32(gate_a), decay_rate(a.a_log[h]), a.dt_bias[h]);
+    const double sum = wave_sums(lane < m ? (double)(x < -200.0f ? -200.0f : x) * 1.4426950408889634 : 0.0);
     // two floats: differences of nearby sums keep the bits of what lies between them
-    s.g_hi[lane] = (float)sum, s.g_lo[lane] = (float)(sum - (double)(float)sum), s.beta[lane] = beta;
+    s.g_hi[lane] = (float)sum, s.g_lo[lane] = (float)(sum - (double)(float)sum);
+    s.beta[lane] = lane < m ? sigmoid(bf16_f32(gate_b)) : 0.0f;
   }
-  v8h kf[4][kSteps], qf[kSteps];
-  float rk[4];
+  // rows scaled to fp16, one over their lengths
+  const auto scaled = [&](const v4i x[kSteps], v8h y[kSteps]) {
+    typedef uint16_t v2u __attribute__((ext_vector_type(2)));
+    v2u most = {};
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    float squares, scale;
-    scaled(raw[t], kf[t], squares, scale);
-    rk[t] = 1.0f / sqrtf(fmaf(a.eps * scale, scale, squares));
-    if (t == w && g == 0) s.rk[16 * w + col] = rk[t];
-  }
-  {
-    float squares, scale;
-    scaled(raw_q, qf, squares, scale);
-    if (g == 0) s.rq[16 * w + col] = 1.0f / sqrtf(fmaf(a.eps * scale, scale, squares));
-  }
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2u, x[i][j] & 0x7FFF7FFF));
+    const float scale = scale_to(max_groups((uint32_t)max(most[0], most[1]) << 16));
+    float squares = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float z = element(x[i], j) * scale, z1 = element(x[i], j + 1) * scale;
+        const v2h both = half2(z, z1);
+        y[i][j] = both[0], y[i][j + 1] = both[1], squares = fmaf(z1, z1, fmaf(z, z, squares));
+      }
+    return 1.0f / sqrtf(fmaf(a.eps * scale, scale, sum_groups(squares)));
+  };
+  v8h kf[kSteps], qf[kSteps];
+  const float rk = scaled(raw_k, kf);
+  __builtin_amdgcn_sched_barrier(0);    // (one after the other: both at once spill)
+  const float rq = scaled(raw_q, qf);
+  if (g == 0) s.rk[16 * w + col] = rk, s.rq[16 * w + col] = rq;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) s.k[w][i][lane] = kf[i];
   __syncthreads();
-  v4f p[4] = {};
+  v4f p[4];
   {
-    v8h mine[kSteps];                   // (the row tile is a number that the compiler does not know)
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) mine[i] = w < 2 ? (w ? kf[1][i] : kf[0][i]) : w == 2 ? kf[2][i] : kf[3][i];
     const v4f rki = *(const v4f*)&s.rk[16 * w + 4 * g], rqi = *(const v4f*)&s.rq[16 * w + 4 * g];
     const v4f hi = *(const v4f*)&s.g_hi[16 * w + 4 * g], lo = *(const v4f*)&s.g_lo[16 * w + 4 * g];
     const v4f beta = *(const v4f*)&s.beta[16 * w + 4 * g];
@@ -220,13 +237,16 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
       if (t > (w | 1)) break;
       v4f ak = {}, aq = {};
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) ak = mfma(mine[i], kf[t][i], ak), aq = mfma(qf[i], kf[t][i], aq);
+      for (int i = 0; i < kSteps; ++i) {
+        const v8h x = s.k[t][i][lane];
+        ak = mfma(kf[i], x, ak), aq = mfma(qf[i], x, aq);
+      }
       const int j = 16 * t + col;
-      const float hj = s.g_hi[j], lj = s.g_lo[j];
+      const float hj = s.g_hi[j], lj = s.g_lo[j], rkj = s.rk[j];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * w + 4 * g + r;
-        const float d = j <= i ? expf((hi[r] - hj) + (lo[r] - lj)) * rk[t] : 0.0f;
+        const float d = j <= i ? exp2_raw((hi[r] - hj) + (lo[r] - lj)) * rkj : 0.0f;
         s.a[i][j] = j < i ? beta[r] * d * rki[r] * ak[r] : 0.0f;
         p[t][r] = j <= i ? d * rqi[r] * aq[r] : 0.0f;
       }
@@ -247,6 +267,7 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
           if (j + l < i) x[l] = fmaf(-y[l], t[j + l], x[l]);
       }
       t[i] = (x[0] + x[1]) + (x[2] + x[3]);
+      asm volatile("" : "+v"(t[i]) : : "memory");     // (all rows read at once would spill)
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -303,11 +324,11 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
   }
   if (w == 0) {
     const float hi = s.g_hi[lane], lo = s.g_lo[lane], last = s.g_hi[C - 1], rest = s.g_lo[C - 1];
-    const float in = expf(hi), there = lane < m ? 1.0f : 0.0f;
+    const float in = exp2_raw(hi + lo), there = lane < m ? 1.0f : 0.0f;
     out.k_factor[lane] = there * (in * s.rk[lane]);
     out.q_factor[lane] = in * s.rq[lane];
-    out.u_factor[lane] = there * (expf((last - hi) + (rest - lo)) * s.rk[lane]);
-    if (lane == 0) out.decay = expf(last);
+    out.u_factor[lane] = there * (exp2_raw((last - hi) + (rest - lo)) * s.rk[lane]);
+    if (lane == 0) out.decay = exp2_raw(last + rest);
   }
   if (hk * (a.Hv / a.Hk) == h) {        // K and Q once for the heads that share them
     ChunkKeys<DK>& keys = delta_keys<DK>(a, c, hk);
@@ -317,7 +338,7 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaArgs a) {
     _Float16(*kt)[C + 8] = (_Float16(*)[C + 8]) s.a;       // [DK][C], over a and t
 #pragma unroll
     for (int step = 0; step < kSteps; ++step) {
-      const v8h x = w < 2 ? (w ? kf[1][step] : kf[0][step]) : w == 2 ? kf[2][step] : kf[3][step];
+      const v8h x = kf[step];
       keys.k[tile][step][16 * g + row] = x;
       keys.q[tile][step][16 * g + row] = qf[step];
 #pragma unroll
