@@ -37,6 +37,8 @@ DECODE_LIB_NAME = "libdecode_ops.so"
 DECODE_SOURCES = ["dec_api.hip", "dec_conv.hip", "dec_delta_steps.hip", "dec_delta_chunks.hip",
                   "dec_sample.hip"]
 DECODE_TORCH_NAME = "_decode_torch.so"
+# matrix instructions' results in vector registers: the delta rule's are vector instructions' operands next
+DECODE_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 # binding -> its source and the library that it is over
 BINDINGS = {os.path.basename(KV4_TORCH_PATH): ("kv4_torch.cpp", os.path.basename(KV4_LIB_PATH)),
             DECODE_TORCH_NAME: ("decode_torch.cpp", DECODE_LIB_NAME)}
@@ -63,7 +65,8 @@ def hipcc() -> str:
 
 def _command(sources, out) -> list[str]:
     srcs = [os.path.join(CSRC, s) for s in sources]
-    return [hipcc(), *FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", out]
+    more = DECODE_FLAGS if sources is DECODE_SOURCES else []
+    return [hipcc(), *FLAGS, *more, f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", out]
 
 
 def _torch_commands(out) -> tuple[list[str], list[str]]:

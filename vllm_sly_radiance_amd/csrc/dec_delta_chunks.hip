@@ -66,13 +66,21 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
 
 __device__ __forceinline__ v2h half2(float a, float b) { return __builtin_convertvector(v2f{a, b}, v2h); }
 
-// x as two parts that add up to it, 8 values.
-__device__ __forceinline__ void split(const float x[8], v8h& hi, v8h& lo) {
+// x scale as two parts that add up to it, 8 values, in two operations a value: fused multiply-adds that round
+// to fp16 (scale is a power of two, so that what the first part leaves is exact).
+__device__ __forceinline__ void split(const float x[8], float scale, v8h& hi, v8h& lo) {
+  v4i a, b;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const v2h a = half2(x[i], x[i + 1]), b = half2(x[i] - (float)a[0], x[i + 1] - (float)a[1]);
-    hi[i] = a[0], hi[i + 1] = a[1], lo[i] = b[0], lo[i + 1] = b[1];
+    const v2h part = {(_Float16)__builtin_fmaf(x[i], scale, 0.0f), (_Float16)__builtin_fmaf(x[i + 1], scale, 0.0f)};
+    int bits = __builtin_bit_cast(int, part);
+    asm("" : "+v"(bits));               // (both halves are read from here)
+    a[i / 2] = bits;
+    const v2h first = __builtin_bit_cast(v2h, bits);
+    b[i / 2] = __builtin_bit_cast(int, v2h{(_Float16)__builtin_fmaf(x[i], scale, -(float)first[0]),
+                                           (_Float16)__builtin_fmaf(x[i + 1], scale, -(float)first[1])});
   }
+  hi = __builtin_bit_cast(v8h, a), lo = __builtin_bit_cast(v8h, b);
 }
 
 // The power of two that brings a magnitude (its bits) to 2^13 .. 2^14, and one over it. What is below 2^-113
@@ -316,9 +324,9 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaArgs a) {
     const int i = place(t, col), j = 32 * k + 8 * g;
     float y[8];
 #pragma unroll
-    for (int l = 0; l < 8; ++l) y[l] = is_p ? s.a[i][j + l] * kUnit : s.t[i][j + l] * (s.beta[j + l] * kUnit);
+    for (int l = 0; l < 8; ++l) y[l] = is_p ? s.a[i][j + l] : s.t[i][j + l] * s.beta[j + l];
     v8h hi, lo;
-    split(y, hi, lo);
+    split(y, kUnit, hi, lo);
     v8h(*to)[kLower][64] = is_p ? out.p : out.t;
     to[0][f][lane] = hi, to[1][f][lane] = lo;
   }
@@ -371,6 +379,16 @@ __device__ __forceinline__ void lds_barrier() {
 // LDS reads above this are not moved below it, nor those below above.
 __device__ __forceinline__ void hold_reads() { __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x8 | 0x10 | 0x200 | 0x400); }
 
+// N times a matrix instruction and three vector instructions.
+template <int N>
+__device__ __forceinline__ void mix_products() {
+  if constexpr (N > 0) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+    mix_products<N - 1>();
+  }
+}
+
 // Waits for all loads but the last N.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -394,7 +412,7 @@ struct ChunkShared {
   } stage[3];
   struct {
     v8h s[2][DK / 32][64];              // parts of the state before the chunk
-    v4f u[4][64];
+    v4f u[4][64];                       // U of the chunk, and before that its values
     float s_back[16], x_back[16], u_back[16];      // one over the columns' scales
   } wave[NW];
 };
@@ -424,9 +442,9 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
   const auto head_of = [&](int c) -> const ChunkHead& { return ((const ChunkHead*)a.workspace)[(size_t)(c0 + c) * a.Hv + h]; };
 
   if (outputs) {
-    // operands of chunk c to stage c % 3, this wave's share of them: kMoves loads or one more
+    // operands of chunk c to stage c % 3, this wave's share of them
     const int lane16 = lane * 16;
-    constexpr int kHead = kHeadStage / kFrag, kKeys = 4 * kSteps + 2 * kTiles, kMoves = kKeys / NW + kHead / NW;
+    constexpr int kHead = kHeadStage / kFrag, kKeys = 4 * kSteps + 2 * kTiles;
     const auto move = [&](int c) {
       const auto head = __builtin_amdgcn_make_buffer_rsrc((char*)&head_of(c) + mine * kFrag, 0, kHeadStage - mine * kFrag, kBufferWord3);
       const auto keys = __builtin_amdgcn_make_buffer_rsrc((char*)&delta_keys<DK>(a, c0 + c, hk) + mine * kFrag, 0, kKeys * kFrag, kBufferWord3);
@@ -440,11 +458,25 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
         if (x + NW <= kHead || x + mine < kHead)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(head, (lds_ptr)(to + x * kFrag), 16, lane16, x * kFrag, 0, 0);
     };
-    if (chunks > 0) move(0);
-    if (chunks > 1) move(1);
-    wait_loads<kMoves>();               // (of one chunk only: all but one load, which has until B)
-    if (chunks == 1) wait_loads<0>();
-    lds_barrier();                      // stage 0 is there
+    // values of chunk c, rows as results have them; rows past the sequence read as zero
+    uint16_t raw[16];
+    v4f v[4];
+    const int v_row = (int)a.v_ts * 2, v_at = 8 * g * v_row + 2 * col;
+    const auto load_v = [&](int c) {
+      const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + ((size_t)first + c * C) * a.v_ts + h * a.v_hs + col0), 0,
+                                                          (min(n - c * C, C) - 1) * v_row + 32, kBufferWord3);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        raw[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(from, v_at + place(i >> 2, i & 3) * v_row, 0, 0);
+    };
+    const auto take_v = [&] {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i >> 2][i & 3] = bf16_f32(raw[i]);
+    };
+    const auto give_v = [&] {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) ex.u[t][lane] = v[t];
+    };
     v8h q[4][kSteps], p[2][kLower], sp[2][kSteps];
     v4f u[4], s_back;
     float q_factor[4], o_factor[4], x_back;
@@ -464,6 +496,12 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
         for (int f = 0; f < kLower; ++f)
           p[l][f] = load_frag(head, lane16, (int)offsetof(ChunkHead, p) + (l * kLower + f) * kFrag);
     };
+    if (chunks > 0) load_v(0), move(0);
+    if (chunks > 1) move(1);
+    if (chunks > 0) take_v(), give_v();
+    if (chunks > 1) load_v(1);
+    wait_loads<0>();
+    lds_barrier();                      // stage 0 and its values are there
     for (int c = 0; c <= chunks; ++c) {
       lds_barrier();                    // A: all have taken what chunk c - 1 left
       uint32_t top = 0;
@@ -485,8 +523,8 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
         for (int k = 0; k < 2; ++k) {
           float y[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = u[2 * k + i / 4][i & 3] * up;
-          split(y, uh[k], ul[k]);
+          for (int i = 0; i < 8; ++i) y[i] = u[2 * k + i / 4][i & 3];
+          split(y, up, uh[k], ul[k]);
         }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
@@ -505,7 +543,9 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
         for (int t = 0; t < 4; ++t) o_factor[t] = a.scale * q_factor[t];
       }
       wait_loads<0>();                  // stage c + 1 is there
+      if (c + 1 < chunks) take_v();
       if (c < chunks) load(c);
+      if (c + 2 < chunks) load_v(c + 2);
       if (mine_to_write) {
         const v4f u_back = *(const v4f*)&ex.u_back[4 * g] * a.scale;
         const int m = min(n - (c - 1) * C, C);
@@ -530,6 +570,7 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
         for (int i = 0; i < kSteps; ++i) sp[l][i] = ex.s[l][i][lane];
 #pragma unroll
       for (int t = 0; t < 4; ++t) u[t] = ex.u[t][lane];
+      if (c + 1 < chunks) give_v();
       if (c + 2 < chunks) move(c + 2);  // (to where chunk c - 1 was, which all are through with)
     }
     return;
@@ -546,17 +587,6 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
       S[j][r] = read >= 0 && read < a.s.slots
                     ? a.state[read * a.s.slot_stride + at + (size_t)place(j, 4 * g + r) * dv]
                     : fill;
-  // values of chunk c, rows as results have them; rows past the sequence read as zero
-  uint32_t v[16];
-  const int v_row = (int)a.v_ts * 2, v_at = 8 * g * v_row + 2 * col;
-  const auto values = [&](int c) {
-    const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + ((size_t)first + c * C) * a.v_ts + h * a.v_hs + col0), 0,
-                                                        (min(n - c * C, C) - 1) * v_row + 32, kBufferWord3);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      v[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(from, v_at + place(i >> 2, i & 3) * v_row, 0, 0);
-  };
-  if (chunks) values(0);
   // What chunk c adds to the state, K^T U, is formed with the products that chunk c + 1 takes of it, tile
   // pair after tile pair: the vector instructions on one pair under the matrix instructions on the next.
   v8h uh[2], ul[2];                     // U of the chunk before, decayed to its end
@@ -597,7 +627,12 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
     };
     read_kt(0), read_k(0), read_kt(1);
     hold_reads();
+    v4f y[2][2];
+    if (adds) added(kt[0], y[0]);
     lds_barrier();                      // A
+    v4f v[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) v[t] = ex.u[t][lane];
     // The scale of the state's columns: by their largest element, or where the state is still to be
     // formed by a bound of it, decay max |S| + 64 max |u| (keys are no longer than 1).
     if (!adds) {
@@ -613,46 +648,48 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
     if (g == 0) ex.s_back[col] = s_back;
     s_top = 0.0f;
     v4f x[4] = {};
-    const auto step = [&](int i) {
+    v8h sh_[2], sl[2];
+    const auto parts_of = [&](int i) {
       float y[8];
 #pragma unroll
-      for (int l = 0; l < 8; ++l) {
-        const float z = S[2 * i + l / 4][l & 3];
-        y[l] = z * s_to, s_top = larger(s_top, z);
-      }
-      v8h hi, lo;
-      split(y, hi, lo);
-      ex.s[0][i][lane] = hi, ex.s[1][i][lane] = lo;
+      for (int l = 0; l < 8; ++l) y[l] = S[2 * i + l / 4][l & 3], s_top = larger(s_top, y[l]);
+      split(y, s_to, sh_[i & 1], sl[i & 1]);
+      ex.s[0][i][lane] = sh_[i & 1], ex.s[1][i][lane] = sl[i & 1];
+    };
+    const auto products = [&](int i) {
 #pragma unroll
       for (int l = 1; l >= 0; --l)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = mfma(kf[i & 1][t], l ? lo : hi, x[t]);
+        for (int t = 0; t < 4; ++t) x[t] = mfma(kf[i & 1][t], l ? sl[i & 1] : sh_[i & 1], x[t]);
     };
     const auto read_t = [&](int l) {
 #pragma unroll
       for (int f = 0; f < kLower; ++f) tf[l][f] = st.t[l][f][lane];
     };
-    // (operands are read a step before their products: alone on its SIMD, a wave waits for every read)
+    // Operands are read a step before their products: alone on its SIMD, a wave waits for every read. The
+    // products that a step issues do not depend on its vector instructions, which go between them.
     if (adds) {
-      v4f y[2][2];
-      added(kt[0], y[0]);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         if (i + 2 < kSteps) read_kt(i + 2);
-        if (i + 1 < kSteps) read_k(i + 1);
         if (i == kSteps - 2) read_t(0);
         if (i == kSteps - 1) read_t(1);
         hold_reads();
+        if (i > 0) products(i - 1);
         if (i + 1 < kSteps) added(kt[(i + 1) % 3], y[(i + 1) & 1]);
         add(i, y[i & 1]);
-        step(i);
+        parts_of(i);
+        mix_products<16>();
+        if (i + 1 < kSteps) read_k(i + 1);
       }
+      products(kSteps - 1);
     } else {
       read_t(0), read_t(1);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         if (i + 1 < kSteps) read_k(i + 1);
-        step(i);
+        parts_of(i);
+        products(i);
       }
     }
     s_top = __uint_as_float(max_groups(__float_as_uint(s_top)));
@@ -662,23 +699,22 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
       const v4f f = *(const v4f*)&st.k_factor[place(t, 4 * g)];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[t][r] = fmaf(-(f[r] * s_back), x[t][r], __uint_as_float(v[4 * t + r] << 16));
+        x[t][r] = fmaf(-(f[r] * s_back), x[t][r], v[t][r]);
         x_top = larger(x_top, x[t][r]);
       }
     }
-    if (c + 1 < chunks) values(c + 1);
     const uint32_t x_most = max_groups(__float_as_uint(x_top));
     const float x_to = scale_to(x_most), x_back = scale_back(x_most) * (1.0f / kUnit);
     if (g == 0) ex.x_back[col] = x_back;
     v8h xh[2], xl[2];
+    v4f u[4] = {};                      // U, in X's scale
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       float y[8];
 #pragma unroll
-      for (int l = 0; l < 8; ++l) y[l] = x[2 * k + l / 4][l & 3] * x_to;
-      split(y, xh[k], xl[k]);
+      for (int l = 0; l < 8; ++l) y[l] = x[2 * k + l / 4][l & 3];
+      split(y, x_to, xh[k], xl[k]);
     }
-    v4f u[4] = {};                      // U, in X's scale
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -745,8 +781,8 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
     for (int k = 0; k < 2; ++k) {
       float y[8];
 #pragma unroll
-      for (int l = 0; l < 8; ++l) y[l] = u[2 * k + l / 4][l & 3] * u_to;
-      split(y, uh[k], ul[k]);
+      for (int l = 0; l < 8; ++l) y[l] = u[2 * k + l / 4][l & 3];
+      split(y, u_to, uh[k], ul[k]);
     }
     adds = true;
   }
