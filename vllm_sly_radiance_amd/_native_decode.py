@@ -85,7 +85,7 @@ def gated_delta_workspace(total, batch, max_q, write_cols, k_heads, v_heads, dk,
     return n.value
 
 
-def sample_workspace(rows, vocabulary, flags=0) -> int:
+def sample_workspace(rows, vocabulary, filters=True) -> int:
     n = _sz()
-    check(lib().dec_sample_workspace(rows, vocabulary, flags, _c.byref(n)))
+    check(lib().dec_sample_workspace(rows, vocabulary, int(filters), _c.byref(n)))
     return n.value

@@ -97,7 +97,9 @@ struct SampleArgs {
   float temperature_all, top_p_all, min_p_all;
   bool bf16;
 };
-size_t sample_workspace(int rows, int V, bool logprobs);
+bool sample_filters(const SampleArgs& a);      // whether any row may be filtered
+size_t sample_workspace(int rows, int V, bool filters);
+long sample_workgroups(int rows, int V);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace dec

@@ -160,7 +160,8 @@ PyObject* sample(const Args& a) {
   const Tensor lp = at::empty({logprobs ? rows : 0}, at::TensorOptions().dtype(at::kFloat).device(dev));
   const int flags = (bf16 ? DEC_BF16 : 0) | (logprobs ? DEC_LOGPROBS : 0);
   size_t need = 0;
-  check(dec_sample_workspace(rows, V, flags, &need));
+  const bool filters = k.defined() || p.defined() || mp.defined() || (k_all >= 1 && k_all < V) || p_all < 1.0f || mp_all > 0.0f;
+  check(dec_sample_workspace(rows, V, filters, &need));
   const Tensor space = new_bytes(dev, need);
   launch(dev, [&](void* stream) {
     return dec_sample(address(x), rows > 1 ? x.stride(0) : V, address_as<const float>(u),
