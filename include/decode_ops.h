@@ -94,7 +94,7 @@ int dec_gated_delta_workspace(int total, int batch, int max_q, int write_cols, i
  * (uniform held to [0, 1); NaN counts as 0). t <= 0: the first in the order. top_k < 1 or past the
  * vocabulary, top_p >= 1 or NaN, min_p <= 0 or NaN filter nothing. A row that holds NaN or nothing above
  * -infinity, and one whose t is NaN, gives token -1 and log probability NaN. Weights are added as
- * integers of 2^-(62 - ceil(log2 vocabulary)), so that results do not depend on an order of additions.
+ * integers of 2^-min(51, 62 - ceil(log2 vocabulary)), so that results do not depend on an order of additions.
  * temperature fp32, top_k int32, top_p fp32, min_p fp32 [rows], or null: the value *_all for all rows.
  * uniform fp32 [rows]; tokens int64 [rows]; logprobs (DEC_LOGPROBS) fp32 [rows], of the softmax of the
  * logits as they are (no temperature, no filter). `workspace`: dec_sample_workspace bytes (filters: whether

@@ -36,33 +36,46 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// 2^y in 64 bits, y <= 0: 2^(k / 64) from a table, and a polynomial for the rest of at most 2^-7 (ln 2 / 128 =
-// 0.0054; the first term left out, r^5 / 120, is below 4e-14).
-__device__ __forceinline__ double exp2_64(double y, const double* table) {
-  if (y < -1100.0) return 0.0;
-  const double k = __builtin_rint(y * 64.0);
-  const double r = (y - k * 0.015625) * 0.6931471805599453;
+// 2^(y + scale) in 64 bits, y <= 0: 2^(k / 64) from a table, and a polynomial for the rest x of at most 2^-7 (the
+// first term left out, (x ln 2)^5 / 120, is below 4e-14).
+__device__ __forceinline__ double exp2_64(double y, const double* table, int scale = 0) {
+  const double k = __builtin_rint(fmax(y, -1100.0) * 64.0);
+  const double x = fma(k, -0.015625, fmax(y, -1100.0));
   const int n = (int)k;
-  const double p = fma(fma(fma(fma(r, 1.0 / 24.0, 1.0 / 6.0), r, 0.5), r, 1.0), r, 1.0);
-  return __builtin_ldexp(table[n & 63] * p, n >> 6);
+  double p = fma(x, 0.009618129107628477, 0.05550410866482158);
+  p = fma(p, x, 0.24022650695910072);
+  p = fma(p, x, 0.6931471805599453);
+  p = fma(p, x, 1.0);
+  return __builtin_ldexp(table[n & 63] * p, (n >> 6) + scale);
 }
 __device__ __forceinline__ void fill_table(double* table) {
   if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
 }
-// A non-negative double below 2^52 rounded to an integer, others by the conversion.
-__device__ __forceinline__ u64 to_units(double x) { return (u64)__double2ull_rn(x); }
+// x of 0 .. 2^52 - 1 rounded to an integer: the low bits of 2^52 + x.
+__device__ __forceinline__ u64 to_units(double x) {
+  return (u64)__double_as_longlong(x + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+}
 
 struct Weights {
   float top;
-  double rate, unit;                    // log2(e) / t, 2^s
+  double rate;                          // log2(e) / t
+  int shift;                            // integers of 2^-shift
   const double* table;
   __device__ double real(float x) const {
     return x == top ? 1.0 : exp2_64(((double)x - (double)top) * rate, table);
   }
-  __device__ u64 operator()(float x) const { return x == -INFINITY ? 0 : to_units(real(x) * unit); }
+  __device__ u64 operator()(float x) const {
+    if (x == top) return 1ull << shift;
+    return x == -INFINITY ? 0 : to_units(exp2_64(((double)x - (double)top) * rate, table, shift));
+  }
+  // the weight where it is at least min_p (over 0)
+  __device__ u64 at_least(float x, float min_p) const {
+    return min_p > 0.0f && !(real(x) >= (double)min_p) ? 0 : (*this)(x);
+  }
 };
 constexpr double kLog2e = 1.4426950408889634;
-__device__ __forceinline__ int unit_shift(int V) { return 62 - (V > 1 ? 32 - __clz(V - 1) : 0); }
+// The integers of a row's weights: 2^-51 at the finest, and the sum of V of them below 2^63.
+__device__ __forceinline__ int unit_shift(int V) { return min(51, 62 - (V > 1 ? 32 - __clz(V - 1) : 0)); }
 
 struct Shared {
   u64 mass[kBins];
@@ -77,22 +90,34 @@ struct Shared {
   int flag, found;
 };
 
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ uint32_t lane_sums(uint32_t x) {
+#define STEP(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false);
+  STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+#undef STEP
+  return x;
+}
+__device__ __forceinline__ u64 lane_sums(u64 x) {
+#define STEP(ctrl, rows)                                                                                        \
+  x += (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, ctrl, rows, 0xF, false) |                \
+       (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), ctrl, rows, 0xF, false) << 32;
+  STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+#undef STEP
+  return x;
+}
+
 // Sums of the threads before this one, and of all.
 template <int N>
 __device__ void scan(u64* wave_mass, uint32_t* wave_count, u64 m, uint32_t c, u64& before_m, uint32_t& before_c,
                      u64& all_m) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 im = m;
-  uint32_t ic = c;
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 pm = __shfl_up(im, d);
-    const uint32_t pc = __shfl_up(ic, d);
-    if (lane >= d) im += pm, ic += pc;
-  }
+  const u64 im = lane_sums(m);
+  const uint32_t ic = lane_sums(c);
   __syncthreads();
   if (lane == 63) wave_mass[wave] = im, wave_count[wave] = ic;
   __syncthreads();
   before_m = im - m, before_c = ic - c, all_m = 0;
+#pragma unroll
   for (int w = 0; w < N / 64; ++w) {
     if (w < wave) before_m += wave_mass[w], before_c += wave_count[w];
     all_m += wave_mass[w];
@@ -132,13 +157,13 @@ __device__ __forceinline__ u64 target_of(float uniform, u64 Z) {
 }
 
 // The cut at which the prefix of the order has `target` elements (BY_MASS: that much weight, > 0): its key,
-// and what lies above the key. at(i, key, weight): element i < n; weight is asked for where it counts.
+// and what lies above the key. Element i < n has at.key(i) and at.weight(i); `key` comes with the bits of the
+// digits before `level`, which all elements that can be at the cut share.
 template <bool BY_MASS, typename Source>
 __device__ void find_cut(Shared& s, int n, const Source& at, u64 target, uint32_t& key, u64& above_count,
-                         u64& above_mass) {
+                         u64& above_mass, int level = 0) {
   const int tid = threadIdx.x;
-  key = 0;
-  for (int level = 0; level < 3; ++level) {
+  for (; level < 3; ++level) {
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
     const uint32_t fixed = level == 0 ? 0u : ~0u << (shift + bits);
     __syncthreads();
@@ -202,7 +227,7 @@ __device__ void whole_row(const SampleArgs& a, int row_at, Shared& s) {
   __syncthreads();
   if (top == s.key) atomicMin(&s.index, at);
   __syncthreads();
-  const Weights w = {of_key(s.key), kLog2e / (double)t, ldexp(1.0, unit_shift(V)), s.table};
+  const Weights w = {of_key(s.key), kLog2e / (double)t, unit_shift(V), s.table};
   const int first = (int)s.index;
   const bool none = s.flag || w.top == -INFINITY;
   if (none) {
@@ -234,7 +259,7 @@ __device__ void whole_row(const SampleArgs& a, int row_at, Shared& s) {
       const double want = ceil((double)par.p * (double)total);
       if (want >= 1.0) {
         const u64 target = min((u64)want, total);
-        above_count = above_mass = 0;
+        above_count = above_mass = cut = 0;
         find_cut<true>(s, V, source, target, cut, above_count, above_mass);
         const u64 each = w(of_key(cut));
         ties = (target - above_mass + each - 1) / each;
@@ -247,8 +272,7 @@ __device__ void whole_row(const SampleArgs& a, int row_at, Shared& s) {
     const auto weight = [&](float x, uint32_t& tie) -> u64 {
       const uint32_t key = key_of(x);
       tie = key == cut && (by_k || by_p);
-      if (key < cut || (mp > 0.0f && !(w.real(x) >= (double)mp))) return 0;
-      return w(x);
+      return key < cut ? 0 : w.at_least(x, mp);
     };
     for (int i = tid; i < kMaxTiles; i += kThreads) s.tile_mass[i] = 0, s.tile_ties[i] = 0;
     __syncthreads();
@@ -301,7 +325,7 @@ __device__ void whole_row(const SampleArgs& a, int row_at, Shared& s) {
     token = s.found;
   }
   if (a.logprobs) {
-    const Weights one = {w.top, kLog2e, w.unit, s.table};
+    const Weights one = {w.top, kLog2e, w.shift, s.table};
     u64 mine = 0, before, total;
     uint32_t c;
     for (int i = tid; i < V; i += kThreads) mine += one(logit<BF16>(row, i));
@@ -309,7 +333,7 @@ __device__ void whole_row(const SampleArgs& a, int row_at, Shared& s) {
     if (tid == 0) {
       const float x = logit<BF16>(row, token);
       a.logprobs[row_at] =
-          (float)((x == w.top ? 0.0 : (double)x - (double)w.top) - log((double)total / w.unit));
+          (float)((x == w.top ? 0.0 : (double)x - (double)w.top) - log(ldexp((double)total, -w.shift)));
     }
   }
   if (tid == 0) a.tokens[row_at] = token;
@@ -446,13 +470,15 @@ __device__ __forceinline__ double sum_all(WideShared& s, double x) {
   return (s.wave_sum[0] + s.wave_sum[1]) + (s.wave_sum[2] + s.wave_sum[3]);
 }
 
+// Sum of exp(x - top). A logarithm of it is asked for in fp32: exponentials in fp32 are off by less than 2^-22 of
+// each that counts, a thread's sum of at most 32 by as much again, and so is the logarithm, in all below 2^-21.
 template <typename M, int N>
 __device__ double exp_sum(WideShared& s, const M& m, float top) {
-  double sum = 0.0;
+  float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (m.x[i] > -INFINITY) sum += m.x[i] == top ? 1.0 : exp2_64(((double)m.x[i] - (double)top) * kLog2e, s.table);
-  return sum_all(s, sum);
+    sum += m.x[i] == top ? 1.0f : __builtin_amdgcn_exp2f((m.x[i] - top) * 1.44269504f);
+  return sum_all(s, (double)sum);
 }
 
 constexpr int kPartUnit = 49;           // a part's weights against its own largest: 2^-49, at most 8192 of them
@@ -470,7 +496,7 @@ __global__ __launch_bounds__(kWide) void weigh(SampleArgs a, Shape sh) {
   const float top = of_key(largest<decltype(m), N>(s, m, part));
   u64 sum = 0;
   if (!par.greedy() && top > -INFINITY) {
-    const Weights w = {top, kLog2e / (double)par.t, ldexp(1.0, kPartUnit), s.table};
+    const Weights w = {top, kLog2e / (double)par.t, kPartUnit, s.table};
 #pragma unroll
     for (int i = 0; i < N; ++i) sum += w(m.x[i]);
     u64 before;
@@ -598,11 +624,11 @@ __global__ __launch_bounds__(kThreads) void pick(SampleArgs a, Shape sh) {
       const float x = of_key(parts[i].top);
       return x == -INFINITY ? 0.0 : x == top ? 1.0 : exp2_64(((double)x - (double)top) * rate, s.table);
     };
-    for (int i = threadIdx.x; i < n; i += kThreads) s.tile_mass[i] = to_units((double)parts[i].kept * factor(i) * unit);
+    for (int i = threadIdx.x; i < n; i += kThreads) s.tile_mass[i] = (u64)((double)parts[i].kept * factor(i) * unit + 0.5);
     __syncthreads();
     u64 target;
     const int at = part_of(s, n, a.uniform[row_at], target);
-    const Weights w = {of_key(parts[at].top), rate, ldexp(1.0, kPartUnit), s.table};
+    const Weights w = {of_key(parts[at].top), rate, kPartUnit, s.table};
     // what is left of the target, in the part's own units
     const u64 inside = (u64)((double)target / (double)s.tile_mass[at] * (double)parts[at].kept);
     token = pass_at<BF16>(s, row_of(a, row_at), at * sh.l.per, min((at + 1) * sh.l.per, a.V), inside,
@@ -632,7 +658,7 @@ __global__ __launch_bounds__(kWide) void survey(SampleArgs a, Shape sh) {
     // bin's largest possible value it could be all but nothing. No other bin's value is above the row's largest.
     const double rate = kLog2e / (double)par.t;
     const uint32_t top_bin = part.top >> kBinShift;
-    const Weights w = {top, rate, ldexp(1.0, kPartUnit), s.table};
+    const Weights w = {top, rate, kPartUnit, s.table};
     u64 near = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -641,7 +667,7 @@ __global__ __launch_bounds__(kWide) void survey(SampleArgs a, Shape sh) {
       u64 x = 0;
       if (par.by_p) {
         if (bin == top_bin) near += w(m.x[i]);
-        else x = to_units(exp2_64(((double)m.x[i] - (double)bin_value(bin)) * rate, s.table) * (double)(1ull << kRelative));
+        else x = to_units(exp2_64(((double)m.x[i] - (double)bin_value(bin)) * rate, s.table, kRelative));
       }
       atomicAdd(&s.bins[bin], x << kCountBits | 1);
     }
@@ -690,14 +716,14 @@ __global__ __launch_bounds__(kWide) void collect(SampleArgs a, Shape sh) {
   if (s.bad || top == -INFINITY) return;
   const double rate = kLog2e / (double)par.t;
   const int shift = unit_shift(a.V);
-  const Weights w = {top, rate, ldexp(1.0, shift), s.table};
+  const Weights w = {top, rate, shift, s.table};
   bool by_k = false;
   if (par.by_k || par.by_p) {
     if (par.by_p) {
       for (int i = tid; i < sh.l.parts; i += kWide)
         if (parts[i].near)
           atomicAdd(&s.bins[parts[i].top >> kBinShift],
-                    to_units((double)parts[i].near * w.real(of_key(parts[i].top)) * ldexp(1.0, shift - kPartUnit)));
+                    (u64)((double)parts[i].near * w.real(of_key(parts[i].top)) * ldexp(1.0, shift - kPartUnit) + 0.5));
       __syncthreads();
     }
     // bins from the highest, 8 a thread
@@ -711,7 +737,7 @@ __global__ __launch_bounds__(kWide) void collect(SampleArgs a, Shape sh) {
       if (par.by_p && count[j]) {
         mass[j] = s.bins[bin];
         const u64 x = row.mass[bin];    // (none in the bin of the row's largest)
-        if (x) mass[j] += to_units((double)x * w.real(bin_value(bin)) * ldexp(1.0, shift - kRelative));
+        if (x) mass[j] += (u64)((double)x * w.real(bin_value(bin)) * ldexp(1.0, shift - kRelative) + 0.5);
       }
       have += count[j], mine += mass[j];
     }
@@ -771,9 +797,7 @@ __global__ __launch_bounds__(kWide) void collect(SampleArgs a, Shape sh) {
       continue;
     }
     if (x < skip) continue;
-    const double r = w.real(x);
-    if (par.mp > 0.0f && !(r >= (double)par.mp)) continue;
-    sum += to_units(r * w.unit);
+    sum += w.at_least(x, par.mp);
   }
   u64 before_m, all_m;
   uint32_t before_c;
@@ -847,7 +871,7 @@ __global__ __launch_bounds__(kThreads) void choose(SampleArgs a, Shape sh) {
   if (!par.greedy()) {
     const int listed = (int)row.listed;
     if (listed > sh.l.most) return whole_row<BF16>(a, row_at, s);
-    const Weights w = {top, kLog2e / (double)par.t, ldexp(1.0, unit_shift(a.V)), s.table};
+    const Weights w = {top, kLog2e / (double)par.t, unit_shift(a.V), s.table};
     const Entry* list = sh.list(a, row_at);
     const ListSource source = {list};
     if (threadIdx.x == 0) s.key = 0, s.above_count = s.above_mass = 0;
@@ -862,12 +886,15 @@ __global__ __launch_bounds__(kThreads) void choose(SampleArgs a, Shape sh) {
       scan(s, mine, 0, before, c, in_list);
     }
     // (Where min-p takes from what is above the list it takes all of the list, and the cuts do not matter.)
+    // (the digit that the listed keys share, where they lie in one bin, is not looked at)
+    const int level = row.high - row.low == 1u << kBinShift;
     uint32_t cut = 0;
     u64 ties = 0, total = above + in_list + row.below;
     bool whole = true;                  // all of the list is kept
     if (row.by_k) {
       u64 ac = row.above_count, am = above;
-      find_cut<false>(s, listed, source, (u64)par.k, cut, ac, am);
+      cut = level ? row.low : 0;
+      find_cut<false>(s, listed, source, (u64)par.k, cut, ac, am, level);
       ties = (u64)par.k - ac, whole = false;
       total = am + ties * w(of_key(cut));
     }
@@ -881,7 +908,8 @@ __global__ __launch_bounds__(kThreads) void choose(SampleArgs a, Shape sh) {
       } else if ((u64)want <= above + in_list) {
         u64 ac = row.above_count, am = above;
         const u64 target = min((u64)want, total);
-        find_cut<true>(s, listed, source, target, cut, ac, am);
+        cut = level ? row.low : 0;
+        find_cut<true>(s, listed, source, target, cut, ac, am, level);
         const u64 each = max(w(of_key(cut)), 1ull);
         ties = (target - am + each - 1) / each, whole = false;
       }
@@ -913,7 +941,7 @@ __global__ __launch_bounds__(kThreads) void choose(SampleArgs a, Shape sh) {
                             const uint32_t key = key_of(x);
                             if (x == -INFINITY || key < low) return 0;
                             if (key < high) return listed_kept(key, i, w(x));
-                            return par.mp > 0.0f && !(w.real(x) >= (double)par.mp) ? 0 : w(x);
+                            return w.at_least(x, par.mp);
                           });
   }
   write_token<BF16>(a, row_at, token, top, parts, n, s);
