@@ -106,8 +106,8 @@ def test_delta_wants_its_workspace(lib):
 
 
 def sample(lib, **kw):
-    a = dict(x=P, stride=100, u=P, t=P, ta=1.0, k=P, ka=0, p=P, pa=1.0, mp=P, ma=0.0, tokens=P, lp=P, work=P,
-             wb=1 << 40, rows=3, V=100, flags=N.LOGPROBS)
+    a = dict(x=P, stride=100, u=P, t=P, ta=1.0, k=P, ka=0, p=P, pa=1.0, mp=P, ma=0.0, tokens=P, lp=P,
+             rows=3, V=100, flags=N.LOGPROBS)
     a.update(kw)
     return lib.dec_sample(*a.values(), None)
 
@@ -122,22 +122,11 @@ def test_sample_refuses(lib, kw, msg):
     assert sample(lib, **kw) == EINVAL and msg in lib.dec_last_error()
 
 
-def test_sample_wants_its_workspace(lib):
-    need = N.sample_workspace(3, 100, N.LOGPROBS)
-    if need:
-        for kw in (dict(wb=need - 1), dict(work=None), dict(work=P + 8)):
-            assert sample(lib, **kw) == EINVAL and b"workspace" in lib.dec_last_error()
-    assert N.sample_workspace(0, 100) == 0
-    with pytest.raises(RuntimeError, match="vocabulary"):
-        N.sample_workspace(3, 0)
-    assert lib.dec_sample_workspace(3, 100, 0, None) == EINVAL
-
-
 def test_nothing_to_do_needs_no_gpu(lib):
     assert conv(lib, B=0, T=0, x=None, w=None, state=None, starts=None, read=None, write=None, out=None) == 0
     assert delta(lib, B=0, T=0, q=None, k=None, v=None, state=None, starts=None, read=None, write=None, out=None,
                  work=None, wb=0) == 0
-    assert sample(lib, rows=0, x=None, u=None, tokens=None, lp=None, work=None, wb=0) == 0
+    assert sample(lib, rows=0, x=None, u=None, tokens=None, lp=None) == 0
 
 
 def test_errors_are_the_last_ones(lib):

@@ -164,25 +164,14 @@ int check_sample_sizes(const char* who, int rows, int vocabulary, int flags) {
   if (vocabulary <= 0 || vocabulary > 1 << 24)
     return fail(DEC_EINVAL, "%s: a vocabulary of %d: need 1..2^24", who, vocabulary);
   if (flags & ~(DEC_BF16 | DEC_LOGPROBS)) return fail(DEC_EINVAL, "%s: unknown flags %d", who, flags);
-  if (rows && sample_workgroups(rows, vocabulary) > kMaxGrid / 4)
-    return fail(DEC_EINVAL, "%s: %d rows of %d are too many", who, rows, vocabulary);
   return DEC_OK;
 }
 }  // namespace
 
-DEC_API int dec_sample_workspace(int rows, int vocabulary, int filters, size_t* bytes) {
-  const char* who = "sample_workspace";
-  if (!bytes) return fail(DEC_EINVAL, "%s: null output", who);
-  if (int rc = check_sample_sizes(who, rows, vocabulary, 0)) return rc;
-  *bytes = rows ? sample_workspace(rows, vocabulary, filters) : 0;
-  return DEC_OK;
-}
-
 DEC_API int dec_sample(const void* logits, long row_stride, const float* uniform, const float* temperature,
                        float temperature_all, const int* top_k, int top_k_all, const float* top_p,
                        float top_p_all, const float* min_p, float min_p_all, int64_t* tokens, float* logprobs,
-                       void* workspace, size_t workspace_bytes, int rows, int vocabulary, int flags,
-                       void* stream) {
+                       int rows, int vocabulary, int flags, void* stream) {
   const char* who = "sample";
   if (int rc = check_sample_sizes(who, rows, vocabulary, flags)) return rc;
   const int size = flags & DEC_BF16 ? 2 : 4;
@@ -198,12 +187,8 @@ DEC_API int dec_sample(const void* logits, long row_stride, const float* uniform
   SampleArgs a = {};
   a.logits = logits, a.uniform = uniform, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p;
   a.min_p = min_p, a.tokens = tokens, a.logprobs = flags & DEC_LOGPROBS ? logprobs : nullptr;
-  a.workspace = workspace, a.row_stride = rows > 1 ? row_stride : 0, a.rows = rows, a.V = vocabulary;
+  a.row_stride = rows > 1 ? row_stride : 0, a.rows = rows, a.V = vocabulary;
   a.temperature_all = temperature_all, a.top_k_all = top_k_all, a.top_p_all = top_p_all, a.min_p_all = min_p_all;
   a.bf16 = flags & DEC_BF16;
-  const size_t need = sample_workspace(rows, vocabulary, sample_filters(a));
-  if (need > workspace_bytes || (need && (!workspace || !aligned(workspace, 16))))
-    return fail(DEC_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, need,
-                workspace_bytes);
   return hip_status(launch_sample(a, (hipStream_t)stream), who);
 }

@@ -91,15 +91,11 @@ struct SampleArgs {
   const float* min_p;
   int64_t* tokens;
   float* logprobs;
-  void* workspace;
   long row_stride;
   int rows, V, top_k_all;
   float temperature_all, top_p_all, min_p_all;
   bool bf16;
 };
-bool sample_filters(const SampleArgs& a);      // whether any row may be filtered
-size_t sample_workspace(int rows, int V, bool filters);
-long sample_workgroups(int rows, int V);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace dec

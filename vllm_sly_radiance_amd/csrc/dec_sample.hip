@@ -1,31 +1,31 @@
 // One token of each row of logits by temperature, top-k, top-p and min-p from a given uniform number, for
-// gfx950.
+// gfx950: a workgroup a row, which stays in the die's L2 between its passes.
 //
-// What top-k and top-p keep is a prefix of the row in descending order, ties by index: all elements above a
-// cut key and the first few at it. Weights are exp in 64 bits, added as integers of 2^-s: such sums are exact
-// and the same in any order, which the atomics of a histogram need, and with s = 62 - ceil(log2 V) a row's sum
-// is off by no more than 2^-(s + 1) an element, 3e-12 of the largest weight in all for V = 131072 in the mean.
-//
-// A row is read by as many workgroups as fill the card, twice:
-//   survey    the largest logit, and how many elements and how much weight (against the largest value of the
-//             bin, as the row's is not known yet) there are in each of 2048 bins of the keys' upper bits
-//   collect   finds the bins in which the cut lies, adds up what is above them, and lists their elements
-//   choose    one workgroup a row: the cut from the listed elements, digit by digit, then the part of the row
-//             in which the sum of the kept weights passes uniform times their sum, and the token in it
-// Without filters the row is read once (weigh, against the part's own largest logit, and pick). Rows of few
-// elements, and those of which too many share a bin, are done by one workgroup (whole_row).
+// What top-k and top-p keep is a prefix of the row in descending order, ties by index. Weights are exp in 64
+// bits, added as integers of 2^-s: such sums are exact and the same in any order, which atomics need, and with
+// s = min(51, 62 - ceil(log2 V)) a row's sum is off by no more than 2^-(s + 1) an element, 3e-12 of the largest
+// weight in all for V = 131072 in the mean.
+//   top-k, up to 512   the k-th of the threads' own maxima is no more than the k-th of the row: one pass lists what is
+//                      at least that (some 700 elements for 512), the list is sorted, the cuts are places in it, and
+//                      sorted by place it gives the token
+//   otherwise          a pass makes a histogram of the distance to the largest logit in 2048 steps, counts and
+//                      weights; the next lists the elements of the steps in which the cuts lie and adds up the
+//                      weight above them by tiles of the row; the cuts are found in the list digit by digit, and the
+//                      token in the tile where the sum of what is kept passes uniform times all of it
+//   rows of which too many elements share a step: the cuts digit by digit of the 32-bit keys, over the row
 #include "decode_ops.h"
 #include "dec_internal.h"
 
 namespace dec {
 namespace {
 
-constexpr int kThreads = 1024, kBins = 2048, kBinShift = 21, kTile = 4096, kMaxTiles = 4096;
-constexpr int kWide = 256;              // threads of the workgroups that share a row
-constexpr int kCountBits = 14;          // of a bin's word in a workgroup: elements, at most 8192
-constexpr int kRelative = 36;           // and weight above them, in 2^-36 of the bin's largest possible
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kBins = 2048, kList = 4096, kTiles = 1024, kTable = 1024;
+constexpr int kSorted = 512;            // top-k up to this by sorting a list
 typedef unsigned long long u64;
 constexpr float kNaN = __builtin_nanf("");
+constexpr double kLog2e = 1.4426950408889634;
+constexpr uint32_t kLowest = 0x007FFFFFu;       // key of -infinity
 
 // Order-preserving bits of a float that is not NaN; -0 as 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -36,105 +36,288 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// 2^(y + scale) in 64 bits, y <= 0: 2^(k / 64) from a table, and a polynomial for the rest x of at most 2^-7 (the
-// first term left out, (x ln 2)^5 / 120, is below 4e-14).
-__device__ __forceinline__ double exp2_64(double y, const double* table, int scale = 0) {
-  const double k = __builtin_rint(fmax(y, -1100.0) * 64.0);
-  const double x = fma(k, -0.015625, fmax(y, -1100.0));
-  const int n = (int)k;
-  double p = fma(x, 0.009618129107628477, 0.05550410866482158);
-  p = fma(p, x, 0.24022650695910072);
-  p = fma(p, x, 0.6931471805599453);
-  p = fma(p, x, 1.0);
-  return __builtin_ldexp(table[n & 63] * p, (n >> 6) + scale);
-}
-__device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
-}
-// x of 0 .. 2^52 - 1 rounded to an integer: the low bits of 2^52 + x.
-__device__ __forceinline__ u64 to_units(double x) {
-  return (u64)__double_as_longlong(x + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
-}
-
-struct Weights {
-  float top;
-  double rate;                          // log2(e) / t
-  int shift;                            // integers of 2^-shift
-  const double* table;
-  __device__ double real(float x) const {
-    return x == top ? 1.0 : exp2_64(((double)x - (double)top) * rate, table);
-  }
-  __device__ u64 operator()(float x) const {
-    if (x == top) return 1ull << shift;
-    return x == -INFINITY ? 0 : to_units(exp2_64(((double)x - (double)top) * rate, table, shift));
-  }
-  // the weight where it is at least min_p (over 0)
-  __device__ u64 at_least(float x, float min_p) const {
-    return min_p > 0.0f && !(real(x) >= (double)min_p) ? 0 : (*this)(x);
-  }
-};
-constexpr double kLog2e = 1.4426950408889634;
 // The integers of a row's weights: 2^-51 at the finest, and the sum of V of them below 2^63.
 __device__ __forceinline__ int unit_shift(int V) { return min(51, 62 - (V > 1 ? 32 - __clz(V - 1) : 0)); }
 
-struct Shared {
-  u64 mass[kBins];
-  uint32_t count[kBins];
-  u64 wave_mass[16];
-  uint32_t wave_count[16];
-  u64 tile_mass[kMaxTiles];
-  uint32_t tile_ties[kMaxTiles];
-  double table[64];
-  uint32_t key, index;
-  u64 above_count, above_mass;
-  int flag, found;
+// 2^((x - top) rate) in units of 2^-shift, with rate = log2(e) / t. y = 1024 (x - top) rate = k + r, |r| <= 1/2: from
+// a table of 2^(i / 1024), and 2^(r / 1024) - 1 as a polynomial whose first term left out, (r ln 2 / 1024)^4 / 24,
+// is below 1e-15. k comes from the low bits of y + 1.5 2^52, and the rounding to an integer from adding 2^52.
+struct Weights {
+  float top;
+  double rate, offset;                  // 1024 log2(e) / t, and top times it
+  int shift;
+  const double* table;
+  __device__ Weights(float top, double t, int shift, const double* table)
+      : top(top), rate(1024.0 * kLog2e / t), offset((double)top * (1024.0 * kLog2e / t)), shift(shift), table(table) {}
+  // in units, not rounded to whole ones, for x below top
+  __device__ __forceinline__ double units(float x) const {
+    const double y = fmax(fma((double)x, rate, -offset), -1024.0 * 1000.0);
+    const double k = y + 6755399441055744.0;
+    const int n = (int)(uint32_t)__double_as_longlong(k);
+    const double r = y - (k - 6755399441055744.0);
+    const double q = r * fma(fma(r, 5.169222938345892e-11, 2.290978498068816e-07), r, 0.0006769015435155716);
+    const u64 bits = (u64)__double_as_longlong(table[n & (kTable - 1)]) + ((u64)(uint32_t)((n >> 10) + shift) << 52);
+    const double v = __longlong_as_double((long long)bits);
+    return fma(v, q, v);
+  }
+  static __device__ __forceinline__ u64 whole(double units) {
+    return (u64)__double_as_longlong(units + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    return x == top ? 1ull << shift : x == -INFINITY ? 0 : whole(units(x));
+  }
+  // the weight where it is at least min_p, `least` in units (0: any)
+  __device__ __forceinline__ u64 from(float x, double least) const {
+    if (x == top) return 1ull << shift;
+    if (x == -INFINITY) return 0;
+    const double u = units(x);
+    return u >= least ? whole(u) : 0;
+  }
 };
 
+struct Shared {
+  double table[kTable];
+  u64 mass[kBins];
+  uint32_t count[kBins];
+  uint32_t key[kList];                  // the list: keys and places
+  int at[kList];
+  u64 tile[kTiles];
+  u64 wave[kWaves], wave2[kWaves];
+  u64 value[4];
+  uint32_t listed;
+};
+
+// ---- over lanes and the workgroup ---------------------------------------------------------------
+// (row_shr:1, 2, 4, 8, then the rows' last lanes: row_bcast:15 and 31)
+#define LANE_STEPS STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 x) {
+  return (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false) |
+         (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false) << 32;
+}
 // Inclusive sums over the wave's lanes.
-__device__ __forceinline__ uint32_t lane_sums(uint32_t x) {
-#define STEP(ctrl, rows) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false);
-  STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
-#undef STEP
-  return x;
-}
 __device__ __forceinline__ u64 lane_sums(u64 x) {
-#define STEP(ctrl, rows)                                                                                        \
-  x += (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, ctrl, rows, 0xF, false) |                \
-       (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), ctrl, rows, 0xF, false) << 32;
-  STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+#define STEP(ctrl, rows) x += moved<ctrl, rows>(x);
+  LANE_STEPS
+#undef STEP
+  return x;
+}
+// The largest of the wave's lanes, in the last of them.
+__device__ __forceinline__ u64 lane_max(u64 x) {
+#define STEP(ctrl, rows) x = max(x, moved<ctrl, rows>(x));
+  LANE_STEPS
 #undef STEP
   return x;
 }
 
-// Sums of the threads before this one, and of all.
-template <int N>
-__device__ void scan(u64* wave_mass, uint32_t* wave_count, u64 m, uint32_t c, u64& before_m, uint32_t& before_c,
-                     u64& all_m) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 im = lane_sums(m);
-  const uint32_t ic = lane_sums(c);
+// The largest of all threads.
+__device__ u64 all_max(Shared& s, u64 x) {
+  x = lane_max(x);
   __syncthreads();
-  if (lane == 63) wave_mass[wave] = im, wave_count[wave] = ic;
+  if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = x;
   __syncthreads();
-  before_m = im - m, before_c = ic - c, all_m = 0;
+  x = s.wave[0];
 #pragma unroll
-  for (int w = 0; w < N / 64; ++w) {
-    if (w < wave) before_m += wave_mass[w], before_c += wave_count[w];
-    all_m += wave_mass[w];
-  }
-}
-__device__ __forceinline__ void scan(Shared& s, u64 m, uint32_t c, u64& before_m, uint32_t& before_c, u64& all_m) {
-  scan<kThreads>(s.wave_mass, s.wave_count, m, c, before_m, before_c, all_m);
+  for (int w = 1; w < kWaves; ++w) x = max(x, s.wave[w]);
+  __syncthreads();
+  return x;
 }
 
+// Sum of the threads before this one, and of all.
+__device__ void sums(Shared& s, u64 x, u64& before, u64& all) {
+  const u64 up_to = lane_sums(x);
+  const int wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s.wave[wave] = up_to;
+  __syncthreads();
+  before = up_to - x, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += s.wave[w];
+    all += s.wave[w];
+  }
+  __syncthreads();
+}
+
+// The value that the one thread with `mine` has (0 where none has), for all.
+__device__ u64 from_one(Shared& s, bool mine, u64 x) {
+  if (threadIdx.x == 0) s.value[0] = 0;
+  __syncthreads();
+  if (mine) s.value[0] = x;
+  __syncthreads();
+  x = s.value[0];
+  __syncthreads();
+  return x;
+}
+
+// Values in descending order, one a thread: a sorting network over the first `size` threads (a power of two, 64 at
+// least; the others' values stay among themselves).
+template <typename T>
+__device__ T sorted(Shared& s, T x, int size) {
+  const int tid = threadIdx.x;
+  T* lds = (T*)s.mass;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j; j >>= 1) {
+      T y;
+      if (j < 64) {
+        y = __shfl_xor(x, j);
+      } else {
+        __syncthreads();
+        lds[tid] = x;
+        __syncthreads();
+        y = lds[tid ^ j];
+      }
+      const bool larger = ((tid & k) == 0) == ((tid & j) == 0);
+      x = larger ? max(x, y) : min(x, y);
+    }
+  __syncthreads();
+  return x;
+}
+__device__ __forceinline__ int power_from(int n) {
+  int size = 64;
+  while (size < n) size <<= 1;
+  return size;
+}
+
+// ---- the row ------------------------------------------------------------------------------------
 template <bool BF16>
 __device__ __forceinline__ float logit(const void* row, int i) {
   return BF16 ? bf16_f32(((const uint16_t*)row)[i]) : ((const float*)row)[i];
 }
 
-// A row's parameters.
+// A row in tiles of consecutive elements, a wave each in turn, 16 bytes of a thread at a time: counted from the
+// address of 16 bytes that the row begins in, `lead` elements before it.
+template <bool BF16>
+struct Row {
+  static constexpr int kRun = BF16 ? 8 : 4, kAhead = BF16 ? 4 : 8;
+  const void* p;
+  int V, lead, tile;                    // elements of a tile: kTiles of them hold the row
+  __device__ Row(const void* p, int V) : p(p), V(V), lead((int)((uintptr_t)p % 16) / (BF16 ? 2 : 4)) {
+    tile = 64 * kRun * kAhead;
+    while ((long)tile * kTiles < (long)V + lead) tile <<= 1;
+  }
+  // f(x, place) for each element of this thread's in turn; end(tile) after each of its wave's tiles.
+  template <typename F, typename G>
+  __device__ void sweep(const F& f, const G& end) const {
+    const int lane = threadIdx.x & 63;
+    for (int t = threadIdx.x >> 6; (long)t * tile < (long)V + lead; t += kWaves) {
+      const int to = (int)min((long)(t + 1) * tile - lead, (long)V);
+      for (int from = t * tile - lead; from < to; from += 64 * kRun * kAhead) {
+        uint4 u[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int i = from + (a * 64 + lane) * kRun;
+          u[a] = {};
+          if (i >= 0 && i + kRun <= to) {
+            u[a] = BF16 ? *(const uint4*)((const uint16_t*)p + i) : *(const uint4*)((const float*)p + i);
+          } else if (i < to) {          // the row's ends
+            uint32_t w[4] = {};
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) {
+              const bool in = i + j >= 0 && i + j < to;
+              if constexpr (BF16) w[j / 2] |= in ? (uint32_t)((const uint16_t*)p)[i + j] << (16 * (j % 2)) : 0u;
+              else w[j] = in ? ((const uint32_t*)p)[i + j] : 0u;
+            }
+            u[a] = {w[0], w[1], w[2], w[3]};
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int i = from + (a * 64 + lane) * kRun;
+          const uint32_t w[4] = {u[a].x, u[a].y, u[a].z, u[a].w};
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) {
+            const float x = !BF16 ? __uint_as_float(w[j % 4]) : j % 2 ? bf16_hi(w[j / 2 % 4]) : bf16_lo(w[j / 2 % 4]);
+            if (i + j >= 0 && i + j < to) f(x, i + j);
+          }
+        }
+      }
+      end(t);
+    }
+  }
+  template <typename F>
+  __device__ void sweep(const F& f) const {
+    sweep(f, [](int) {});
+  }
+};
+
+// Elements of a row with their weights, for find_cut.
+template <typename R>
+struct OfRow {
+  const R& row;
+  const Weights& w;
+  template <typename F>
+  __device__ void each(const F& f) const {
+    row.sweep([&](float x, int) { f(key_of(x), [&] { return w(x); }); });
+  }
+};
+struct OfList {
+  const Shared& s;
+  int n;
+  const Weights& w;
+  template <typename F>
+  __device__ void each(const F& f) const {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint32_t key = s.key[i];
+      f(key, [&] { return w(of_key(key)); });
+    }
+  }
+};
+
+// The bin, of those that the threads have two each from the highest, in which the sum passes to `target` or more, and
+// what lies above it. (~0: none.)
+__device__ uint32_t find_bin(Shared& s, const u64 m[2], u64 from, u64 target, u64& above) {
+  u64 before, all;
+  sums(s, m[0] + m[1], before, all);
+  u64 x = from + before, hit = 0, at = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (x < target && x + m[j] >= target) hit = 2 * threadIdx.x + j + 1, at = x;
+    x += m[j];
+  }
+  above = from_one(s, hit != 0, at);
+  return (uint32_t)from_one(s, hit != 0, hit) - 1;
+}
+
+// The key at which the prefix of the order has `target` elements (BY_MASS: that much weight, over 0), digit by digit
+// (11, 11 and 10 bits), and the elements and the weight above it. `count` and `mass` come with what lies above all
+// elements of `from`.
+template <bool BY_MASS, typename From>
+__device__ uint32_t find_cut(Shared& s, const From& from, u64 target, u64& count, u64& mass) {
+  const int tid = threadIdx.x;
+  uint32_t key = 0;
+  for (int level = 0; level < 3; ++level) {
+    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+    const uint32_t fixed = level == 0 ? 0u : ~0u << (shift + bits);
+    for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+    __syncthreads();
+    from.each([&](uint32_t k, auto weight) {
+      if ((k & fixed) != key) return;
+      const uint32_t bin = (k >> shift) & ((1u << bits) - 1);
+      atomicAdd(&s.count[bin], 1u);
+      atomicAdd(&s.mass[bin], weight());
+    });
+    __syncthreads();
+    u64 m[2], c[2], other;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) m[j] = s.mass[kBins - 1 - 2 * tid - j], c[j] = s.count[kBins - 1 - 2 * tid - j];
+    const uint32_t bin = find_bin(s, BY_MASS ? m : c, BY_MASS ? mass : count, target, other);
+    // what lies above it by the other measure
+    u64 before, all;
+    const u64 mine0 = BY_MASS ? c[0] : m[0], mine1 = BY_MASS ? c[1] : m[1];
+    sums(s, mine0 + mine1, before, all);
+    const u64 up_to = from_one(s, bin >> 1 == (uint32_t)tid, before + (bin & 1 ? mine0 : 0));
+    if (BY_MASS) mass = other, count += up_to;
+    else count = other, mass += up_to;
+    key |= (kBins - 1 - bin) << shift;
+  }
+  return key;
+}
+
+// ---- parameters ---------------------------------------------------------------------------------
 struct Params {
   float t, p, mp;
+  double least;                         // min-p in units
   int k;
   bool by_k, by_p;
   __device__ Params(const SampleArgs& a, int row) {
@@ -142,861 +325,325 @@ struct Params {
     k = a.top_k ? a.top_k[row] : a.top_k_all;
     p = a.top_p ? a.top_p[row] : a.top_p_all;
     mp = a.min_p ? a.min_p[row] : a.min_p_all;
+    least = mp > 0.0f ? ldexp((double)mp, unit_shift(a.V)) : 0.0;
     by_k = k >= 1 && k < a.V, by_p = p < 1.0f;
   }
   // the first of the largest, whatever the uniform number
   __device__ bool greedy() const { return !(t > 0.0f) || mp > 1.0f; }
+  // how much weight top-p asks of `total`
+  __device__ double asked(u64 total) const { return ceil((double)p * (double)total); }
 };
-__device__ __forceinline__ const void* row_of(const SampleArgs& a, int row) {
-  return (const char*)a.logits + (size_t)row * a.row_stride * (a.bf16 ? 2 : 4);
-}
-__device__ __forceinline__ u64 target_of(float uniform, u64 Z) {
-  // (a cumulated sum exceeds u Z where it exceeds what whole number there is in u Z)
+
+// A cumulated sum exceeds uniform times all of it where it exceeds what whole number there is in that.
+__device__ __forceinline__ u64 target_of(float uniform, u64 all) {
   const float u = fminf(fmaxf(uniform, 0.0f), 1.0f);
-  return min((u64)((double)u * (double)Z), Z - 1);
+  return min((u64)((double)u * (double)all), all - 1);
 }
 
-// The cut at which the prefix of the order has `target` elements (BY_MASS: that much weight, > 0): its key,
-// and what lies above the key. Element i < n has at.key(i) and at.weight(i); `key` comes with the bits of the
-// digits before `level`, which all elements that can be at the cut share.
-template <bool BY_MASS, typename Source>
-__device__ void find_cut(Shared& s, int n, const Source& at, u64 target, uint32_t& key, u64& above_count,
-                         u64& above_mass, int level = 0) {
-  const int tid = threadIdx.x;
-  for (; level < 3; ++level) {
-    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-    const uint32_t fixed = level == 0 ? 0u : ~0u << (shift + bits);
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const uint32_t k = at.key(i);
-      if ((k & fixed) != key) continue;
-      const uint32_t bin = (k >> shift) & ((1u << bits) - 1);
-      atomicAdd(&s.count[bin], 1u);
-      atomicAdd(&s.mass[bin], at.weight(i));
-    }
-    __syncthreads();
-    u64 m[2], before_m, all_m;
-    uint32_t c[2], before_c;
-    for (int j = 0; j < 2; ++j) m[j] = s.mass[kBins - 1 - 2 * tid - j], c[j] = s.count[kBins - 1 - 2 * tid - j];
-    scan(s, m[0] + m[1], c[0] + c[1], before_m, before_c, all_m);
-    u64 am = above_mass + before_m, ac = above_count + before_c;
-    for (int j = 0; j < 2; ++j) {
-      const u64 x = BY_MASS ? am : ac, more = BY_MASS ? m[j] : (u64)c[j];
-      if (x < target && x + more >= target)
-        s.key = key | (uint32_t)(kBins - 1 - 2 * tid - j) << shift, s.above_count = ac, s.above_mass = am;
-      am += m[j], ac += c[j];
-    }
-    __syncthreads();
-    key = s.key, above_count = s.above_count, above_mass = s.above_mass;
-  }
-}
-
-template <bool BF16>
-struct RowSource {
-  const void* row;
-  const Weights& w;
-  __device__ uint32_t key(int i) const { return key_of(logit<BF16>(row, i)); }
-  __device__ u64 weight(int i) const { return w(logit<BF16>(row, i)); }
+// What is kept: keys above `key`, and those at it up to place `last`.
+struct Cut {
+  uint32_t key;
+  int last;
+  __device__ __forceinline__ bool keeps(uint32_t k, int at) const { return k > key || (k == key && at <= last); }
 };
 
-// A row in one workgroup.
-template <bool BF16>
-__device__ void whole_row(const SampleArgs& a, int row_at, Shared& s) {
-  const int tid = threadIdx.x, V = a.V;
-  const void* row = row_of(a, row_at);
-  const Params par(a, row_at);
-  const float t = par.t, mp = par.mp;
-  __syncthreads();
-  fill_table(s.table);
+// The place of the `ties`-th of the elements with this key, in order of places: 8 of its 24 bits at a time.
+template <typename Each>
+__device__ int last_tie(Shared& s, u64 ties, const Each& each) {
+  uint32_t at = 0;
+  for (int shift = 16; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += kThreads) s.count[i] = 0;
+    __syncthreads();
+    each([&](uint32_t place) {
+      if (place >> (shift + 8) == at >> (shift + 8)) atomicAdd(&s.count[(place >> shift) & 255], 1u);
+    });
+    __syncthreads();
+    const u64 c = threadIdx.x < 256 ? s.count[threadIdx.x] : 0;
+    u64 before, all;
+    sums(s, c, before, all);
+    const bool hit = before < ties && before + c >= ties;
+    at |= (uint32_t)from_one(s, hit, threadIdx.x) << shift;
+    ties -= from_one(s, hit, before);
+  }
+  return (int)at;
+}
 
-  // the largest logit and where it is first
-  uint32_t top = 0, at = 0xFFFFFFFFu;
-  bool bad = t != t;
-  for (int i = tid; i < V; i += kThreads) {
-    const float x = logit<BF16>(row, i);
-    bad |= x != x;
-    const uint32_t key = x != x ? 0 : key_of(x);
-    if (key > top) top = key, at = i;
+// The token where tiles hold the kept weight of the row's tiles and weight(x, place) that of an element.
+template <bool BF16, typename R, typename F>
+__device__ int locate(Shared& s, const R& row, float uniform, const F& weight) {
+  u64 before, all;
+  const u64 mine = s.tile[threadIdx.x];
+  sums(s, mine, before, all);
+  const u64 target = target_of(uniform, all);
+  const bool hit = before <= target && before + mine > target;
+  const int tile = (int)from_one(s, hit, threadIdx.x);
+  const u64 left = target - from_one(s, hit, before);
+  // runs of consecutive elements a thread
+  const int run = row.tile / kThreads, to = (int)min((long)(tile + 1) * row.tile - row.lead, (long)row.V);
+  const long i0 = (long)tile * row.tile - row.lead + (long)threadIdx.x * run;
+  u64 sum = 0;
+  for (int i = 0; i < run; ++i)
+    if (i0 + i >= 0 && i0 + i < to) sum += weight(logit<BF16>(row.p, (int)i0 + i), (int)i0 + i);
+  sums(s, sum, before, all);
+  int at = -1;
+  if (before <= left && before + sum > left) {
+    u64 x = before;
+    for (int i = 0; i < run && at < 0; ++i) {
+      if (i0 + i >= 0 && i0 + i < to) x += weight(logit<BF16>(row.p, (int)i0 + i), (int)i0 + i);
+      if (x > left) at = (int)i0 + i;
+    }
   }
-  if (tid == 0) s.key = 0, s.index = 0xFFFFFFFFu, s.flag = 0, s.found = -1;
+  return (int)from_one(s, at >= 0, (u64)(at + 1)) - 1;
+}
+
+// The weight of each tile into s.tile.
+template <typename R, typename F>
+__device__ void weigh_tiles(Shared& s, const R& row, const F& weight) {
+  s.tile[threadIdx.x] = 0;
   __syncthreads();
-  atomicMax(&s.key, top);
-  if (bad) s.flag = 1;
+  u64 sum = 0;
+  row.sweep([&](float x, int at) { sum += weight(x, at); },
+            [&](int t) {
+              const u64 all = lane_sums(sum);
+              if ((threadIdx.x & 63) == 63) s.tile[t] = all;
+              sum = 0;
+            });
   __syncthreads();
-  if (top == s.key) atomicMin(&s.index, at);
+}
+
+// top-k by sorting what is at least the k-th of the threads' maxima; -2: too many.
+template <typename R>
+__device__ int by_sorting(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, uint32_t mine) {
+  const int tid = threadIdx.x;
+  const uint32_t order = sorted(s, mine, kThreads);
+  const uint32_t least = max((uint32_t)from_one(s, tid + 1 == par.k, order), kLowest + 1);
+  if (tid == 0) s.listed = 0;
   __syncthreads();
-  const Weights w = {of_key(s.key), kLog2e / (double)t, unit_shift(V), s.table};
-  const int first = (int)s.index;
-  const bool none = s.flag || w.top == -INFINITY;
-  if (none) {
-    if (tid == 0) {
-      a.tokens[row_at] = -1;
-      if (a.logprobs) a.logprobs[row_at] = kNaN;
-    }
-    return;
+  row.sweep([&](float x, int at) {
+    const uint32_t key = key_of(x);
+    if (key < least) return;
+    const uint32_t i = atomicAdd(&s.listed, 1u);
+    if (i < (uint32_t)kThreads) s.key[i] = key, s.at[i] = at;
+  });
+  __syncthreads();
+  const int n = (int)s.listed;
+  __syncthreads();                      // (by_steps clears it)
+  if (n > kThreads) return -2;
+  const int size = power_from(n);
+  const u64 e = sorted(s, tid < n ? (u64)s.key[tid] << 32 | (uint32_t)~s.at[tid] : 0, size);
+  const float x = of_key((uint32_t)(e >> 32));
+  const bool there = tid < min(n, par.k);
+  u64 weight = there ? w(x) : 0, before, all;
+  sums(s, weight, before, all);
+  const bool kept = there && (tid == 0 || (double)before < (par.by_p ? par.asked(all) : 1e300)) &&
+                    w.from(x, par.least);
+  // by place: ~place, descending
+  const u64 f = sorted(s, kept ? (u64)(uint32_t)e << 32 | (uint32_t)(e >> 32) : 0, size);
+  weight = f ? w(of_key((uint32_t)f)) : 0;
+  sums(s, weight, before, all);
+  const u64 target = target_of(uniform, all);
+  const bool hit = before <= target && before + weight > target;
+  return (int)from_one(s, hit, (u64)(~(uint32_t)(f >> 32)) + 1) - 1;
+}
+
+// No cut.
+template <bool BF16, typename R>
+__device__ int by_weight(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
+  const auto weight = [&](float x, int) { return w.from(x, par.least); };
+  weigh_tiles(s, row, weight);
+  return locate<BF16>(s, row, uniform, weight);
+}
+
+// top-k and top-p by steps of the distance to the largest logit; -2: too many in a step.
+template <bool BF16, typename R>
+__device__ int by_steps(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, float lowest) {
+  const int tid = threadIdx.x;
+  if (!par.by_k && !par.by_p) return by_weight<BF16>(s, row, par, w, uniform);
+  // 2046 steps over the finite logits, or over 48 t where that is less: what is further has 2^-69 of the weight
+  const float range = fminf(w.top - lowest, 48.0f * par.t), scale = 2046.0f / range;
+  if (!(range > 0.0f) || !(scale < 3e38f)) return -2;
+  const auto step = [&](float x) { return x == w.top ? 0 : (int)fminf((w.top - x) * scale, 2047.0f); };
+  for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  row.sweep([&](float x, int) {
+    if (!(x > -INFINITY)) return;
+    const int i = step(x);
+    if (par.by_k) atomicAdd(&s.count[i], 1u);
+    if (par.by_p) atomicAdd(&s.mass[i], w(x));
+  });
+  __syncthreads();
+  u64 m[2], c[2], before, all, elements;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) m[j] = s.mass[2 * tid + j], c[j] = s.count[2 * tid + j];
+  sums(s, c[0] + c[1], before, elements);
+  const u64 count_before = before;
+  sums(s, m[0] + m[1], before, all);
+  const bool by_k = par.by_k && elements > (u64)par.k;
+  if (!by_k && !par.by_p) return by_weight<BF16>(s, row, par, w, uniform);
+  // The steps to list: that of the cut by top-k; that by top-p; with both all from the first in which the cut by
+  // top-p can be (if nothing of top-k's step counts) to top-k's.
+  uint32_t begin = 0, end = 0;
+  u64 count_above = 0, mass_above = 0, total = all;
+  if (by_k) {
+    begin = end = find_bin(s, c, 0, (u64)par.k, count_above);
+    mass_above = from_one(s, end >> 1 == (uint32_t)tid, before + (end & 1 ? m[0] : 0));
   }
-  int token = first;
-  if (!par.greedy()) {
-    uint32_t cut = 0;                   // kept: keys above it, and the first `ties` at it
-    u64 ties = 0, above_count = 0, above_mass = 0;
-    const bool by_k = par.by_k, by_p = par.by_p;
-    const RowSource<BF16> source = {row, w};
-    u64 total = 0;
-    if (by_k) {
-      find_cut<false>(s, V, source, (u64)par.k, cut, above_count, above_mass);
-      ties = (u64)par.k - above_count;
-      total = above_mass + ties * w(of_key(cut));
-    }
-    if (by_p) {
-      if (!by_k) {
-        u64 mine = 0, before;
-        uint32_t c;
-        for (int i = tid; i < V; i += kThreads) mine += w(logit<BF16>(row, i));
-        scan(s, mine, 0, before, c, total);
-      }
-      const double want = ceil((double)par.p * (double)total);
-      if (want >= 1.0) {
-        const u64 target = min((u64)want, total);
-        above_count = above_mass = cut = 0;
-        find_cut<true>(s, V, source, target, cut, above_count, above_mass);
-        const u64 each = w(of_key(cut));
-        ties = (target - above_mass + each - 1) / each;
-      } else {
-        cut = key_of(w.top), ties = 1;
-      }
-    }
-    // kept weight and ties of each tile, in index order
-    const int tile = max(kTile, (ceil_div(V, kMaxTiles) + kThreads - 1) / kThreads * kThreads);
-    const auto weight = [&](float x, uint32_t& tie) -> u64 {
-      const uint32_t key = key_of(x);
-      tie = key == cut && (by_k || by_p);
-      return key < cut ? 0 : w.at_least(x, mp);
-    };
-    for (int i = tid; i < kMaxTiles; i += kThreads) s.tile_mass[i] = 0, s.tile_ties[i] = 0;
-    __syncthreads();
-    for (int t0 = 0, n = 0; t0 < V; t0 += tile, ++n) {
-      u64 m = 0;
-      uint32_t c = 0;
-      for (int i = t0 + tid; i < min(V, t0 + tile); i += kThreads) {
-        uint32_t tie;
-        const u64 x = weight(logit<BF16>(row, i), tie);
-        c += tie;
-        if (!tie) m += x;
-      }
-      for (int d = 32; d; d >>= 1) m += __shfl_xor(m, d), c += __shfl_xor(c, d);
-      if ((tid & 63) == 0) atomicAdd(&s.tile_mass[n], m), atomicAdd(&s.tile_ties[n], c);
-    }
-    __syncthreads();
-    const int tiles = ceil_div(V, tile);
-    uint32_t unused;
-    const u64 each = by_k || by_p ? weight(of_key(cut), unused) : 0;
-    u64 Z = 0, left = ties;
-    for (int n = 0; n < tiles; ++n) {
-      const u64 here = min((u64)s.tile_ties[n], left);
-      Z += s.tile_mass[n] + here * each, left -= here;
-    }
-    const u64 target = target_of(a.uniform[row_at], Z);
-    u64 sum = 0;
-    left = ties;
-    int n = 0;
-    for (; n < tiles; ++n) {
-      const u64 here = min((u64)s.tile_ties[n], left), next = sum + s.tile_mass[n] + here * each;
-      if (next > target) break;
-      sum = next, left -= here;
-    }
-    // the token inside that tile, a round of kThreads elements at a time
-    for (int t0 = n * tile; t0 < min(V, (n + 1) * tile) && s.found < 0; t0 += kThreads) {
-      const int i = t0 + tid;
-      uint32_t tie = 0, ties_before, c;
-      u64 x = 0, before, all;
-      if (i < min(V, (n + 1) * tile)) x = weight(logit<BF16>(row, i), tie);
-      scan(s, 0, tie, before, ties_before, all);
-      if (tie && ties_before >= left) x = 0;
-      scan(s, x, tie, before, c, all);
-      if (x && sum + before <= target && sum + before + x > target) s.found = i;
-      if (tid == kThreads - 1) s.index = c + tie;
-      __syncthreads();
-      sum += all, left -= min((u64)s.index, left);
-      __syncthreads();
-    }
-    __syncthreads();
-    token = s.found;
+  if (par.by_p) {
+    const double asked = par.asked(by_k ? mass_above : all);
+    begin = find_bin(s, m, 0, (u64)fmax(asked, 1.0), mass_above);
+    if (!by_k) end = begin;
+    else count_above = from_one(s, begin >> 1 == (uint32_t)tid, count_before + (begin & 1 ? c[0] : 0));
   }
-  if (a.logprobs) {
-    const Weights one = {w.top, kLog2e, w.shift, s.table};
-    u64 mine = 0, before, total;
-    uint32_t c;
-    for (int i = tid; i < V; i += kThreads) mine += one(logit<BF16>(row, i));
-    scan(s, mine, 0, before, c, total);
-    if (tid == 0) {
-      const float x = logit<BF16>(row, token);
-      a.logprobs[row_at] =
-          (float)((x == w.top ? 0.0 : (double)x - (double)w.top) - log(ldexp((double)total, -w.shift)));
+  if (end >= 2047) return -2;           // (the last step is all that is further)
+  // the list, and the weight above it
+  weigh_tiles(s, row, [&](float x, int at) -> u64 {
+    if (!(x > -INFINITY)) return 0;
+    const uint32_t i = (uint32_t)step(x);
+    if (i > end) return 0;
+    if (i >= begin) {
+      const uint32_t to = atomicAdd(&s.listed, 1u);
+      if (to < (uint32_t)kList) s.key[to] = key_of(x), s.at[to] = at;
+      return 0;
+    }
+    return w.from(x, par.least);
+  });
+  const int n = (int)s.listed;
+  if (n > kList) return -2;
+  // the cuts
+  const OfList list = {s, n, w};
+  Cut cut = {0, 0x7FFFFFFF};
+  u64 ties = 0;
+  if (by_k) {
+    u64 count = count_above, mass = mass_above;
+    cut.key = find_cut<false>(s, list, (u64)par.k, count, mass);
+    ties = (u64)par.k - count;
+    total = mass + ties * w(of_key(cut.key));
+  }
+  if (par.by_p) {
+    u64 count = count_above, mass = mass_above;
+    const u64 target = max((u64)fmax(par.asked(total), 1.0), mass_above + 1);
+    if (target <= total) {
+      cut.key = find_cut<true>(s, list, target, count, mass);
+      const u64 each = max(w(of_key(cut.key)), 1ull);
+      ties = (target - mass + each - 1) / each;
     }
   }
-  if (tid == 0) a.tokens[row_at] = token;
+  cut.last = last_tie(s, ties, [&](auto f) {
+    for (int i = tid; i < n; i += kThreads)
+      if (s.key[i] == cut.key) f((uint32_t)s.at[i]);
+  });
+  for (int i = tid; i < n; i += kThreads) {
+    const float x = of_key(s.key[i]);
+    if (cut.keeps(s.key[i], s.at[i])) atomicAdd(&s.tile[(s.at[i] + row.lead) / row.tile], w.from(x, par.least));
+  }
+  __syncthreads();
+  return locate<BF16>(s, row, uniform, [&](float x, int at) -> u64 {
+    return cut.keeps(key_of(x), at) ? w.from(x, par.least) : 0;
+  });
+}
+
+// The cuts digit by digit over the row.
+template <bool BF16, typename R>
+__device__ int by_digits(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
+  Cut cut = {0, 0x7FFFFFFF};
+  u64 ties = 0, count, mass, total = 0;
+  bool some = false;
+  const OfRow<R> from = {row, w};
+  if (par.by_k) {
+    count = mass = 0;
+    cut.key = find_cut<false>(s, from, (u64)par.k, count, mass);
+    ties = (u64)par.k - count, some = true;
+    total = mass + ties * w(of_key(cut.key));
+  }
+  if (par.by_p) {
+    if (!par.by_k) {
+      u64 mine = 0, before;
+      row.sweep([&](float x, int) { mine += w(x); });
+      sums(s, mine, before, total);
+    }
+    const u64 target = (u64)fmax(par.asked(total), 1.0);
+    if (target <= total) {
+      count = mass = 0;
+      cut.key = find_cut<true>(s, from, target, count, mass);
+      const u64 each = max(w(of_key(cut.key)), 1ull);
+      ties = (target - mass + each - 1) / each, some = true;
+    }
+  }
+  if (some)
+    cut.last = last_tie(s, ties, [&](auto f) {
+      row.sweep([&](float x, int at) {
+        if (key_of(x) == cut.key) f((uint32_t)at);
+      });
+    });
+  const auto weight = [&](float x, int at) -> u64 {
+    return cut.keeps(key_of(x), at) ? w.from(x, par.least) : 0;
+  };
+  weigh_tiles(s, row, weight);
+  return locate<BF16>(s, row, uniform, weight);
 }
 
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   __shared__ Shared s;
-  whole_row<BF16>(a, blockIdx.x, s);
-}
-
-// ---- a row shared by workgroups -----------------------------------------------------------------
-// What a workgroup found in its part of a row.
-struct Part {
-  u64 kept;                             // weight above the listed bins (weigh: of all, against `top`)
-  u64 near;                             // weight of the bin of `top`, against it
-  double sum;                           // for log probabilities: of exp(x - top)
-  uint32_t top;                         // key of the largest
-  int at;                               // and its first place
-  int bad, pad;                         // NaN among them
-};
-struct Entry {
-  u64 weight;
-  uint32_t key;
-  int at;
-};
-// A row's part of the workspace, followed by its parts and its list.
-struct RowSpace {
-  u64 mass[kBins];
-  uint32_t count[kBins];
-  u64 below, above_count;               // weight of the bins below those listed, elements above them
-  uint32_t listed, low, high;           // entries of the list; keys of its bins, low <= key < high
-  uint32_t by_k;                        // there are top_k elements
-};
-struct Layout {
-  int per, parts, most;                 // elements of a part, parts, entries of the list
-  size_t list, row;                     // offsets in a row's space, and its size
-};
-__host__ __device__ inline Layout layout_of(int rows, int V, bool filters) {
-  Layout l;
-  l.per = (long)rows * ((V + 8191) / 8192) >= 2 * kCUs || V > 2048 * kMaxTiles ? 8192 : 2048;
-  l.parts = (V + l.per - 1) / l.per;
-  l.most = filters ? min(V, max(16384, V / 8)) : 0;
-  l.list = (filters ? sizeof(RowSpace) : 0) + l.parts * sizeof(Part);
-  l.row = l.list + (size_t)l.most * sizeof(Entry);
-  return l;
-}
-
-struct Shape {
-  Layout l;
-  bool filters;
-  __device__ char* row(const SampleArgs& a, int r) const { return (char*)a.workspace + r * l.row; }
-  __device__ RowSpace& space(const SampleArgs& a, int r) const { return *(RowSpace*)row(a, r); }
-  __device__ Part* parts(const SampleArgs& a, int r) const { return (Part*)(row(a, r) + (filters ? sizeof(RowSpace) : 0)); }
-  __device__ Entry* list(const SampleArgs& a, int r) const { return (Entry*)(row(a, r) + l.list); }
-};
-
-__global__ __launch_bounds__(kWide) void clear_rows(SampleArgs a, Shape sh) {
-  u64* p = (u64*)sh.row(a, blockIdx.x);
-  for (unsigned i = threadIdx.x; i < sizeof(RowSpace) / 8; i += kWide) p[i] = 0;
-}
-
-// The elements that a thread has of its workgroup's part, N of them, -infinity past the end. VEC: 16 bytes
-// at a time from aligned rows.
-template <bool BF16, bool VEC, int N>
-struct Mine {
-  float x[N];
-  int base, step;                       // places of the first, and from one run to the next
-  static constexpr int kRun = VEC ? (BF16 ? 8 : 4) : 1;
-  __device__ void load(const void* row, int from, int V) {
-    base = from + (int)threadIdx.x * kRun;
-    step = kWide * kRun;
-#pragma unroll
-    for (int i = 0; i < N; i += kRun) {
-      const int at = place(i);
-      if constexpr (VEC) {
-        if (at + kRun <= V) {
-          const uint4 u = BF16 ? *(const uint4*)((const uint16_t*)row + at) : *(const uint4*)((const float*)row + at);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (BF16) x[i + 2 * j] = bf16_lo(w[j]), x[i + 2 * j + 1] = bf16_hi(w[j]);
-            else x[i + j] = __uint_as_float(w[j]);
-          }
-          continue;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) x[i + j] = at + j < V ? logit<BF16>(row, at + j) : -INFINITY;
-    }
-  }
-  __device__ int place(int i) const { return base + i / kRun * step + i % kRun; }
-};
-
-struct WideShared {
-  u64 bins[kBins];
-  u64 wave_mass[4];
-  uint32_t wave_count[4];
-  double table[64], wave_sum[4];
-  uint32_t top, at;
-  int bad;
-};
-
-// The part's largest logit and first place, and whether it holds NaN; returns the key.
-template <typename M, int N>
-__device__ uint32_t largest(WideShared& s, const M& m, Part& part) {
-  if (threadIdx.x == 0) s.top = 0, s.at = 0xFFFFFFFFu, s.bad = 0;
-  uint32_t top = 0, at = 0;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    bad |= m.x[i] != m.x[i];
-    const uint32_t k = m.x[i] != m.x[i] ? 0 : key_of(m.x[i]);
-    if (k > top) top = k, at = (uint32_t)m.place(i);
-  }
-  uint32_t most = top;
-  for (int d = 32; d; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) atomicMax(&s.top, most);
-  if (__any(bad) && (threadIdx.x & 63) == 0) s.bad = 1;
-  __syncthreads();
-  if (top == s.top) atomicMin(&s.at, at);
-  __syncthreads();
-  part.top = s.top, part.at = (int)s.at, part.bad = s.bad;
-  return s.top;
-}
-
-// Sum over the workgroup in a fixed order.
-__device__ __forceinline__ double sum_all(WideShared& s, double x) {
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.wave_sum[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return (s.wave_sum[0] + s.wave_sum[1]) + (s.wave_sum[2] + s.wave_sum[3]);
-}
-
-// Sum of exp(x - top). A logarithm of it is asked for in fp32: exponentials in fp32 are off by less than 2^-22 of
-// each that counts, a thread's sum of at most 32 by as much again, and so is the logarithm, in all below 2^-21.
-template <typename M, int N>
-__device__ double exp_sum(WideShared& s, const M& m, float top) {
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    sum += m.x[i] == top ? 1.0f : __builtin_amdgcn_exp2f((m.x[i] - top) * 1.44269504f);
-  return sum_all(s, (double)sum);
-}
-
-constexpr int kPartUnit = 49;           // a part's weights against its own largest: 2^-49, at most 8192 of them
-
-// Without filters: a part's weight against its largest logit.
-template <bool BF16, bool VEC, int N>
-__global__ __launch_bounds__(kWide) void weigh(SampleArgs a, Shape sh) {
-  __shared__ WideShared s;
-  const int row_at = (int)blockIdx.x / sh.l.parts, n = (int)blockIdx.x % sh.l.parts;
-  Mine<BF16, VEC, N> m;
-  m.load(row_of(a, row_at), n * sh.l.per, a.V);
-  fill_table(s.table);
-  const Params par(a, row_at);
-  Part part = {};
-  const float top = of_key(largest<decltype(m), N>(s, m, part));
-  u64 sum = 0;
-  if (!par.greedy() && top > -INFINITY) {
-    const Weights w = {top, kLog2e / (double)par.t, kPartUnit, s.table};
-#pragma unroll
-    for (int i = 0; i < N; ++i) sum += w(m.x[i]);
-    u64 before;
-    uint32_t c;
-    scan<kWide>(s.wave_mass, s.wave_count, sum, 0, before, c, part.kept);
-  }
-  if (a.logprobs && top > -INFINITY) part.sum = exp_sum<decltype(m), N>(s, m, top);
-  if (threadIdx.x == 0) sh.parts(a, row_at)[n] = part;
-}
-
-// The row's largest logit and its first place from the parts; false where the row gives no token.
-__device__ bool largest_of_parts(Shared& s, const Part* parts, int n, float t, uint32_t& top, int& first) {
-  if (threadIdx.x == 0) s.key = 0, s.index = 0xFFFFFFFFu, s.flag = t != t;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    if (parts[i].bad) s.flag = 1;
-    atomicMax(&s.key, parts[i].top);
-  }
-  __syncthreads();
-  top = s.key;
-  for (int i = threadIdx.x; i < n; i += kThreads)
-    if (parts[i].top == top) atomicMin(&s.index, (uint32_t)parts[i].at);
-  __syncthreads();
-  first = (int)s.index;
-  return !s.flag && of_key(top) > -INFINITY;
-}
-
-__device__ void write_none(const SampleArgs& a, int row) {
-  if (threadIdx.x == 0) {
-    a.tokens[row] = -1;
-    if (a.logprobs) a.logprobs[row] = kNaN;
-  }
-}
-template <bool BF16>
-__device__ void write_token(const SampleArgs& a, int row_at, int token, float top, const Part* parts, int n,
-                            Shared& s) {
-  if (a.logprobs) {                     // (a sum in a fixed order)
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const float part = of_key(parts[i].top);
-      if (part > -INFINITY)
-        sum += parts[i].sum * (part == top ? 1.0 : exp2_64(((double)part - (double)top) * kLog2e, s.table));
-    }
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.wave_mass[threadIdx.x >> 6] = (u64)__double_as_longlong(sum);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      sum = 0.0;
-      for (int i = 0; i < kThreads / 64; ++i) sum += __longlong_as_double((long long)s.wave_mass[i]);
-      const float x = logit<BF16>(row_of(a, row_at), token);
-      a.logprobs[row_at] = (float)((x == top ? 0.0 : (double)x - (double)top) - log(sum));
-    }
-  }
-  if (threadIdx.x == 0) a.tokens[row_at] = token;
-}
-
-// The first place in [from, to) at which the cumulated weight exceeds target, in order of places: runs of
-// consecutive elements a thread.
-template <bool BF16, typename F>
-__device__ int pass_at(Shared& s, const void* row, int from, int to, u64 target, const F& weight) {
-  if (threadIdx.x == 0) s.found = -1;
-  const int run = ceil_div(to - from, kThreads), i0 = from + (int)threadIdx.x * run, i1 = min(i0 + run, to);
-  u64 mine = 0, before, all;
-  uint32_t c;
-  for (int i = i0; i < i1; ++i) mine += weight(logit<BF16>(row, i), i);
-  scan(s, mine, 0, before, c, all);
-  // (a target past the sum, by rounding, takes the last element of any weight)
-  target = min(target, all - 1);
-  if (before <= target && before + mine > target) {
-    u64 sum = before;
-    for (int i = i0; i < i1; ++i) {
-      sum += weight(logit<BF16>(row, i), i);
-      if (sum > target) {
-        s.found = i;
-        break;
-      }
-    }
-  }
-  __syncthreads();
-  return s.found;
-}
-
-// The part in which the cumulated sum of weight_of(part) passes uniform times all of it: the part, and what is
-// left of the target in it. Sums of the parts lie in s.tile_mass.
-__device__ int part_of(Shared& s, int parts, float uniform, u64& target) {
-  // runs of consecutive parts a thread
-  if (threadIdx.x == 0) s.found = parts - 1, s.above_mass = 0;
-  const int run = ceil_div(parts, kThreads), i0 = (int)threadIdx.x * run, i1 = min(i0 + run, parts);
-  u64 mine = 0, before, Z;
-  uint32_t c;
-  for (int i = i0; i < i1; ++i) mine += s.tile_mass[i];
-  scan(s, mine, 0, before, c, Z);
-  const u64 all = target_of(uniform, Z);
-  if (before <= all && before + mine > all) {
-    u64 sum = before;
-    for (int i = i0; i < i1; ++i) {
-      if (sum + s.tile_mass[i] > all) {
-        s.found = i, s.above_mass = all - sum;
-        break;
-      }
-      sum += s.tile_mass[i];
-    }
-  }
-  __syncthreads();
-  target = s.above_mass;
-  return s.found;
-}
-
-// Without filters: the token from the parts' weights.
-template <bool BF16>
-__global__ __launch_bounds__(kThreads) void pick(SampleArgs a, Shape sh) {
-  __shared__ Shared s;
-  const int row_at = blockIdx.x, n = sh.l.parts;
-  const Part* parts = sh.parts(a, row_at);
-  const Params par(a, row_at);
-  fill_table(s.table);
-  uint32_t top_key;
-  int token;
-  if (!largest_of_parts(s, parts, n, par.t, top_key, token)) return write_none(a, row_at);
-  const float top = of_key(top_key);
-  if (!par.greedy()) {
-    const double rate = kLog2e / (double)par.t, unit = ldexp(1.0, unit_shift(a.V) - kPartUnit);
-    const auto factor = [&](int i) {
-      const float x = of_key(parts[i].top);
-      return x == -INFINITY ? 0.0 : x == top ? 1.0 : exp2_64(((double)x - (double)top) * rate, s.table);
-    };
-    for (int i = threadIdx.x; i < n; i += kThreads) s.tile_mass[i] = (u64)((double)parts[i].kept * factor(i) * unit + 0.5);
-    __syncthreads();
-    u64 target;
-    const int at = part_of(s, n, a.uniform[row_at], target);
-    const Weights w = {of_key(parts[at].top), rate, kPartUnit, s.table};
-    // what is left of the target, in the part's own units
-    const u64 inside = (u64)((double)target / (double)s.tile_mass[at] * (double)parts[at].kept);
-    token = pass_at<BF16>(s, row_of(a, row_at), at * sh.l.per, min((at + 1) * sh.l.per, a.V), inside,
-                          [&](float x, int) { return w(x); });
-  }
-  write_token<BF16>(a, row_at, token, top, parts, n, s);
-}
-
-// The largest value of a bin of keys (of finite ones).
-__device__ __forceinline__ float bin_value(uint32_t bin) { return of_key(bin << kBinShift | ((1u << kBinShift) - 1)); }
-
-template <bool BF16, bool VEC, int N>
-__global__ __launch_bounds__(kWide) void survey(SampleArgs a, Shape sh) {
-  __shared__ WideShared s;
-  const int row_at = (int)blockIdx.x / sh.l.parts, n = (int)blockIdx.x % sh.l.parts, tid = threadIdx.x;
-  Mine<BF16, VEC, N> m;
-  m.load(row_of(a, row_at), n * sh.l.per, a.V);
-  fill_table(s.table);
-  const Params par(a, row_at);
-  const bool bins = !par.greedy() && (par.by_k || par.by_p);
-  if (bins)
-    for (int i = tid; i < kBins; i += kWide) s.bins[i] = 0;
-  Part part = {};
-  const float top = of_key(largest<decltype(m), N>(s, m, part));
-  if (bins) {
-    // The bin of the part's largest logit, which may be the row's, counts against that logit: against the
-    // bin's largest possible value it could be all but nothing. No other bin's value is above the row's largest.
-    const double rate = kLog2e / (double)par.t;
-    const uint32_t top_bin = part.top >> kBinShift;
-    const Weights w = {top, rate, kPartUnit, s.table};
-    u64 near = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (!(m.x[i] > -INFINITY)) continue;
-      const uint32_t bin = key_of(m.x[i]) >> kBinShift;
-      u64 x = 0;
-      if (par.by_p) {
-        if (bin == top_bin) near += w(m.x[i]);
-        else x = to_units(exp2_64(((double)m.x[i] - (double)bin_value(bin)) * rate, s.table, kRelative));
-      }
-      atomicAdd(&s.bins[bin], x << kCountBits | 1);
-    }
-    u64 before;
-    uint32_t c;
-    scan<kWide>(s.wave_mass, s.wave_count, near, 0, before, c, part.near);
-    __syncthreads();
-    RowSpace& row = sh.space(a, row_at);
-    for (int i = tid; i < kBins; i += kWide) {
-      const u64 x = s.bins[i];
-      if (!x) continue;
-      atomicAdd(&row.count[i], (uint32_t)(x & ((1u << kCountBits) - 1)));
-      if (x >> kCountBits) atomicAdd(&row.mass[i], x >> kCountBits);
-    }
-  }
-  if (a.logprobs && top > -INFINITY) part.sum = exp_sum<decltype(m), N>(s, m, top);
-  if (tid == 0) sh.parts(a, row_at)[n] = part;
-}
-
-struct CollectShared : WideShared {
-  uint32_t low, high;                   // keys of the listed bins: low <= key < high
-  uint32_t elements, begin;
-  u64 below, above_count, above_mass;
-};
-
-template <bool BF16, bool VEC, int N>
-__global__ __launch_bounds__(kWide) void collect(SampleArgs a, Shape sh) {
-  __shared__ CollectShared s;
-  const int row_at = (int)blockIdx.x / sh.l.parts, n = (int)blockIdx.x % sh.l.parts, tid = threadIdx.x;
-  const Params par(a, row_at);
-  if (par.greedy()) return;
-  Mine<BF16, VEC, N> m;
-  m.load(row_of(a, row_at), n * sh.l.per, a.V);
-  Part* parts = sh.parts(a, row_at);
-  RowSpace& row = sh.space(a, row_at);
-  fill_table(s.table);
-  if (tid == 0) s.top = 0, s.bad = 0, s.low = s.high = 0, s.below = s.above_count = s.above_mass = 0;
-  for (int i = tid; i < kBins; i += kWide) s.bins[i] = 0;
-  __syncthreads();
-  for (int i = tid; i < sh.l.parts; i += kWide) {
-    atomicMax(&s.top, parts[i].top);
-    if (parts[i].bad) s.bad = 1;
-  }
-  __syncthreads();
-  const float top = of_key(s.top);
-  if (s.bad || top == -INFINITY) return;
-  const double rate = kLog2e / (double)par.t;
-  const int shift = unit_shift(a.V);
-  const Weights w = {top, rate, shift, s.table};
-  bool by_k = false;
-  if (par.by_k || par.by_p) {
-    if (par.by_p) {
-      for (int i = tid; i < sh.l.parts; i += kWide)
-        if (parts[i].near)
-          atomicAdd(&s.bins[parts[i].top >> kBinShift],
-                    (u64)((double)parts[i].near * w.real(of_key(parts[i].top)) * ldexp(1.0, shift - kPartUnit) + 0.5));
-      __syncthreads();
-    }
-    // bins from the highest, 8 a thread
-    constexpr int kEach = kBins / kWide;
-    u64 mass[kEach], mine = 0, before_m, all_m;
-    uint32_t count[kEach], have = 0, before_c;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const uint32_t bin = kBins - 1 - kEach * tid - j;
-      count[j] = row.count[bin], mass[j] = 0;
-      if (par.by_p && count[j]) {
-        mass[j] = s.bins[bin];
-        const u64 x = row.mass[bin];    // (none in the bin of the row's largest)
-        if (x) mass[j] += (u64)((double)x * w.real(bin_value(bin)) * ldexp(1.0, shift - kRelative) + 0.5);
-      }
-      have += count[j], mine += mass[j];
-    }
-    scan<kWide>(s.wave_mass, s.wave_count, mine, have, before_m, before_c, all_m);
-    if (tid == kWide - 1) s.elements = before_c + have;
-    __syncthreads();
-    by_k = par.by_k && s.elements >= (uint32_t)par.k;
-    // The bins to list: that of the cut by top-k; that by top-p; with both all from the highest in which the cut
-    // by top-p can be (if nothing of top-k's bin counts) to top-k's.
-    if (by_k) {
-      u64 ac = before_c, am = before_m;
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        if (ac < (u64)par.k && ac + count[j] >= (u64)par.k) {
-          const uint32_t bin = kBins - 1 - kEach * tid - j;
-          s.low = bin << kBinShift, s.high = (bin + 1) << kBinShift;
-          s.above_count = ac, s.above_mass = am;
-        }
-        ac += count[j], am += mass[j];
-      }
-      __syncthreads();
-    }
-    if (par.by_p) {
-      // (with top-k a little less: the bins' sums are rounded)
-      const double want = ceil((double)par.p * (by_k ? (double)s.above_mass * (1.0 - 1e-9) : (double)all_m));
-      const u64 target = (u64)fmax(want, 1.0);
-      __syncthreads();
-      u64 ac = before_c, am = before_m;
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        if (am < target && am + mass[j] >= target) {
-          const uint32_t bin = kBins - 1 - kEach * tid - j;
-          s.high = (bin + 1) << kBinShift;
-          if (!by_k) s.low = bin << kBinShift, s.below = all_m - am - mass[j];
-          s.above_count = ac;
-        }
-        ac += count[j], am += mass[j];
-      }
-      __syncthreads();
-    }
-  }
-  const uint32_t low = s.low, high = s.high;
-  // Weight of what is above, and the list. (Below `skip` a weight is certainly below min-p: no exponential.)
-  const float skip = par.mp > 0.0f
-                         ? (float)((double)top + log2((double)par.mp) / rate * 1.0001) - 1e-6f * (1.0f + fabsf(top))
-                         : -INFINITY;
-  u64 sum = 0;
-  uint32_t entries = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = m.x[i];
-    if (!(x > -INFINITY)) continue;
+  const int at = blockIdx.x, tid = threadIdx.x;
+  const Row<BF16> row((const char*)a.logits + (size_t)at * a.row_stride * (BF16 ? 2 : 4), a.V);
+  const Params par(a, at);
+  s.table[tid] = exp2((double)tid / kTable);
+  // the largest and its first place, the lowest above -infinity, and each thread's largest
+  uint32_t top = 0, mine_at = 0xFFFFFFFFu, low = 0xFFFFFFFFu;
+  bool bad = par.t != par.t;
+  row.sweep([&](float x, int i) {
+    bad |= x != x;
     const uint32_t key = key_of(x);
-    if (key < low) continue;
-    if (key < high) {
-      ++entries;
-      continue;
+    if (key > top) top = key, mine_at = (uint32_t)i;
+    if (key > kLowest) low = min(low, key);
+  });
+  const u64 first = all_max(s, (u64)top << 32 | (uint32_t)~mine_at);
+  const u64 far = all_max(s, (u64)(uint32_t)~low | (u64)bad << 32);
+  const float most = of_key((uint32_t)(first >> 32));
+  if (far >> 32 || !(most > -INFINITY)) {
+    if (tid == 0) {
+      a.tokens[at] = -1;
+      if (a.logprobs) a.logprobs[at] = kNaN;
     }
-    if (x < skip) continue;
-    sum += w.at_least(x, par.mp);
-  }
-  u64 before_m, all_m;
-  uint32_t before_c;
-  scan<kWide>(s.wave_mass, s.wave_count, sum, entries, before_m, before_c, all_m);
-  if (tid == kWide - 1) {
-    const uint32_t all = before_c + entries;
-    s.begin = all ? atomicAdd(&row.listed, all) : 0;
-  }
-  __syncthreads();
-  Entry* list = sh.list(a, row_at);
-  uint32_t at = s.begin + before_c;
-  if (entries)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float x = m.x[i];
-      const uint32_t key = key_of(x);
-      if (!(x > -INFINITY) || key < low || key >= high) continue;
-      if (at < (uint32_t)sh.l.most) list[at] = {w(x), key, m.place(i)};
-      ++at;
-    }
-  if (tid == 0) {
-    parts[n].kept = all_m;
-    if (n == 0) row.below = s.below, row.above_count = s.above_count, row.low = low, row.high = high,
-                row.by_k = by_k;
-  }
-}
-
-struct ListSource {
-  const Entry* list;
-  __device__ uint32_t key(int i) const { return list[i].key; }
-  __device__ u64 weight(int i) const { return list[i].weight; }
-};
-
-// The place of the `ties`-th of the entries at `cut`, in order of places: 8 of its 24 bits at a time.
-__device__ int last_tie(Shared& s, const Entry* list, int n, uint32_t cut, u64 ties) {
-  uint32_t at = 0;
-  u64 left = ties;
-  for (int level = 0; level < 3; ++level) {
-    const int shift = 16 - 8 * level;
-    __syncthreads();
-    for (int i = threadIdx.x; i < 256; i += kThreads) s.count[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads)
-      if (list[i].key == cut && (level == 0 || (uint32_t)list[i].at >> (shift + 8) == at >> (shift + 8)))
-        atomicAdd(&s.count[((uint32_t)list[i].at >> shift) & 255], 1u);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      u64 sum = 0;
-      uint32_t d = 0;
-      while (d < 255 && sum + s.count[d] < left) sum += s.count[d++];
-      s.key = d, s.above_count = sum;
-    }
-    __syncthreads();
-    at |= s.key << shift, left -= s.above_count;
-  }
-  return (int)at;
-}
-
-template <bool BF16>
-__global__ __launch_bounds__(kThreads) void choose(SampleArgs a, Shape sh) {
-  __shared__ Shared s;
-  const int row_at = blockIdx.x, n = sh.l.parts;
-  const Part* parts = sh.parts(a, row_at);
-  const RowSpace& row = sh.space(a, row_at);
-  const Params par(a, row_at);
-  fill_table(s.table);
-  uint32_t top_key;
-  int token;
-  if (!largest_of_parts(s, parts, n, par.t, top_key, token)) return write_none(a, row_at);
-  const float top = of_key(top_key);
-  if (!par.greedy()) {
-    const int listed = (int)row.listed;
-    if (listed > sh.l.most) return whole_row<BF16>(a, row_at, s);
-    const Weights w = {top, kLog2e / (double)par.t, unit_shift(a.V), s.table};
-    const Entry* list = sh.list(a, row_at);
-    const ListSource source = {list};
-    if (threadIdx.x == 0) s.key = 0, s.above_count = s.above_mass = 0;
-    u64 above = 0, in_list = 0, before;
-    uint32_t c;
-    {
-      u64 mine = 0;
-      for (int i = threadIdx.x; i < n; i += kThreads) mine += parts[i].kept, s.tile_mass[i] = parts[i].kept;
-      scan(s, mine, 0, before, c, above);
-      mine = 0;
-      for (int i = threadIdx.x; i < listed; i += kThreads) mine += list[i].weight;
-      scan(s, mine, 0, before, c, in_list);
-    }
-    // (Where min-p takes from what is above the list it takes all of the list, and the cuts do not matter.)
-    // (the digit that the listed keys share, where they lie in one bin, is not looked at)
-    const int level = row.high - row.low == 1u << kBinShift;
-    uint32_t cut = 0;
-    u64 ties = 0, total = above + in_list + row.below;
-    bool whole = true;                  // all of the list is kept
-    if (row.by_k) {
-      u64 ac = row.above_count, am = above;
-      cut = level ? row.low : 0;
-      find_cut<false>(s, listed, source, (u64)par.k, cut, ac, am, level);
-      ties = (u64)par.k - ac, whole = false;
-      total = am + ties * w(of_key(cut));
-    }
-    bool none = false;                  // nothing of it is
-    if (par.by_p) {
-      const double want = ceil((double)par.p * (double)total);
-      if (!(want >= 1.0)) {
-        cut = top_key, ties = 1, whole = false;
-      } else if ((u64)want <= above) {
-        none = true;
-      } else if ((u64)want <= above + in_list) {
-        u64 ac = row.above_count, am = above;
-        const u64 target = min((u64)want, total);
-        cut = level ? row.low : 0;
-        find_cut<true>(s, listed, source, target, cut, ac, am, level);
-        const u64 each = max(w(of_key(cut)), 1ull);
-        ties = (target - am + each - 1) / each, whole = false;
-      }
-    }
-    // the first `ties` elements at the cut: the place of the last of them
-    int last = 0x7FFFFFFF;
-    if (!whole && !none) {
-      u64 mine = 0, at_cut;
-      for (int i = threadIdx.x; i < listed; i += kThreads) mine += list[i].key == cut;
-      scan(s, mine, 0, before, c, at_cut);
-      if (ties < at_cut) last = last_tie(s, list, listed, cut, ties);
-    }
-    const auto listed_kept = [&](uint32_t key, int at, u64 weight) -> u64 {
-      if (none || (!whole && (key < cut || (key == cut && at > last)))) return 0;
-      return par.mp > 0.0f && !(w.real(of_key(key)) >= (double)par.mp) ? 0 : weight;
-    };
-    __syncthreads();
-    for (int i = threadIdx.x; i < listed; i += kThreads) {
-      const u64 x = listed_kept(list[i].key, list[i].at, list[i].weight);
-      if (x) atomicAdd(&s.tile_mass[list[i].at / sh.l.per], x);
-    }
-    __syncthreads();
-    u64 target;
-    const int at = part_of(s, n, a.uniform[row_at], target);
-    // the listed bins again, to tell what is above them
-    const uint32_t low = row.low, high = row.high;
-    token = pass_at<BF16>(s, row_of(a, row_at), at * sh.l.per, min((at + 1) * sh.l.per, a.V), target,
-                          [&](float x, int i) -> u64 {
-                            const uint32_t key = key_of(x);
-                            if (x == -INFINITY || key < low) return 0;
-                            if (key < high) return listed_kept(key, i, w(x));
-                            return w.at_least(x, par.mp);
-                          });
-  }
-  write_token<BF16>(a, row_at, token, top, parts, n, s);
-}
-
-}  // namespace
-
-bool sample_filters(const SampleArgs& a) {
-  return a.top_k || a.top_p || a.min_p || (a.top_k_all >= 1 && a.top_k_all < a.V) || a.top_p_all < 1.0f ||
-         a.min_p_all > 0.0f;
-}
-
-namespace {
-
-template <bool BF16, bool VEC, int N>
-void launch_wide(const SampleArgs& a, const Shape& sh, hipStream_t stream) {
-  const unsigned grid = (unsigned)(a.rows * sh.l.parts);
-  if (!sh.filters) {
-    weigh<BF16, VEC, N><<<grid, kWide, 0, stream>>>(a, sh);
-    pick<BF16><<<a.rows, kThreads, 0, stream>>>(a, sh);
     return;
   }
-  clear_rows<<<a.rows, kWide, 0, stream>>>(a, sh);
-  survey<BF16, VEC, N><<<grid, kWide, 0, stream>>>(a, sh);
-  collect<BF16, VEC, N><<<grid, kWide, 0, stream>>>(a, sh);
-  choose<BF16><<<a.rows, kThreads, 0, stream>>>(a, sh);
+  int token = (int)~(uint32_t)first;
+  if (!par.greedy()) {
+    const Weights w(most, (double)par.t, unit_shift(a.V), s.table);
+    const float u = a.uniform[at];
+    int found = -2;
+    if (par.by_k && par.k <= kSorted) found = by_sorting(s, row, par, w, u, top);
+    if (found < 0) found = by_steps<BF16>(s, row, par, w, u, of_key(~(uint32_t)far));
+    if (found < 0) found = by_digits<BF16>(s, row, par, w, u);
+    if (found >= 0) token = found;
+  }
+  if (a.logprobs) {
+    // A logarithm in fp32 of the sum of exp(x - top): exponentials in fp32, a tile's sum of a thread in fp32.
+    double sum = 0.0;
+    float part = 0.0f;
+    row.sweep([&](float x, int) { part += x == most ? 1.0f : __builtin_amdgcn_exp2f((x - most) * 1.44269504f); },
+              [&](int) { sum += (double)part, part = 0.0f; });
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    __syncthreads();
+    if ((tid & 63) == 0) s.wave2[tid >> 6] = (u64)__double_as_longlong(sum);
+    __syncthreads();
+    if (tid == 0) {
+      sum = 0.0;
+      for (int i = 0; i < kWaves; ++i) sum += __longlong_as_double((long long)s.wave2[i]);
+      const float x = logit<BF16>(row.p, token);
+      a.logprobs[at] = (float)((x == most ? 0.0 : (double)x - (double)most) - log(sum));
+    }
+  }
+  if (tid == 0) a.tokens[at] = token;
 }
-template <bool BF16>
-void launch_wide(const SampleArgs& a, const Shape& sh, hipStream_t stream) {
-  const bool vec = ((uintptr_t)a.logits | (size_t)(a.rows > 1 ? a.row_stride * (BF16 ? 2 : 4) : 0)) % 16 == 0;
-  if (sh.l.per == 8192) vec ? launch_wide<BF16, true, 32>(a, sh, stream) : launch_wide<BF16, false, 32>(a, sh, stream);
-  else vec ? launch_wide<BF16, true, 8>(a, sh, stream) : launch_wide<BF16, false, 8>(a, sh, stream);
-}
-
-// Vocabularies up to this take one workgroup a row.
-constexpr int kSmall = 4096;
 
 }  // namespace
 
-long sample_workgroups(int rows, int V) { return V <= kSmall ? rows : (long)rows * layout_of(rows, V, false).parts; }
-
-size_t sample_workspace(int rows, int V, bool filters) {
-  return V <= kSmall ? 0 : rows * layout_of(rows, V, filters).row;
-}
-
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
-  if (a.V <= kSmall) {
-    if (a.bf16) sample_rows<true><<<a.rows, kThreads, 0, stream>>>(a);
-    else sample_rows<false><<<a.rows, kThreads, 0, stream>>>(a);
-  } else {
-    const bool filters = sample_filters(a);
-    const Shape sh = {layout_of(a.rows, a.V, filters), filters};
-    if (a.bf16) launch_wide<true>(a, sh, stream);
-    else launch_wide<false>(a, sh, stream);
-  }
+  if (a.bf16) sample_rows<true><<<a.rows, kThreads, 0, stream>>>(a);
+  else sample_rows<false><<<a.rows, kThreads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
