@@ -47,9 +47,9 @@ struct Weights {
   double rate, offset;                  // 1024 log2(e) / t, and top times it
   int shift;
   const double* table;
-  __device__ Weights(float top, double t, int shift, const double* table)
+  __device__ __forceinline__ Weights(float top, double t, int shift, const double* table)
       : top(top), rate(1024.0 * kLog2e / t), offset((double)top * (1024.0 * kLog2e / t)), shift(shift), table(table) {}
-  // in units, not rounded to whole ones, for x below top
+  // in units, not rounded to whole ones, for x below top; less than half of one for -infinity
   __device__ __forceinline__ double units(float x) const {
     const double y = fmax(fma((double)x, rate, -offset), -1024.0 * 1000.0);
     const double k = y + 6755399441055744.0;
@@ -64,14 +64,14 @@ struct Weights {
     return (u64)__double_as_longlong(units + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
   }
   __device__ __forceinline__ u64 operator()(float x) const {
-    return x == top ? 1ull << shift : x == -INFINITY ? 0 : whole(units(x));
+    const u64 w = whole(units(x));
+    return x == top ? 1ull << shift : w;
   }
   // the weight where it is at least min_p, `least` in units (0: any)
   __device__ __forceinline__ u64 from(float x, double least) const {
-    if (x == top) return 1ull << shift;
-    if (x == -INFINITY) return 0;
     const double u = units(x);
-    return u >= least ? whole(u) : 0;
+    const u64 w = u >= least ? whole(u) : 0;
+    return x == top ? 1ull << shift : w;
   }
 };
 
@@ -88,12 +88,47 @@ struct Shared {
 };
 
 // ---- over lanes and the workgroup ---------------------------------------------------------------
-// (row_shr:1, 2, 4, 8, then the rows' last lanes: row_bcast:15 and 31)
-#define LANE_STEPS STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+// (as instructions: fmaxf comes with one more an operand that makes signalling NaN quiet; rows with NaN have no token)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float max4(const float x[4]) { return max3(max3(x[0], x[1], x[2]), x[3], x[3]); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false);
+}
 template <int CTRL, int ROWS>
 __device__ __forceinline__ u64 moved(u64 x) {
-  return (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false) |
-         (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xF, false) << 32;
+  return (u64)moved<CTRL, ROWS>((uint32_t)x) | (u64)moved<CTRL, ROWS>((uint32_t)(x >> 32)) << 32;
+}
+// (row_shr:1, 2, 4, 8, then the rows' last lanes: row_bcast:15 and 31)
+#define LANE_STEPS STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+// The value of lane ^ J.
+template <int J>
+__device__ __forceinline__ uint32_t across(uint32_t x) {
+  if constexpr (J == 1) return moved<0xB1, 0xF>(x);                        // quad_perm:[1,0,3,2]
+  else if constexpr (J == 2) return moved<0x4E, 0xF>(x);                   // quad_perm:[2,3,0,1]
+  else if constexpr (J == 4) return moved<0x141, 0xF>(moved<0x1B, 0xF>(x));  // each four reversed, then each eight
+  else if constexpr (J == 8) return moved<0x128, 0xF>(x);                  // row_ror:8
+  else if constexpr (J == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);   // even rows' values, odd rows'
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int J>
+__device__ __forceinline__ u64 across(u64 x) {
+  return (u64)across<J>((uint32_t)x) | (u64)across<J>((uint32_t)(x >> 32)) << 32;
 }
 // Inclusive sums over the wave's lanes.
 __device__ __forceinline__ u64 lane_sums(u64 x) {
@@ -111,7 +146,7 @@ __device__ __forceinline__ u64 lane_max(u64 x) {
 }
 
 // The largest of all threads.
-__device__ u64 all_max(Shared& s, u64 x) {
+__device__ __forceinline__ u64 all_max(Shared& s, u64 x) {
   x = lane_max(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = x;
@@ -124,7 +159,7 @@ __device__ u64 all_max(Shared& s, u64 x) {
 }
 
 // Sum of the threads before this one, and of all.
-__device__ void sums(Shared& s, u64 x, u64& before, u64& all) {
+__device__ __forceinline__ void sums(Shared& s, u64 x, u64& before, u64& all) {
   const u64 up_to = lane_sums(x);
   const int wave = threadIdx.x >> 6;
   __syncthreads();
@@ -140,7 +175,7 @@ __device__ void sums(Shared& s, u64 x, u64& before, u64& all) {
 }
 
 // The value that the one thread with `mine` has (0 where none has), for all.
-__device__ u64 from_one(Shared& s, bool mine, u64 x) {
+__device__ __forceinline__ u64 from_one(Shared& s, bool mine, u64 x) {
   if (threadIdx.x == 0) s.value[0] = 0;
   __syncthreads();
   if (mine) s.value[0] = x;
@@ -152,24 +187,30 @@ __device__ u64 from_one(Shared& s, bool mine, u64 x) {
 
 // Values in descending order, one a thread: a sorting network over the first `size` threads (a power of two, 64 at
 // least; the others' values stay among themselves).
-template <typename T>
-__device__ T sorted(Shared& s, T x, int size) {
+template <int J>
+__device__ __forceinline__ u64 sorted_step(u64 x, int k) {
+  const u64 y = across<J>(x);
+  const bool larger = ((threadIdx.x & k) == 0) == ((threadIdx.x & J) == 0);
+  return (x > y) == larger ? x : y;
+}
+__device__ __forceinline__ u64 sorted(Shared& s, u64 x, int size) {
   const int tid = threadIdx.x;
-  T* lds = (T*)s.mass;
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j; j >>= 1) {
-      T y;
-      if (j < 64) {
-        y = __shfl_xor(x, j);
-      } else {
-        __syncthreads();
-        lds[tid] = x;
-        __syncthreads();
-        y = lds[tid ^ j];
-      }
+  for (int k = 2; k <= size; k <<= 1) {
+    for (int j = k >> 1; j >= 64; j >>= 1) {
+      __syncthreads();
+      s.mass[tid] = x;
+      __syncthreads();
+      const u64 y = s.mass[tid ^ j];
       const bool larger = ((tid & k) == 0) == ((tid & j) == 0);
-      x = larger ? max(x, y) : min(x, y);
+      x = (x > y) == larger ? x : y;
     }
+    if (k > 32) x = sorted_step<32>(x, k);
+    if (k > 16) x = sorted_step<16>(x, k);
+    if (k > 8) x = sorted_step<8>(x, k);
+    if (k > 4) x = sorted_step<4>(x, k);
+    if (k > 2) x = sorted_step<2>(x, k);
+    x = sorted_step<1>(x, k);
+  }
   __syncthreads();
   return x;
 }
@@ -185,59 +226,95 @@ __device__ __forceinline__ float logit(const void* row, int i) {
   return BF16 ? bf16_f32(((const uint16_t*)row)[i]) : ((const float*)row)[i];
 }
 
-// A row in tiles of consecutive elements, a wave each in turn, 16 bytes of a thread at a time: counted from the
-// address of 16 bytes that the row begins in, `lead` elements before it.
+// A row in tiles of consecutive elements, a wave each in turn, in groups of 16 bytes a thread four times, loaded
+// while the group before is worked on. Counted from the address of 16 bytes that the row begins in, `lead` elements
+// before it; what is not of the row reads as -infinity. (Code stays small: with 32 elements of a thread unrolled, the
+// passes waited for instructions, up to 1500 cycles an element of a wave.)
 template <bool BF16>
 struct Row {
-  static constexpr int kRun = BF16 ? 8 : 4, kAhead = BF16 ? 4 : 8;
+  static constexpr int kRun = BF16 ? 8 : 4, kGroup = 64 * kRun * 4;
   const void* p;
   int V, lead, tile;                    // elements of a tile: kTiles of them hold the row
-  __device__ Row(const void* p, int V) : p(p), V(V), lead((int)((uintptr_t)p % 16) / (BF16 ? 2 : 4)) {
-    tile = 64 * kRun * kAhead;
+  __device__ __forceinline__ Row(const void* p, int V) : p(p), V(V), lead((int)((uintptr_t)p % 16) / (BF16 ? 2 : 4)) {
+    tile = kGroup;
     while ((long)tile * kTiles < (long)V + lead) tile <<= 1;
   }
-  // f(x, place) for each element of this thread's in turn; end(tile) after each of its wave's tiles.
-  template <typename F, typename G>
-  __device__ void sweep(const F& f, const G& end) const {
-    const int lane = threadIdx.x & 63;
-    for (int t = threadIdx.x >> 6; (long)t * tile < (long)V + lead; t += kWaves) {
-      const int to = (int)min((long)(t + 1) * tile - lead, (long)V);
-      for (int from = t * tile - lead; from < to; from += 64 * kRun * kAhead) {
-        uint4 u[kAhead];
+  __device__ __forceinline__ void load(uint4 (&u)[4], int from) const {
+    const int at = from + (int)(threadIdx.x & 63) * kRun;
+    const bool inside = from >= 0 && from + kGroup <= V;
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          const int i = from + (a * 64 + lane) * kRun;
-          u[a] = {};
-          if (i >= 0 && i + kRun <= to) {
-            u[a] = BF16 ? *(const uint4*)((const uint16_t*)p + i) : *(const uint4*)((const float*)p + i);
-          } else if (i < to) {          // the row's ends
-            uint32_t w[4] = {};
-#pragma unroll
-            for (int j = 0; j < kRun; ++j) {
-              const bool in = i + j >= 0 && i + j < to;
-              if constexpr (BF16) w[j / 2] |= in ? (uint32_t)((const uint16_t*)p)[i + j] << (16 * (j % 2)) : 0u;
-              else w[j] = in ? ((const uint32_t*)p)[i + j] : 0u;
+    for (int a = 0; a < 4; ++a) {
+      const int i = at + a * 64 * kRun;
+      if (inside || (i >= 0 && i + kRun <= V)) {
+        u[a] = BF16 ? *(const uint4*)((const uint16_t*)p + i) : *(const uint4*)((const float*)p + i);
+      } else {
+        constexpr uint32_t kNone = BF16 ? 0xFF80FF80u : 0xFF800000u;
+        u[a] = {kNone, kNone, kNone, kNone};
+        if (i < V && i + kRun > 0) {    // the row's ends: element by element, shifted in from above
+#pragma unroll 1
+          for (int j = i; j < i + kRun; ++j) {
+            const bool in = j >= 0 && j < V;
+            if constexpr (BF16) {
+              const uint32_t x = in ? ((const uint16_t*)p)[j] : 0xFF80u;
+              u[a] = {u[a].x >> 16 | u[a].y << 16, u[a].y >> 16 | u[a].z << 16, u[a].z >> 16 | u[a].w << 16,
+                      u[a].w >> 16 | x << 16};
+            } else {
+              u[a] = {u[a].y, u[a].z, u[a].w, in ? ((const uint32_t*)p)[j] : kNone};
             }
-            u[a] = {w[0], w[1], w[2], w[3]};
-          }
-        }
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          const int i = from + (a * 64 + lane) * kRun;
-          const uint32_t w[4] = {u[a].x, u[a].y, u[a].z, u[a].w};
-#pragma unroll
-          for (int j = 0; j < kRun; ++j) {
-            const float x = !BF16 ? __uint_as_float(w[j % 4]) : j % 2 ? bf16_hi(w[j / 2 % 4]) : bf16_lo(w[j / 2 % 4]);
-            if (i + j >= 0 && i + j < to) f(x, i + j);
           }
         }
       }
-      end(t);
     }
   }
-  template <typename F>
-  __device__ void sweep(const F& f) const {
-    sweep(f, [](int) {});
+  // f(x, place) for four consecutive elements of this thread's in turn; end(tile) after each of its wave's tiles.
+  template <bool LONG, typename F, typename G>
+  __device__ __forceinline__ void sweep(const F& f, const G& end) const {
+    int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = t * tile - lead;
+    if (from >= V) return;
+    uint4 u[4], next[4] = {};
+    load(u, from);
+#pragma unroll 1
+    for (;;) {
+      int then = from + kGroup;
+      const bool last = then >= (t + 1) * tile - lead || then >= V;
+      if (last) then = (t + kWaves) * tile - lead;
+      if (then < V) load(next, then);
+      const int at = from + (int)(threadIdx.x & 63) * kRun;
+      // (one group of four elements in the code where f is long)
+      const auto four = [&](const uint4& v, int i) {
+        if constexpr (BF16) {
+          uint32_t w0 = v.x, w1 = v.y;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const float x[4] = {bf16_lo(w0), bf16_hi(w0), bf16_lo(w1), bf16_hi(w1)};
+            f(x, i + 4 * half);
+            w0 = v.z, w1 = v.w;
+          }
+        } else {
+          const float x[4] = {bits_f32(v.x), bits_f32(v.y), bits_f32(v.z), bits_f32(v.w)};
+          f(x, i);
+        }
+      };
+      if constexpr (LONG) {
+#pragma unroll 1
+        for (int a = 0; a < 4; ++a) {
+          four(u[0], at + a * 64 * kRun);
+          u[0] = u[1], u[1] = u[2], u[2] = u[3];
+        }
+      } else {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) four(u[a], at + a * 64 * kRun);
+      }
+      if (last) end(t), t += kWaves;
+      if (then >= V) return;
+      from = then;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) u[a] = next[a];
+    }
+  }
+  template <bool LONG, typename F>
+  __device__ __forceinline__ void sweep(const F& f) const {
+    sweep<LONG>(f, [](int) {});
   }
 };
 
@@ -247,8 +324,11 @@ struct OfRow {
   const R& row;
   const Weights& w;
   template <typename F>
-  __device__ void each(const F& f) const {
-    row.sweep([&](float x, int) { f(key_of(x), [&] { return w(x); }); });
+  __device__ __forceinline__ void each(const F& f) const {
+    row.template sweep<true>([&](const float (&x)[4], int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(key_of(x[j]), [&] { return w(x[j]); });
+    });
   }
 };
 struct OfList {
@@ -256,7 +336,7 @@ struct OfList {
   int n;
   const Weights& w;
   template <typename F>
-  __device__ void each(const F& f) const {
+  __device__ __forceinline__ void each(const F& f) const {
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const uint32_t key = s.key[i];
       f(key, [&] { return w(of_key(key)); });
@@ -266,7 +346,7 @@ struct OfList {
 
 // The bin, of those that the threads have two each from the highest, in which the sum passes to `target` or more, and
 // what lies above it. (~0: none.)
-__device__ uint32_t find_bin(Shared& s, const u64 m[2], u64 from, u64 target, u64& above) {
+__device__ __forceinline__ uint32_t find_bin(Shared& s, const u64 m[2], u64 from, u64 target, u64& above) {
   u64 before, all;
   sums(s, m[0] + m[1], before, all);
   u64 x = from + before, hit = 0, at = 0;
@@ -283,9 +363,10 @@ __device__ uint32_t find_bin(Shared& s, const u64 m[2], u64 from, u64 target, u6
 // (11, 11 and 10 bits), and the elements and the weight above it. `count` and `mass` come with what lies above all
 // elements of `from`.
 template <bool BY_MASS, typename From>
-__device__ uint32_t find_cut(Shared& s, const From& from, u64 target, u64& count, u64& mass) {
+__device__ __forceinline__ uint32_t find_cut(Shared& s, const From& from, u64 target, u64& count, u64& mass) {
   const int tid = threadIdx.x;
   uint32_t key = 0;
+#pragma unroll 1
   for (int level = 0; level < 3; ++level) {
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
     const uint32_t fixed = level == 0 ? 0u : ~0u << (shift + bits);
@@ -320,7 +401,7 @@ struct Params {
   double least;                         // min-p in units
   int k;
   bool by_k, by_p;
-  __device__ Params(const SampleArgs& a, int row) {
+  __device__ __forceinline__ Params(const SampleArgs& a, int row) {
     t = a.temperature ? a.temperature[row] : a.temperature_all;
     k = a.top_k ? a.top_k[row] : a.top_k_all;
     p = a.top_p ? a.top_p[row] : a.top_p_all;
@@ -349,8 +430,9 @@ struct Cut {
 
 // The place of the `ties`-th of the elements with this key, in order of places: 8 of its 24 bits at a time.
 template <typename Each>
-__device__ int last_tie(Shared& s, u64 ties, const Each& each) {
+__device__ __forceinline__ int last_tie(Shared& s, u64 ties, const Each& each) {
   uint32_t at = 0;
+#pragma unroll 1
   for (int shift = 16; shift >= 0; shift -= 8) {
     for (int i = threadIdx.x; i < 256; i += kThreads) s.count[i] = 0;
     __syncthreads();
@@ -370,7 +452,7 @@ __device__ int last_tie(Shared& s, u64 ties, const Each& each) {
 
 // The token where tiles hold the kept weight of the row's tiles and weight(x, place) that of an element.
 template <bool BF16, typename R, typename F>
-__device__ int locate(Shared& s, const R& row, float uniform, const F& weight) {
+__device__ __forceinline__ int locate(Shared& s, const R& row, float uniform, const F& weight) {
   u64 before, all;
   const u64 mine = s.tile[threadIdx.x];
   sums(s, mine, before, all);
@@ -398,11 +480,14 @@ __device__ int locate(Shared& s, const R& row, float uniform, const F& weight) {
 
 // The weight of each tile into s.tile.
 template <typename R, typename F>
-__device__ void weigh_tiles(Shared& s, const R& row, const F& weight) {
+__device__ __forceinline__ void weigh_tiles(Shared& s, const R& row, const F& weight) {
   s.tile[threadIdx.x] = 0;
   __syncthreads();
   u64 sum = 0;
-  row.sweep([&](float x, int at) { sum += weight(x, at); },
+  row.template sweep<true>([&](const float (&x)[4], int at) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sum += weight(x[j], at + j);
+            },
             [&](int t) {
               const u64 all = lane_sums(sum);
               if ((threadIdx.x & 63) == 63) s.tile[t] = all;
@@ -411,19 +496,32 @@ __device__ void weigh_tiles(Shared& s, const R& row, const F& weight) {
   __syncthreads();
 }
 
-// top-k by sorting what is at least the k-th of the threads' maxima; -2: too many.
+// top-k by sorting what is at least the k-th of the threads' maxima, or a little less; -2: too many.
 template <typename R>
-__device__ int by_sorting(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, uint32_t mine) {
+__device__ __forceinline__ int by_sorting(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, float mine) {
   const int tid = threadIdx.x;
-  const uint32_t order = sorted(s, mine, kThreads);
-  const uint32_t least = max((uint32_t)from_one(s, tid + 1 == par.k, order), kLowest + 1);
+  // the lower end of the step, of 2048 from the largest of the threads' maxima to the least, that the k-th lies in
+  const bool some = mine > -INFINITY;
+  const float lowest = of_key(~(uint32_t)all_max(s, some ? ~key_of(mine) : 0u)), scale = 2047.0f / (w.top - lowest);
+  const int step = mine == w.top ? 0 : (int)fminf((w.top - mine) * scale, 2047.0f);
+  for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
   if (tid == 0) s.listed = 0;
   __syncthreads();
-  row.sweep([&](float x, int at) {
-    const uint32_t key = key_of(x);
-    if (key < least) return;
-    const uint32_t i = atomicAdd(&s.listed, 1u);
-    if (i < (uint32_t)kThreads) s.key[i] = key, s.at[i] = at;
+  if (some) atomicAdd(&s.count[step], 1u);
+  __syncthreads();
+  const u64 c[2] = {s.count[2 * tid], s.count[2 * tid + 1]};
+  u64 above;
+  const uint32_t bin = find_bin(s, c, 0, (u64)par.k, above);
+  const uint32_t key = ~(uint32_t)all_max(s, some && (uint32_t)step <= bin ? ~key_of(mine) : 0u);
+  const float least = of_key(bin == ~0u ? kLowest + 1 : key);
+  row.template sweep<false>([&](const float (&x)[4], int at) {
+    if (!(max4(x) >= least)) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+      if (x[j] >= least) {
+        const uint32_t i = atomicAdd(&s.listed, 1u);
+        if (i < (uint32_t)kThreads) s.key[i] = key_of(x[j]), s.at[i] = at + j;
+      }
   });
   __syncthreads();
   const int n = (int)s.listed;
@@ -448,7 +546,7 @@ __device__ int by_sorting(Shared& s, const R& row, const Params& par, const Weig
 
 // No cut.
 template <bool BF16, typename R>
-__device__ int by_weight(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
+__device__ __forceinline__ int by_weight(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
   const auto weight = [&](float x, int) { return w.from(x, par.least); };
   weigh_tiles(s, row, weight);
   return locate<BF16>(s, row, uniform, weight);
@@ -456,7 +554,7 @@ __device__ int by_weight(Shared& s, const R& row, const Params& par, const Weigh
 
 // top-k and top-p by steps of the distance to the largest logit; -2: too many in a step.
 template <bool BF16, typename R>
-__device__ int by_steps(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, float lowest) {
+__device__ __forceinline__ int by_steps(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, float lowest) {
   const int tid = threadIdx.x;
   if (!par.by_k && !par.by_p) return by_weight<BF16>(s, row, par, w, uniform);
   // 2046 steps over the finite logits, or over 48 t where that is less: what is further has 2^-69 of the weight
@@ -466,11 +564,16 @@ __device__ int by_steps(Shared& s, const R& row, const Params& par, const Weight
   for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
   if (tid == 0) s.listed = 0;
   __syncthreads();
-  row.sweep([&](float x, int) {
-    if (!(x > -INFINITY)) return;
-    const int i = step(x);
-    if (par.by_k) atomicAdd(&s.count[i], 1u);
-    if (par.by_p) atomicAdd(&s.mass[i], w(x));
+  row.template sweep<true>([&](const float (&x)[4], int) {
+    u64 m[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = w(x[j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = step(x[j]);
+      if (par.by_k && x[j] > -INFINITY) atomicAdd(&s.count[i], 1u);
+      if (par.by_p && m[j]) atomicAdd(&s.mass[i], m[j]);
+    }
   });
   __syncthreads();
   u64 m[2], c[2], before, all, elements;
@@ -497,16 +600,14 @@ __device__ int by_steps(Shared& s, const R& row, const Params& par, const Weight
   }
   if (end >= 2047) return -2;           // (the last step is all that is further)
   // the list, and the weight above it
-  weigh_tiles(s, row, [&](float x, int at) -> u64 {
-    if (!(x > -INFINITY)) return 0;
+  weigh_tiles(s, row, [&](float x, int at) {
     const uint32_t i = (uint32_t)step(x);
-    if (i > end) return 0;
-    if (i >= begin) {
+    const u64 m = w.from(x, par.least);
+    if (i >= begin && i <= end) {       // (not -infinity, whose step is the last)
       const uint32_t to = atomicAdd(&s.listed, 1u);
       if (to < (uint32_t)kList) s.key[to] = key_of(x), s.at[to] = at;
-      return 0;
     }
-    return w.from(x, par.least);
+    return i < begin ? m : 0;
   });
   const int n = (int)s.listed;
   if (n > kList) return -2;
@@ -545,7 +646,7 @@ __device__ int by_steps(Shared& s, const R& row, const Params& par, const Weight
 
 // The cuts digit by digit over the row.
 template <bool BF16, typename R>
-__device__ int by_digits(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
+__device__ __forceinline__ int by_digits(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
   Cut cut = {0, 0x7FFFFFFF};
   u64 ties = 0, count, mass, total = 0;
   bool some = false;
@@ -559,7 +660,10 @@ __device__ int by_digits(Shared& s, const R& row, const Params& par, const Weigh
   if (par.by_p) {
     if (!par.by_k) {
       u64 mine = 0, before;
-      row.sweep([&](float x, int) { mine += w(x); });
+      row.template sweep<true>([&](const float (&x)[4], int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mine += w(x[j]);
+      });
       sums(s, mine, before, total);
     }
     const u64 target = (u64)fmax(par.asked(total), 1.0);
@@ -572,8 +676,10 @@ __device__ int by_digits(Shared& s, const R& row, const Params& par, const Weigh
   }
   if (some)
     cut.last = last_tie(s, ties, [&](auto f) {
-      row.sweep([&](float x, int at) {
-        if (key_of(x) == cut.key) f((uint32_t)at);
+      row.template sweep<true>([&](const float (&x)[4], int at) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+          if (key_of(x[j]) == cut.key) f((uint32_t)(at + j));
       });
     });
   const auto weight = [&](float x, int at) -> u64 {
@@ -590,40 +696,50 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   const Row<BF16> row((const char*)a.logits + (size_t)at * a.row_stride * (BF16 ? 2 : 4), a.V);
   const Params par(a, at);
   s.table[tid] = exp2((double)tid / kTable);
-  // the largest and its first place, the lowest above -infinity, and each thread's largest
-  uint32_t top = 0, mine_at = 0xFFFFFFFFu, low = 0xFFFFFFFFu;
+  // the largest, the lowest that is finite, and each thread's largest and the first four elements that it is among
+  float mine = -INFINITY, low = INFINITY;
+  int mine_at = row.V;
   bool bad = par.t != par.t;
-  row.sweep([&](float x, int i) {
-    bad |= x != x;
-    const uint32_t key = key_of(x);
-    if (key > top) top = key, mine_at = (uint32_t)i;
-    if (key > kLowest) low = min(low, key);
+  row.template sweep<false>([&](const float (&x)[4], int i) {
+    bad |= __builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]);
+    // (infinity times 0 is NaN, which a minimum passes by)
+    low = min3(min3(low, fmaf(x[0], 0.0f, x[0]), fmaf(x[1], 0.0f, x[1])), fmaf(x[2], 0.0f, x[2]), fmaf(x[3], 0.0f, x[3]));
+    const float m = max4(x);
+    if (m > mine) mine = m, mine_at = i;
   });
-  const u64 first = all_max(s, (u64)top << 32 | (uint32_t)~mine_at);
-  const u64 far = all_max(s, (u64)(uint32_t)~low | (u64)bad << 32);
-  const float most = of_key((uint32_t)(first >> 32));
-  if (far >> 32 || !(most > -INFINITY)) {
+  const u64 ends = all_max(s, (u64)(bad ? ~0u : key_of(mine)) << 32 | (uint32_t)~key_of(low));
+  const float top = of_key((uint32_t)(ends >> 32));
+  if (!(top > -INFINITY)) {             // (~0 is the key of a NaN)
     if (tid == 0) {
       a.tokens[at] = -1;
       if (a.logprobs) a.logprobs[at] = kNaN;
     }
     return;
   }
-  int token = (int)~(uint32_t)first;
+  int token = -1;
   if (!par.greedy()) {
-    const Weights w(most, (double)par.t, unit_shift(a.V), s.table);
+    const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
     const float u = a.uniform[at];
-    int found = -2;
-    if (par.by_k && par.k <= kSorted) found = by_sorting(s, row, par, w, u, top);
-    if (found < 0) found = by_steps<BF16>(s, row, par, w, u, of_key(~(uint32_t)far));
-    if (found < 0) found = by_digits<BF16>(s, row, par, w, u);
-    if (found >= 0) token = found;
+    if (par.by_k && par.k <= kSorted) token = by_sorting(s, row, par, w, u, mine);
+    if (token < 0) token = by_steps<BF16>(s, row, par, w, u, of_key(~(uint32_t)all_max(s, (uint32_t)~key_of(low))));
+    if (token < 0) token = by_digits<BF16>(s, row, par, w, u);
+  }
+  if (token < 0) {
+    int place = 0x7FFFFFFF;
+    for (int j = 3; j >= 0; --j) {
+      const int i = mine_at + j;
+      if (i >= 0 && i < row.V && logit<BF16>(row.p, i) == top) place = i;
+    }
+    token = (int)~(uint32_t)all_max(s, (uint32_t)~place);
   }
   if (a.logprobs) {
     // A logarithm in fp32 of the sum of exp(x - top): exponentials in fp32, a tile's sum of a thread in fp32.
     double sum = 0.0;
     float part = 0.0f;
-    row.sweep([&](float x, int) { part += x == most ? 1.0f : __builtin_amdgcn_exp2f((x - most) * 1.44269504f); },
+    row.template sweep<true>([&](const float (&x)[4], int) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part += x[j] == top ? 1.0f : __builtin_amdgcn_exp2f((x[j] - top) * 1.44269504f);
+              },
               [&](int) { sum += (double)part, part = 0.0f; });
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     __syncthreads();
@@ -633,7 +749,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
       sum = 0.0;
       for (int i = 0; i < kWaves; ++i) sum += __longlong_as_double((long long)s.wave2[i]);
       const float x = logit<BF16>(row.p, token);
-      a.logprobs[at] = (float)((x == most ? 0.0 : (double)x - (double)most) - log(sum));
+      a.logprobs[at] = (float)((x == top ? 0.0 : (double)x - (double)top) - log(sum));
     }
   }
   if (tid == 0) a.tokens[at] = token;
