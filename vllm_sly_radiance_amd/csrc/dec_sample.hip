@@ -56,8 +56,8 @@ struct Weights {
     const int n = (int)(uint32_t)__double_as_longlong(k);
     const double r = y - (k - 6755399441055744.0);
     const double q = r * fma(fma(r, 5.169222938345892e-11, 2.290978498068816e-07), r, 0.0006769015435155716);
-    const u64 bits = (u64)__double_as_longlong(table[n & (kTable - 1)]) + ((u64)(uint32_t)((n >> 10) + shift) << 52);
-    const double v = __longlong_as_double((long long)bits);
+    const u64 bits = (u64)__double_as_longlong(table[n & (kTable - 1)]);
+    const double v = __longlong_as_double((long long)(bits + ((u64)((uint32_t)(n & -kTable) << 10) << 32)));
     return fma(v, q, v);
   }
   static __device__ __forceinline__ u64 whole(double units) {
@@ -83,7 +83,6 @@ struct Shared {
   int at[kList];
   u64 tile[kTiles];
   u64 wave[kWaves], wave2[kWaves];
-  u64 value[4];
   uint32_t listed;
 };
 
@@ -110,7 +109,8 @@ __device__ __forceinline__ u64 moved(u64 x) {
   return (u64)moved<CTRL, ROWS>((uint32_t)x) | (u64)moved<CTRL, ROWS>((uint32_t)(x >> 32)) << 32;
 }
 // (row_shr:1, 2, 4, 8, then the rows' last lanes: row_bcast:15 and 31)
-#define LANE_STEPS STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF) STEP(0x142, 0xA) STEP(0x143, 0xC)
+#define ROW_STEPS STEP(0x111, 0xF) STEP(0x112, 0xF) STEP(0x114, 0xF) STEP(0x118, 0xF)
+#define LANE_STEPS ROW_STEPS STEP(0x142, 0xA) STEP(0x143, 0xC)
 // The value of lane ^ J.
 template <int J>
 __device__ __forceinline__ uint32_t across(uint32_t x) {
@@ -145,43 +145,57 @@ __device__ __forceinline__ u64 lane_max(u64 x) {
   return x;
 }
 
+static_assert(kWaves == 16, "a row of lanes has a value of each wave");
+__device__ __forceinline__ u64 from_lane(u64 x, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
+         (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32;
+}
+__device__ __forceinline__ int this_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 // The largest of all threads.
 __device__ __forceinline__ u64 all_max(Shared& s, u64 x) {
   x = lane_max(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = x;
   __syncthreads();
-  x = s.wave[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) x = max(x, s.wave[w]);
-  __syncthreads();
-  return x;
+  x = s.wave[threadIdx.x & 15];
+#define STEP(ctrl, rows) x = max(x, moved<ctrl, rows>(x));
+  ROW_STEPS
+#undef STEP
+  return from_lane(x, 15);
 }
 
 // Sum of the threads before this one, and of all.
 __device__ __forceinline__ void sums(Shared& s, u64 x, u64& before, u64& all) {
   const u64 up_to = lane_sums(x);
-  const int wave = threadIdx.x >> 6;
+  const int wave = this_wave();
   __syncthreads();
   if ((threadIdx.x & 63) == 63) s.wave[wave] = up_to;
   __syncthreads();
-  before = up_to - x, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += s.wave[w];
-    all += s.wave[w];
-  }
-  __syncthreads();
+  u64 waves = s.wave[threadIdx.x & 15];
+#define STEP(ctrl, rows) waves += moved<ctrl, rows>(waves);
+  ROW_STEPS
+#undef STEP
+  all = from_lane(waves, 15);
+  before = up_to - x + (wave ? from_lane(waves, wave - 1) : 0);
 }
 
-// The value that the one thread with `mine` has (0 where none has), for all.
+// The values that the one thread with `mine` has (0 where none has), for all.
+__device__ __forceinline__ void from_one(Shared& s, bool mine, u64& x, u64& y) {
+  const int wave = this_wave();
+  const bool here = __any(mine);
+  __syncthreads();
+  if (mine || (!here && (threadIdx.x & 63) == 0)) s.wave[wave] = mine ? x : 0, s.wave2[wave] = mine ? y : 0;
+  __syncthreads();
+  x = s.wave[threadIdx.x & 15], y = s.wave2[threadIdx.x & 15];
+#define STEP(ctrl, rows) x |= moved<ctrl, rows>(x), y |= moved<ctrl, rows>(y);
+  ROW_STEPS
+#undef STEP
+  x = from_lane(x, 15), y = from_lane(y, 15);
+}
 __device__ __forceinline__ u64 from_one(Shared& s, bool mine, u64 x) {
-  if (threadIdx.x == 0) s.value[0] = 0;
-  __syncthreads();
-  if (mine) s.value[0] = x;
-  __syncthreads();
-  x = s.value[0];
-  __syncthreads();
+  u64 none = 0;
+  from_one(s, mine, x, none);
   return x;
 }
 
@@ -355,8 +369,9 @@ __device__ __forceinline__ uint32_t find_bin(Shared& s, const u64 m[2], u64 from
     if (x < target && x + m[j] >= target) hit = 2 * threadIdx.x + j + 1, at = x;
     x += m[j];
   }
-  above = from_one(s, hit != 0, at);
-  return (uint32_t)from_one(s, hit != 0, hit) - 1;
+  from_one(s, hit != 0, at, hit);
+  above = at;
+  return (uint32_t)hit - 1;
 }
 
 // The key at which the prefix of the order has `target` elements (BY_MASS: that much weight, over 0), digit by digit
@@ -444,8 +459,10 @@ __device__ __forceinline__ int last_tie(Shared& s, u64 ties, const Each& each) {
     u64 before, all;
     sums(s, c, before, all);
     const bool hit = before < ties && before + c >= ties;
-    at |= (uint32_t)from_one(s, hit, threadIdx.x) << shift;
-    ties -= from_one(s, hit, before);
+    u64 digit = threadIdx.x;
+    from_one(s, hit, digit, before);
+    at |= (uint32_t)digit << shift;
+    ties -= before;
   }
   return (int)at;
 }
@@ -458,8 +475,10 @@ __device__ __forceinline__ int locate(Shared& s, const R& row, float uniform, co
   sums(s, mine, before, all);
   const u64 target = target_of(uniform, all);
   const bool hit = before <= target && before + mine > target;
-  const int tile = (int)from_one(s, hit, threadIdx.x);
-  const u64 left = target - from_one(s, hit, before);
+  u64 where = threadIdx.x;
+  from_one(s, hit, where, before);
+  const int tile = (int)where;
+  const u64 left = target - before;
   // runs of consecutive elements a thread
   const int run = row.tile / kThreads, to = (int)min((long)(tile + 1) * row.tile - row.lead, (long)row.V);
   const long i0 = (long)tile * row.tile - row.lead + (long)threadIdx.x * run;
@@ -695,7 +714,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   const int at = blockIdx.x, tid = threadIdx.x;
   const Row<BF16> row((const char*)a.logits + (size_t)at * a.row_stride * (BF16 ? 2 : 4), a.V);
   const Params par(a, at);
-  s.table[tid] = exp2((double)tid / kTable);
+  s.table[tid] = exp2((double)tid / kTable + unit_shift(row.V));   // (in units)
   // the largest, the lowest that is finite, and each thread's largest and the first four elements that it is among
   float mine = -INFINITY, low = INFINITY;
   int mine_at = row.V;
