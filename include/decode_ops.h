@@ -97,11 +97,14 @@ int dec_gated_delta_workspace(int total, int batch, int max_q, int write_cols, i
  * integers of 2^-min(51, 62 - ceil(log2 vocabulary)), so that results do not depend on an order of additions.
  * temperature fp32, top_k int32, top_p fp32, min_p fp32 [rows], or null: the value *_all for all rows.
  * uniform fp32 [rows]; tokens int64 [rows]; logprobs (DEC_LOGPROBS) fp32 [rows], of the softmax of the
- * logits as they are (no temperature, no filter). */
+ * logits as they are (no temperature, no filter). `workspace`: dec_sample_workspace bytes (top_k: the value
+ * for all rows, or 1 where they have their own), 16-byte aligned, the call's own until it has run. */
 int dec_sample(const void* logits, long row_stride, const float* uniform, const float* temperature,
                float temperature_all, const int* top_k, int top_k_all, const float* top_p,
                float top_p_all, const float* min_p, float min_p_all, int64_t* tokens, float* logprobs,
-               int rows, int vocabulary, int flags, void* stream);
+               void* workspace, size_t workspace_bytes, int rows, int vocabulary, int flags,
+               void* stream);
+int dec_sample_workspace(int rows, int vocabulary, int top_k, int flags, size_t* bytes);
 
 #ifdef __cplusplus
 }

@@ -106,8 +106,8 @@ def test_delta_wants_its_workspace(lib):
 
 
 def sample(lib, **kw):
-    a = dict(x=P, stride=100, u=P, t=P, ta=1.0, k=P, ka=0, p=P, pa=1.0, mp=P, ma=0.0, tokens=P, lp=P,
-             rows=3, V=100, flags=N.LOGPROBS)
+    a = dict(x=P, stride=100, u=P, t=P, ta=1.0, k=P, ka=0, p=P, pa=1.0, mp=P, ma=0.0, tokens=P, lp=P, work=P,
+             wb=1 << 40, rows=3, V=100, flags=N.LOGPROBS)
     a.update(kw)
     return lib.dec_sample(*a.values(), None)
 
@@ -122,11 +122,31 @@ def test_sample_refuses(lib, kw, msg):
     assert sample(lib, **kw) == EINVAL and msg in lib.dec_last_error()
 
 
+def test_sample_wants_its_workspace(lib):
+    # 1024 sums by tiles of a row; what a part leaves: a head of 72 bytes, 2048 steps of 12, 4096 entries of 8
+    def need(rows, parts):
+        return rows * (8192 + parts * (72 + 2048 * 12 + 4096 * 8))
+    for rows, V, top_k, flags, parts in ((64, 131072, 0, 0, 4), (1, 131072, 0, 0, 8), (1, 131072, 0, N.BF16, 4),
+                                         (1, 131072, 513, 0, 8), (100, 131072, 0, 0, 2), (3, 40000, -1, 0, 2),
+                                         (1, 1 << 24, 0, 0, 16)):
+        assert N.sample_workspace(rows, V, top_k, flags) == need(rows, parts)
+        kw = dict(rows=rows, V=V, stride=V, k=None, k_all=top_k, flags=flags)
+        for more in (dict(wb=need(rows, parts) - 1), dict(work=None), dict(work=P + 8)):
+            assert sample(lib, **kw, **more) == EINVAL and b"bytes of 16-byte aligned workspace" in lib.dec_last_error()
+    # a part is 16 tiles of 1024 or 2048 elements at least, and there is one workgroup a compute unit; sorted lists
+    # are a workgroup's
+    for rows, V, top_k, flags in ((129, 131072, 0, 0), (1, 32767, 0, 0), (1, 65535, 0, N.BF16), (1, 131072, 512, 0)):
+        assert N.sample_workspace(rows, V, top_k, flags) == 0
+    for bad in ((-1, 10, 0, 0), (1, 0, 0, 0)):
+        with pytest.raises(RuntimeError, match="sample_workspace: "):
+            N.sample_workspace(*bad)
+
+
 def test_nothing_to_do_needs_no_gpu(lib):
     assert conv(lib, B=0, T=0, x=None, w=None, state=None, starts=None, read=None, write=None, out=None) == 0
     assert delta(lib, B=0, T=0, q=None, k=None, v=None, state=None, starts=None, read=None, write=None, out=None,
                  work=None, wb=0) == 0
-    assert sample(lib, rows=0, x=None, u=None, tokens=None, lp=None) == 0
+    assert sample(lib, rows=0, x=None, u=None, tokens=None, lp=None, work=None, wb=0) == 0
 
 
 def test_errors_are_the_last_ones(lib):

@@ -27,8 +27,9 @@ SIGNATURES = {
                                _long, _vp, _vp, _vp, _long, _long, _vp, _vp, _vp, _long, _int, _vp, _vp,
                                _sz, _int, _int, _int, _int, _int, _int, _int, _f, _f, _vp]),
     "dec_gated_delta_workspace": (_int, [_int] * 8 + [_psz]),
-    "dec_sample": (_int, [_vp, _long, _vp, _vp, _f, _vp, _int, _vp, _f, _vp, _f, _vp, _vp, _int, _int,
-                          _int, _vp]),
+    "dec_sample": (_int, [_vp, _long, _vp, _vp, _f, _vp, _int, _vp, _f, _vp, _f, _vp, _vp, _vp, _sz,
+                          _int, _int, _int, _vp]),
+    "dec_sample_workspace": (_int, [_int, _int, _int, _int, _psz]),
 }
 
 _lock = threading.Lock()
@@ -83,3 +84,8 @@ def gated_delta_workspace(total, batch, max_q, write_cols, k_heads, v_heads, dk,
                                           _c.byref(n)))
     return n.value
 
+
+def sample_workspace(rows, vocabulary, top_k, flags) -> int:
+    n = _sz()
+    check(lib().dec_sample_workspace(rows, vocabulary, top_k, flags, _c.byref(n)))
+    return n.value

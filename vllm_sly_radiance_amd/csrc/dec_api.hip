@@ -168,10 +168,19 @@ int check_sample_sizes(const char* who, int rows, int vocabulary, int flags) {
 }
 }  // namespace
 
+DEC_API int dec_sample_workspace(int rows, int vocabulary, int top_k, int flags, size_t* bytes) {
+  const char* who = "sample_workspace";
+  if (!bytes) return fail(DEC_EINVAL, "%s: null output", who);
+  if (int rc = check_sample_sizes(who, rows, vocabulary, flags)) return rc;
+  *bytes = sample_workspace(rows, sample_parts(rows, vocabulary, flags & DEC_BF16, top_k));
+  return DEC_OK;
+}
+
 DEC_API int dec_sample(const void* logits, long row_stride, const float* uniform, const float* temperature,
                        float temperature_all, const int* top_k, int top_k_all, const float* top_p,
                        float top_p_all, const float* min_p, float min_p_all, int64_t* tokens, float* logprobs,
-                       int rows, int vocabulary, int flags, void* stream) {
+                       void* workspace, size_t workspace_bytes, int rows, int vocabulary, int flags,
+                       void* stream) {
   const char* who = "sample";
   if (int rc = check_sample_sizes(who, rows, vocabulary, flags)) return rc;
   const int size = flags & DEC_BF16 ? 2 : 4;
@@ -184,9 +193,14 @@ DEC_API int dec_sample(const void* logits, long row_stride, const float* uniform
     return fail(DEC_EINVAL, "%s: misaligned parameters", who);
   if (!tokens || !aligned(tokens, 8) || ((flags & DEC_LOGPROBS) && (!logprobs || !aligned(logprobs, 4))))
     return fail(DEC_EINVAL, "%s: null or misaligned output", who);
+  const int parts = sample_parts(rows, vocabulary, flags & DEC_BF16, top_k ? 1 : top_k_all);
+  const size_t need = sample_workspace(rows, parts);
+  if (need > workspace_bytes || (need && (!workspace || !aligned(workspace, 16))))
+    return fail(DEC_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, need, workspace_bytes);
   SampleArgs a = {};
   a.logits = logits, a.uniform = uniform, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p;
   a.min_p = min_p, a.tokens = tokens, a.logprobs = flags & DEC_LOGPROBS ? logprobs : nullptr;
+  a.workspace = workspace, a.parts = parts;
   a.row_stride = rows > 1 ? row_stride : 0, a.rows = rows, a.V = vocabulary;
   a.temperature_all = temperature_all, a.top_k_all = top_k_all, a.top_p_all = top_p_all, a.min_p_all = min_p_all;
   a.bf16 = flags & DEC_BF16;

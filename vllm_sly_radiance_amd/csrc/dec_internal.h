@@ -91,11 +91,14 @@ struct SampleArgs {
   const float* min_p;
   int64_t* tokens;
   float* logprobs;
+  void* workspace;
   long row_stride;
-  int rows, V, top_k_all;
+  int rows, V, top_k_all, parts;        // parts: workgroups of a row
   float temperature_all, top_p_all, min_p_all;
   bool bf16;
 };
+int sample_parts(int rows, int V, bool bf16, int top_k);    // top_k: of all rows; 1 where they have their own
+size_t sample_workspace(int rows, int parts);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace dec

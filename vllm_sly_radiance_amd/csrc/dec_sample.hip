@@ -13,6 +13,8 @@
 //                      weight above them by tiles of the row; the cuts are found in the list digit by digit, and the
 //                      token in the tile where the sum of what is kept passes uniform times all of it
 //   rows of which too many elements share a step: the cuts digit by digit of the 32-bit keys, over the row
+// Where there are fewer rows than compute units, the passes of the second kind are launches of their own with
+// several workgroups a row, which leave to the next what theirs have found, in memory of the call's own.
 #include "decode_ops.h"
 #include "dec_internal.h"
 
@@ -153,16 +155,21 @@ __device__ __forceinline__ u64 from_lane(u64 x, int lane) {
 __device__ __forceinline__ int this_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // The largest of all threads.
-__device__ __forceinline__ u64 all_max(Shared& s, u64 x) {
-  x = lane_max(x);
+__device__ __forceinline__ void all_max(Shared& s, u64& x, u64& y) {
+  x = lane_max(x), y = lane_max(y);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = x;
+  if ((threadIdx.x & 63) == 63) s.wave[threadIdx.x >> 6] = x, s.wave2[threadIdx.x >> 6] = y;
   __syncthreads();
-  x = s.wave[threadIdx.x & 15];
-#define STEP(ctrl, rows) x = max(x, moved<ctrl, rows>(x));
+  x = s.wave[threadIdx.x & 15], y = s.wave2[threadIdx.x & 15];
+#define STEP(ctrl, rows) x = max(x, moved<ctrl, rows>(x)), y = max(y, moved<ctrl, rows>(y));
   ROW_STEPS
 #undef STEP
-  return from_lane(x, 15);
+  x = from_lane(x, 15), y = from_lane(y, 15);
+}
+__device__ __forceinline__ u64 all_max(Shared& s, u64 x) {
+  u64 none = 0;
+  all_max(s, x, none);
+  return x;
 }
 
 // Sum of the threads before this one, and of all.
@@ -249,9 +256,16 @@ struct Row {
   static constexpr int kRun = BF16 ? 8 : 4, kGroup = 64 * kRun * 4;
   const void* p;
   int V, lead, tile;                    // elements of a tile: kTiles of them hold the row
+  int t0, end;                          // the first tile and the end of the elements of a sweep: of all, or of a part
   __device__ __forceinline__ Row(const void* p, int V) : p(p), V(V), lead((int)((uintptr_t)p % 16) / (BF16 ? 2 : 4)) {
     tile = kGroup;
     while ((long)tile * kTiles < (long)V + lead) tile <<= 1;
+    t0 = 0, end = V;
+  }
+  // From here on, sweeps over one of `parts` parts.
+  __device__ __forceinline__ void take_part(int part, int parts) {
+    const int tiles = ((V + lead - 1) / tile + parts) / parts;
+    t0 = part * tiles, end = (int)min((long)(part + 1) * tiles * tile - lead, (long)V);
   }
   __device__ __forceinline__ void load(uint4 (&u)[4], int from) const {
     const int at = from + (int)(threadIdx.x & 63) * kRun;
@@ -280,22 +294,22 @@ struct Row {
       }
     }
   }
-  // f(x, place) for four consecutive elements of this thread's in turn; end(tile) after each of its wave's tiles.
+  // f(x, place) for four consecutive elements of this thread's in turn; done(tile) after each of its wave's tiles.
   template <bool LONG, typename F, typename G>
-  __device__ __forceinline__ void sweep(const F& f, const G& end) const {
-    int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = t * tile - lead;
-    if (from >= V) return;
+  __device__ __forceinline__ void sweep(const F& f, const G& done) const {
+    int t = t0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), from = t * tile - lead;
+    if (from >= end) return;
     uint4 u[4], next[4] = {};
     load(u, from);
 #pragma unroll 1
     for (;;) {
       int then = from + kGroup;
-      const bool last = then >= (t + 1) * tile - lead || then >= V;
+      const bool last = then >= (t + 1) * tile - lead || then >= end;
       if (last) then = (t + kWaves) * tile - lead;
-      if (then < V) load(next, then);
+      if (then < end) load(next, then);
       const int at = from + (int)(threadIdx.x & 63) * kRun;
       // (one group of four elements in the code where f is long)
-      const auto four = [&](const uint4& v, int i) {
+      const auto four = [&](const uint4 v, int i) {
         if constexpr (BF16) {
           uint32_t w0 = v.x, w1 = v.y;
 #pragma unroll 1
@@ -319,8 +333,8 @@ struct Row {
 #pragma unroll
         for (int a = 0; a < 4; ++a) four(u[a], at + a * 64 * kRun);
       }
-      if (last) end(t), t += kWaves;
-      if (then >= V) return;
+      if (last) done(t), t += kWaves;
+      if (then >= end) return;
       from = then;
 #pragma unroll
       for (int a = 0; a < 4; ++a) u[a] = next[a];
@@ -426,6 +440,7 @@ struct Params {
   }
   // the first of the largest, whatever the uniform number
   __device__ bool greedy() const { return !(t > 0.0f) || mp > 1.0f; }
+  __device__ bool by_sorting() const { return by_k && k <= kSorted; }
   // how much weight top-p asks of `total`
   __device__ double asked(u64 total) const { return ceil((double)p * (double)total); }
 };
@@ -563,25 +578,24 @@ __device__ __forceinline__ int by_sorting(Shared& s, const R& row, const Params&
   return (int)from_one(s, hit, (u64)(~(uint32_t)(f >> 32)) + 1) - 1;
 }
 
-// No cut.
-template <bool BF16, typename R>
-__device__ __forceinline__ int by_weight(Shared& s, const R& row, const Params& par, const Weights& w, float uniform) {
-  const auto weight = [&](float x, int) { return w.from(x, par.least); };
-  weigh_tiles(s, row, weight);
-  return locate<BF16>(s, row, uniform, weight);
-}
+// Steps of the distance to the largest logit: 2046 over the finite logits, or over 48 t where that is less (what is
+// further has 2^-69 of the weight, and is the last step).
+struct Steps {
+  float top, scale;
+  bool some;
+  __device__ __forceinline__ Steps(const Params& par, float top, float lowest) : top(top) {
+    const float range = fminf(top - lowest, 48.0f * par.t);
+    scale = 2046.0f / range, some = range > 0.0f && scale < 3e38f;
+  }
+  __device__ __forceinline__ int operator()(float x) const {
+    return x == top ? 0 : (int)fminf((top - x) * scale, 2047.0f);
+  }
+};
 
-// top-k and top-p by steps of the distance to the largest logit; -2: too many in a step.
-template <bool BF16, typename R>
-__device__ __forceinline__ int by_steps(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, float lowest) {
-  const int tid = threadIdx.x;
-  if (!par.by_k && !par.by_p) return by_weight<BF16>(s, row, par, w, uniform);
-  // 2046 steps over the finite logits, or over 48 t where that is less: what is further has 2^-69 of the weight
-  const float range = fminf(w.top - lowest, 48.0f * par.t), scale = 2046.0f / range;
-  if (!(range > 0.0f) || !(scale < 3e38f)) return -2;
-  const auto step = [&](float x) { return x == w.top ? 0 : (int)fminf((w.top - x) * scale, 2047.0f); };
-  for (int i = tid; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
-  if (tid == 0) s.listed = 0;
+// Counts and weights of the steps, where a cut asks for them.
+template <typename R>
+__device__ __forceinline__ void histogram(Shared& s, const R& row, const Params& par, const Weights& w, const Steps& step) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
   __syncthreads();
   row.template sweep<true>([&](const float (&x)[4], int) {
     u64 m[4];
@@ -595,72 +609,159 @@ __device__ __forceinline__ int by_steps(Shared& s, const R& row, const Params& p
     }
   });
   __syncthreads();
-  u64 m[2], c[2], before, all, elements;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) m[j] = s.mass[2 * tid + j], c[j] = s.count[2 * tid + j];
-  sums(s, c[0] + c[1], before, elements);
-  const u64 count_before = before;
-  sums(s, m[0] + m[1], before, all);
-  const bool by_k = par.by_k && elements > (u64)par.k;
-  if (!by_k && !par.by_p) return by_weight<BF16>(s, row, par, w, uniform);
-  // The steps to list: that of the cut by top-k; that by top-p; with both all from the first in which the cut by
-  // top-p can be (if nothing of top-k's step counts) to top-k's.
-  uint32_t begin = 0, end = 0;
-  u64 count_above = 0, mass_above = 0, total = all;
-  if (by_k) {
-    begin = end = find_bin(s, c, 0, (u64)par.k, count_above);
-    mass_above = from_one(s, end >> 1 == (uint32_t)tid, before + (end & 1 ? m[0] : 0));
-  }
-  if (par.by_p) {
-    const double asked = par.asked(by_k ? mass_above : all);
-    begin = find_bin(s, m, 0, (u64)fmax(asked, 1.0), mass_above);
-    if (!by_k) end = begin;
-    else count_above = from_one(s, begin >> 1 == (uint32_t)tid, count_before + (begin & 1 ? c[0] : 0));
-  }
-  if (end >= 2047) return -2;           // (the last step is all that is further)
-  // the list, and the weight above it
-  weigh_tiles(s, row, [&](float x, int at) {
-    const uint32_t i = (uint32_t)step(x);
-    const u64 m = w.from(x, par.least);
-    if (i >= begin && i <= end) {       // (not -infinity, whose step is the last)
-      const uint32_t to = atomicAdd(&s.listed, 1u);
-      if (to < (uint32_t)kList) s.key[to] = key_of(x), s.at[to] = at;
+}
+
+// The steps to list, and what lies above them.
+struct Span {
+  bool by_k, by_p;
+  uint32_t begin, end;
+  u64 count, mass, all;                 // above `begin`; of the row
+  Span() = default;
+  // (m, c: the weights and counts of steps 2 tid and 2 tid + 1)
+  __device__ __forceinline__ Span(Shared& s, const Params& par, const u64 m[2], const u64 c[2]) {
+    const uint32_t tid = threadIdx.x;
+    u64 before = 0, count_before = 0, elements = 0;
+    all = 0;
+    if (par.by_k) sums(s, c[0] + c[1], count_before, elements);
+    if (par.by_p) sums(s, m[0] + m[1], before, all);
+    by_k = par.by_k && elements > (u64)par.k, by_p = par.by_p;
+    begin = end = kBins, count = mass = 0;            // no cut: none
+    // That of the cut by top-k; that by top-p; with both all from the first in which the cut by top-p can be
+    // (if nothing of top-k's step counts) to top-k's.
+    if (by_k) {
+      begin = end = find_bin(s, c, 0, (u64)par.k, count);
+      mass = from_one(s, end >> 1 == tid, before + (end & 1 ? m[0] : 0));
     }
-    return i < begin ? m : 0;
-  });
-  const int n = (int)s.listed;
-  if (n > kList) return -2;
-  // the cuts
+    if (by_p) {
+      const double asked = par.asked(by_k ? mass : all);
+      begin = find_bin(s, m, 0, (u64)fmax(asked, 1.0), mass);
+      if (!by_k) end = begin;
+      else count = from_one(s, begin >> 1 == tid, count_before + (begin & 1 ? c[0] : 0));
+    }
+  }
+  __device__ __forceinline__ bool cuts() const { return by_k || by_p; }
+  // (the last step is all that is further)
+  __device__ __forceinline__ bool usable() const { return !cuts() || end < 2047; }
+};
+
+// The weight above the span by tiles to tile(t, sum), and the span's elements to list(key, place).
+template <typename R, typename T, typename L>
+__device__ __forceinline__ void survey(const R& row, const Params& par, const Weights& w, const Steps& step, const Span& span,
+                                       const T& tile, const L& list) {
+  u64 sum = 0;
+  row.template sweep<true>(
+      [&](const float (&x)[4], int at) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t i = (uint32_t)step(x[j]);
+          const u64 m = w.from(x[j], par.least);
+          if (i >= span.begin && i <= span.end) list(key_of(x[j]), at + j);     // (not -infinity, whose step is the last)
+          sum += i < span.begin ? m : 0;
+        }
+      },
+      [&](int t) {
+        const u64 all = lane_sums(sum);
+        if ((threadIdx.x & 63) == 63) tile(t, all);
+        sum = 0;
+      });
+}
+
+// The token, where s.tile holds the weight above the span by tiles, and s.key and s.at the span's n elements.
+template <bool BF16, typename R>
+__device__ __forceinline__ int by_list(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, const Span& span,
+                                       int n) {
+  const int tid = threadIdx.x;
   const OfList list = {s, n, w};
   Cut cut = {0, 0x7FFFFFFF};
-  u64 ties = 0;
-  if (by_k) {
-    u64 count = count_above, mass = mass_above;
-    cut.key = find_cut<false>(s, list, (u64)par.k, count, mass);
-    ties = (u64)par.k - count;
-    total = mass + ties * w(of_key(cut.key));
-  }
-  if (par.by_p) {
-    u64 count = count_above, mass = mass_above;
-    const u64 target = max((u64)fmax(par.asked(total), 1.0), mass_above + 1);
-    if (target <= total) {
-      cut.key = find_cut<true>(s, list, target, count, mass);
-      const u64 each = max(w(of_key(cut.key)), 1ull);
-      ties = (target - mass + each - 1) / each;
+  if (span.cuts() && n <= kThreads) {
+    // sorted, the cuts are places in it (3 us where the search digit by digit takes 13)
+    const u64 e = sorted(s, tid < n ? (u64)s.key[tid] << 32 | (uint32_t)~s.at[tid] : 0, power_from(n));
+    const float x = of_key((uint32_t)(e >> 32));
+    const bool there = tid < n && (!span.by_k || span.count + tid < (u64)par.k);
+    u64 before, all;
+    sums(s, there ? w(x) : 0, before, all);
+    const double asked = fmax(par.asked(span.by_k ? span.mass + all : span.all), 1.0);
+    const bool kept = there && (!span.by_p || (double)(span.mass + before) < asked);
+    const u64 last = ~all_max(s, kept ? ~e : 0);
+    cut.key = (uint32_t)(last >> 32), cut.last = (int)~(uint32_t)last;
+    if (kept) atomicAdd(&s.tile[((int)~(uint32_t)e + row.lead) / row.tile], w.from(x, par.least));
+    __syncthreads();
+  } else if (span.cuts()) {
+    u64 ties = 0, total = span.all;
+    if (span.by_k) {
+      u64 count = span.count, mass = span.mass;
+      cut.key = find_cut<false>(s, list, (u64)par.k, count, mass);
+      ties = (u64)par.k - count;
+      total = mass + ties * w(of_key(cut.key));
     }
+    if (span.by_p) {
+      u64 count = span.count, mass = span.mass;
+      const u64 target = max((u64)fmax(par.asked(total), 1.0), mass + 1);
+      if (target <= total) {
+        cut.key = find_cut<true>(s, list, target, count, mass);
+        const u64 each = max(w(of_key(cut.key)), 1ull);
+        ties = (target - mass + each - 1) / each;
+      }
+    }
+    cut.last = last_tie(s, ties, [&](auto f) {
+      for (int i = tid; i < n; i += kThreads)
+        if (s.key[i] == cut.key) f((uint32_t)s.at[i]);
+    });
+    for (int i = tid; i < n; i += kThreads) {
+      const float x = of_key(s.key[i]);
+      if (cut.keeps(s.key[i], s.at[i])) atomicAdd(&s.tile[(s.at[i] + row.lead) / row.tile], w.from(x, par.least));
+    }
+    __syncthreads();
   }
-  cut.last = last_tie(s, ties, [&](auto f) {
-    for (int i = tid; i < n; i += kThreads)
-      if (s.key[i] == cut.key) f((uint32_t)s.at[i]);
-  });
-  for (int i = tid; i < n; i += kThreads) {
-    const float x = of_key(s.key[i]);
-    if (cut.keeps(s.key[i], s.at[i])) atomicAdd(&s.tile[(s.at[i] + row.lead) / row.tile], w.from(x, par.least));
-  }
-  __syncthreads();
   return locate<BF16>(s, row, uniform, [&](float x, int at) -> u64 {
     return cut.keeps(key_of(x), at) ? w.from(x, par.least) : 0;
   });
+}
+
+// The weight of each tile to tile(t, sum), where nothing is cut.
+template <typename R, typename T>
+__device__ __forceinline__ void weigh(const R& row, const Params& par, const Weights& w, const T& tile) {
+  u64 sum = 0;
+  row.template sweep<true>(
+      [&](const float (&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += w.from(x[j], par.least);
+      },
+      [&](int t) {
+        const u64 all = lane_sums(sum);
+        if ((threadIdx.x & 63) == 63) tile(t, all);
+        sum = 0;
+      });
+}
+
+// top-k and top-p by steps; -2: too many in a step.
+template <bool BF16, typename R>
+__device__ __forceinline__ int by_steps(Shared& s, const R& row, const Params& par, const Weights& w, float uniform, float lowest) {
+  const int tid = threadIdx.x;
+  const Steps step(par, w.top, lowest);
+  u64 m[2] = {}, c[2] = {};
+  if (par.by_k || par.by_p) {
+    if (!step.some) return -2;
+    histogram(s, row, par, w, step);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) m[j] = s.mass[2 * tid + j], c[j] = s.count[2 * tid + j];
+  }
+  const Span span(s, par, m, c);
+  if (!span.usable()) return -2;
+  s.tile[tid] = 0;
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  const auto tile = [&](int t, u64 sum) { s.tile[t] = sum; };
+  if (!span.cuts())
+    weigh(row, par, w, tile);
+  else
+    survey(row, par, w, step, span, tile, [&](uint32_t key, int at) {
+      const uint32_t to = atomicAdd(&s.listed, 1u);
+      if (to < (uint32_t)kList) s.key[to] = key, s.at[to] = at;
+    });
+  __syncthreads();
+  const int n = (int)s.listed;
+  return n > kList ? -2 : by_list<BF16>(s, row, par, w, uniform, span, n);
 }
 
 // The cuts digit by digit over the row.
@@ -708,27 +809,224 @@ __device__ __forceinline__ int by_digits(Shared& s, const R& row, const Params& 
   return locate<BF16>(s, row, uniform, weight);
 }
 
+// ---- a row in parts -----------------------------------------------------------------------------
+// What the workgroups of a row's parts leave for the next launch.
+struct PartOf {
+  u64 top;                              // the key of the largest; ~0: there is a NaN
+  u64 low;                              // ~ that of the lowest finite
+  double sum;                           // of exp(x - top)
+  uint32_t listed, pad;
+  Span span;                            // of the row: the first part's
+  u64 mass[kBins];
+  uint32_t count[kBins];
+  uint32_t key[kList];
+  int at[kList];
+};
+__device__ __forceinline__ PartOf& part_of(const SampleArgs& a, int row, int part) {
+  return ((PartOf*)((char*)a.workspace + (size_t)a.rows * kTiles * 8))[(size_t)row * a.parts + part];
+}
+__device__ __forceinline__ u64* tiles_of(const SampleArgs& a, int row) { return (u64*)a.workspace + (size_t)row * kTiles; }
+
+template <bool BF16>
+__device__ __forceinline__ Row<BF16> row_of(const SampleArgs& a, int at) {
+  return Row<BF16>((const char*)a.logits + (size_t)at * a.row_stride * (BF16 ? 2 : 4), a.V);
+}
+__device__ __forceinline__ void fill_table(Shared& s, int V) {
+  s.table[threadIdx.x] = exp2((double)threadIdx.x / kTable + unit_shift(V));   // (in units)
+}
+
+// The largest, the lowest that is finite, each thread's largest and the first four elements that it is among.
+struct Ends {
+  float mine, low;
+  int mine_at;
+  u64 top_key, low_key;                 // of all threads; as in PartOf
+  template <typename R>
+  __device__ __forceinline__ Ends(Shared& s, const R& row, const Params& par) : mine(-INFINITY), low(INFINITY), mine_at(row.V) {
+    bool bad = par.t != par.t;
+    row.template sweep<false>([&](const float (&x)[4], int i) {
+      bad |= __builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]);
+      // (infinity times 0 is NaN, which a minimum passes by)
+      low = min3(min3(low, fmaf(x[0], 0.0f, x[0]), fmaf(x[1], 0.0f, x[1])), fmaf(x[2], 0.0f, x[2]), fmaf(x[3], 0.0f, x[3]));
+      const float m = max4(x);
+      if (m > mine) mine = m, mine_at = i;
+    });
+    top_key = bad ? ~0u : key_of(mine), low_key = (uint32_t)~key_of(low);
+    all_max(s, top_key, low_key);
+  }
+};
+// Those of the parts, a lane each.
+__device__ __forceinline__ void ends_of(const SampleArgs& a, int at, u64& top, u64& low) {
+  top = low = 0;
+  const int p = (int)(threadIdx.x & 15);
+  top = low = 0;
+  if (p < a.parts) top = part_of(a, at, p).top, low = part_of(a, at, p).low;
+#define STEP(ctrl, rows) top = max(top, moved<ctrl, rows>(top)), low = max(low, moved<ctrl, rows>(low));
+  ROW_STEPS
+#undef STEP
+  top = from_lane(top, 15), low = from_lane(low, 15);
+}
+// (~0 is the key of a NaN)
+__device__ __forceinline__ bool has_token(u64 top) { return of_key((uint32_t)top) > -INFINITY; }
+
+// The sum of exp(x - top): exponentials in fp32, a tile's sum of a thread in fp32. For thread 0.
+template <typename R>
+__device__ __forceinline__ double exp_sum(Shared& s, const R& row, float top) {
+  const int tid = threadIdx.x;
+  double sum = 0.0;
+  float part = 0.0f;
+  row.template sweep<true>(
+      [&](const float (&x)[4], int) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part += x[j] == top ? 1.0f : __builtin_amdgcn_exp2f((x[j] - top) * 1.44269504f);
+      },
+      [&](int) { sum += (double)part, part = 0.0f; });
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  __syncthreads();
+  if ((tid & 63) == 0) s.wave2[tid >> 6] = (u64)__double_as_longlong(sum);
+  __syncthreads();
+  sum = 0.0;
+  if (tid == 0)
+    for (int i = 0; i < kWaves; ++i) sum += __longlong_as_double((long long)s.wave2[i]);
+  return sum;
+}
+
+// The counts and weights of steps 2 tid and 2 tid + 1 in all parts.
+__device__ __forceinline__ void steps_of(const SampleArgs& a, int at, u64 m[2], u64 c[2]) {
+#pragma unroll 4
+  for (int p = 0; p < a.parts; ++p) {
+    const PartOf& part = part_of(a, at, p);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) m[j] += part.mass[2 * threadIdx.x + j], c[j] += part.count[2 * threadIdx.x + j];
+  }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads) void sample_ends(SampleArgs a) {
+  __shared__ Shared s;
+  const int at = (int)blockIdx.x / a.parts, p = (int)blockIdx.x % a.parts;
+  const Params par(a, at);
+  if (par.greedy() || par.by_sorting()) return;
+  Row<BF16> row = row_of<BF16>(a, at);
+  row.take_part(p, a.parts);
+  const Ends ends(s, row, par);
+  PartOf& part = part_of(a, at, p);
+  if (threadIdx.x == 0) part.top = ends.top_key, part.low = ends.low_key;
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads) void sample_steps(SampleArgs a) {
+  __shared__ Shared s;
+  const int at = (int)blockIdx.x / a.parts, p = (int)blockIdx.x % a.parts, tid = threadIdx.x;
+  const Params par(a, at);
+  if (par.greedy() || par.by_sorting()) return;
+  u64 top_key, low_key;
+  ends_of(a, at, top_key, low_key);
+  if (!has_token(top_key)) return;
+  const float top = of_key((uint32_t)top_key);
+  Row<BF16> row = row_of<BF16>(a, at);
+  row.take_part(p, a.parts);
+  PartOf& part = part_of(a, at, p);
+  const Steps step(par, top, of_key(~(uint32_t)low_key));
+  if (step.some && (par.by_k || par.by_p)) {
+    fill_table(s, a.V);
+    const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
+    histogram(s, row, par, w, step);    // (its first barrier is the table's)
+    for (int i = tid; i < kBins; i += kThreads) part.mass[i] = s.mass[i], part.count[i] = s.count[i];
+  }
+  if (a.logprobs) {
+    const double sum = exp_sum(s, row, top);
+    if (tid == 0) part.sum = sum;
+  }
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kThreads) void sample_lists(SampleArgs a) {
+  __shared__ Shared s;
+  const int at = (int)blockIdx.x / a.parts, p = (int)blockIdx.x % a.parts, tid = threadIdx.x;
+  const Params par(a, at);
+  if (par.greedy() || par.by_sorting()) return;
+  u64 top_key, low_key;
+  ends_of(a, at, top_key, low_key);
+  if (!has_token(top_key)) return;
+  const float top = of_key((uint32_t)top_key);
+  const Steps step(par, top, of_key(~(uint32_t)low_key));
+  u64 m[2] = {}, c[2] = {};
+  if (par.by_k || par.by_p) {
+    if (!step.some) return;
+    steps_of(a, at, m, c);
+  }
+  fill_table(s, a.V);
+  if (tid == 0) s.listed = 0;
+  const Span span(s, par, m, c);
+  if (p == 0 && tid == 0) part_of(a, at, 0).span = span;
+  if (!span.usable()) return;
+  __syncthreads();                      // (the table, and the list's length)
+  const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
+  Row<BF16> row = row_of<BF16>(a, at);
+  row.take_part(p, a.parts);
+  PartOf& part = part_of(a, at, p);
+  u64* const tiles = tiles_of(a, at);
+  const auto tile = [&](int t, u64 sum) { tiles[t] = sum; };
+  if (!span.cuts())
+    weigh(row, par, w, tile);
+  else
+    survey(row, par, w, step, span, tile, [&](uint32_t key, int place) {
+      const uint32_t to = atomicAdd(&s.listed, 1u);
+      if (to < (uint32_t)kList) part.key[to] = key, part.at[to] = place;
+    });
+  __syncthreads();
+  if (tid == 0) part.listed = s.listed;
+}
+
+// by_steps with what the parts' workgroups have left.
+template <bool BF16, typename R>
+__device__ __forceinline__ int by_parts(Shared& s, const SampleArgs& a, int at, const R& row, const Params& par, const Weights& w,
+                                        float uniform, float lowest) {
+  const int tid = threadIdx.x;
+  if ((par.by_k || par.by_p) && !Steps(par, w.top, lowest).some) return -2;
+  // (asked for together: what another die wrote is far)
+  const Span span = part_of(a, at, 0).span;
+  const int lane = tid & 63, wave = this_wave();
+  const uint32_t listed = lane < a.parts ? part_of(a, at, lane).listed : 0;
+  const u64 tile = (long)tid * row.tile < (long)row.V + row.lead ? tiles_of(a, at)[tid] : 0;
+  if (!span.usable()) return -2;
+  s.tile[tid] = tile;
+  int n = 0;
+  if (span.cuts()) {
+    // a wave takes a part's list
+    const u64 up_to = lane_sums((u64)listed);
+    if (from_lane(up_to, 15) > (u64)kList) return -2;
+    n = (int)from_lane(up_to, 15);
+    if (wave < a.parts) {
+      const PartOf& part = part_of(a, at, wave);
+      const int to = (int)from_lane(up_to, wave), more = (int)from_lane((u64)listed, wave);
+      for (int i = lane; i < more; i += 64) s.key[to - more + i] = part.key[i], s.at[to - more + i] = part.at[i];
+    }
+  }
+  __syncthreads();
+  return by_list<BF16>(s, row, par, w, uniform, span, n);
+}
+
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   __shared__ Shared s;
   const int at = blockIdx.x, tid = threadIdx.x;
-  const Row<BF16> row((const char*)a.logits + (size_t)at * a.row_stride * (BF16 ? 2 : 4), a.V);
+  const Row<BF16> row = row_of<BF16>(a, at);
   const Params par(a, at);
-  s.table[tid] = exp2((double)tid / kTable + unit_shift(row.V));   // (in units)
-  // the largest, the lowest that is finite, and each thread's largest and the first four elements that it is among
-  float mine = -INFINITY, low = INFINITY;
+  const bool in_parts = a.parts > 1 && !par.greedy() && !par.by_sorting();
+  fill_table(s, a.V);
+  float mine = 0.0f;
   int mine_at = row.V;
-  bool bad = par.t != par.t;
-  row.template sweep<false>([&](const float (&x)[4], int i) {
-    bad |= __builtin_isunordered(x[0], x[1]) | __builtin_isunordered(x[2], x[3]);
-    // (infinity times 0 is NaN, which a minimum passes by)
-    low = min3(min3(low, fmaf(x[0], 0.0f, x[0]), fmaf(x[1], 0.0f, x[1])), fmaf(x[2], 0.0f, x[2]), fmaf(x[3], 0.0f, x[3]));
-    const float m = max4(x);
-    if (m > mine) mine = m, mine_at = i;
-  });
-  const u64 ends = all_max(s, (u64)(bad ? ~0u : key_of(mine)) << 32 | (uint32_t)~key_of(low));
-  const float top = of_key((uint32_t)(ends >> 32));
-  if (!(top > -INFINITY)) {             // (~0 is the key of a NaN)
+  u64 top_key, low_key;
+  if (in_parts) {
+    ends_of(a, at, top_key, low_key);
+    __syncthreads();                    // (the table)
+  } else {
+    const Ends ends(s, row, par);
+    mine = ends.mine, mine_at = ends.mine_at, top_key = ends.top_key, low_key = ends.low_key;
+  }
+  const float top = of_key((uint32_t)top_key);
+  if (!has_token(top_key)) {
     if (tid == 0) {
       a.tokens[at] = -1;
       if (a.logprobs) a.logprobs[at] = kNaN;
@@ -738,9 +1036,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   int token = -1;
   if (!par.greedy()) {
     const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
-    const float u = a.uniform[at];
-    if (par.by_k && par.k <= kSorted) token = by_sorting(s, row, par, w, u, mine);
-    if (token < 0) token = by_steps<BF16>(s, row, par, w, u, of_key(~(uint32_t)all_max(s, (uint32_t)~key_of(low))));
+    const float u = a.uniform[at], lowest = of_key(~(uint32_t)low_key);
+    if (par.by_sorting()) token = by_sorting(s, row, par, w, u, mine);
+    if (token < 0) token = in_parts ? by_parts<BF16>(s, a, at, row, par, w, u, lowest) : by_steps<BF16>(s, row, par, w, u, lowest);
     if (token < 0) token = by_digits<BF16>(s, row, par, w, u);
   }
   if (token < 0) {
@@ -752,21 +1050,13 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
     token = (int)~(uint32_t)all_max(s, (uint32_t)~place);
   }
   if (a.logprobs) {
-    // A logarithm in fp32 of the sum of exp(x - top): exponentials in fp32, a tile's sum of a thread in fp32.
     double sum = 0.0;
-    float part = 0.0f;
-    row.template sweep<true>([&](const float (&x)[4], int) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part += x[j] == top ? 1.0f : __builtin_amdgcn_exp2f((x[j] - top) * 1.44269504f);
-              },
-              [&](int) { sum += (double)part, part = 0.0f; });
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    __syncthreads();
-    if ((tid & 63) == 0) s.wave2[tid >> 6] = (u64)__double_as_longlong(sum);
-    __syncthreads();
+    if (in_parts)
+#pragma unroll 4
+      for (int p = 0; p < a.parts; ++p) sum += part_of(a, at, p).sum;
+    else
+      sum = exp_sum(s, row, top);
     if (tid == 0) {
-      sum = 0.0;
-      for (int i = 0; i < kWaves; ++i) sum += __longlong_as_double((long long)s.wave2[i]);
       const float x = logit<BF16>(row.p, token);
       a.logprobs[at] = (float)((x == top ? 0.0 : (double)x - (double)top) - log(sum));
     }
@@ -776,10 +1066,34 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
 
 }  // namespace
 
-hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
-  if (a.bf16) sample_rows<true><<<a.rows, kThreads, 0, stream>>>(a);
-  else sample_rows<false><<<a.rows, kThreads, 0, stream>>>(a);
+// Into how many parts the rows go: so that there is a workgroup for each compute unit, with 16 of the smallest tiles
+// each at least, one a wave; 16 parts at most, a lane and a wave of the last launch each. One part where every row goes by a sorted list, whose passes over the row
+// take less than three launches.
+int sample_parts(int rows, int V, bool bf16, int top_k) {
+  if (rows < 1 || (top_k >= 1 && top_k <= kSorted && top_k < V)) return 1;
+  return max(min(min(kCUs / rows, 16), V / (16 * (bf16 ? Row<true>::kGroup : Row<false>::kGroup))), 1);
+}
+size_t sample_workspace(int rows, int parts) {
+  return parts > 1 ? (size_t)rows * (kTiles * 8 + (size_t)parts * sizeof(PartOf)) : 0;
+}
+
+namespace {
+template <bool BF16>
+hipError_t launch(const SampleArgs& a, hipStream_t stream) {
+  if (a.parts > 1) {
+    const int grid = a.rows * a.parts;
+    const bool filters = a.top_k || a.top_p || (a.top_k_all >= 1 && a.top_k_all < a.V) || a.top_p_all < 1.0f;
+    sample_ends<BF16><<<grid, kThreads, 0, stream>>>(a);
+    if (filters || a.logprobs) sample_steps<BF16><<<grid, kThreads, 0, stream>>>(a);
+    sample_lists<BF16><<<grid, kThreads, 0, stream>>>(a);
+  }
+  sample_rows<BF16><<<a.rows, kThreads, 0, stream>>>(a);
   return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
+  return a.bf16 ? launch<true>(a, stream) : launch<false>(a, stream);
 }
 
 }  // namespace dec

@@ -159,11 +159,15 @@ PyObject* sample(const Args& a) {
   const Tensor tokens = at::empty({rows}, at::TensorOptions().dtype(at::kLong).device(dev));
   const Tensor lp = at::empty({logprobs ? rows : 0}, at::TensorOptions().dtype(at::kFloat).device(dev));
   const int flags = (bf16 ? DEC_BF16 : 0) | (logprobs ? DEC_LOGPROBS : 0);
+  size_t need = 0;
+  check(dec_sample_workspace(rows, V, k.defined() ? 1 : k_all, flags, &need));
+  const Tensor space = new_bytes(dev, need);
   launch(dev, [&](void* stream) {
     return dec_sample(address(x), rows > 1 ? x.stride(0) : V, address_as<const float>(u),
                       address_as<const float>(t), t_all, address_as<const int>(k), k_all,
                       address_as<const float>(p), p_all, address_as<const float>(mp), mp_all,
-                      address_as<int64_t>(tokens), address_as<float>(lp), rows, V, flags, stream);
+                      address_as<int64_t>(tokens), address_as<float>(lp), address_as<void>(space), need, rows, V,
+                      flags, stream);
   });
   PyObject* out = PyTuple_New(2);
   if (!out) throw python_error();
