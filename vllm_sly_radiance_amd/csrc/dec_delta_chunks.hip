@@ -835,6 +835,8 @@ hipError_t launch_delta_chunks(const DeltaArgs& a, int dk, int dv, hipStream_t s
 
 DeltaPlan delta_plan(int total, int batch, int max_q, int write_cols, int Hk, int Hv, int dk, int dv) {
   DeltaPlan p = {};
+  // Token after token takes 1.8 us a token, in chunks 2.3 a chunk and two launches: 4001 tokens 7374 us against 188;
+  // few tokens have a chunk's work for 64. Where between 8 and 64 the two meet is not measured.
   p.chunks = max_q > 16 && !write_cols && total > 0;
   if (p.chunks) {
     const size_t chunks = total / C + batch;
