@@ -108,7 +108,7 @@ PyObject* gated_delta_rule(const Args& a) {
   const auto gate = [&](const char* name, const Tensor& x) {
     if (x.scalar_type() != at::kBFloat16 || x.dim() != 2 || x.size(0) != T || x.size(1) != Hv)
       fail(a.op, std::string(name) + " must be bf16 [" + str(T) + ", " + str(Hv) + "], got " + str(x));
-    return x.numel() && (stride(x, 1) > 1 || stride(x, 0) < 0) ? x.contiguous() : x;
+    return x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x;     // (one number for all heads: stride 0)
   };
   const Tensor ga = gate("a", a0), gb = gate("b", b0);
   const auto per_head = [&](const char* name, const Tensor& x) {
