@@ -19,6 +19,11 @@ __device__ __forceinline__ float sum_rows(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
 }
+__device__ __forceinline__ float max_rows(float x) {
+  x = fmaxf(x, __shfl_xor(x, 8));
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
 
 template <int R>
 __device__ __forceinline__ void load_rows(const uint16_t* p, float y[R]) {
@@ -67,21 +72,37 @@ __global__ __launch_bounds__(256) void delta_steps(DeltaArgs a, int units) {
     const float v[4] = {bf16_lo(vv.x), bf16_hi(vv.x), bf16_lo(vv.y), bf16_hi(vv.y)};
     const float alpha = expf(log_decay(bf16_f32(a.a[(size_t)t * a.a_ts + h]), rate, dt));
     const float beta = sigmoid(bf16_f32(a.b[(size_t)t * a.b_ts + h]));
-    float kk = 0.0f, qq = 0.0f, kq = 0.0f, sk[4] = {}, sq[4] = {};
+    float kk = 0.0f, qq = 0.0f, kq = 0.0f, sk[4] = {}, sq[4] = {}, pk = 1.0f, pq = 1.0f;
+    const auto squares = [&] {
+      kk = qq = 0.0f;
+#pragma unroll
+      for (int i = 0; i < R; ++i) kk = fmaf(k[i], k[i], kk), qq = fmaf(q[i], q[i], qq);
+      kk = sum_rows(kk), qq = sum_rows(qq);
+    };
+    squares();
+    if (!(plain_squares(kk) && plain_squares(qq))) {    // (of all lanes or none: they have the same row)
+      float kt = 0.0f, qt = 0.0f;
+#pragma unroll
+      for (int i = 0; i < R; ++i) kt = fmaxf(kt, fabsf(k[i])), qt = fmaxf(qt, fabsf(q[i]));
+      pk = unit_power(max_rows(kt)), pq = unit_power(max_rows(qt));
+#pragma unroll
+      for (int i = 0; i < R; ++i) k[i] *= pk, q[i] *= pq;
+      squares();
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      kk = fmaf(k[i], k[i], kk), qq = fmaf(q[i], q[i], qq), kq = fmaf(k[i], q[i], kq);
+      kq = fmaf(k[i], q[i], kq);
 #pragma unroll
       for (int c = 0; c < 4; ++c) sk[c] = fmaf(S[i][c], k[i], sk[c]), sq[c] = fmaf(S[i][c], q[i], sq[c]);
     }
-    kk = sum_rows(kk), qq = sum_rows(qq), kq = sum_rows(kq);
+    kq = sum_rows(kq);
 #pragma unroll
     for (int c = 0; c < 4; ++c) sk[c] = sum_rows(sk[c]), sq[c] = sum_rows(sq[c]);
-    const float rk = 1.0f / sqrtf(kk + a.eps), rq = a.scale / sqrtf(qq + a.eps);
+    const float rk = over_length(1.0f, kk, a.eps, pk), rq = over_length(a.scale, qq, a.eps, pq);
     float u[4], o[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      u[c] = beta * (v[c] - alpha * rk * sk[c]) * rk;    // times 1 / |k|, for the raw k below
+      u[c] = beta * (v[c] - alpha * rk * sk[c]) * rk;    // times 1 / |k|, for the k below, not of unit length
       o[c] = rq * fmaf(kq, u[c], alpha * sq[c]);
 #pragma unroll
       for (int i = 0; i < R; ++i) S[i][c] = fmaf(k[i], u[c], alpha * S[i][c]);
