@@ -43,3 +43,25 @@ def test_long_keys_meet_large_states():
         d.state *= np.float32(1e30)
         args = d.device(max_q=max_q)
         d.check(G.gated_delta_rule(*args), args[7])
+
+
+@pytest.mark.parametrize("scale", [1e25, 1e-25], ids=str)
+@pytest.mark.parametrize("what", ["q", "k", "qk"])
+def test_lengths_beside_a_value_that_is_not_finite(scale, what):
+    """A chunk with NaN in it goes token after token: the channels and the tokens that the NaN does not reach are
+    what they are without it."""
+    d = Delta(np.random.default_rng(43), [100], (1, 2, 128, 128))
+    for w in what:
+        scaled(d, w, scale)
+    for eps in (1e-6, 0.0):
+        ref, tol, states, bounds = d.expect(eps=eps)
+        args = d.device(max_q=CHUNKS)
+        args[2][70, 1, 7] = float("nan")
+        out, state = host(G.gated_delta_rule(*args, eps=eps)), host(args[7])[d.write[0]]
+        hit = np.zeros(out.shape, bool)
+        hit[70:, 1, 7] = True
+        assert np.isnan(out[hit]).all() and (np.abs(out - ref)[~hit] <= tol[~hit]).all()
+        off = np.sqrt(((state - states[0][-1]) ** 2).sum(1))
+        bad = np.zeros(off.shape, bool)
+        bad[1, 7] = True
+        assert np.isnan(off[bad]).all() and (off[~bad] <= bounds[0][-1][~bad]).all()

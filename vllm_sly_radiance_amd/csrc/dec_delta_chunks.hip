@@ -746,28 +746,34 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
         const float alpha = expf(log_decay(bf16_f32(a.a[row * a.a_ts + h]), rate, dt));
         const float beta = sigmoid(bf16_f32(a.b[row * a.b_ts + h]));
         const float vt = bf16_f32(a.v[row * a.v_ts + h * a.v_hs + col0 + col]);
-        float kk = 0.0f, qq = 0.0f, sk = 0.0f, sq = 0.0f;
+        float kk = 0.0f, qq = 0.0f, sk = 0.0f, sq = 0.0f, kt = 0.0f, qt = 0.0f;
         v4i kf[kSteps], qf[kSteps];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
           kf[i] = load8(a.k + row * a.k_ts + hk * a.k_hs + 32 * i + 8 * g);
           qf[i] = load8(a.q + row * a.q_ts + hk * a.q_hs + 32 * i + 8 * g);
 #pragma unroll
+          for (int l = 0; l < 8; ++l) kt = larger(kt, element(kf[i], l)), qt = larger(qt, element(qf[i], l));
+        }
+        const float pk = unit_power(__uint_as_float(max_groups(__float_as_uint(kt))));
+        const float pq = unit_power(__uint_as_float(max_groups(__float_as_uint(qt))));
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
           for (int l = 0; l < 8; ++l) {
-            const float kx = element(kf[i], l), qx = element(qf[i], l);
+            const float kx = element(kf[i], l) * pk, qx = element(qf[i], l) * pq;
             kk = fmaf(kx, kx, kk), qq = fmaf(qx, qx, qq), sk = fmaf(S[2 * i + l / 4][l & 3], kx, sk);
           }
-        }
         kk = sum_groups(kk), qq = sum_groups(qq), sk = sum_groups(sk);
-        const float rk = 1.0f / sqrtf(kk + a.eps), rq = a.scale / sqrtf(qq + a.eps);
+        const float rk = over_length(1.0f, kk, a.eps, pk), rq = over_length(a.scale, qq, a.eps, pq);
         const float ut = beta * (vt - alpha * rk * sk) * rk;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
           for (int l = 0; l < 8; ++l) {
-            const float y = fmaf(element(kf[i], l), ut, alpha * S[2 * i + l / 4][l & 3]);
+            const float y = fmaf(element(kf[i], l) * pk, ut, alpha * S[2 * i + l / 4][l & 3]);
             S[2 * i + l / 4][l & 3] = y;
-            sq = fmaf(y, element(qf[i], l), sq);
+            sq = fmaf(y, element(qf[i], l) * pq, sq);
           }
         sq = rq * sum_groups(sq);
         if (g == 0) a.out[(row * a.Hv + h) * dv + col0 + col] = (uint16_t)bf16x2(sq, sq);
