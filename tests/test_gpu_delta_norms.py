@@ -65,3 +65,47 @@ def test_lengths_beside_a_value_that_is_not_finite(scale, what):
         bad = np.zeros(off.shape, bool)
         bad[1, 7] = True
         assert np.isnan(off[bad]).all() and (off[~bad] <= bounds[0][-1][~bad]).all()
+
+
+# A row of length s far below sqrt(eps) counts as one of length s / sqrt(eps), in which outputs (of queries) and states (from
+# zeros, of keys) are linear: their bounds are those for length 1 times that.
+def unit_length(x, eps):
+    return np.minimum(np.sqrt((O.bf16_to_f32(x).astype(np.float64) ** 2).sum(-1) / eps), 1.0)
+
+
+@pytest.mark.parametrize("max_q", [STEPS, CHUNKS])
+@pytest.mark.parametrize("scale", [1e-6, 1e-16, 1e-20, 1e-25, 1e-30], ids=str)
+@pytest.mark.parametrize("eps", [1e-6, 1e-2], ids=str)
+def test_short_queries_beside_eps(scale, eps, max_q):
+    """(Of a state that no token adds to: beta is 0.)"""
+    d = Delta(np.random.default_rng(44), [70], (1, 2, 128, 128))
+    scaled(d, "q", scale)
+    d.b[:] = 0xFF80                                 # -infinity
+    args = d.device(max_q=max_q)
+    out = host(G.gated_delta_rule(*args, eps=eps))
+    ref, tol, *_ = d.expect(eps=eps)
+    half = 2.0 ** -8 * np.abs(ref)
+    assert (np.abs(out - ref) <= (tol - half) * unit_length(d.q, eps)[..., None] + half + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("max_q", [STEPS, CHUNKS])
+@pytest.mark.parametrize("scale", [1e-6, 1e-16, 1e-20, 1e-25, 1e-30], ids=str)
+def test_short_keys_beside_eps(scale, max_q):
+    d = Delta(np.random.default_rng(45), [70], (1, 2, 128, 128), read=[-1])
+    scaled(d, "k", scale)
+    args = d.device(max_q=max_q)
+    G.gated_delta_rule(*args)
+    *_, states, bounds = d.expect()
+    off = np.sqrt(((host(args[7])[d.write[0]] - states[0][-1]) ** 2).sum(1))
+    assert (off <= bounds[0][-1] * unit_length(d.k, 1e-6).max() + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("scale", [1e36, 1e25, 1e16, 1e-16, 1e-25, 1e-36], ids=str)
+@pytest.mark.parametrize("what", ["q", "k", "qk"])
+@pytest.mark.parametrize("eps", [1e-6, 0.0], ids=str)
+def test_lengths_in_chunks(scale, what, eps):
+    d = Delta(np.random.default_rng(46), [90, 3], (2, 4, 128, 64))
+    for w in what:
+        scaled(d, w, scale)
+    args = d.device(max_q=CHUNKS)
+    d.check(G.gated_delta_rule(*args, eps=eps), args[7], eps=eps)

@@ -13,6 +13,8 @@
 // split into two parts that add up to it, the second the rounding of what the first leaves: 22 bits, and
 // products of two such as three instructions. Two parts of bf16 hold 16 bits, and three of them took 182
 // instructions a chunk in place of 132. A state is as far from the definition as a plain evaluation in fp32.
+// T and P are at most 1 and held to 2^-37. So an output has what its own chunk adds to within 2^-37 of the values
+// there, which a query or a key that is shorter than sqrt(eps) / 2^28 makes smaller than that.
 //
 // A wave has 16 columns of a state, which do not meet others, so that its products need no other wave. As a
 // matrix instruction's result a column is a lane and 4 rows of 16 lie in a lane's registers; as its operand a
@@ -225,7 +227,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaArgs a) {
         const v2h both = half2(z, z1);
         y[i][j] = both[0], y[i][j + 1] = both[1], squares = fmaf(z1, z1, fmaf(z, z, squares));
       }
-    return 1.0f / sqrtf(fmaf(a.eps * scale, scale, sum_groups(squares)));
+    return over_length(1.0f, sum_groups(squares), a.eps, scale);
   };
   v8h kf[kSteps], qf[kSteps];
   const float rk = scaled(raw_k, kf);
