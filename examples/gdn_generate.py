@@ -80,9 +80,11 @@ class Hybrid:
 
     def fork(self, sequence):
         other = self.pool.fork(sequence)
-        self.base[other] = self.now[other] = self.free.pop()
-        for pool in (self.conv_state, self.state):
-            pool[:, self.base[other]] = pool[:, self.now[sequence]]
+        self.base[other], self.now[other] = self.free.pop(), -1
+        if self.now[sequence] >= 0:         # (else there is nothing to go on from)
+            self.now[other] = self.base[other]
+            for pool in (self.conv_state, self.state):
+                pool[:, self.base[other]] = pool[:, self.now[sequence]]
         return other
 
     def drop(self, sequence):

@@ -1,0 +1,28 @@
+"""The sequences of the example's stack where they have no tokens, none yet, or more than there is room for."""
+import numpy as np
+import pytest
+import torch
+
+from examples.gdn_generate import Hybrid
+from tests.test_gpu_gdn_generate import close
+from vllm_sly_radiance_amd import _native, _native_decode, _native_kv4
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _lib(gpu_lib):
+    return _native.lib(), _native_kv4.lib(), _native_decode.lib()
+
+
+@torch.no_grad()
+def test_a_fork_of_nothing_begins_from_nothing():
+    s = Hybrid(layers=4, pages=96)
+    rng = np.random.default_rng(5)
+    tokens = rng.integers(0, 512, 50).tolist()
+    a = s.add()
+    s.forward([a], [tokens[:4]], drafts=True)           # states that are not zero in the last slots
+    b = s.add()
+    c = s.fork(b)
+    want = s.forward([b], [tokens])[-1]
+    close(s.forward([c], [tokens])[-1], want)
