@@ -119,7 +119,8 @@ class Hybrid:
                 linear += 1
             x = x + torch.nn.functional.rms_norm(y, y.shape[-1:])
         for s, t in zip(sequences, tokens):
-            self.now[s] = self.base[s] + (len(t) - 1 if drafts else 0)
+            if t or not drafts:             # (the state after each of no tokens is written nowhere)
+                self.now[s] = self.base[s] + (len(t) - 1 if drafts else 0)
         return x.float() @ self.unembedding.float().T / x.shape[1] ** 0.5
 
 

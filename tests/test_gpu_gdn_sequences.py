@@ -26,3 +26,15 @@ def test_a_fork_of_nothing_begins_from_nothing():
     c = s.fork(b)
     want = s.forward([b], [tokens])[-1]
     close(s.forward([c], [tokens])[-1], want)
+
+
+@torch.no_grad()
+def test_a_sequence_without_tokens_among_drafts_keeps_its_state():
+    s = Hybrid(layers=4, pages=96)
+    rng = np.random.default_rng(6)
+    tokens = rng.integers(0, 512, 50).tolist()
+    a, b, c = s.add(), s.add(), s.add()
+    s.forward([a, b, c], [tokens, tokens, tokens[::-1]])
+    want = s.forward([a], [tokens[:1]])[-1]
+    s.forward([b, c], [[], tokens[:2]], drafts=True)
+    close(s.forward([b], [tokens[:1]])[-1], want)
