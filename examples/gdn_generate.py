@@ -99,7 +99,9 @@ class Hybrid:
 
     def forward(self, sequences, tokens, drafts=False):
         """Logits fp32 [total, vocabulary] of the new tokens (a list a sequence). drafts: the states after
-        each are kept, for `keep` to choose from."""
+        each are kept, for `keep` to choose from; one and DRAFT behind it at most."""
+        if drafts and max(map(len, tokens), default=0) > 1 + DRAFT:
+            raise ValueError(f"more than {DRAFT} drafted tokens behind one of a sequence")
         step = self.pool.extend(sequences, [len(t) for t in tokens])
         _, _, starts, max_q, _ = step.attention
         device = self.embedding.device

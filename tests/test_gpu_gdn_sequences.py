@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from examples.gdn_generate import Hybrid
+from examples.gdn_generate import DRAFT, Hybrid
 from tests.test_gpu_gdn_generate import close
 from vllm_sly_radiance_amd import _native, _native_decode, _native_kv4
 
@@ -38,3 +38,15 @@ def test_a_sequence_without_tokens_among_drafts_keeps_its_state():
     want = s.forward([a], [tokens[:1]])[-1]
     s.forward([b, c], [[], tokens[:2]], drafts=True)
     close(s.forward([b], [tokens[:1]])[-1], want)
+
+
+@torch.no_grad()
+def test_more_drafts_than_a_sequence_has_slots_are_refused():
+    s = Hybrid(layers=4, pages=96)
+    a = s.add()
+    s.forward([a], [[1, 2, 3]])
+    before = s.conv_state.clone(), s.state.clone(), dict(s.now), s.pool.length(a)
+    with pytest.raises(ValueError, match="drafted"):
+        s.forward([a], [list(range(2 + DRAFT))], drafts=True)
+    assert torch.equal(before[0], s.conv_state) and torch.equal(before[1], s.state)
+    assert before[2:] == (s.now, s.pool.length(a))
