@@ -73,12 +73,18 @@ class Hybrid:
             torch.from_numpy(g.standard_normal((vocabulary, hidden), np.float32))
             .to(device, torch.bfloat16) for _ in range(2))
 
+    def _room(self):
+        if not self.free:
+            raise RuntimeError(f"there are {len(self.base)} sequences, as many as there is room for")
+
     def add(self):
+        self._room()
         sequence = self.pool.add()
         self.base[sequence], self.now[sequence] = self.free.pop(), -1
         return sequence
 
     def fork(self, sequence):
+        self._room()
         other = self.pool.fork(sequence)
         self.base[other], self.now[other] = self.free.pop(), -1
         if self.now[sequence] >= 0:         # (else there is nothing to go on from)

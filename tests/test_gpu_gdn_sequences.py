@@ -50,3 +50,13 @@ def test_more_drafts_than_a_sequence_has_slots_are_refused():
         s.forward([a], [list(range(2 + DRAFT))], drafts=True)
     assert torch.equal(before[0], s.conv_state) and torch.equal(before[1], s.state)
     assert before[2:] == (s.now, s.pool.length(a))
+
+
+def test_no_room_for_a_sequence_changes_nothing():
+    s = Hybrid(layers=1, pages=96, sequences=1)
+    a = s.add()
+    for more in (s.add, lambda: s.fork(a)):
+        with pytest.raises(RuntimeError, match="1 sequences, as many as"):
+            more()
+    s.drop(a)
+    assert not s.pool._sequences and s.free == [0]
