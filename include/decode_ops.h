@@ -53,7 +53,7 @@ int dec_abi_version(void);
 /* Description of this thread's most recent failing call. */
 const char* dec_last_error(void);
 
-/* Depthwise causal convolution of `width` 2, 3 or 4 over each sequence's tokens:
+/* Depthwise causal convolution of `width` 2, 3 or 4 over each sequence's tokens, `total` 2^30 at most:
  *   out[t][c] = f(bias[c] + sum_i weight[c][i] x[t - width + 1 + i][c]), f SiLU or nothing,
  * in fp32, rounded once. x bf16 [total][channels] with rows x_ts elements apart (16-byte aligned, x_ts
  * and channels multiples of 8); weight bf16 [channels][width] and bias bf16 [channels] (or null),

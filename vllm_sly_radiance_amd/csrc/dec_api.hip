@@ -89,6 +89,8 @@ DEC_API int dec_causal_conv(const void* x, long x_ts, const void* weight, const 
   ConvArgs a = {};
   a.s = {q_starts, read_slots, write_slots, write_stride, slots, slot_stride, write_cols, total, batch, max_q};
   if (int rc = check_sequences(who, a.s, (long)(width - 1) * channels, 8)) return rc;
+  if (total > 1 << 30)                  // (a lane's next run of tokens is counted in 32 bits)
+    return fail(DEC_EINVAL, "%s: total=%d: need 2^30 at most", who, total);
   if ((long)batch * kv4::ceil_div(channels / 8, 256) > kMaxGrid)
     return fail(DEC_EINVAL, "%s: batch=%d of %d channels is too large", who, batch, channels);
   if (!batch) return DEC_OK;
