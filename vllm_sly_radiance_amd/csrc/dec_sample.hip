@@ -836,6 +836,18 @@ __device__ __forceinline__ Row<BF16> row_of(const SampleArgs& a, int at) {
 __device__ __forceinline__ void fill_table(Shared& s, int V) {
   s.table[threadIdx.x] = exp2((double)threadIdx.x / kTable + unit_shift(V));   // (in units)
 }
+// A row's weights, over the table that this thread has filled its entry of. What the rounding of `offset` leaves out is
+// the same for all of the row's exponents, and goes into the table where it is more than 2^-36, 2^-46 of a weight: from
+// |top| / t of some 88. (From 1 on nothing else has weight: logits next to each other are 2^29 times as far apart.)
+__device__ __forceinline__ Weights row_weights(Shared& s, float top, const Params& par, int V) {
+  const Weights w(top, (double)par.t, unit_shift(V), s.table);
+  const double rest = fma((double)top, w.rate, -w.offset);
+  if (fabs(rest) > 0x1p-36 && fabs(rest) < 1.0) {
+    s.table[threadIdx.x] *= exp2(-rest / kTable);
+    __syncthreads();
+  }
+  return w;
+}
 
 // The largest, the lowest that is finite, each thread's largest and the first four elements that it is among.
 struct Ends {
@@ -931,7 +943,7 @@ __global__ __launch_bounds__(kThreads) void sample_steps(SampleArgs a) {
   const Steps step(par, top, of_key(~(uint32_t)low_key));
   if (step.some && (par.by_k || par.by_p)) {
     fill_table(s, a.V);
-    const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
+    const Weights w = row_weights(s, top, par, a.V);
     histogram(s, row, par, w, step);    // (its first barrier is the table's)
     for (int i = tid; i < kBins; i += kThreads) part.mass[i] = s.mass[i], part.count[i] = s.count[i];
   }
@@ -963,7 +975,7 @@ __global__ __launch_bounds__(kThreads) void sample_lists(SampleArgs a) {
   if (p == 0 && tid == 0) part_of(a, at, 0).span = span;
   if (!span.usable()) return;
   __syncthreads();                      // (the table, and the list's length)
-  const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
+  const Weights w = row_weights(s, top, par, a.V);
   Row<BF16> row = row_of<BF16>(a, at);
   row.take_part(p, a.parts);
   PartOf& part = part_of(a, at, p);
@@ -1037,7 +1049,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   }
   int token = -1;
   if (!par.greedy()) {
-    const Weights w(top, (double)par.t, unit_shift(a.V), s.table);
+    const Weights w = row_weights(s, top, par, a.V);
     const float u = a.uniform[at], lowest = of_key(~(uint32_t)low_key);
     if (par.by_sorting()) token = by_sorting(s, row, par, w, u, mine);
     if (token < 0) token = in_parts ? by_parts<BF16>(s, a, at, row, par, w, u, lowest) : by_steps<BF16>(s, row, par, w, u, lowest);
