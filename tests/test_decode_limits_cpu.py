@@ -29,3 +29,14 @@ def test_conv_of_more_tokens_is_refused(lib, T):  # noqa: F811
 
 def test_delta_rule_of_as_many_is_too_large(lib):  # noqa: F811
     assert delta(lib, T=(1 << 30) + 1, Hk=1, Hv=1, ss=128 * 128, B=1) == EINVAL and b"too large" in lib.dec_last_error()
+
+
+def test_rows_with_a_top_k_of_their_own_are_one_part():
+    """(dec_sample.hip relies on it: of rows in parts none goes by a sorted list)"""
+    from vllm_sly_radiance_amd import _native_decode as N
+    for rows in (1, 2, 64, 300):
+        for V in (1, 2, 511, 512, 513, 32768, 131072, 1 << 24):
+            for flags in (0, N.BF16, N.LOGPROBS):
+                assert N.sample_workspace(rows, V, 1, flags) == 0
+                for k in (1, 50, 512):
+                    assert N.sample_workspace(rows, V, k, flags) == 0 or k >= V
