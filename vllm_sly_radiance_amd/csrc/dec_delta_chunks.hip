@@ -23,6 +23,7 @@
 // two result tiles are one operand as they are: S, X and U go from product to product without leaving their
 // lanes. The other operands come from memory in the order in which lanes want them.
 #include "decode_ops.h"
+#include "dec_chunks.h"
 #include "dec_delta.h"
 #include "dec_internal.h"
 
@@ -118,31 +119,6 @@ __device__ __forceinline__ ChunkKeys<DK>& delta_keys(const DeltaArgs& a, int c, 
   return ((ChunkKeys<DK>*)((char*)a.workspace + a.keys))[(size_t)c * a.Hk + hk];
 }
 
-// Chunk slots: sequence b's begin at starts[b] / 64 + b, so that total / 64 + batch slots hold all.
-__device__ __forceinline__ int first_chunk(const Sequences& s, int b) {
-  return min(max(s.starts[b], 0), s.total) / C + b;
-}
-
-// The sequence that chunk slot c belongs to, the last whose slots begin at it or before (-1 for none), its first
-// row and its number of rows.
-__device__ __forceinline__ int sequence_of(const Sequences& s, int c, int& first, int& n) {
-  const int lane = threadIdx.x & 63;
-  int b = -1;
-  for (int b0 = 0; b0 < s.batch; b0 += 64) {
-    const int start = s.starts[min(b0 + lane, s.batch)];
-    const int m = __popcll(__ballot(b0 + lane < s.batch && min(max(start, 0), s.total) / C + b0 + lane <= c));
-    b += m;
-    if (m < 64 && m) {                  // its start and the next are here
-      first = min(max(__builtin_amdgcn_readlane(start, m - 1), 0), s.total);
-      n = max(min(__builtin_amdgcn_readlane(start, m), s.total) - first, 0);
-      return b;
-    }
-    if (m < 64) break;
-  }
-  if (b >= 0) rows_of(s, b, first, n);
-  return b;
-}
-
 // Inclusive sum over the wave's lanes.
 __device__ __forceinline__ double wave_sums(double x) {
 #define STEP(ctrl, rows)                                                                                      \
@@ -176,13 +152,9 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaArgs a) {
   __shared__ __attribute__((aligned(16))) PrepareShared<DK> s;
   const int c = a.by_heads((int)blockIdx.x), h = (int)blockIdx.x - c * a.Hv;
   const int hk = a.by_group(h);
-  int first, n;
-  const int b = sequence_of(a.s, c, first, n);
-  if (b < 0) return;
-  const int i0 = (c - first / C - b) * C;
-  if (i0 >= n) return;
-  const int m = min(n - i0, C);
-  const size_t row0 = (size_t)first + i0;
+  size_t row0;
+  int m;
+  if (!rows_of_chunk(a.s, c, row0, m)) return;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
 
   constexpr int kSteps = DK / 32;
@@ -440,7 +412,7 @@ void delta_chunks(DeltaArgs a, int dv, int parts, int sequences) {
   auto& ex = sh.wave[mine];
   int first, n;
   rows_of(a.s, b, first, n);
-  const int chunks = ceil_div(n, C), c0 = first_chunk(a.s, b);
+  const int chunks = ceil_div(n, kChunk), c0 = first_chunk(a.s, b);
   const auto head_of = [&](int c) -> const ChunkHead& { return ((const ChunkHead*)a.workspace)[(size_t)(c0 + c) * a.Hv + h]; };
 
   if (outputs) {

@@ -39,7 +39,7 @@ struct Sequences {
 // First row and number of rows of sequence b, in [0, total] whatever the starts hold.
 __device__ __forceinline__ void rows_of(const Sequences& s, int b, int& first, int& n) {
   first = min(max(s.starts[b], 0), s.total);
-  n = max(min(s.starts[b + 1], s.total) - first, 0);
+  n = min(max(s.starts[b + 1], first), s.total) - first;
 }
 
 struct ConvArgs {
