@@ -46,7 +46,7 @@ def main(path, seed):
         own = int(rng.integers(batch))
         write[own, 0] = 0
         read[(read == 0) & (np.arange(batch) != own)] = -1
-        ordered = (np.diff(starts) >= 0).all()
+        ordered = (np.diff(starts.astype(np.int64)) >= 0).all()
         lens = np.diff(np.clip(starts, 0, total)) if ordered else None
         at, at_end = int(np.clip(starts[0], 0, total)), bool(rng.integers(2))
         held = [guarded(a, at_end) for a in (starts, read, write)]
