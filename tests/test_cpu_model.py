@@ -1,5 +1,6 @@
 """Kernels of libdecode_ops.so on the CPU, over a model of a workgroup (cpu_model/), with memory that ends where the data
-does: what the convolution and the delta rule read and write has to be in range whatever starts and slots hold."""
+does: sampling as a whole, with its waves in random order; and what the convolution and the delta rule read and write, which
+has to be in range whatever starts and slots hold."""
 import concurrent.futures
 import ctypes
 import os
@@ -42,12 +43,36 @@ def for_cpu(name, replace=("", "")):
     return source
 
 
+SAMPLE = """
+extern "C" int model_sample(const dec::SampleArgs* a) { return dec::launch_sample(*a, nullptr); }
+extern "C" size_t model_workspace(int rows, int parts) { return dec::sample_workspace(rows, parts); }
+extern "C" size_t model_args() { return sizeof(dec::SampleArgs); }
+"""
+
+
 def run(cases, library, seeds):
     def one(seed):
         return subprocess.run([sys.executable, "-u", "-m", "tests.cpu_model." + cases, library, str(seed)], cwd=ROOT,
                               capture_output=True, text=True, timeout=300)
     with concurrent.futures.ThreadPoolExecutor(4) as pool:
         return list(pool.map(one, seeds))
+
+
+def test_sampling_in_any_order_of_waves(tmp_path):
+    for r in run("sample", compiled(str(tmp_path), "sample", for_cpu("dec_sample.hip") + SAMPLE), range(16)):
+        assert r.returncode == 0, (r.returncode, r.stdout[-500:], r.stderr[-1500:])
+
+
+@pytest.mark.parametrize("mistake", ["a missing barrier", "a read in front of the row"])
+def test_the_model_shows_mistakes(tmp_path, mistake):
+    """(planted in a copy for the CPU)"""
+    if mistake == "a missing barrier":          # what one thread has found, read before it has left it
+        old = "s.wave[wave] = mine ? x : 0, s.wave2[wave] = mine ? y : 0;\n  __syncthreads();"
+        new = old.replace("\n  __syncthreads();", "")
+    else:
+        old, new = "if (inside || (i >= 0 && i + kRun <= V)) {", "if (inside || i + kRun <= V) {"
+    library = compiled(str(tmp_path), "wrong", for_cpu("dec_sample.hip", (old, new)) + SAMPLE)
+    assert any(r.returncode for r in run("sample", library, (3, 5, 6, 7)))
 
 
 # ---- sequences ----------------------------------------------------------------------------------
