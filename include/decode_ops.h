@@ -74,7 +74,9 @@ int dec_causal_conv(const void* x, long x_ts, const void* weight, const void* bi
  * k_heads). a, b bf16 [total][v_heads], tokens a_ts and b_ts elements apart; a_log, dt_bias fp32
  * [v_heads]. state fp32 [slots][v_heads][dk][dv], slots slot_stride elements apart (a multiple of 4),
  * 16-byte aligned. out bf16 [total][v_heads][dv]. dk and dv: 64 or 128. `workspace`:
- * dec_gated_delta_workspace bytes, 16-byte aligned, the call's own until it has run. */
+ * dec_gated_delta_workspace bytes, 16-byte aligned, the call's own until it has run: none with max_q 16 at most or
+ * write_cols > 0, else 25600 a value head and 49152 a key head (24576 with dk 64) for each of total / 64 + batch chunks, 31
+ * KB a token of 48 and 16 heads. */
 int dec_gated_delta(const void* q, long q_ts, long q_hs, const void* k, long k_ts, long k_hs,
                     const void* v, long v_ts, long v_hs, const void* a, long a_ts, const void* b,
                     long b_ts, const float* a_log, const float* dt_bias, float* state, long slots,

@@ -40,3 +40,12 @@ def test_rows_with_a_top_k_of_their_own_are_one_part():
                 assert N.sample_workspace(rows, V, 1, flags) == 0
                 for k in (1, 50, 512):
                     assert N.sample_workspace(rows, V, k, flags) == 0 or k >= V
+
+
+def test_workspace_of_the_chunks_is_as_documented():
+    from vllm_sly_radiance_amd import _native_decode as N
+    for total, batch, Hk, Hv, dk, dv in ((4001, 1, 16, 48, 128, 128), (30000, 16, 8, 16, 64, 64), (63, 2, 1, 4, 64, 128)):
+        need = (total // 64 + batch) * (25600 * Hv + (49152 if dk == 128 else 24576) * Hk)
+        assert N.gated_delta_workspace(total, batch, 17, 0, Hk, Hv, dk, dv) == need
+        for max_q, cols in ((16, 0), (17, 1)):
+            assert N.gated_delta_workspace(total, batch, max_q, cols, Hk, Hv, dk, dv) == 0

@@ -815,8 +815,11 @@ hipError_t launch_delta_chunks(const DeltaArgs& a, int dk, int dv, hipStream_t s
 
 DeltaPlan delta_plan(int total, int batch, int max_q, int write_cols, int Hk, int Hv, int dk, int dv) {
   DeltaPlan p = {};
-  // Token after token takes 1.8 us a token, in chunks 2.3 a chunk and two launches: 4001 tokens 7374 us against 188;
-  // few tokens have a chunk's work for 64. Where between 8 and 64 the two meet is not measured.
+  // Token after token takes 1.6 us a token at least, in chunks 2.3 a chunk and two launches, whatever a chunk holds: 4001
+  // tokens 7374 us against 188. Where they meet depends on how many workgroups there are. us, token after token and in
+  // chunks, at 16, 24 and 32 tokens a sequence: 1 sequence of 48 heads 31 43 55, 17 17 17 (8 tokens: 18, 17); 8 of
+  // them 44 61 78, 46 46 46; 61 of 8 heads 46 64 81, 57 57 56; 61 of 48 heads 191 267 348, 294 297 301. The rule looks at
+  // the longest sequence alone, so that all go one way: 61 of one token beside one of 17 take 289, in two calls 85.
   p.chunks = max_q > 16 && !write_cols && total > 0;
   if (p.chunks) {
     const size_t chunks = total / C + batch;

@@ -1,5 +1,5 @@
 // One token of each row of logits by temperature, top-k, top-p and min-p from a given uniform number, for
-// gfx950: a workgroup a row, which stays in the die's L2 between its passes.
+// gfx950: a workgroup a row. (Few rows stay in the dies' L2s between its passes; 256 of 131072 are read twice.)
 //
 // What top-k and top-p keep is a prefix of the row in descending order, ties by index. Weights are exp in 64
 // bits, added as integers of 2^-s: such sums are exact and the same in any order, which atomics need, and with
@@ -14,7 +14,7 @@
 //                      token in the tile where the sum of what is kept passes uniform times all of it
 //   rows of which too many elements share a step: the cuts digit by digit of the 32-bit keys, over the row
 // Exponentials bound the passes: some 30 instructions an element, 40 us a pass for a row of 131072 in one workgroup.
-// 1 row of 131072 by a sorted list takes 24 us, 64 by top-p 78 in parts (121 in one piece), 256 uncut 66.
+// 1 row of 131072 by a sorted list takes 25 us, 64 by top-p 78 in parts (121 in one piece), 256 uncut 66.
 // Where there are fewer rows than compute units, the passes of the second kind are launches of their own with
 // several workgroups a row, which leave to the next what theirs have found, in memory of the call's own.
 #include "decode_ops.h"

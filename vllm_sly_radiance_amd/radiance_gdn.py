@@ -14,8 +14,10 @@ that of the last one accepted. A slot that one sequence writes may be read by no
 written by no other.
 
 A batch's tokens lie one sequence after the other, q_starts as in radiance_kv4.attention; PagePool's steps
-have them. max_q, at least the most tokens of a sequence, chooses how the work is done, not what comes out:
-a graph captured with it serves any starts and slots.
+have them. max_q, at least the most tokens of a sequence, chooses how the work is done, not what comes out (the
+delta rule's two forms round differently): a graph captured with it serves any starts and slots. With max_q above 16 all
+sequences of a call go in chunks of 64 tokens, also those of one; decoding sequences beside a prompt are better a
+call of their own. Chunks take a workspace while the call runs (include/decode_ops.h has its size).
 
 The HIP library does the work; there is no torch fallback. Every call runs on the current stream of its
 tensors' device and allocates through torch only, so it can be captured into a graph. What the host can

@@ -52,8 +52,8 @@ def sample(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, min_p=No
     stay; of those the shortest prefix with at least top_p of their weight; of those the ones whose weight
     is at least min_p times the largest. The token is the lowest index at which the sum of what stays, up
     to it, exceeds uniform (fp32 [rows], in [0, 1)) times their sum. Each parameter is a number or a tensor
-    for the rows (temperature, top_p, min_p fp32, top_k int32 [rows]); None or a value out of its range
-    filters nothing, temperature 0 takes the first of the largest. A row that holds NaN, or nothing above
+    for the rows (temperature, top_p, min_p fp32, top_k int32 [rows]; numbers have these ranges too); None or
+    a value outside of what filters filters nothing, temperature 0 takes the first of the largest. A row that holds NaN, or nothing above
     -infinity, gives -1 (log probability NaN). Weights are added as whole numbers of 2^-min(51, 62 -
     ceil(log2 vocabulary)), so that no order of additions changes a token; one of less than half of that is
     none."""
